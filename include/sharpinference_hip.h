@@ -458,6 +458,147 @@ int si_hip_batch_values_workspace_bytes(int batch, int query_heads, int context,
 int si_hip_batch_select_last(si_hip_context* ctx, const float* input, const int32_t* control, float* output,
                              int batch, int64_t width);
 
+/* ---- many sequences at once: rows in 8 bits -------------------------------------- */
+
+/* The products of a step over many sequences (each token row a row of its
+ * operands) in 8-bit integers: rows of codes with one FP32 scale each,
+ * value = code * scale.  Rows 1..2097152, widths 1..1048576, dense
+ * row-major.  A row that holds an infinity or NaN has the scale NaN and
+ * codes 0; a row of zeros has the scale 0. */
+
+/* u = hidden + residual, updated = u (residual and updated both NULL: u =
+ * hidden), y = u * (1 / sqrt(sum(u^2) / n + eps)) * weight, scale[r] =
+ * max |y| / 127, codes[r][i] = y_i / scale[r] rounded to the nearest (ties
+ * to even), decided in FP64: the same codes in any batch.  eps finite and
+ * >= 0; outputs may not overlap any input.  Replaces: transformer.
+ * batch-residual-rms-norm (GpuBatchTransformerInstructions.cs:158-222) in
+ * front of products in 8 bits, which the reference does not have. */
+int si_hip_residual_rms_norm_i8(si_hip_context* ctx, const float* hidden, const float* residual, const float* weight,
+                                float* updated, int8_t* codes, float* scale, int64_t rows, int64_t n, float eps);
+
+/* The codes and scales of rows as they are: weights laid out once, or
+ * activations that no norm produces.  format is SI_HIP_F32, F16 or BF16
+ * (GGUF blocks: si_hip_dequant first).  No counterpart in the reference. */
+int si_hip_quantize_i8(si_hip_context* ctx, int format, const void* x, int8_t* codes, float* scale, int64_t rows,
+                       int64_t n);
+
+/* output[r][i] = codes[r][i] * scale[r].  Test and inspection entry point,
+ * as si_hip_dequant is for GGUF blocks. */
+int si_hip_dequant_i8(si_hip_context* ctx, const int8_t* codes, const float* scale, float* output, int64_t rows,
+                      int64_t n);
+
+/* y[t][o] = x_scale[t] * w_scale[o] * sum_k x[t][k] w[o][k] (+
+ * residual[t][o], which may be y), x [m, cols] and w [rows, cols] codes,
+ * 16-byte aligned, cols a multiple of 16 in 16..65536: exact int32 sums on
+ * the matrix cores, one FP32 rounding for each scale and for the residual.
+ * Small grids use the context's split buffer, so a call allocates nothing.
+ * Replaces: transformer.batch-shared-matvec (GpuBatchTransformerInstructions.cs:
+ * 224-279) for weights kept in 8 bits. */
+int si_hip_gemm_i8(si_hip_context* ctx, const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale,
+                   float* y, int64_t m, int64_t rows, int64_t cols, const float* residual);
+
+/* ---- many sequences at once: a cache in pages ----------------------------------------- */
+
+/* Keys and values of many sequences in pools of equal pages, each page
+ * `page_size` positions of one sequence, in any order.  One page of one KV
+ * head (si_hip_paged_page_bytes) is
+ *   SI_HIP_F16:  fp16 [page_size][head_size]
+ *   SI_HIP_Q4_0: bytes [page_size][head_size / 2], byte j of a position
+ *                holding values 2j (low nibble) and 2j + 1 (high), then fp16
+ *                scales [head_size / 32][page_size]; value = scale * (nibble
+ *                - 8): the values of a Q4_0 block, nibbles and scales apart
+ * and a pool is [pages][kv_heads] of them. */
+typedef struct si_hip_paged_cache {
+    void* key_pages;           /* 16-byte aligned */
+    void* value_pages;         /* 16-byte aligned */
+    int64_t pages;             /* of the pool, 1..2^31 - 1 */
+    int32_t page_size;         /* 16, 32, 64, 128 or 256 */
+    int32_t kv_heads;          /* 1..256 */
+    int32_t head_size;         /* 64 or 128 */
+    int32_t cache_format;      /* SI_HIP_F16 or SI_HIP_Q4_0 */
+} si_hip_paged_cache;
+
+/* The newest positions of `sequences` sequences, row after row: rows
+ * row_starts[s] .. row_starts[s + 1] - 1 are the last positions of sequence
+ * s, whose cache holds lengths[s] positions with them, so row t is position
+ * lengths[s] - row_starts[s + 1] + t.  A sequence may bring no row.  Rows
+ * from row_starts[sequences] on belong to none and are neither read nor
+ * written.  The arrays are read on the GPU when the call runs there, so a
+ * recorded plan serves whatever they hold at each replay. */
+typedef struct si_hip_paged_batch {
+    const int32_t* page_table; /* device [sequences][max_pages]: the page of positions page_size * i and on;
+                                  entries behind a sequence's end are not looked at */
+    const int32_t* row_starts; /* device [sequences + 1], from 0 up */
+    const int32_t* lengths;    /* device [sequences] */
+    int32_t sequences;         /* 1..4096 */
+    int32_t max_pages;         /* max_pages * page_size at most 2^30 */
+    int32_t rows;              /* rows of the batch's buffers, 1..1048576 */
+    int32_t max_rows;          /* most rows that one sequence brings, 1..rows */
+} si_hip_paged_batch;
+
+/* Bytes of one page of one KV head. */
+int si_hip_paged_page_bytes(int cache_format, int page_size, int head_size, uint64_t* bytes);
+
+typedef struct si_hip_paged_append_args {
+    si_hip_paged_batch batch;
+    si_hip_paged_cache cache;
+    const float* qkv;          /* [rows][(query_heads + 2 * kv_heads) * head_size] */
+    const float* frequencies;  /* [rotary_size / 2]: angle of pair i = position * frequencies[i] */
+    float* query;              /* [rows][query_heads * head_size] rotated queries */
+    int32_t query_heads;       /* 1..16 times kv_heads */
+    int32_t rotary_size;       /* even, 0..head_size */
+    float rope_scale;          /* multiplies cos and sin */
+} si_hip_paged_append_args;
+
+/* Every row of the batch: rotate-half rotary embedding of the first
+ * rotary_size values of each q and k head (in FP64, rounded to FP32), q to
+ * `query`, k and v to the row's place in the pages, rounded to fp16 or to
+ * blocks of 32 4-bit values: scale = the block's value of largest magnitude
+ * (the first of equals) / -8 in fp16, nibble = value / scale rounded to the
+ * nearest + 8, at most 15.  A 4-bit block with a value beyond +-65504 or
+ * NaN reads back as NaN.  A row whose position lies outside 0..max_pages *
+ * page_size - 1, or in a page outside 0..pages - 1, writes nothing.  Two
+ * rows of one call may not share a place.  Replaces: transformer.
+ * batch-rope-kv-write (GpuBatchTransformerInstructions.cs:318-413), whose
+ * cache is one dense array of one sequence. */
+int si_hip_paged_kv_append(si_hip_context* ctx, const si_hip_paged_append_args* args);
+
+/* keys, values [rows][kv_heads * head_size]: the values that the pages hold
+ * for the batch's rows (row_starts spanning whole lengths reads whole
+ * sequences); NaN for a row without a place.  Test and inspection entry
+ * point, and the way to take a sequence out of a cache. */
+int si_hip_paged_kv_read(si_hip_context* ctx, const si_hip_paged_batch* batch, const si_hip_paged_cache* cache,
+                         float* keys, float* values);
+
+typedef struct si_hip_paged_attention_args {
+    si_hip_paged_batch batch;
+    si_hip_paged_cache cache;
+    const float* query;        /* [rows][query_heads * head_size], 16-byte aligned */
+    void* output;              /* [rows][query_heads * head_size] of output_format, 16-byte aligned */
+    void* workspace;           /* si_hip_paged_attention_workspace_bytes, 16-byte aligned; any contents on entry;
+                                  calls sharing one workspace must not overlap on the GPU */
+    int32_t query_heads;       /* 1..16 times kv_heads */
+    int32_t output_format;     /* SI_HIP_F16 or SI_HIP_BF16 */
+} si_hip_paged_attention_args;
+
+int si_hip_paged_attention_workspace_bytes(int query_heads, int kv_heads, int head_size, uint64_t* bytes);
+
+/* output_t,h = softmax(q_t,h . K^T / sqrt(head_size)) . V over the positions
+ * of row t's sequence up to its own, KV head h / (query_heads / kv_heads),
+ * for every row of the batch (appended before).  Products in FP16 on the
+ * matrix cores (queries / sqrt(head_size) times log2(e), cached values and
+ * exponentials rounded to fp16), statistics and sums in FP32.  A row before
+ * position 0 (a sequence with fewer positions than rows) sees nothing and
+ * is 0.  A row that sees a page outside 0..pages - 1, a cached infinity or
+ * NaN or a 4-bit scale beyond +-8188 (values that fp16 cannot hold; append
+ * writes none) holds NaN or infinities; all rows of a sequence with a negative length,
+ * one beyond max_pages * page_size, or more than max_rows rows hold NaN.  What a row
+ * does not see (later positions, the rest of the last page) changes nothing
+ * of it, whatever it holds.  Replaces: transformer.batch-gqa-scores,
+ * batch-causal-softmax and batch-gqa-values (GpuBatchTransformerInstructions.cs:
+ * 415-598) for many sequences over pages. */
+int si_hip_paged_attention(si_hip_context* ctx, const si_hip_paged_attention_args* args);
+
 /* ---- Phi-4 decode step ------------------------------------------------------------ */
 
 typedef struct si_hip_phi4_layer {

@@ -44,6 +44,12 @@ SOURCES = [
     "si_batch_abi.cpp",
     "si_t0.hip",
     "si_t0_abi.cpp",
+    "si_i8.hip",
+    "si_i8_gemm.hip",
+    "si_i8_abi.cpp",
+    "si_paged.hip",
+    "si_paged_attention.hip",
+    "si_paged_abi.cpp",
 ]
 
 

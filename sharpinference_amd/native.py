@@ -117,6 +117,30 @@ class BatchAttentionArgs(ctypes.Structure):
                 ("kv_heads", _i32), ("head_size", _i32), ("context", _i32)]
 
 
+class PagedBatch(ctypes.Structure):
+    """si_hip_paged_batch."""
+    _fields_ = [("page_table", _vp), ("row_starts", _vp), ("lengths", _vp), ("sequences", _i32),
+                ("max_pages", _i32), ("rows", _i32), ("max_rows", _i32)]
+
+
+class PagedCache(ctypes.Structure):
+    """si_hip_paged_cache."""
+    _fields_ = [("key_pages", _vp), ("value_pages", _vp), ("pages", _i64), ("page_size", _i32),
+                ("kv_heads", _i32), ("head_size", _i32), ("cache_format", _i32)]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """si_hip_paged_append_args."""
+    _fields_ = [("batch", PagedBatch), ("cache", PagedCache), ("qkv", _vp), ("frequencies", _vp), ("query", _vp),
+                ("query_heads", _i32), ("rotary_size", _i32), ("rope_scale", ctypes.c_float)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """si_hip_paged_attention_args."""
+    _fields_ = [("batch", PagedBatch), ("cache", PagedCache), ("query", _vp), ("output", _vp), ("workspace", _vp),
+                ("query_heads", _i32), ("output_format", _i32)]
+
+
 class Phi4Layer(ctypes.Structure):
     """si_hip_phi4_layer."""
     _fields_ = [("attn_norm", _vp), ("qkv", _vp), ("o", _vp), ("ffn_norm", _vp), ("up", _vp), ("down", _vp),
@@ -221,6 +245,15 @@ SIGNATURES.update({
     "si_hip_batch_gqa_attention": ([_vp, ctypes.POINTER(BatchAttentionArgs), _vp], _i32),
     "si_hip_batch_values_workspace_bytes": ([_i32, _i32, _i32, ctypes.POINTER(_u64)], _i32),
     "si_hip_batch_select_last": ([_vp, _vp, _vp, _vp, _i32, _i64], _i32),
+    "si_hip_residual_rms_norm_i8": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_float], _i32),
+    "si_hip_quantize_i8": ([_vp, _i32, _vp, _vp, _vp, _i64, _i64], _i32),
+    "si_hip_dequant_i8": ([_vp, _vp, _vp, _vp, _i64, _i64], _i32),
+    "si_hip_gemm_i8": ([_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp], _i32),
+    "si_hip_paged_page_bytes": ([_i32, _i32, _i32, ctypes.POINTER(_u64)], _i32),
+    "si_hip_paged_kv_append": ([_vp, ctypes.POINTER(PagedAppendArgs)], _i32),
+    "si_hip_paged_kv_read": ([_vp, ctypes.POINTER(PagedBatch), ctypes.POINTER(PagedCache), _vp, _vp], _i32),
+    "si_hip_paged_attention_workspace_bytes": ([_i32, _i32, _i32, ctypes.POINTER(_u64)], _i32),
+    "si_hip_paged_attention": ([_vp, ctypes.POINTER(PagedAttentionArgs)], _i32),
     "si_hip_phi4_workspace_bytes": ([ctypes.POINTER(Phi4Model), ctypes.POINTER(_u64)], _i32),
     "si_hip_phi4_decode": ([_vp, ctypes.POINTER(Phi4Model)], _i32),
     "si_hip_phi4_decode_bounded": ([_vp, ctypes.POINTER(Phi4Model), _i32], _i32),
@@ -502,6 +535,34 @@ class HipContext:
     def batch_select_last(self, x: int, control: int, out: int, batch: int, width: int) -> None:
         self._call(lib().si_hip_batch_select_last, _p(x), _p(control), _p(out), batch, width)
 
+    # many sequences at once: rows in 8 bits
+    def residual_rms_norm_i8(self, hidden: int, residual: int, w: int, updated: int, codes: int, scale: int, rows: int,
+                             n: int, eps: float) -> None:
+        """residual and updated both 0: the norm of `hidden` alone."""
+        self._call(lib().si_hip_residual_rms_norm_i8, _p(hidden), _p(residual), _p(w), _p(updated), _p(codes), _p(scale),
+                   rows, n, ctypes.c_float(eps))
+
+    def quantize_i8(self, fmt: int, x: int, codes: int, scale: int, rows: int, n: int) -> None:
+        self._call(lib().si_hip_quantize_i8, fmt, _p(x), _p(codes), _p(scale), rows, n)
+
+    def dequant_i8(self, codes: int, scale: int, out: int, rows: int, n: int) -> None:
+        self._call(lib().si_hip_dequant_i8, _p(codes), _p(scale), _p(out), rows, n)
+
+    def gemm_i8(self, x: int, x_scale: int, w: int, w_scale: int, y: int, m: int, rows: int, cols: int,
+                residual: int = 0) -> None:
+        """y[m, rows] = (x . w^T) * x_scale[:, None] * w_scale (+ residual), 8-bit codes, FP32 y."""
+        self._call(lib().si_hip_gemm_i8, _p(x), _p(x_scale), _p(w), _p(w_scale), _p(y), m, rows, cols, _p(residual))
+
+    # many sequences at once: a cache in pages
+    def paged_kv_append(self, args: PagedAppendArgs) -> None:
+        self._call(lib().si_hip_paged_kv_append, ctypes.byref(args))
+
+    def paged_kv_read(self, batch: PagedBatch, cache: PagedCache, keys: int, values: int) -> None:
+        self._call(lib().si_hip_paged_kv_read, ctypes.byref(batch), ctypes.byref(cache), _p(keys), _p(values))
+
+    def paged_attention(self, args: PagedAttentionArgs) -> None:
+        self._call(lib().si_hip_paged_attention, ctypes.byref(args))
+
     def phi4_decode(self, model: Phi4Model) -> None:
         self._call(lib().si_hip_phi4_decode, ctypes.byref(model))
 
@@ -603,6 +664,19 @@ def gqa_workspace_bytes(query_heads: int, head_size: int, context: int) -> int:
 def batch_values_workspace_bytes(batch: int, query_heads: int, context: int) -> int:
     n = ctypes.c_uint64(0)
     _check(lib().si_hip_batch_values_workspace_bytes(batch, query_heads, context, ctypes.byref(n)))
+    return n.value
+
+
+def paged_page_bytes(fmt: int, page_size: int, head_size: int) -> int:
+    """Bytes of one page of one KV head."""
+    n = ctypes.c_uint64(0)
+    _check(lib().si_hip_paged_page_bytes(fmt, page_size, head_size, ctypes.byref(n)))
+    return n.value
+
+
+def paged_attention_workspace_bytes(query_heads: int, kv_heads: int, head_size: int) -> int:
+    n = ctypes.c_uint64(0)
+    _check(lib().si_hip_paged_attention_workspace_bytes(query_heads, kv_heads, head_size, ctypes.byref(n)))
     return n.value
 
 
