@@ -578,16 +578,18 @@ typedef struct si_hip_paged_attention_args {
     void* workspace;           /* si_hip_paged_attention_workspace_bytes, 16-byte aligned; any contents on entry;
                                   calls sharing one workspace must not overlap on the GPU */
     int32_t query_heads;       /* 1..16 times kv_heads */
-    int32_t output_format;     /* SI_HIP_F16 or SI_HIP_BF16 */
+    int32_t output_format;     /* SI_HIP_F32, SI_HIP_F16 or SI_HIP_BF16 */
 } si_hip_paged_attention_args;
 
 int si_hip_paged_attention_workspace_bytes(int query_heads, int kv_heads, int head_size, uint64_t* bytes);
 
 /* output_t,h = softmax(q_t,h . K^T / sqrt(head_size)) . V over the positions
  * of row t's sequence up to its own, KV head h / (query_heads / kv_heads),
- * for every row of the batch (appended before).  Products in FP16 on the
- * matrix cores (queries / sqrt(head_size) times log2(e), cached values and
- * exponentials rounded to fp16), statistics and sums in FP32.  A row before
+ * for every row of the batch (appended before).  Products on the matrix
+ * cores, statistics and sums in FP32: for BF16 outputs of FP16 operands
+ * (queries / sqrt(head_size) times log2(e), cached values and exponentials
+ * rounded to fp16 once), for F16 and F32 outputs of operands in two fp16
+ * terms (22 bits; cached values exact).  A row before
  * position 0 (a sequence with fewer positions than rows) sees nothing and
  * is 0.  A row that sees a page outside 0..pages - 1, a cached infinity or
  * NaN or a 4-bit scale beyond +-8188 (values that fp16 cannot hold; append

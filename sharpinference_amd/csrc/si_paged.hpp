@@ -54,14 +54,16 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s);
 hipError_t launch_paged_read(const PagedBatch& batch, const PagedCache& cache, float* keys, float* values,
                              hipStream_t s);
 
+enum PagedOut : int { PAGED_OUT_F32, PAGED_OUT_F16, PAGED_OUT_BF16 };
+
 struct PagedAttentionArgs {
     PagedBatch batch;
     PagedCache cache;
     const float* query;        // [rows][heads * head], 16-byte aligned
-    uint16_t* out;             // [rows][heads * head] FP16 or BF16, 16-byte aligned
+    void* out;                 // [rows][heads * head], 16-byte aligned
     float* workspace;
     int heads;
-    bool bf16;
+    int out_format;            // PagedOut
 };
 
 int64_t paged_attention_workspace_floats(int heads, int kv_heads, int head);

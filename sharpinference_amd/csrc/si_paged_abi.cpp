@@ -216,8 +216,8 @@ int si_hip_paged_attention(si_hip_context* ctx, const si_hip_paged_attention_arg
     const int d = p.cache.head;
     if (check_heads(ctx, op, args->query_heads, p.cache.kv_heads))
         return SI_HIP_ERR_ARGUMENT;
-    if (args->output_format != SI_HIP_F16 && args->output_format != SI_HIP_BF16)
-        return fail(ctx, SI_HIP_ERR_UNSUPPORTED, "%s: output of %s (%d) is not F16 or BF16", op,
+    if (args->output_format != SI_HIP_F32 && args->output_format != SI_HIP_F16 && args->output_format != SI_HIP_BF16)
+        return fail(ctx, SI_HIP_ERR_UNSUPPORTED, "%s: output of %s (%d) is not F32, F16 or BF16", op,
                     fmt_name(args->output_format), args->output_format);
     if (check_ptr(ctx, op, args->query, "query", 16) || check_ptr(ctx, op, args->output, "output", 16) ||
         check_ptr(ctx, op, args->workspace, "workspace", 16))
@@ -225,7 +225,7 @@ int si_hip_paged_attention(si_hip_context* ctx, const si_hip_paged_attention_arg
     const uint64_t count = static_cast<uint64_t>(p.batch.rows) * args->query_heads * d;
     const uint64_t ws_b =
         static_cast<uint64_t>(si::paged_attention_workspace_floats(args->query_heads, p.cache.kv_heads, d)) * 4;
-    if (check_apart(ctx, op, {{args->output, count * 2}, {args->workspace, ws_b}},
+    if (check_apart(ctx, op, {{args->output, count * (args->output_format == SI_HIP_F32 ? 4 : 2)}, {args->workspace, ws_b}},
                     {{args->query, count * 4},
                      {p.cache.keys, p.pool_bytes},
                      {p.cache.values, p.pool_bytes},
@@ -233,9 +233,11 @@ int si_hip_paged_attention(si_hip_context* ctx, const si_hip_paged_attention_arg
                      {p.batch.starts, p.starts_bytes},
                      {p.batch.lengths, p.lengths_bytes}}))
         return SI_HIP_ERR_ARGUMENT;
-    const si::PagedAttentionArgs a{p.batch, p.cache, args->query, static_cast<uint16_t*>(args->output),
-                                   static_cast<float*>(args->workspace), args->query_heads,
-                                   args->output_format == SI_HIP_BF16};
+    const si::PagedAttentionArgs a{p.batch, p.cache, args->query, args->output, static_cast<float*>(args->workspace),
+                                   args->query_heads,
+                                   args->output_format == SI_HIP_F32   ? si::PAGED_OUT_F32
+                                   : args->output_format == SI_HIP_F16 ? si::PAGED_OUT_F16
+                                                                       : si::PAGED_OUT_BF16};
     return launched(ctx, si::launch_paged_attention(a, ctx->stream), op);
 }
 

@@ -10,7 +10,9 @@ slack) in numerator and denominator, and once h for their own rounding and
 once h for the value's: |error| <= (exp(4 h slack) - 1 + 2 h) * (weighted
 mean of |v|), plus half a step of the output, plus 1e-5 of the mean for FP32
 sums and exponentials.  Over a whole output the roundings average out: its
-norm is off by no more than half a step of the output and 6 h.
+norm is off by no more than half a step of the output and 6 h.  Outputs of
+F16 and F32 come of two-term operands: h = 2^-18 stands for their 2^-22, the
+terms' floor of 2^-25 and FP32 sums of up to 128 products.
 """
 import itertools
 
@@ -20,7 +22,7 @@ import pytest
 from sharpinference_amd import native
 from tests import paged_reference as ref
 
-F16, BF16, Q4 = native.F16, native.BF16, native.Q4_0
+F32, F16, BF16, Q4 = native.F32, native.F16, native.BF16, native.Q4_0
 gpu = pytest.mark.gpu
 SENTINEL = 0x7B
 
@@ -236,7 +238,8 @@ def test_append_rows_without_a_place(hip):
 
 def _attend(hip, st, heads, q, out_fmt=BF16, ws_fill=0xFF):
     """Output [rows, heads, d] in 64 bits; the workspace starts with NaN in it."""
-    nbytes = st.rows * heads * st.d * 2
+    wide = out_fmt == F32
+    nbytes = st.rows * heads * st.d * (4 if wide else 2)
     out = hip.to_device(np.full(nbytes + 64, SENTINEL, np.uint8))
     dq = hip.to_device(q)
     size = native.paged_attention_workspace_bytes(heads, st.kv, st.d)
@@ -246,18 +249,20 @@ def _attend(hip, st, heads, q, out_fmt=BF16, ws_fill=0xFF):
     assert np.all(ws.readback(np.uint8, 64, size) == ws_fill)
     raw = out.readback(np.uint8)
     assert np.all(raw[nbytes:] == SENTINEL)
-    u = raw[:nbytes].view(np.uint16).reshape(st.rows, heads, st.d)
-    assert np.all(u[st.used:] == SENTINEL * 0x0101), "rows behind the last sequence"
+    u = raw[:nbytes].view(np.uint32 if wide else np.uint16).reshape(st.rows, heads, st.d)
+    assert np.all(u[st.used:] == SENTINEL * (0x01010101 if wide else 0x0101)), "rows behind the last sequence"
+    if wide:
+        return u.view(np.float32).astype(np.float64)
     if out_fmt == F16:
         return u.view(np.float16).astype(np.float64)
     return (u.astype(np.uint32) << 16).view(np.float32).astype(np.float64)
 
 
 def _check_rows(st, heads, q, got, out_fmt, rows=None):
-    half_out = 2.0 ** -11 if out_fmt == F16 else 2.0 ** -8
+    half_out = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}[out_fmt]
     # (FP16 outputs among the subnormals have a step of their own)
     floor = 2.0 ** -25 if out_fmt == F16 else 0.0
-    h = 2.0 ** -11
+    h = 2.0 ** -11 if out_fmt == BF16 else 2.0 ** -18
     err2 = norm2 = 0.0
     for s, (new, length) in enumerate(st.seqs):
         if rows is not None and not set(rows) & set(range(st.starts[s], st.starts[s + 1])):
@@ -294,7 +299,7 @@ ATTENDS = [
 
 @gpu
 @pytest.mark.parametrize("head,heads,kv,page,seqs", ATTENDS)
-@pytest.mark.parametrize("fmt,out_fmt", [(Q4, BF16), (F16, F16)])
+@pytest.mark.parametrize("fmt,out_fmt", [(Q4, BF16), (F16, F16), (Q4, F32), (F16, BF16)])
 def test_attention(hip, fmt, out_fmt, head, heads, kv, page, seqs):
     st = Setup(hip, fmt, head, kv, page, seqs, seed=heads).fill().upload()
     q = st.rng.standard_normal((st.rows, heads * head)).astype(np.float32)
@@ -607,7 +612,7 @@ def test_refusals(hip):
               {"workspace": ws.ptr + 4}, {"query_heads": 0}, {"query_heads": 5}, {"query_heads": 34},
               {"output": query.ptr}, {"output": st.cache.key_pages}, {"workspace": out.ptr}):
         refused(arg, hip.paged_attention, with_(att, **c))
-    refused(uns, hip.paged_attention, with_(att, output_format=native.F32))
+    refused(uns, hip.paged_attention, with_(att, output_format=native.Q8_0))
     for keys, vals in ((0, out.ptr), (query.ptr, 0), (query.ptr, query.ptr), (st.cache.key_pages, query.ptr)):
         refused(arg, hip.paged_kv_read, st.batch, st.cache, keys, vals)
     assert np.array_equal(before, st.dev[3].readback(np.uint8))
