@@ -230,9 +230,14 @@ struct Attend {
         }
     }
 
-    // Loads the unit of 64 positions from `base` on; pages[u]: the page of
-    // granule u, -1 for one that is not there (page 0 is read in its place).
-    __device__ __forceinline__ void load(Raw<D, Q4>& r, int kvh, int base, const int* pages) const
+    __device__ __forceinline__ int64_t page_at(int page, int kvh) const
+    {
+        return (int64_t(page < 0 ? 0 : page) * a.cache.kv_heads + kvh) * head_bytes;
+    }
+
+    // Loads the keys of the unit of 64 positions from `base` on; pages[u]: the
+    // page of granule u, -1 for one that is not there (page 0 is read in its place).
+    __device__ __forceinline__ void load_keys(Raw<D, Q4>& r, int kvh, int base, const int* pages) const
     {
         const int ps = a.cache.page_size;
         r.lost = 0;
@@ -240,9 +245,7 @@ struct Attend {
         for (int u = 0; u < 4; u++) {
             const int slot = (base + GRANULE * u) & (ps - 1);
             r.lost |= pages[u] < 0 ? 1u << u : 0u;
-            const int64_t off = (int64_t(pages[u] < 0 ? 0 : pages[u]) * a.cache.kv_heads + kvh) * head_bytes;
-            const char* kp = a.cache.keys + off;
-            const char* vp = a.cache.values + off;
+            const char* kp = a.cache.keys + page_at(pages[u], kvh);
             if constexpr (Q4) {
                 const char* kr = kp + slot * (D / 2) + (D / 2 * c + D / 8 * g);
                 if constexpr (D == 128) {
@@ -253,6 +256,25 @@ struct Attend {
                     r.k[u][0] = t.x, r.k[u][1] = t.y;
                 }
                 r.kd[u] = *reinterpret_cast<const uint16_t*>(kp + ps * (D / 2) + 2 * slot + 2 * ((D == 128 ? g : g >> 1) * ps + c));
+            } else {
+                const char* kr = kp + slot * (2 * D) + (2 * D * c + 16 * g);
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    const uint4 t = *reinterpret_cast<const uint4*>(kr + 64 * j);
+                    r.k[u][4 * j] = t.x, r.k[u][4 * j + 1] = t.y, r.k[u][4 * j + 2] = t.z, r.k[u][4 * j + 3] = t.w;
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void load_values(Raw<D, Q4>& r, int kvh, int base, const int* pages) const
+    {
+        const int ps = a.cache.page_size;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int slot = (base + GRANULE * u) & (ps - 1);
+            const char* vp = a.cache.values + page_at(pages[u], kvh);
+            if constexpr (Q4) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const char* vr = vp + slot * (D / 2) + (4 * g + i) * (D / 2) + NV / 2 * c;
@@ -262,12 +284,6 @@ struct Attend {
                                                                 2 * ((D == 128 ? c >> 2 : c >> 3) * ps + 4 * g));
                 r.vd[u][0] = t.x, r.vd[u][1] = t.y;
             } else {
-                const char* kr = kp + slot * (2 * D) + (2 * D * c + 16 * g);
-#pragma unroll
-                for (int j = 0; j < NJ; j++) {
-                    const uint4 t = *reinterpret_cast<const uint4*>(kr + 64 * j);
-                    r.k[u][4 * j] = t.x, r.k[u][4 * j + 1] = t.y, r.k[u][4 * j + 2] = t.z, r.k[u][4 * j + 3] = t.w;
-                }
                 const char* vr = vp + slot * (2 * D) + (2 * D * 4 * g + 2 * NV * c);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -308,11 +324,8 @@ struct Attend {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(k.v, q[j], s, 0, 0, 0);
     }
 
-    // One unit of 64 positions from `base` on: positions up to `limit` count
-    // for this lane's row, `full`: the whole unit for every row.
-    __device__ __forceinline__ void unit(State<D>& st, Raw<D, Q4>& r, int base, int limit, bool full) const
+    __device__ __forceinline__ void scores(const Raw<D, Q4>& r, f32x4* s) const
     {
-        f32x4 s[4];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -320,6 +333,14 @@ struct Attend {
             for (int j = 0; j < NJ; j++)
                 s[u] = score(r, u, j, s[u]);
         }
+    }
+
+    // One unit of 64 positions from `base` on, its scores in s: positions up
+    // to `limit` count for this lane's row, `full`: the whole unit for every
+    // row; bit u of `lost`: granule u has no page.
+    __device__ __forceinline__ void unit(State<D>& st, Raw<D, Q4>& r, f32x4* s, uint32_t lost, int base, int limit,
+                                         bool full) const
+    {
         if (!full) {
             // what a row does not see scores -inf
 #pragma unroll
@@ -329,12 +350,12 @@ struct Attend {
                     s[u][i] = base + GRANULE * u + 4 * g + i > limit ? -INFINITY : s[u][i];
             take_out_odd(r, s, base, limit);
         }
-        if (r.lost) {
+        if (lost) {
 #pragma unroll
             for (int u = 0; u < 4; u++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    s[u][i] = (r.lost >> u & 1) && base + GRANULE * u + 4 * g + i <= limit ? NAN : s[u][i];
+                    s[u][i] = (lost >> u & 1) && base + GRANULE * u + 4 * g + i <= limit ? NAN : s[u][i];
         }
         float top = st.top;
 #pragma unroll
@@ -534,19 +555,27 @@ paged_attention_kernel(const PagedAttentionArgs a)
             for (int k = 0; k < 4; k++)
                 pages[k] = __builtin_amdgcn_readlane(held, (u & 15) * 4 + k);
         };
+        // One set of registers: the next unit's keys are on their way while
+        // this one's weights and values are worked on, its values while the
+        // next scores are.
         int pages[4];
-        Raw<D, Q4> now, next;
+        Raw<D, Q4> raw;
         if (unit0 < stop) {
             pages_of(unit0, pages);
-            w.load(next, kvh, unit0 * UNIT, pages);
+            w.load_keys(raw, kvh, unit0 * UNIT, pages);
+            w.load_values(raw, kvh, unit0 * UNIT, pages);
         }
         for (int u = unit0; u < stop; u++) {
-            now = next;
+            f32x4 s[4];
+            w.scores(raw, s);
+            const uint32_t lost = raw.lost;
             if (u + 1 < stop) {
                 pages_of(u + 1, pages);
-                w.load(next, kvh, (u + 1) * UNIT, pages);
+                w.load_keys(raw, kvh, (u + 1) * UNIT, pages);
             }
-            w.unit(st, now, u * UNIT, limit, u * UNIT + UNIT - 1 <= least);
+            w.unit(st, raw, s, lost, u * UNIT, limit, u * UNIT + UNIT - 1 <= least);
+            if (u + 1 < stop)
+                w.load_values(raw, kvh, (u + 1) * UNIT, pages);
         }
         const float sum = rows_sum(st.sum);
         if (tile_start >= begin && tile_end <= end) {
