@@ -22,6 +22,7 @@
 // Caches are [context][kv_heads][head] (FP32 as in the reference, or fp16).
 // The attention launches are built for 128-value heads.
 #include "si_batch.hpp"
+#include "si_copies.hpp"
 #include "si_internal.hpp"
 #include "si_lanes.hpp"
 
@@ -946,23 +947,6 @@ constexpr int RING_COPIES = 3;                  // copy instructions per stage
 
 __device__ __forceinline__ uint32_t lds_u16(const uint8_t* p) { return *reinterpret_cast<const uint16_t*>(p); }
 __device__ __forceinline__ uint32_t lds_u32(const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
-
-// One asynchronous 16-byte copy per lane from global memory into LDS at
-// lds_base + 16 x lane.  The wave-uniform LDS base goes in M0 (the compiler
-// writes it there as the operand's register); the s_nop is the wait state an
-// LDS-bound load needs after an M0 write.
-__device__ __forceinline__ void copy16_to_lds(const void* src, uint32_t lds_base)
-{
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(lds_base) : "memory");
-}
-
-// Waits until at most N of this wave's memory loads (copies included) are in
-// flight.
-template <int N>
-__device__ __forceinline__ void wait_copies()
-{
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
 
 // Source of weight piece j (0..2) of block b in a row: Q4_K the header (j =
 // 0) and the quant bytes of the sub-block pair; Q4_0 the 16-byte aligned 32
