@@ -60,7 +60,7 @@ bool on(const void* p, uintptr_t align) { return (reinterpret_cast<uintptr_t>(p)
 // where its bytes land, still 128 whole bytes of a row to eight lanes.
 template <int MT, int NT, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : 2)
-gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles, bool wide)
+gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
 {
     constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN, WAVES = WM * WN;
     constexpr int COPIES = (BM + BN) / 8 / WAVES;         // of a wave and step, 8 rows each
@@ -119,60 +119,111 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles, bool wide)
             for (int e = 0; e < 16; e++)
                 acc[i][j][e] = 0;
 
-    const int64_t steps = (a.cols + 127) / 128;
-    copy(0, 0);
-    wait_copies<0>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    for (int64_t s = 0; s < steps; s++) {
-        const int buffer = int(s & 1);
-        if (s + 1 < steps)
-            copy((s + 1) * 128, buffer ^ 1);
-        const int8_t* wl = lds[buffer] + wm * (32 * MT) * 128;
-        const int8_t* xl = lds[buffer] + (BM + wn * (32 * NT)) * 128;
+    const int8_t* const wl = lds[0] + wm * (32 * MT) * 128;
+    const int8_t* const xl = lds[0] + (BM + wn * (32 * NT)) * 128;
+    i32x4 fw[2][MT], fx[2][NT];
+    auto read = [&](int buffer, int k, int set) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            i32x4 fw[MT], fx[NT];
+        for (int i = 0; i < MT; i++)
+            fw[set][i] = *reinterpret_cast<const i32x4*>(wl + buffer * ((BM + BN) * 128) + at[k] + i * 4096);
 #pragma unroll
-            for (int i = 0; i < MT; i++)
-                fw[i] = *reinterpret_cast<const i32x4*>(wl + at[k] + i * 4096);
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-                fx[j] = *reinterpret_cast<const i32x4*>(xl + at[k] + j * 4096);
-#pragma unroll
-            for (int i = 0; i < MT; i++)
-#pragma unroll
-                for (int j = 0; j < NT; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[i], fx[j], acc[i][j], 0, 0, 0);
-        }
-        wait_copies<0>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    }
-#pragma unroll
-    for (int j = 0; j < NT; j++) {
-        const int64_t t = t0 + (wn * NT + j) * 32 + r;
-        if (t >= a.m)
-            continue;
-        const float sx = a.x_scale[t];
+        for (int j = 0; j < NT; j++)
+            fx[set][j] = *reinterpret_cast<const i32x4*>(xl + buffer * ((BM + BN) * 128) + at[k] + j * 4096);
+    };
+    auto multiply = [&](int set) {
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int64_t o = o0 + (wm * MT + i) * 32 + 8 * e + 4 * h;
-                const i32x4 sum = {acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
-                store_y4(a, t, o, sx, sum, wide && o + 4 <= a.rows);
+            for (int j = 0; j < NT; j++)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[set][j], fw[set][i], acc[i][j], 0, 0, 0);
+    };
+    // One of a step's four quarters: the next fragments are read among the products.
+    auto interleave = [&] {
+#pragma unroll
+        for (int i = 0; i < MT + NT; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // one LDS read
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // one MFMA
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, MT * NT, 0);
+    };
+    const int64_t steps = (a.cols + 127) / 128;
+    copy(0, 0);
+    if (steps > 1)
+        copy(128, 1);
+    if (steps > 1)
+        wait_copies<COPIES>();
+    else
+        wait_copies<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(0, 0, 0);
+    for (int64_t s = 0; s < steps; s++) {
+        const int buffer = int(s & 1);
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            read(buffer, k + 1, (k + 1) & 1);
+            multiply(k & 1);
+            interleave();
+        }
+        // All of this step is in registers: when every wave says so, its
+        // buffer takes the step after the next one, and the next one's first
+        // fragments are read while the last products run.
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + 2 < steps)
+            copy((s + 2) * 128, buffer);
+        if (s + 1 < steps)
+            read(buffer ^ 1, 0, 0);
+        multiply(1);
+    }
+    // A lane holds one channel of each block, its registers the tokens: a
+    // store instruction writes whole 128-byte lines of two tokens (four
+    // channels a lane, 32 tokens an instruction, took three times as long).
+    float sw[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+        sw[i] = a.w_scale[min(o0 + (wm * MT + i) * 32 + r, a.rows - 1)];
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+        const int64_t tj = t0 + (wn * NT + j) * 32 + 4 * h;
+        float sx[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            sx[e] = a.x_scale[min(tj + 8 * (e >> 2) + (e & 3), a.m - 1)];
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            const int64_t o = o0 + (wm * MT + i) * 32 + r;
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                v[e] = float(acc[i][j][e]) * sx[e] * sw[i];
+            if (a.residual) {
+                float add[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    add[e] = a.residual[min(tj + 8 * (e >> 2) + (e & 3), a.m - 1) * a.rows + min(o, a.rows - 1)];
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    v[e] += add[e];
             }
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int64_t t = tj + 8 * (e >> 2) + (e & 3);
+                if (t < a.m && o < a.rows)
+                    a.y[t * a.rows + o] = v[e];
+            }
+        }
     }
 }
 
 template <int MT, int NT, int WM, int WN>
-hipError_t launch_tiles(const GemmI8Args& a, bool wide, hipStream_t s)
+hipError_t launch_tiles(const GemmI8Args& a, hipStream_t s)
 {
     constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN;
     const int64_t o_tiles = (a.rows + BM - 1) / BM, t_tiles = (a.m + BN - 1) / BN;
     gemm_i8_tile_kernel<MT, NT, WM, WN>
-        <<<unsigned(o_tiles * t_tiles), 64 * WM * WN, 0, s>>>(a, int(o_tiles), int(t_tiles), wide);
+        <<<unsigned(o_tiles * t_tiles), 64 * WM * WN, 0, s>>>(a, int(o_tiles), int(t_tiles));
     return hipGetLastError();
 }
 
@@ -265,8 +316,8 @@ hipError_t launch_gemm_i8(const GemmI8Args& a, hipStream_t s)
         return launch_few<2, 4, 16>(a, wide, s);
     const int64_t big = ((a.rows + 255) / 256) * ((a.m + 255) / 256);
     if (big >= 192)
-        return launch_tiles<4, 2, 2, 4>(a, wide, s);
-    return launch_tiles<2, 2, 2, 2>(a, wide, s);
+        return launch_tiles<4, 2, 2, 4>(a, s);
+    return launch_tiles<2, 2, 2, 2>(a, s);
 }
 
 }  // namespace si
