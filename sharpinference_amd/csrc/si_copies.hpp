@@ -15,6 +15,12 @@ __device__ __forceinline__ void copy16_to_lds(const void* src, uint32_t lds_base
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(lds_base) : "memory");
 }
 
+// The same from a wave-uniform base and a byte offset of each lane.
+__device__ __forceinline__ void copy16_to_lds(uint32_t offset, const void* base, uint32_t lds_base)
+{
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "{m0}"(lds_base) : "memory");
+}
+
 // Waits until at most N of this wave's memory loads (copies included) are in
 // flight.
 template <int N>

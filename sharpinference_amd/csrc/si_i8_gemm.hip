@@ -4,6 +4,7 @@
 #include "si_i8.hpp"
 
 #include "si_copies.hpp"
+#include <cstdlib>
 
 namespace si {
 
@@ -49,6 +50,90 @@ bool on(const void* p, uintptr_t align) { return (reinterpret_cast<uintptr_t>(p)
 
 // ---- many tokens: tiles in LDS ----------------------------------------------------------
 
+// Tile `id` of the launch.  Tiles go in the order of the dies that run them:
+// workgroup b runs on die b % 8, and each die takes a run of tiles of its
+// own, eight token tiles beside one another, so their operands meet in its L2.
+__device__ __forceinline__ void tile_of(int id, int o_tiles, int t_tiles, int bm, int bn, int64_t* o0, int64_t* t0)
+{
+    const int tiles = o_tiles * t_tiles, per = tiles / 8, more = tiles % 8, die = id % 8;
+    id = die * per + min(die, more) + id / 8;
+    constexpr int ROW = 8;
+    const int band = id / (ROW * o_tiles), in = id % (ROW * o_tiles), height = min(ROW, t_tiles - band * ROW);
+    *t0 = int64_t(band * ROW + in % height) * bn;
+    *o0 = int64_t(in / height) * bm;
+}
+
+// A pointer that is the same in all lanes, in scalar registers.
+__device__ __forceinline__ const int8_t* uniform(const int8_t* p)
+{
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<const int8_t*>(uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(v)))) |
+                                           uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(v >> 32)))) << 32);
+}
+
+// A 32 x 32 block of sums: this lane holds channel o, register e token t0 + 8
+// (e / 4) + e % 4, whose scales are sx[8 (e / 4) + e % 4] in LDS.  A store
+// instruction writes whole 128-byte lines of two tokens (four channels a
+// lane, 32 tokens an instruction, took three times as long).  WHOLE: every
+// token and channel of the tile is there.  Kept in one piece: spread over
+// the blocks before it, its values would need registers that the sums hold.
+template <bool WHOLE>
+__device__ __forceinline__ void store_block(const GemmI8Args& a, const i32x16& acc, const float* sx, int64_t t0, int64_t o,
+                                            float sw)
+{
+    const int64_t first = WHOLE ? t0 * a.rows + o : min(t0, a.m - 1) * a.rows + min(o, a.rows - 1);
+    float* const y = a.y + first;
+    const float* const add = a.residual + first;
+    const uint32_t rows = uint32_t(a.rows);
+    float v[16];
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+        v[e] = float(acc[e]) * sx[8 * (e >> 2) + (e & 3)] * sw;
+    if (a.residual) {
+        float r[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int t = 8 * (e >> 2) + (e & 3);
+            r[e] = WHOLE || (t0 + t < a.m && o < a.rows) ? add[t * rows] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            v[e] += r[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const int t = 8 * (e >> 2) + (e & 3);
+        if (WHOLE || (t0 + t < a.m && o < a.rows))
+            y[t * rows] = v[e];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The blocks of a wave, MT of channels from o0 on and NT of tokens from t0 on.
+template <int MT, int NT>
+__device__ __forceinline__ void store_blocks(const GemmI8Args& a, const i32x16 (&acc)[MT][NT], const float* sx, int64_t t0,
+                                             int64_t o0)
+{
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    float sw[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+        sw[i] = a.w_scale[min(o0 + i * 32 + r, a.rows - 1)];
+    if (o0 + 32 * MT <= a.rows && t0 + 32 * NT <= a.m) {
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+                store_block<true>(a, acc[i][j], sx + j * 32 + 4 * h, t0 + j * 32 + 4 * h, o0 + i * 32 + r, sw[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+                store_block<false>(a, acc[i][j], sx + j * 32 + 4 * h, t0 + j * 32 + 4 * h, o0 + i * 32 + r, sw[i]);
+    }
+}
+
 // A workgroup of WM x WN waves owns 32 MT WM channels x 32 NT WN tokens; a
 // wave MT x NT blocks of v_mfma_i32_32x32x32_i8.  Steps of 128 columns go
 // through two LDS buffers: the copies of the next step (16 bytes a lane,
@@ -58,28 +143,23 @@ bool on(const void* p, uintptr_t align) { return (reinterpret_cast<uintptr_t>(p)
 // 7), so the 32 rows that a fragment read takes hit every bank evenly.  The
 // copies write LDS in lane order; each lane asks for the piece that belongs
 // where its bytes land, still 128 whole bytes of a row to eight lanes.
-template <int MT, int NT, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : 2)
+template <int MT, int NT, int WM, int WN, int WK, int RING>
+__global__ void __launch_bounds__(64 * WM * WN * WK)
 gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
 {
-    constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN, WAVES = WM * WN;
+    constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN, WAVES = WM * WN * WK;
+    constexpr int QUARTERS = 4 / WK;                      // of a step's 128 columns, of a wave
     constexpr int COPIES = (BM + BN) / 8 / WAVES;         // of a wave and step, 8 rows each
     static_assert(COPIES * 8 * WAVES == BM + BN && BM % 8 == 0, "whole copies");
-    __shared__ __align__(16) int8_t lds[2][(BM + BN) * 128];
+    static_assert((RING & (RING - 1)) == 0 && (RING - 1) * COPIES < 64, "buffers by mask, vmcnt range");
+    __shared__ __align__(16) int8_t lds[RING][(BM + BN) * 128];
+    __shared__ __align__(16) float sx[BN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    // Tiles in the order of the dies that run them: workgroup b runs on die b
-    // % 8, and each die takes a run of tiles of its own, eight token tiles
-    // beside one another, so their operands meet in its L2.
-    const int tiles = o_tiles * t_tiles;
-    int id = blockIdx.x;
-    {
-        const int per = tiles / 8, more = tiles % 8, die = id % 8;
-        id = die * per + min(die, more) + id / 8;
-    }
-    constexpr int ROW = 8;
-    const int band = id / (ROW * o_tiles), in = id % (ROW * o_tiles), height = min(ROW, t_tiles - band * ROW);
-    const int64_t t0 = int64_t(band * ROW + in % height) * BN, o0 = int64_t(in / height) * BM;
+    int64_t o0, t0;
+    tile_of(blockIdx.x, o_tiles, t_tiles, BM, BN, &o0, &t0);
+    for (int i = threadIdx.x; i < BN; i += 64 * WAVES)
+        sx[i] = a.x_scale[min(t0 + i, a.m - 1)];
 
     const int8_t* src[COPIES];
 #pragma unroll
@@ -104,12 +184,12 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
         }
     };
 
-    const int wm = wave % WM, wn = wave / WM;
+    const int wm = wave % WM, wn = wave / WM % WN, wk = wave / (WM * WN);
     const int r = lane & 31, h = lane >> 5;
-    int at[4];
+    int at[QUARTERS];
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-        at[k] = r * 128 + (((2 * k + h) ^ ((r >> 1) & 7)) << 4);
+    for (int k = 0; k < QUARTERS; k++)
+        at[k] = r * 128 + (((2 * (wk * QUARTERS + k) + h) ^ ((r >> 1) & 7)) << 4);
     i32x16 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; i++)
@@ -147,84 +227,236 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
         __builtin_amdgcn_sched_group_barrier(0x008, MT * NT, 0);
     };
     const int64_t steps = (a.cols + 127) / 128;
-    copy(0, 0);
-    if (steps > 1)
-        copy(128, 1);
-    if (steps > 1)
-        wait_copies<COPIES>();
+    for (int i = 0; i < RING && i < steps; i++)
+        copy(i * 128, i);
+    if (steps >= RING)
+        wait_copies<(RING - 1) * COPIES>();
     else
         wait_copies<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     read(0, 0, 0);
     for (int64_t s = 0; s < steps; s++) {
-        const int buffer = int(s & 1);
+        const int buffer = int(s) & (RING - 1);
 #pragma unroll
-        for (int k = 0; k < 3; k++) {
+        for (int k = 0; k + 1 < QUARTERS; k++) {
             read(buffer, k + 1, (k + 1) & 1);
             multiply(k & 1);
             interleave();
         }
         // All of this step is in registers: when every wave says so, its
-        // buffer takes the step after the next one, and the next one's first
+        // buffer takes the step RING steps on, and the next one's first
         // fragments are read while the last products run.
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (s + RING <= steps)
+            wait_copies<(RING - 2) * COPIES>();
+        else
+            wait_copies<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s + 2 < steps)
-            copy((s + 2) * 128, buffer);
+        if (s + RING < steps)
+            copy((s + RING) * 128, buffer);
+        constexpr int LAST = (QUARTERS - 1) & 1;
         if (s + 1 < steps)
-            read(buffer ^ 1, 0, 0);
-        multiply(1);
-    }
-    // A lane holds one channel of each block, its registers the tokens: a
-    // store instruction writes whole 128-byte lines of two tokens (four
-    // channels a lane, 32 tokens an instruction, took three times as long).
-    float sw[MT];
+            read((buffer + 1) & (RING - 1), 0, LAST ^ 1);
+        multiply(LAST);
+        if constexpr (LAST == 0) {
 #pragma unroll
-    for (int i = 0; i < MT; i++)
-        sw[i] = a.w_scale[min(o0 + (wm * MT + i) * 32 + r, a.rows - 1)];
+            for (int i = 0; i < MT; i++)
+                fw[0][i] = fw[1][i];
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-        const int64_t tj = t0 + (wn * NT + j) * 32 + 4 * h;
-        float sx[16];
-#pragma unroll
-        for (int e = 0; e < 16; e++)
-            sx[e] = a.x_scale[min(tj + 8 * (e >> 2) + (e & 3), a.m - 1)];
-#pragma unroll
-        for (int i = 0; i < MT; i++) {
-            const int64_t o = o0 + (wm * MT + i) * 32 + r;
-            float v[16];
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                v[e] = float(acc[i][j][e]) * sx[e] * sw[i];
-            if (a.residual) {
-                float add[16];
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    add[e] = a.residual[min(tj + 8 * (e >> 2) + (e & 3), a.m - 1) * a.rows + min(o, a.rows - 1)];
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    v[e] += add[e];
-            }
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int64_t t = tj + 8 * (e >> 2) + (e & 3);
-                if (t < a.m && o < a.rows)
-                    a.y[t * a.rows + o] = v[e];
-            }
+            for (int j = 0; j < NT; j++)
+                fx[0][j] = fx[1][j];
         }
     }
+    if constexpr (WK > 1) {
+        // The waves that shared a block's columns add their sums in LDS.
+        static_assert(WK * BM * BN * 4 <= sizeof(lds), "the sums fit the ring");
+        int* const sums = reinterpret_cast<int*>(&lds[0][0]);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    sums[(wk * BN + (wn * NT + j) * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) * BM + (wm * MT + i) * 32 + r] =
+                        acc[i][j][e];
+        __syncthreads();
+        constexpr int PER = BM * BN / (64 * WAVES);       // outputs of a thread
+        const int o_in = threadIdx.x % BM;
+        const int64_t o = o0 + o_in;
+        float v[PER], add[PER];
+        const float sw = a.w_scale[min(o, a.rows - 1)];
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+            const int t_in = int(threadIdx.x) / BM + e * (64 * WAVES / BM);
+            const int64_t t = min(t0 + t_in, a.m - 1);
+            int sum = 0;
+#pragma unroll
+            for (int k = 0; k < WK; k++)
+                sum += sums[(k * BN + t_in) * BM + o_in];
+            v[e] = float(sum) * sx[t_in];
+            add[e] = a.residual ? a.residual[t * a.rows + min(o, a.rows - 1)] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+            const int64_t t = t0 + int(threadIdx.x) / BM + e * (64 * WAVES / BM);
+            if (t < a.m && o < a.rows) {
+                float y = v[e] * sw;
+                if (a.residual)
+                    y += add[e];
+                a.y[t * a.rows + o] = y;
+            }
+        }
+        return;
+    }
+    store_blocks<MT, NT>(a, acc, sx + wn * NT * 32, t0 + wn * NT * 32, o0 + wm * MT * 32);
 }
 
-template <int MT, int NT, int WM, int WN>
+template <int MT, int NT, int WM, int WN, int WK, int RING>
 hipError_t launch_tiles(const GemmI8Args& a, hipStream_t s)
 {
     constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN;
     const int64_t o_tiles = (a.rows + BM - 1) / BM, t_tiles = (a.m + BN - 1) / BN;
-    gemm_i8_tile_kernel<MT, NT, WM, WN>
-        <<<unsigned(o_tiles * t_tiles), 64 * WM * WN, 0, s>>>(a, int(o_tiles), int(t_tiles));
+    gemm_i8_tile_kernel<MT, NT, WM, WN, WK, RING>
+        <<<unsigned(o_tiles * t_tiles), 64 * WM * WN * WK, 0, s>>>(a, int(o_tiles), int(t_tiles));
     return hipGetLastError();
+}
+
+// The largest grids: a workgroup of four waves, one on each SIMD, owns 256
+// channels x 256 tokens, a wave 128 x 128 in 256 accumulators: each fragment
+// read from LDS meets four others, which halves the LDS traffic of an MFMA
+// against 128 x 64.  With one wave to a SIMD nothing hides behind another
+// wave, so the order of a step is written out: between two MFMAs one LDS
+// read of the next half step and (in its first half) one copy.
+//
+// Steps of 64 columns through four buffers: step s copies step s + 3 into
+// the buffer that the barrier of step s - 1 has freed.  LDS rows are 64
+// bytes, piece p of row r at p ^ ((r >> 2) & 3).
+constexpr int BIG = 256;                                  // channels and tokens of a tile
+
+__global__ void __launch_bounds__(256, 1)
+gemm_i8_big_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
+{
+    constexpr int STAGE = 2 * BIG * 64, COPIES = 8;
+    __shared__ __align__(16) int8_t lds[4][STAGE];
+    __shared__ __align__(16) float sx[BIG];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int64_t o0, t0;
+    tile_of(blockIdx.x, o_tiles, t_tiles, BIG, BIG, &o0, &t0);
+    sx[threadIdx.x] = a.x_scale[min(t0 + int(threadIdx.x), a.m - 1)];
+
+    // copies i < 4 of a wave fetch weights, i >= 4 tokens, 16 rows each
+    uint32_t off[COPIES];
+#pragma unroll
+    for (int i = 0; i < COPIES; i++) {
+        const int r = ((i & 3) * 4 + wave) * 16 + (lane >> 2), piece = (lane & 3) ^ ((r >> 2) & 3);
+        const int64_t row = i < 4 ? min(int64_t(r), a.rows - 1 - o0) : min(int64_t(r), a.m - 1 - t0);
+        off[i] = uint32_t(row * a.cols) + 16 * piece;
+    }
+    const uint32_t lds_base = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>(&lds[0][0])));
+    const int8_t* const w0 = uniform(a.w + o0 * a.cols);
+    const int8_t* const x0 = uniform(a.x + t0 * a.cols);
+    auto copy = [&](int i, int64_t k, bool whole) {
+        const uint32_t to = lds_base + uint32_t(int(k >> 6) & 3) * STAGE + uint32_t(((i >> 2) * 16 + (i & 3) * 4 + wave) * 1024);
+        const int8_t* const base = (i < 4 ? w0 : x0) + k;
+        if (whole) {
+            copy16_to_lds(off[i], base, to);
+        } else {
+            // (the piece's column: its place in the row's 64 bytes)
+            const int r = ((i & 3) * 4 + wave) * 16 + (lane >> 2);
+            const bool in = k + 16 * ((lane & 3) ^ ((r >> 2) & 3)) < a.cols;
+            copy16_to_lds(in ? base + off[i] : reinterpret_cast<const int8_t*>(no_columns), to);
+        }
+    };
+
+    const int wm = wave & 1, wn = wave >> 1;
+    const int r = lane & 31, h = lane >> 5;
+    const int8_t* at[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+        at[k] = lds[0] + r * 64 + (((2 * k + h) ^ ((r >> 2) & 3)) << 4);
+    i32x16 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                acc[i][j][e] = 0;
+    i32x4 f[2][8];                                        // fragments of a half step: 4 of weights, 4 of tokens
+    auto read = [&](int n, int64_t s, int k) {
+        const int row = n < 4 ? wm * 128 + n * 32 : BIG + wn * 128 + (n - 4) * 32;
+        f[k][n] = *reinterpret_cast<const i32x4*>(at[k] + (int(s) & 3) * STAGE + row * 64);
+    };
+    // MFMAs 2 g and 2 g + 1 of half step k
+    auto multiply = [&](int g, int k) {
+#pragma unroll
+        for (int n = 2 * g; n < 2 * g + 2; n++)
+            acc[n >> 2][n & 3] =
+                __builtin_amdgcn_mfma_i32_32x32x32_i8(f[k][4 + (n & 3)], f[k][n >> 2], acc[n >> 2][n & 3], 0, 0, 0);
+    };
+    const int64_t steps = (a.cols + 63) / 64, wholes = a.cols / 64;
+    for (int s = 0; s < 3 && s < steps; s++)
+#pragma unroll
+        for (int i = 0; i < COPIES; i++)
+            copy(i, int64_t(s) * 64, s < wholes);
+    if (steps >= 3)
+        wait_copies<2 * COPIES>();
+    else
+        wait_copies<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int n = 0; n < 8; n++)
+        read(n, 0, 0);
+    int64_t s = 0;
+    // the steps whose copy is of a whole step, then the last ones
+    for (; s + 3 < wholes; s++) {
+#pragma unroll
+        for (int g = 0; g < 8; g++) {
+            multiply(g, 0);
+            read(g, s, 1);
+            copy(g, (s + 3) * 64, true);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        wait_copies<2 * COPIES>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int g = 0; g < 8; g++) {
+            multiply(g, 1);
+            read(g, s + 1, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    for (; s < steps; s++) {
+        if (s + 3 < steps)
+#pragma unroll
+            for (int i = 0; i < COPIES; i++)
+                copy(i, (s + 3) * 64, false);
+#pragma unroll
+        for (int n = 0; n < 8; n++)
+            read(n, s, 1);
+#pragma unroll
+        for (int g = 0; g < 8; g++)
+            multiply(g, 0);
+        wait_copies<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + 1 < steps)
+#pragma unroll
+            for (int n = 0; n < 8; n++)
+                read(n, s + 1, 0);
+#pragma unroll
+        for (int g = 0; g < 8; g++)
+            multiply(g, 1);
+    }
+    store_blocks<4, 4>(a, acc, sx + wn * 128, t0 + wn * 128, o0 + wm * 128);
 }
 
 // ---- few tokens: weights straight into registers -------------------------------------------
@@ -308,6 +540,33 @@ hipError_t launch_few(const GemmI8Args& a, bool wide, hipStream_t s)
 hipError_t launch_gemm_i8(const GemmI8Args& a, hipStream_t s)
 {
     const bool wide = a.rows % 4 == 0 && on(a.y, 16) && on(a.w_scale, 16) && on(a.residual, 16);
+    if (getenv("GI8") && atoi(getenv("GI8")) == 40) {
+        const int64_t ot = (a.rows + BIG - 1) / BIG, tt = (a.m + BIG - 1) / BIG;
+        gemm_i8_big_kernel<<<unsigned(ot * tt), 256, 0, s>>>(a, int(ot), int(tt));
+        return hipGetLastError();
+    }
+    static const int force = getenv("GI8") ? atoi(getenv("GI8")) : -1;
+    switch (force) {
+    case 0: return launch_few<1, 1, 8>(a, wide, s);
+    case 1: return launch_few<2, 2, 16>(a, wide, s);
+    case 2: return launch_few<2, 4, 16>(a, wide, s);
+    case 3: return launch_few<4, 4, 8>(a, wide, s);
+    case 4: return launch_few<4, 4, 16>(a, wide, s);
+    case 5: return launch_few<2, 3, 16>(a, wide, s);
+    case 6: return launch_few<4, 2, 8>(a, wide, s);
+    case 7: return launch_few<2, 4, 8>(a, wide, s);
+    case 8: return launch_few<1, 1, 4>(a, wide, s);
+    case 9: return launch_few<1, 1, 16>(a, wide, s);
+    case 10: return launch_few<2, 1, 8>(a, wide, s);
+    case 11: return launch_few<2, 1, 16>(a, wide, s);
+    case 20: return launch_tiles<4, 2, 2, 4, 1, 2>(a, s);
+    case 21: return launch_tiles<2, 2, 2, 2, 1, 2>(a, s);
+    case 22: return launch_tiles<2, 2, 2, 2, 2, 4>(a, s);
+    case 23: return launch_tiles<1, 1, 2, 2, 4, 4>(a, s);
+    case 24: return launch_tiles<1, 1, 2, 2, 4, 8>(a, s);
+    case 25: return launch_tiles<1, 1, 2, 2, 2, 4>(a, s);
+    case 30: return launch_tiles<2, 1, 2, 4, 2, 4>(a, s);
+    }
     if (a.m <= 16)
         return launch_few<1, 1, 8>(a, wide, s);
     if (a.m <= 32)
@@ -316,8 +575,8 @@ hipError_t launch_gemm_i8(const GemmI8Args& a, hipStream_t s)
         return launch_few<2, 4, 16>(a, wide, s);
     const int64_t big = ((a.rows + 255) / 256) * ((a.m + 255) / 256);
     if (big >= 192)
-        return launch_tiles<4, 2, 2, 4>(a, s);
-    return launch_tiles<2, 2, 2, 2>(a, s);
+        return launch_tiles<4, 2, 2, 4, 1, 2>(a, s);
+    return launch_tiles<2, 2, 2, 2, 1, 2>(a, s);
 }
 
 }  // namespace si
