@@ -4,7 +4,6 @@
 #include "si_i8.hpp"
 
 #include "si_copies.hpp"
-#include <cstdlib>
 
 namespace si {
 
@@ -134,15 +133,27 @@ __device__ __forceinline__ void store_blocks(const GemmI8Args& a, const i32x16 (
     }
 }
 
-// A workgroup of WM x WN waves owns 32 MT WM channels x 32 NT WN tokens; a
-// wave MT x NT blocks of v_mfma_i32_32x32x32_i8.  Steps of 128 columns go
-// through two LDS buffers: the copies of the next step (16 bytes a lane,
-// straight into LDS) are in flight while this one is multiplied.
+// A workgroup owns 32 MT WM channels x 32 NT WN tokens: WM x WN waves with
+// MT x NT blocks of v_mfma_i32_32x32x32_i8 each, WK times over with the
+// columns of a step shared between them (their sums meet in LDS at the end).
+// Steps of 128 columns go through a ring of LDS buffers that asynchronous
+// copies fill, 16 bytes a lane straight into LDS, RING - 1 steps ahead; a
+// copy's address is a scalar base that moves and an offset that does not
+// (with 64-bit addresses per lane a step of the 64 x 64 tile took half as
+// long again).
 //
 // LDS rows are 128 bytes; piece p (16 bytes) of row r lies at p ^ ((r >> 1) &
-// 7), so the 32 rows that a fragment read takes hit every bank evenly.  The
-// copies write LDS in lane order; each lane asks for the piece that belongs
-// where its bytes land, still 128 whole bytes of a row to eight lanes.
+// 7), so the 32 rows that a fragment read takes hit every bank evenly
+// (no conflicts counted).  The copies write LDS in lane order; each lane asks
+// for the piece that belongs where its bytes land, still 128 whole bytes of a
+// row to eight lanes.
+//
+// 4093 x 8192 x 4096 takes 143 us (1.92 POP/s), 4096 x 16384 x 8192 519 us
+// (2.12); the vendor's plain product of 8-bit integers, int32 out and no
+// scales, reaches 2.18 and 2.10 on such shapes.  In a single workgroup a step
+// of the 256 x 256 tile takes 1.2 us, near the LDS traffic of its fragments;
+// with all CUs at work 1.6 us, and a form with half that traffic (128 x 128
+// a wave, one wave a SIMD, 0.9 us a step alone) gained nothing there.
 template <int MT, int NT, int WM, int WN, int WK, int RING>
 __global__ void __launch_bounds__(64 * WM * WN * WK)
 gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
@@ -161,26 +172,33 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
     for (int i = threadIdx.x; i < BN; i += 64 * WAVES)
         sx[i] = a.x_scale[min(t0 + i, a.m - 1)];
 
-    const int8_t* src[COPIES];
+    // copy i of this wave: eight rows of the weights or of the tokens
+    uint32_t off[COPIES];
+    const int8_t* base[COPIES];
 #pragma unroll
     for (int i = 0; i < COPIES; i++) {
-        const int r = (wave * COPIES + i) * 8 + (lane >> 3);
-        const int piece = (lane & 7) ^ ((r >> 1) & 7);
-        const int64_t row = r < BM ? min(o0 + r, a.rows - 1) : min(t0 + r - BM, a.m - 1);
-        src[i] = (r < BM ? a.w : a.x) + row * a.cols + 16 * piece;
+        const int r0 = (wave * COPIES + i) * 8, r = r0 + (lane >> 3), piece = (lane & 7) ^ ((r >> 1) & 7);
+        const bool of_w = r0 < BM;
+        const int64_t row = of_w ? min(int64_t(r), a.rows - 1 - o0) : min(int64_t(r - BM), a.m - 1 - t0);
+        off[i] = uint32_t(row * a.cols) + 16 * piece;
+        base[i] = uniform(of_w ? a.w + o0 * a.cols : a.x + t0 * a.cols);
     }
-    const uint32_t lds_base = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>(&lds[0][0])));
-    auto copy = [&](int64_t k, int buffer) {
-        const bool whole = k + 128 <= a.cols;
+    const uint32_t lds_base =
+        __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>(&lds[0][0])) + wave * COPIES * 1024);
+    const int cols = int(a.cols), steps = (cols + 127) / 128, wholes = cols / 128;
+    auto copy = [&](int s) {
+        const uint32_t to = lds_base + (s & (RING - 1)) * ((BM + BN) * 128);
+        if (s < wholes) {
 #pragma unroll
-        for (int i = 0; i < COPIES; i++) {
-            const int8_t* p = src[i] + k;
-            if (!whole) {
-                const int r = (wave * COPIES + i) * 8 + (lane >> 3);
-                if (k + 16 * ((lane & 7) ^ ((r >> 1) & 7)) >= a.cols)
-                    p = reinterpret_cast<const int8_t*>(no_columns);
+            for (int i = 0; i < COPIES; i++)
+                copy16_to_lds(off[i], base[i] + s * 128, to + i * 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < COPIES; i++) {
+                const int r = (wave * COPIES + i) * 8 + (lane >> 3), piece = (lane & 7) ^ ((r >> 1) & 7);
+                const bool in = s * 128 + 16 * piece < cols;
+                copy16_to_lds(in ? base[i] + s * 128 + off[i] : reinterpret_cast<const int8_t*>(no_columns), to + i * 1024);
             }
-            copy16_to_lds(p, lds_base + uint32_t(buffer * (BM + BN) * 128 + (wave * COPIES + i) * 1024));
         }
     };
 
@@ -226,9 +244,8 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
         }
         __builtin_amdgcn_sched_group_barrier(0x008, MT * NT, 0);
     };
-    const int64_t steps = (a.cols + 127) / 128;
     for (int i = 0; i < RING && i < steps; i++)
-        copy(i * 128, i);
+        copy(i);
     if (steps >= RING)
         wait_copies<(RING - 1) * COPIES>();
     else
@@ -236,8 +253,8 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     read(0, 0, 0);
-    for (int64_t s = 0; s < steps; s++) {
-        const int buffer = int(s) & (RING - 1);
+    for (int s = 0; s < steps; s++) {
+        const int buffer = s & (RING - 1);
 #pragma unroll
         for (int k = 0; k + 1 < QUARTERS; k++) {
             read(buffer, k + 1, (k + 1) & 1);
@@ -255,7 +272,7 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         if (s + RING < steps)
-            copy((s + RING) * 128, buffer);
+            copy(s + RING);
         constexpr int LAST = (QUARTERS - 1) & 1;
         if (s + 1 < steps)
             read((buffer + 1) & (RING - 1), 0, LAST ^ 1);
@@ -325,213 +342,57 @@ hipError_t launch_tiles(const GemmI8Args& a, hipStream_t s)
     return hipGetLastError();
 }
 
-// The largest grids: a workgroup of four waves, one on each SIMD, owns 256
-// channels x 256 tokens, a wave 128 x 128 in 256 accumulators: each fragment
-// read from LDS meets four others, which halves the LDS traffic of an MFMA
-// against 128 x 64.  With one wave to a SIMD nothing hides behind another
-// wave, so the order of a step is written out: between two MFMAs one LDS
-// read of the next half step and (in its first half) one copy.
-//
-// Steps of 64 columns through four buffers: step s copies step s + 3 into
-// the buffer that the barrier of step s - 1 has freed.  LDS rows are 64
-// bytes, piece p of row r at p ^ ((r >> 2) & 3).
-constexpr int BIG = 256;                                  // channels and tokens of a tile
-
-__global__ void __launch_bounds__(256, 1)
-gemm_i8_big_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
-{
-    constexpr int STAGE = 2 * BIG * 64, COPIES = 8;
-    __shared__ __align__(16) int8_t lds[4][STAGE];
-    __shared__ __align__(16) float sx[BIG];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int64_t o0, t0;
-    tile_of(blockIdx.x, o_tiles, t_tiles, BIG, BIG, &o0, &t0);
-    sx[threadIdx.x] = a.x_scale[min(t0 + int(threadIdx.x), a.m - 1)];
-
-    // copies i < 4 of a wave fetch weights, i >= 4 tokens, 16 rows each
-    uint32_t off[COPIES];
-#pragma unroll
-    for (int i = 0; i < COPIES; i++) {
-        const int r = ((i & 3) * 4 + wave) * 16 + (lane >> 2), piece = (lane & 3) ^ ((r >> 2) & 3);
-        const int64_t row = i < 4 ? min(int64_t(r), a.rows - 1 - o0) : min(int64_t(r), a.m - 1 - t0);
-        off[i] = uint32_t(row * a.cols) + 16 * piece;
-    }
-    const uint32_t lds_base = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>(&lds[0][0])));
-    const int8_t* const w0 = uniform(a.w + o0 * a.cols);
-    const int8_t* const x0 = uniform(a.x + t0 * a.cols);
-    auto copy = [&](int i, int64_t k, bool whole) {
-        const uint32_t to = lds_base + uint32_t(int(k >> 6) & 3) * STAGE + uint32_t(((i >> 2) * 16 + (i & 3) * 4 + wave) * 1024);
-        const int8_t* const base = (i < 4 ? w0 : x0) + k;
-        if (whole) {
-            copy16_to_lds(off[i], base, to);
-        } else {
-            // (the piece's column: its place in the row's 64 bytes)
-            const int r = ((i & 3) * 4 + wave) * 16 + (lane >> 2);
-            const bool in = k + 16 * ((lane & 3) ^ ((r >> 2) & 3)) < a.cols;
-            copy16_to_lds(in ? base + off[i] : reinterpret_cast<const int8_t*>(no_columns), to);
-        }
-    };
-
-    const int wm = wave & 1, wn = wave >> 1;
-    const int r = lane & 31, h = lane >> 5;
-    const int8_t* at[2];
-#pragma unroll
-    for (int k = 0; k < 2; k++)
-        at[k] = lds[0] + r * 64 + (((2 * k + h) ^ ((r >> 2) & 3)) << 4);
-    i32x16 acc[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                acc[i][j][e] = 0;
-    i32x4 f[2][8];                                        // fragments of a half step: 4 of weights, 4 of tokens
-    auto read = [&](int n, int64_t s, int k) {
-        const int row = n < 4 ? wm * 128 + n * 32 : BIG + wn * 128 + (n - 4) * 32;
-        f[k][n] = *reinterpret_cast<const i32x4*>(at[k] + (int(s) & 3) * STAGE + row * 64);
-    };
-    // MFMAs 2 g and 2 g + 1 of half step k
-    auto multiply = [&](int g, int k) {
-#pragma unroll
-        for (int n = 2 * g; n < 2 * g + 2; n++)
-            acc[n >> 2][n & 3] =
-                __builtin_amdgcn_mfma_i32_32x32x32_i8(f[k][4 + (n & 3)], f[k][n >> 2], acc[n >> 2][n & 3], 0, 0, 0);
-    };
-    const int64_t steps = (a.cols + 63) / 64, wholes = a.cols / 64;
-    for (int s = 0; s < 3 && s < steps; s++)
-#pragma unroll
-        for (int i = 0; i < COPIES; i++)
-            copy(i, int64_t(s) * 64, s < wholes);
-    if (steps >= 3)
-        wait_copies<2 * COPIES>();
-    else
-        wait_copies<0>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int n = 0; n < 8; n++)
-        read(n, 0, 0);
-    int64_t s = 0;
-    // the steps whose copy is of a whole step, then the last ones
-    for (; s + 3 < wholes; s++) {
-#pragma unroll
-        for (int g = 0; g < 8; g++) {
-            multiply(g, 0);
-            read(g, s, 1);
-            copy(g, (s + 3) * 64, true);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        wait_copies<2 * COPIES>();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-#pragma unroll
-        for (int g = 0; g < 8; g++) {
-            multiply(g, 1);
-            read(g, s + 1, 0);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-    for (; s < steps; s++) {
-        if (s + 3 < steps)
-#pragma unroll
-            for (int i = 0; i < COPIES; i++)
-                copy(i, (s + 3) * 64, false);
-#pragma unroll
-        for (int n = 0; n < 8; n++)
-            read(n, s, 1);
-#pragma unroll
-        for (int g = 0; g < 8; g++)
-            multiply(g, 0);
-        wait_copies<0>();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (s + 1 < steps)
-#pragma unroll
-            for (int n = 0; n < 8; n++)
-                read(n, s + 1, 0);
-#pragma unroll
-        for (int g = 0; g < 8; g++)
-            multiply(g, 1);
-    }
-    store_blocks<4, 4>(a, acc, sx + wn * 128, t0 + wn * 128, o0 + wm * 128);
-}
-
 // ---- few tokens: weights straight into registers -------------------------------------------
 
-// A workgroup owns 16 MT channels and all tokens (up to 16 NT); its waves
-// share the columns, 64 at a time in turn, and add their int32 sums in LDS (in
-// any order: integers).  A wave's fragments come straight from memory: the
-// weights are read once, the tokens from L2.
-template <int MT, int NT, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES)
+// Up to 16 tokens: a workgroup owns 16 channels, its waves share the columns,
+// 64 at a time in turn, and add their int32 sums in LDS (in any order:
+// integers).  Fragments of v_mfma_i32_16x16x64_i8 come straight from memory,
+// four steps of them in flight: the weights are read once, the tokens from
+// L2.  Bound by the weights' stream: 16384 x 4096 with four tokens runs at
+// 4.6 TB/s of weights, 8192 x 2048 with one (5.0 us) at 3.3 TB/s, most of the
+// rest being the launch.
+__global__ void __launch_bounds__(512)
 gemm_i8_few_kernel(const GemmI8Args a, bool wide)
 {
-    constexpr int DEPTH = NT <= 2 ? 4 : 2;               // steps of loads in flight
-    __shared__ __align__(16) int sums[16 * NT][16 * MT + 4];
+    constexpr int DEPTH = 4, WAVES = 8;
+    __shared__ __align__(16) int sums[16][16 + 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    const int64_t o0 = int64_t(blockIdx.x) * (16 * MT);
-    const int8_t* wp[MT];
-    const int8_t* xp[NT];
-#pragma unroll
-    for (int i = 0; i < MT; i++)
-        wp[i] = a.w + min(o0 + 16 * i + r, a.rows - 1) * a.cols + 16 * g;
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-        xp[j] = a.x + min(int64_t(16 * j + r), a.m - 1) * a.cols + 16 * g;
-    for (int i = threadIdx.x; i < 16 * NT * (16 * MT + 4); i += 64 * WAVES)
+    const int64_t o0 = int64_t(blockIdx.x) * 16;
+    const int8_t* const wp = a.w + min(o0 + r, a.rows - 1) * a.cols + 16 * g;
+    const int8_t* const xp = a.x + min(int64_t(r), a.m - 1) * a.cols + 16 * g;
+    for (int i = threadIdx.x; i < 16 * (16 + 4); i += 64 * WAVES)
         (&sums[0][0])[i] = 0;
-    i32x4 acc[MT][NT];
-#pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-            acc[i][j] = i32x4{0, 0, 0, 0};
-    const int64_t steps = (a.cols + 63) / 64;
-    for (int64_t s0 = wave; s0 < steps; s0 += WAVES * DEPTH) {
-        i32x4 fw[DEPTH][MT], fx[DEPTH][NT];
+    i32x4 acc = {0, 0, 0, 0};
+    const int cols = int(a.cols), steps = (cols + 63) / 64;
+    for (int s0 = wave; s0 < steps; s0 += WAVES * DEPTH) {
+        i32x4 fw[DEPTH], fx[DEPTH];
 #pragma unroll
         for (int d = 0; d < DEPTH; d++) {
-            const int64_t k = (s0 + d * WAVES) * 64;
-            const bool in = k + 16 * g < a.cols;
-#pragma unroll
-            for (int i = 0; i < MT; i++)
-                fw[d][i] = in ? *reinterpret_cast<const i32x4*>(wp[i] + k) : i32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-                fx[d][j] = in ? *reinterpret_cast<const i32x4*>(xp[j] + k) : i32x4{0, 0, 0, 0};
+            const int k = (s0 + d * WAVES) * 64;
+            const bool in = k + 16 * g < cols;
+            fw[d] = in ? *reinterpret_cast<const i32x4*>(wp + k) : i32x4{0, 0, 0, 0};
+            fx[d] = in ? *reinterpret_cast<const i32x4*>(xp + k) : i32x4{0, 0, 0, 0};
         }
 #pragma unroll
         for (int d = 0; d < DEPTH; d++)
-#pragma unroll
-            for (int i = 0; i < MT; i++)
-#pragma unroll
-                for (int j = 0; j < NT; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[d][i], fx[d][j], acc[i][j], 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[d], fx[d], acc, 0, 0, 0);
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                atomicAdd(&sums[16 * j + r][16 * i + 4 * g + e], acc[i][j][e]);
+    for (int e = 0; e < 4; e++)
+        atomicAdd(&sums[r][4 * g + e], acc[e]);
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * NT * (4 * MT); i += 64 * WAVES) {
-        const int64_t t = i / (4 * MT), o = o0 + 4 * (i % (4 * MT));
+    if (threadIdx.x < 64) {
+        const int64_t t = threadIdx.x / 4, o = o0 + 4 * (threadIdx.x % 4);
         if (t < a.m && o < a.rows)
-            store_y4(a, t, o, a.x_scale[t], *reinterpret_cast<const i32x4*>(&sums[t][4 * (i % (4 * MT))]),
+            store_y4(a, t, o, a.x_scale[t], *reinterpret_cast<const i32x4*>(&sums[t][4 * (threadIdx.x % 4)]),
                      wide && o + 4 <= a.rows);
     }
 }
 
-template <int MT, int NT, int WAVES>
 hipError_t launch_few(const GemmI8Args& a, bool wide, hipStream_t s)
 {
-    gemm_i8_few_kernel<MT, NT, WAVES><<<unsigned((a.rows + 16 * MT - 1) / (16 * MT)), 64 * WAVES, 0, s>>>(a, wide);
+    gemm_i8_few_kernel<<<unsigned((a.rows + 15) / 16), 512, 0, s>>>(a, wide);
     return hipGetLastError();
 }
 
@@ -540,43 +401,23 @@ hipError_t launch_few(const GemmI8Args& a, bool wide, hipStream_t s)
 hipError_t launch_gemm_i8(const GemmI8Args& a, hipStream_t s)
 {
     const bool wide = a.rows % 4 == 0 && on(a.y, 16) && on(a.w_scale, 16) && on(a.residual, 16);
-    if (getenv("GI8") && atoi(getenv("GI8")) == 40) {
-        const int64_t ot = (a.rows + BIG - 1) / BIG, tt = (a.m + BIG - 1) / BIG;
-        gemm_i8_big_kernel<<<unsigned(ot * tt), 256, 0, s>>>(a, int(ot), int(tt));
-        return hipGetLastError();
-    }
-    static const int force = getenv("GI8") ? atoi(getenv("GI8")) : -1;
-    switch (force) {
-    case 0: return launch_few<1, 1, 8>(a, wide, s);
-    case 1: return launch_few<2, 2, 16>(a, wide, s);
-    case 2: return launch_few<2, 4, 16>(a, wide, s);
-    case 3: return launch_few<4, 4, 8>(a, wide, s);
-    case 4: return launch_few<4, 4, 16>(a, wide, s);
-    case 5: return launch_few<2, 3, 16>(a, wide, s);
-    case 6: return launch_few<4, 2, 8>(a, wide, s);
-    case 7: return launch_few<2, 4, 8>(a, wide, s);
-    case 8: return launch_few<1, 1, 4>(a, wide, s);
-    case 9: return launch_few<1, 1, 16>(a, wide, s);
-    case 10: return launch_few<2, 1, 8>(a, wide, s);
-    case 11: return launch_few<2, 1, 16>(a, wide, s);
-    case 20: return launch_tiles<4, 2, 2, 4, 1, 2>(a, s);
-    case 21: return launch_tiles<2, 2, 2, 2, 1, 2>(a, s);
-    case 22: return launch_tiles<2, 2, 2, 2, 2, 4>(a, s);
-    case 23: return launch_tiles<1, 1, 2, 2, 4, 4>(a, s);
-    case 24: return launch_tiles<1, 1, 2, 2, 4, 8>(a, s);
-    case 25: return launch_tiles<1, 1, 2, 2, 2, 4>(a, s);
-    case 30: return launch_tiles<2, 1, 2, 4, 2, 4>(a, s);
-    }
     if (a.m <= 16)
-        return launch_few<1, 1, 8>(a, wide, s);
-    if (a.m <= 32)
-        return launch_few<2, 2, 16>(a, wide, s);
-    if (a.m <= 64)
-        return launch_few<2, 4, 16>(a, wide, s);
-    const int64_t big = ((a.rows + 255) / 256) * ((a.m + 255) / 256);
-    if (big >= 192)
+        return launch_few(a, wide, s);
+    // The largest tile that still gives the 256 CUs one each: large tiles
+    // read less per product, small ones fill the chip.  Both sides measured
+    // at 4096 columns (us, tokens x channels): 256 x 256 and 128 x 128 at 2048
+    // x 8192 74 / 80, at 2048 x 4096 (128 tiles) 50 / 41; 128 and 64 at 1024 x
+    // 4096 27 / 33, at 512 x 4096 (128 tiles) 25 / 18; 64 and 32 at 65 x 8192
+    // 11 / 20, at 64 x 4096 (64 tiles) 10.4 / 9.0 - but tiles of 32 in more
+    // than one round lose to 64 (64 x 16384, 1024 tiles: 16.6 / 24.8).
+    auto tiles = [&](int64_t n) { return ((a.rows + n - 1) / n) * ((a.m + n - 1) / n); };
+    if (tiles(256) >= 224)
         return launch_tiles<4, 2, 2, 4, 1, 2>(a, s);
-    return launch_tiles<2, 2, 2, 2, 1, 2>(a, s);
+    if (tiles(128) >= 192)
+        return launch_tiles<2, 2, 2, 2, 1, 2>(a, s);
+    if (tiles(32) > 320)
+        return launch_tiles<1, 1, 2, 2, 2, 4>(a, s);
+    return launch_tiles<1, 1, 1, 1, 4, 8>(a, s);
 }
 
 }  // namespace si
