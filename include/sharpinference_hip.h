@@ -491,7 +491,7 @@ int si_hip_dequant_i8(si_hip_context* ctx, const int8_t* codes, const float* sca
  * residual[t][o], which may be y), x [m, cols] and w [rows, cols] codes,
  * 16-byte aligned, cols a multiple of 16 in 16..65536: exact int32 sums on
  * the matrix cores, one FP32 rounding for each scale and for the residual.
- * Small grids use the context's split buffer, so a call allocates nothing.
+ * A call allocates nothing.
  * Replaces: transformer.batch-shared-matvec (GpuBatchTransformerInstructions.cs:
  * 224-279) for weights kept in 8 bits. */
 int si_hip_gemm_i8(si_hip_context* ctx, const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale,

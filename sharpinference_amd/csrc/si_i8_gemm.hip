@@ -136,11 +136,13 @@ __device__ __forceinline__ void store_blocks(const GemmI8Args& a, const i32x16 (
 // A workgroup owns 32 MT WM channels x 32 NT WN tokens: WM x WN waves with
 // MT x NT blocks of v_mfma_i32_32x32x32_i8 each, WK times over with the
 // columns of a step shared between them (their sums meet in LDS at the end).
-// Steps of 128 columns go through a ring of LDS buffers that asynchronous
+// Steps of 128 PER columns go through a ring of LDS buffers that asynchronous
 // copies fill, 16 bytes a lane straight into LDS, RING - 1 steps ahead; a
 // copy's address is a scalar base that moves and an offset that does not
 // (with 64-bit addresses per lane a step of the 64 x 64 tile took half as
-// long again).
+// long again).  PER 2 halves the barriers of the smallest tile, whose step
+// is otherwise a barrier, two LDS reads and one MFMA (64 x 4096 x 4096 9.0 ->
+// 6.9 us); the larger tiles gain nothing from it.
 //
 // LDS rows are 128 bytes; piece p (16 bytes) of row r lies at p ^ ((r >> 1) &
 // 7), so the 32 rows that a fragment read takes hit every bank evenly
@@ -154,16 +156,18 @@ __device__ __forceinline__ void store_blocks(const GemmI8Args& a, const i32x16 (
 // of the 256 x 256 tile takes 1.2 us, near the LDS traffic of its fragments;
 // with all CUs at work 1.6 us, and a form with half that traffic (128 x 128
 // a wave, one wave a SIMD, 0.9 us a step alone) gained nothing there.
-template <int MT, int NT, int WM, int WN, int WK, int RING>
+template <int MT, int NT, int WM, int WN, int WK, int RING, int PER>
 __global__ void __launch_bounds__(64 * WM * WN * WK)
 gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
 {
     constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN, WAVES = WM * WN * WK;
-    constexpr int QUARTERS = 4 / WK;                      // of a step's 128 columns, of a wave
-    constexpr int COPIES = (BM + BN) / 8 / WAVES;         // of a wave and step, 8 rows each
-    static_assert(COPIES * 8 * WAVES == BM + BN && BM % 8 == 0, "whole copies");
+    constexpr int QUARTERS = 4 / WK * PER;                // 32-column pieces of a step, of a wave
+    constexpr int ROUNDS = (BM + BN) / 8 / WAVES;         // copies of a wave for 128 columns, 8 rows each
+    constexpr int COPIES = ROUNDS * PER;
+    constexpr int SLAB = (BM + BN) * 128;
+    static_assert(ROUNDS * 8 * WAVES == BM + BN && BM % 8 == 0, "whole copies");
     static_assert((RING & (RING - 1)) == 0 && (RING - 1) * COPIES < 64, "buffers by mask, vmcnt range");
-    __shared__ __align__(16) int8_t lds[RING][(BM + BN) * 128];
+    __shared__ __align__(16) int8_t lds[RING][PER * SLAB];
     __shared__ __align__(16) float sx[BN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -173,31 +177,36 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
         sx[i] = a.x_scale[min(t0 + i, a.m - 1)];
 
     // copy i of this wave: eight rows of the weights or of the tokens
-    uint32_t off[COPIES];
-    const int8_t* base[COPIES];
+    uint32_t off[ROUNDS];
+    const int8_t* base[ROUNDS];
 #pragma unroll
-    for (int i = 0; i < COPIES; i++) {
-        const int r0 = (wave * COPIES + i) * 8, r = r0 + (lane >> 3), piece = (lane & 7) ^ ((r >> 1) & 7);
+    for (int i = 0; i < ROUNDS; i++) {
+        const int r0 = (wave * ROUNDS + i) * 8, r = r0 + (lane >> 3), piece = (lane & 7) ^ ((r >> 1) & 7);
         const bool of_w = r0 < BM;
         const int64_t row = of_w ? min(int64_t(r), a.rows - 1 - o0) : min(int64_t(r - BM), a.m - 1 - t0);
         off[i] = uint32_t(row * a.cols) + 16 * piece;
         base[i] = uniform(of_w ? a.w + o0 * a.cols : a.x + t0 * a.cols);
     }
     const uint32_t lds_base =
-        __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>(&lds[0][0])) + wave * COPIES * 1024);
-    const int cols = int(a.cols), steps = (cols + 127) / 128, wholes = cols / 128;
+        __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>(&lds[0][0])) + wave * ROUNDS * 1024);
+    const int cols = int(a.cols), steps = (cols + 128 * PER - 1) / (128 * PER), wholes = cols / (128 * PER);
     auto copy = [&](int s) {
-        const uint32_t to = lds_base + (s & (RING - 1)) * ((BM + BN) * 128);
-        if (s < wholes) {
+        const uint32_t to = lds_base + (s & (RING - 1)) * (PER * SLAB);
 #pragma unroll
-            for (int i = 0; i < COPIES; i++)
-                copy16_to_lds(off[i], base[i] + s * 128, to + i * 1024);
-        } else {
+        for (int p = 0; p < PER; p++) {
+            const int k = (s * PER + p) * 128;
+            if (s < wholes) {
 #pragma unroll
-            for (int i = 0; i < COPIES; i++) {
-                const int r = (wave * COPIES + i) * 8 + (lane >> 3), piece = (lane & 7) ^ ((r >> 1) & 7);
-                const bool in = s * 128 + 16 * piece < cols;
-                copy16_to_lds(in ? base[i] + s * 128 + off[i] : reinterpret_cast<const int8_t*>(no_columns), to + i * 1024);
+                for (int i = 0; i < ROUNDS; i++)
+                    copy16_to_lds(off[i], base[i] + k, to + p * SLAB + i * 1024);
+            } else {
+#pragma unroll
+                for (int i = 0; i < ROUNDS; i++) {
+                    const int r = (wave * ROUNDS + i) * 8 + (lane >> 3), piece = (lane & 7) ^ ((r >> 1) & 7);
+                    const bool in = k + 16 * piece < cols;
+                    copy16_to_lds(in ? base[i] + k + off[i] : reinterpret_cast<const int8_t*>(no_columns),
+                                  to + p * SLAB + i * 1024);
+                }
             }
         }
     };
@@ -207,7 +216,7 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
     int at[QUARTERS];
 #pragma unroll
     for (int k = 0; k < QUARTERS; k++)
-        at[k] = r * 128 + (((2 * (wk * QUARTERS + k) + h) ^ ((r >> 1) & 7)) << 4);
+        at[k] = r * 128 + (((2 * (wk * (4 / WK) + k % (4 / WK)) + h) ^ ((r >> 1) & 7)) << 4) + k / (4 / WK) * SLAB;
     i32x16 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; i++)
@@ -223,10 +232,10 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
     auto read = [&](int buffer, int k, int set) {
 #pragma unroll
         for (int i = 0; i < MT; i++)
-            fw[set][i] = *reinterpret_cast<const i32x4*>(wl + buffer * ((BM + BN) * 128) + at[k] + i * 4096);
+            fw[set][i] = *reinterpret_cast<const i32x4*>(wl + buffer * (PER * SLAB) + at[k] + i * 4096);
 #pragma unroll
         for (int j = 0; j < NT; j++)
-            fx[set][j] = *reinterpret_cast<const i32x4*>(xl + buffer * ((BM + BN) * 128) + at[k] + j * 4096);
+            fx[set][j] = *reinterpret_cast<const i32x4*>(xl + buffer * (PER * SLAB) + at[k] + j * 4096);
     };
     auto multiply = [&](int set) {
 #pragma unroll
@@ -301,13 +310,13 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
                     sums[(wk * BN + (wn * NT + j) * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) * BM + (wm * MT + i) * 32 + r] =
                         acc[i][j][e];
         __syncthreads();
-        constexpr int PER = BM * BN / (64 * WAVES);       // outputs of a thread
+        constexpr int OUTS = BM * BN / (64 * WAVES);      // of a thread
         const int o_in = threadIdx.x % BM;
         const int64_t o = o0 + o_in;
-        float v[PER], add[PER];
+        float v[OUTS], add[OUTS];
         const float sw = a.w_scale[min(o, a.rows - 1)];
 #pragma unroll
-        for (int e = 0; e < PER; e++) {
+        for (int e = 0; e < OUTS; e++) {
             const int t_in = int(threadIdx.x) / BM + e * (64 * WAVES / BM);
             const int64_t t = min(t0 + t_in, a.m - 1);
             int sum = 0;
@@ -318,7 +327,7 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
             add[e] = a.residual ? a.residual[t * a.rows + min(o, a.rows - 1)] : 0.0f;
         }
 #pragma unroll
-        for (int e = 0; e < PER; e++) {
+        for (int e = 0; e < OUTS; e++) {
             const int64_t t = t0 + int(threadIdx.x) / BM + e * (64 * WAVES / BM);
             if (t < a.m && o < a.rows) {
                 float y = v[e] * sw;
@@ -332,25 +341,24 @@ gemm_i8_tile_kernel(const GemmI8Args a, int o_tiles, int t_tiles)
     store_blocks<MT, NT>(a, acc, sx + wn * NT * 32, t0 + wn * NT * 32, o0 + wm * MT * 32);
 }
 
-template <int MT, int NT, int WM, int WN, int WK, int RING>
+template <int MT, int NT, int WM, int WN, int WK, int RING, int PER>
 hipError_t launch_tiles(const GemmI8Args& a, hipStream_t s)
 {
     constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN;
     const int64_t o_tiles = (a.rows + BM - 1) / BM, t_tiles = (a.m + BN - 1) / BN;
-    gemm_i8_tile_kernel<MT, NT, WM, WN, WK, RING>
+    gemm_i8_tile_kernel<MT, NT, WM, WN, WK, RING, PER>
         <<<unsigned(o_tiles * t_tiles), 64 * WM * WN * WK, 0, s>>>(a, int(o_tiles), int(t_tiles));
     return hipGetLastError();
 }
 
 // ---- few tokens: weights straight into registers -------------------------------------------
 
-// Up to 16 tokens: a workgroup owns 16 channels, its waves share the columns,
+// Up to 16 tokens on few channels: a workgroup owns 16 channels, its waves share the columns,
 // 64 at a time in turn, and add their int32 sums in LDS (in any order:
 // integers).  Fragments of v_mfma_i32_16x16x64_i8 come straight from memory,
 // four steps of them in flight: the weights are read once, the tokens from
-// L2.  Bound by the weights' stream: 16384 x 4096 with four tokens runs at
-// 4.6 TB/s of weights, 8192 x 2048 with one (5.0 us) at 3.3 TB/s, most of the
-// rest being the launch.
+// L2.  2048 channels of 8192 columns take 6.8 us with one token, 2.5 TB/s of
+// weights: 128 workgroups, and the launch.
 __global__ void __launch_bounds__(512)
 gemm_i8_few_kernel(const GemmI8Args a, bool wide)
 {
@@ -401,23 +409,26 @@ hipError_t launch_few(const GemmI8Args& a, bool wide, hipStream_t s)
 hipError_t launch_gemm_i8(const GemmI8Args& a, hipStream_t s)
 {
     const bool wide = a.rows % 4 == 0 && on(a.y, 16) && on(a.w_scale, 16) && on(a.residual, 16);
-    if (a.m <= 16)
+    auto tiles = [&](int64_t n) { return ((a.rows + n - 1) / n) * ((a.m + n - 1) / n); };
+    // Few tokens and too few channels for a tile of 32 on half the CUs: the
+    // form whose workgroups take 16 (one token, 2048 channels of 8192 columns
+    // 6.8 / 9.7 us; at 8192 channels of 4096 columns and 16 tokens 9.7 / 7.7).
+    if (a.m <= 16 && tiles(32) < 128)
         return launch_few(a, wide, s);
     // The largest tile that still gives the 256 CUs one each: large tiles
     // read less per product, small ones fill the chip.  Both sides measured
     // at 4096 columns (us, tokens x channels): 256 x 256 and 128 x 128 at 2048
     // x 8192 74 / 80, at 2048 x 4096 (128 tiles) 50 / 41; 128 and 64 at 1024 x
-    // 4096 27 / 33, at 512 x 4096 (128 tiles) 25 / 18; 64 and 32 at 65 x 8192
-    // 11 / 20, at 64 x 4096 (64 tiles) 10.4 / 9.0 - but tiles of 32 in more
-    // than one round lose to 64 (64 x 16384, 1024 tiles: 16.6 / 24.8).
-    auto tiles = [&](int64_t n) { return ((a.rows + n - 1) / n) * ((a.m + n - 1) / n); };
+    // 4096 27 / 33, at 512 x 4096 (128 tiles) 25 / 18; 64 and 32 at 64 x 16384
+    // 16.7 / 23, at 32 x 16384 (512 tiles of 32: two a CU) 15.0 / 14.1, at 64 x
+    // 4096 10.4 / 6.9.
     if (tiles(256) >= 224)
-        return launch_tiles<4, 2, 2, 4, 1, 2>(a, s);
+        return launch_tiles<4, 2, 2, 4, 1, 2, 1>(a, s);
     if (tiles(128) >= 192)
-        return launch_tiles<2, 2, 2, 2, 1, 2>(a, s);
-    if (tiles(32) > 320)
-        return launch_tiles<1, 1, 2, 2, 2, 4>(a, s);
-    return launch_tiles<1, 1, 1, 1, 4, 8>(a, s);
+        return launch_tiles<2, 2, 2, 2, 1, 2, 1>(a, s);
+    if (tiles(32) > 512)
+        return launch_tiles<1, 1, 2, 2, 2, 4, 1>(a, s);
+    return launch_tiles<1, 1, 1, 1, 4, 4, 2>(a, s);
 }
 
 }  // namespace si
