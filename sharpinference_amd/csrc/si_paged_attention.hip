@@ -24,6 +24,7 @@ using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
 using f32x4 = float __attribute__((ext_vector_type(4)));
 
 constexpr int TILE_ROWS = 16;            // packed query rows (position, head of the group) of a tile
+constexpr int FEW_ROWS = 64;             // sequences of more packed rows go to the prompt kernel
 constexpr int UNIT = 64;                 // positions of a step: four granules of 16
 constexpr int GRANULE = 16;              // positions that always lie in one page
 
@@ -32,10 +33,15 @@ __device__ __forceinline__ uint32_t as_u32(f16x2 v) { return __builtin_bit_cast(
 
 // 4-bit values at bits 0..3 and 16..19 of w as FP16 value - 8 (exact): the
 // nibble under the exponent of 1024 is 1024 + nibble.
+// (mask and exponent in registers: one v_and_or_b32, which takes no literals)
 __device__ __forceinline__ f16x2 nibbles(uint32_t w)
 {
     const f16x2 k = {_Float16(1032.0f), _Float16(1032.0f)};
-    return as_f16x2((w & 0x000F000Fu) | 0x64006400u) - k;
+    uint32_t mask = 0x000F000Fu, magic = 0x64006400u, v;
+    asm("" : "+s"(mask));
+    asm("" : "+v"(magic));
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(v) : "v"(w), "s"(mask), "v"(magic));
+    return as_f16x2(v) - k;
 }
 
 union Frag {
@@ -71,7 +77,7 @@ __device__ __forceinline__ Sequence take_sequence(const PagedBatch& b, int page_
     q.length = b.lengths[s];
     if (q.length < 0 || q.length > int64_t(b.max_pages) << page_shift || q.count > b.max_rows)
         q.length = -1;
-    q.tiles = (q.count * group + TILE_ROWS - 1) / TILE_ROWS;
+    q.tiles = q.count * group > FEW_ROWS ? 0 : (q.count * group + TILE_ROWS - 1) / TILE_ROWS;
     q.units = max(1, (q.length + UNIT - 1) / UNIT);
     return q;
 }
@@ -164,7 +170,10 @@ struct Shares {
 // accumulators [TILE_ROWS][D], largest scores and sums [TILE_ROWS] each.
 // Slot 2 w: of the tile that began before wave w's units, slot 2 w + 1: of
 // the one that goes on behind them.
+constexpr int COUNTER_FLOATS = 4;        // a workspace begins with the prompt kernel's counter
 constexpr int slot_floats(int d) { return TILE_ROWS * d + 2 * TILE_ROWS; }
+// where the prompt kernel's slots begin
+constexpr int64_t prompt_workspace(int d) { return COUNTER_FLOATS + int64_t(WAVES) * 2 * slot_floats(d); }
 
 // Running state of a tile: the lane's packed row is lane & 15.
 template <int D>
@@ -496,6 +505,9 @@ paged_attention_kernel(const PagedAttentionArgs a)
     constexpr int NV = D / 16;
     const int kv = a.cache.kv_heads, group = a.heads / kv;
     const int64_t wave = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    // (the prompt kernel behind this one draws its items from here)
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        *reinterpret_cast<int32_t*>(a.workspace) = 0;
     const Line line{a.batch, a.cache.page_shift, group, kv};
     const int64_t total = line.total();
     if (total == 0)
@@ -590,7 +602,7 @@ paged_attention_kernel(const PagedAttentionArgs a)
                                   st.acc[n + 3][r] * inv);
             }
         } else if (live) {
-            float* slot = a.workspace + (2 * wave + (tile_start >= begin)) * slot_floats(D);
+            float* slot = a.workspace + COUNTER_FLOATS + (2 * wave + (tile_start >= begin)) * slot_floats(D);
             float* at = slot + w.c * D + NV * 4 * w.g;
 #pragma unroll
             for (int r = 0; r < 4; r++)
@@ -636,7 +648,7 @@ paged_merge_kernel(const PagedAttentionArgs a)
     bool seen_nan = false;
     if (live) {
         for (int64_t p = w0 + wave; p <= w1; p += 4) {
-            const float* slot = a.workspace + (2 * p + (p == w0)) * slot_floats(D);
+            const float* slot = a.workspace + COUNTER_FLOATS + (2 * p + (p == w0)) * slot_floats(D);
             const float m = slot[TILE_ROWS * D + r], l = slot[TILE_ROWS * D + TILE_ROWS + r];
             const f32x4 v = *reinterpret_cast<const f32x4*>(slot + r * D + col);
             const float t = fmaxf(top, m), at = fmaxf(t, -3.4028235e38f);
@@ -670,33 +682,587 @@ paged_merge_kernel(const PagedAttentionArgs a)
               acc[2] * inv, acc[3] * inv);
 }
 
+// ---- many rows of a sequence ------------------------------------------------------------
+
+// A workgroup of four waves takes 128 packed rows of one sequence and KV
+// head, 32 a wave, through units of 64 positions.  The unit's keys and values
+// go through LDS as FP16, dequantized once for the four waves (two waves
+// convert keys, two values), two buffers: the next unit's bytes are loaded
+// while this one is multiplied.  Scores stay transposed here too, with
+// v_mfma_f32_32x32x16_f16.
+constexpr int PROMPT_ROWS = 128;
+constexpr int PROMPT_WORKERS = 512;      // two workgroups a CU
+constexpr int PROMPT_SLOTS = 2 * PROMPT_WORKERS;   // see Prompt
+constexpr int PROMPT_MIN = 8;            // units that a workgroup takes at least
+
+using f32x16 = float __attribute__((ext_vector_type(16)));
+
+constexpr int prompt_slot_floats(int d) { return PROMPT_ROWS * d + 2 * PROMPT_ROWS; }
+
+// The items of a launch: sequence after sequence, its tiles from the last
+// (which see most) to the first, a tile's `parts` runs of units, the KV
+// heads.  A sequence is split where its units are at least 1.5 times what
+// each worker would take of an equal division; then parts is at most 4/3 of
+// units / share, so no more than 4/3 PROMPT_WORKERS items have slots.
+struct PromptSequence {
+    int index, first, count, length, tiles, units, parts;
+};
+struct PromptItem {
+    PromptSequence q;
+    int tile, part, kvh;
+    int64_t slot;              // of the tile's first part; parts > 1
+};
+
+struct Prompt {
+    const PagedBatch& b;
+    int page_shift, group, kv;
+    int64_t share;             // units of a worker
+
+    __device__ __forceinline__ PromptSequence take(int s) const
+    {
+        PromptSequence q{s, 0, 0, 0, 0, 0, 1};
+        if (s >= b.sequences)
+            return q;
+        sequence_rows(b, s, &q.first, &q.count);
+        q.length = b.lengths[s];
+        if (q.length < 0 || q.length > int64_t(b.max_pages) << page_shift || q.count > b.max_rows)
+            q.length = -1;
+        q.tiles = q.count * group > FEW_ROWS ? (q.count * group + PROMPT_ROWS - 1) / PROMPT_ROWS : 0;
+        q.units = max(1, (q.length + UNIT - 1) / UNIT);
+        if (share > 0)
+            q.parts = int((q.units + share - 1) / share);
+        return q;
+    }
+    __device__ __forceinline__ void set_share()
+    {
+        share = 0;
+        int64_t sum = 0;
+        for (int base = 0; base < b.sequences; base += 64) {
+            const PromptSequence q = take(base + int(threadIdx.x & 63));
+            sum += int64_t(kv) * q.tiles * q.units;
+        }
+        sum = __shfl(wave_scan(sum), 63);
+        share = max(int64_t(PROMPT_MIN), (sum + PROMPT_WORKERS - 1) / PROMPT_WORKERS);
+    }
+    // Item x, or (TILES) the first part of tile x of the launch.
+    template <bool TILES>
+    __device__ __forceinline__ bool find(int64_t x, PromptItem* out) const
+    {
+        int64_t before = 0, slots = 0;
+        for (int base = 0; base < b.sequences; base += 64) {
+            const PromptSequence mine = take(base + int(threadIdx.x & 63));
+            const int64_t own = int64_t(kv) * mine.tiles * (TILES ? 1 : mine.parts);
+            const int64_t own_slots = mine.parts > 1 ? int64_t(kv) * mine.tiles * mine.parts : 0;
+            const int64_t upto = before + wave_scan(own), slots_upto = slots + wave_scan(own_slots);
+            const uint64_t past = __ballot(upto > x);
+            if (past) {
+                const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+                out->q = {__shfl(mine.index, at), __shfl(mine.first, at), __shfl(mine.count, at), __shfl(mine.length, at),
+                          __shfl(mine.tiles, at), __shfl(mine.units, at), __shfl(mine.parts, at)};
+                const int64_t in = x - __shfl(upto - own, at);
+                const int parts = TILES ? 1 : out->q.parts;
+                out->kvh = int(in % kv);
+                out->part = int(in / kv % parts);
+                out->tile = out->q.tiles - 1 - int(in / kv / parts);
+                // a tile's parts and KV heads lie together in the slots
+                out->slot = __shfl(slots_upto - own_slots, at) +
+                            (int64_t(out->q.tiles - 1 - out->tile) * kv + out->kvh) * out->q.parts;
+                return true;
+            }
+            before = __shfl(upto, 63);
+            slots = __shfl(slots_upto, 63);
+        }
+        return false;
+    }
+};
+
+template <int D>
+__device__ __forceinline__ int key_at(int row, int piece)      // bytes of 16-byte piece `piece` of a key
+{
+    return row * (2 * D) + ((piece ^ (D == 128 ? row & 15 : (row >> 1) & 7)) << 4);
+}
+__device__ __forceinline__ int value_at(int col, int piece)    // of eight positions of a column
+{
+    return col * 128 + ((piece ^ (((col >> 1) ^ (col >> 4)) & 7)) << 4);
+}
+
+// What a thread loads of a unit.  Threads 0..127 take keys: 16-byte pieces of
+// rows; threads 128..255 values: NV columns of eight positions, those that
+// piece q = (thread - 128) / 16 of a column holds: 16 (q / 2) + 4 (q % 2) + {0..3, 8..11}.
+template <int D, bool Q4, bool FINE>
+struct PromptLoad {
+    static constexpr int NV = D / 16;
+    static constexpr int KEYS = Q4 ? D / 64 : D / 16;          // 16-byte loads of a key thread
+    static constexpr int PIECES = Q4 ? D / 32 : D / 8;         // of a row
+    uint4 k[KEYS];
+    uint32_t kd[KEYS];
+    uint32_t v[8][Q4 ? 1 : NV / 2];
+    uint32_t vd[4];
+
+    // The thread among its 128, as a new value each time: what follows from it
+    // is worked out where it is needed and holds no register through the products.
+    static __device__ __forceinline__ int thread()
+    {
+        int t = threadIdx.x & 127;
+        asm volatile("" : "+v"(t));
+        return t;
+    }
+    // the row of a key thread's load i, and its piece of it
+    static __device__ __forceinline__ int row(int t, int i) { return t / PIECES + i * (128 / PIECES); }
+    static __device__ __forceinline__ int piece(int t) { return t % PIECES; }
+
+    // pages: the unit's four pages (a page that is not there: page 0)
+    __device__ __forceinline__ void load(const PagedAttentionArgs& a, int kvh, int base, const int* pages, int64_t head_bytes)
+    {
+        const int ps = a.cache.page_size, t = thread();
+        // (selects: an array indexed by a lane's value would live in memory)
+        auto page_at = [&](int u) {
+            const int page = u < 2 ? (u ? pages[1] : pages[0]) : (u == 2 ? pages[2] : pages[3]);
+            return (int64_t(max(page, 0)) * a.cache.kv_heads + kvh) * head_bytes;
+        };
+        if (threadIdx.x < 128) {
+#pragma unroll
+            for (int i = 0; i < KEYS; i++) {
+                const int r = row(t, i), slot = (base + r) & (ps - 1);
+                const char* const p = a.cache.keys + page_at(r >> 4);
+                k[i] = *reinterpret_cast<const uint4*>(p + slot * (Q4 ? D / 2 : 2 * D) + 16 * piece(t));
+                if constexpr (Q4)
+                    kd[i] = reinterpret_cast<const uint16_t*>(p + ps * (D / 2))[piece(t) * ps + slot];
+            }
+        } else {
+            const int c = t & 15, q = t >> 4;
+            const int r = 16 * (q >> 1) + 4 * (q & 1), slot = (base + r) & (ps - 1);
+            const char* const p = a.cache.values + page_at(q >> 1);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int s = slot + (i & 3) + 8 * (i >> 2);
+                if constexpr (Q4) {
+                    const char* const at = p + s * (D / 2) + NV / 2 * c;
+                    v[i][0] = D == 128 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at);
+                } else if constexpr (D == 128) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(p + s * (2 * D) + 2 * NV * c);
+                    v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(p + s * (2 * D) + 2 * NV * c);
+                    v[i][0] = x.x, v[i][1] = x.y;
+                }
+            }
+            if constexpr (Q4) {
+                const uint16_t* const d = reinterpret_cast<const uint16_t*>(p + ps * (D / 2)) + (D == 128 ? c >> 2 : c >> 3) * ps + slot;
+                const uint2 x = *reinterpret_cast<const uint2*>(d), y = *reinterpret_cast<const uint2*>(d + 8);
+                vd[0] = x.x, vd[1] = x.y, vd[2] = y.x, vd[3] = y.y;
+            }
+        }
+    }
+
+    // Into LDS as FP16 (FINE 4-bit: and what is left of the products beside
+    // it).  `partial`: some row does not see all of the unit; values that are
+    // not finite are then taken out and their positions marked in `odd`.
+    __device__ __forceinline__ void store(char* keys, char* values, int lo, bool partial, uint32_t* odd)
+    {
+        const int t = thread();
+        if (threadIdx.x < 128) {
+#pragma unroll
+            for (int i = 0; i < KEYS; i++) {
+                const int r = row(t, i);
+                if constexpr (Q4) {
+                    const f16x2 d = as_f16x2(kd[i] | kd[i] << 16);
+                    const uint32_t w[4] = {k[i].x, k[i].y, k[i].z, k[i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        uint4 x, y;
+                        uint32_t* const xs[4] = {&x.x, &x.y, &x.z, &x.w};
+                        uint32_t* const ys[4] = {&y.x, &y.y, &y.z, &y.w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const f16x2 n = nibbles(w[j] >> (4 * e)), p = n * d;
+                            *xs[e] = as_u32(p);
+                            if constexpr (FINE)
+                                *ys[e] = as_u32(__builtin_elementwise_fma(n, d, -p));
+                        }
+                        *reinterpret_cast<uint4*>(keys + key_at<D>(r, 4 * piece(t) + j)) = x;
+                        if constexpr (FINE)
+                            *reinterpret_cast<uint4*>(keys + lo + key_at<D>(r, 4 * piece(t) + j)) = y;
+                    }
+                } else {
+                    *reinterpret_cast<uint4*>(keys + key_at<D>(r, piece(t))) = k[i];
+                }
+            }
+        } else {
+            const int c = t & 15, q = t >> 4;
+            if (partial) {
+                uint32_t mask = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    bool bad = false;
+                    if constexpr (Q4) {
+                        const uint32_t e = 0x7000u << (16 * (i & 1));      // (8192 and up, as above)
+                        bad = (vd[i >> 1] & e) == e;
+                        if (bad)
+                            vd[i >> 1] &= ~(0xFFFFu << (16 * (i & 1)));
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < NV / 2; n++)
+                            if ((v[i][n] & 0x7C00u) == 0x7C00u || (v[i][n] & 0x7C000000u) == 0x7C000000u) {
+                                bad = true;
+                                v[i][n] = 0;
+                            }
+                    }
+                    const int pos = 16 * (q >> 1) + 4 * (q & 1) + (i & 3) + 8 * (i >> 2);
+                    mask |= bad ? 1u << (pos & 31) : 0u;
+                }
+                if (mask)
+                    atomicOr(&odd[q >> 2], mask);
+            }
+            uint32_t lo16[4], hi16[4];
+            if constexpr (Q4) {
+#pragma unroll
+                for (int p = 0; p < 4; p++) {
+                    lo16[p] = __builtin_amdgcn_perm(v[2 * p + 1][0], v[2 * p][0], 0x05040100u);
+                    hi16[p] = __builtin_amdgcn_perm(v[2 * p + 1][0], v[2 * p][0], 0x07060302u);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NV; n++) {
+                uint4 x, y;
+                uint32_t* const xs[4] = {&x.x, &x.y, &x.z, &x.w};
+                uint32_t* const ys[4] = {&y.x, &y.y, &y.z, &y.w};
+#pragma unroll
+                for (int p = 0; p < 4; p++) {
+                    if constexpr (Q4) {
+                        const f16x2 d = as_f16x2(vd[p]);
+                        const f16x2 m = nibbles((n < 4 ? lo16[p] : hi16[p]) >> (4 * (n & 3))), z = m * d;
+                        *xs[p] = as_u32(z);
+                        if constexpr (FINE)
+                            *ys[p] = as_u32(__builtin_elementwise_fma(m, d, -z));
+                    } else {
+                        *xs[p] = __builtin_amdgcn_perm(v[2 * p + 1][n >> 1], v[2 * p][n >> 1], n & 1 ? 0x07060302u : 0x05040100u);
+                    }
+                }
+                *reinterpret_cast<uint4*>(values + value_at(NV * c + n, q)) = x;
+                if constexpr (FINE && Q4)
+                    *reinterpret_cast<uint4*>(values + lo + value_at(NV * c + n, q)) = y;
+            }
+        }
+    }
+};
+
+template <int D, bool Q4, bool FINE>
+__global__ void __launch_bounds__(256, FINE && Q4 && D == 128 ? 1 : 2)
+paged_prompt_kernel(const PagedAttentionArgs a)
+{
+    constexpr int NK = D / 16, NC = D / 32;
+    constexpr int PLANE = UNIT * D * 2;                   // bytes of a unit's keys, and of its values
+    constexpr int PLANES = FINE && Q4 ? 4 : 2;
+    __shared__ __align__(16) char lds[2][PLANES * PLANE];
+    __shared__ uint32_t odd[3][2];
+    const int kv = a.cache.kv_heads, group = a.heads / kv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
+    const int64_t head_bytes = paged_head_bytes(Q4, a.cache.page_size, D);
+    Prompt prompt{a.batch, a.cache.page_shift, group, kv, 0};
+    prompt.set_share();
+    PromptItem it;
+    __shared__ int drawn;
+    int32_t* const counter = reinterpret_cast<int32_t*>(a.workspace);
+    for (;;) {
+        // whoever is done takes the next item: long ones first, so the last end together
+        if (threadIdx.x == 0)
+            drawn = atomicAdd(counter, 1);
+        __syncthreads();
+        if (!prompt.find<false>(drawn, &it))
+            return;
+        const PromptSequence& q = it.q;
+        const bool wrong = q.length < 0;
+        const int row0 = it.tile * PROMPT_ROWS;
+        const int packed = row0 + 32 * wave + r, i = packed / group;
+        const bool live = i < q.count;
+        const int64_t row = int64_t(q.first) + i;
+        const int head = it.kvh * group + packed % group;
+        const int limit = live && !wrong ? q.length - q.count + i : -1;
+        const int last_row = min(q.count - 1, (row0 + PROMPT_ROWS - 1) / group);
+        const int most = __builtin_amdgcn_readfirstlane(wrong ? -1 : q.length - q.count + last_row);
+        const int least = __builtin_amdgcn_readfirstlane(q.length - q.count + row0 / group);
+        const int units = (most + UNIT) / UNIT;           // of this tile, 0 where no row sees anything
+        const int unit0 = __builtin_amdgcn_readfirstlane(int(int64_t(units) * it.part / q.parts));
+        const int unit1 = __builtin_amdgcn_readfirstlane(int(int64_t(units) * (it.part + 1) / q.parts));
+        const int32_t* const table = a.batch.table + int64_t(q.index) * a.batch.max_pages;
+
+        // queries of this lane's row: piece 2 k + h of its values for product k
+        f16x8 qf[NK], ql[FINE ? NK : 1];
+        {
+            const float f = 1.44269504088896340736f / sqrtf(float(D));
+            const float* const p = live ? a.query + (row * a.heads + head) * D : nullptr;
+#pragma unroll
+            for (int k = 0; k < NK; k++) {
+                float4 x = make_float4(0, 0, 0, 0), y = x;
+                if (p) {
+                    x = *reinterpret_cast<const float4*>(p + 16 * k + 8 * h);
+                    y = *reinterpret_cast<const float4*>(p + 16 * k + 8 * h + 4);
+                }
+                const float v[8] = {x.x * f, x.y * f, x.z * f, x.w * f, y.x * f, y.y * f, y.z * f, y.w * f};
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float t = Q4 ? v[(e >> 1) + 4 * (e & 1)] : v[e];
+                    qf[k][e] = _Float16(t);
+                    if constexpr (FINE)
+                        ql[k][e] = _Float16(t - float(qf[k][e]));
+                }
+            }
+        }
+        f32x16 acc[NC];
+#pragma unroll
+        for (int n = 0; n < NC; n++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                acc[n][e] = 0.0f;
+        float ref = -INFINITY, sum = 0.0f;
+        // Places of the lane's fragments: rows 32 apart share their swizzle,
+        // columns 32 apart differ in it by 2 n, so eight and four offsets do.
+        int key_of[NK], value_of[4];
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+            key_of[k] = key_at<D>(r, 2 * k + h);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            value_of[k] = PLANE + value_at(r, 2 * k + h);
+
+        // pages of the 64 granules around a unit, one a lane of every wave
+        int held = 0, held_at = -1;
+        auto pages_of = [&](int u, int* pages) {
+            if (u >> 4 != held_at) {
+                held_at = u >> 4;
+                const int pos = (held_at * 64 + lane) * GRANULE;
+                held = pos <= most ? table[pos >> a.cache.page_shift] : 0;
+                if (held >= a.cache.pages)
+                    held = -1;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                pages[k] = __builtin_amdgcn_readlane(held, (u & 15) * 4 + k);
+        };
+        auto lost_of = [](const int* pages) {
+            return (pages[0] < 0 ? 1u : 0u) | (pages[1] < 0 ? 2u : 0u) | (pages[2] < 0 ? 4u : 0u) | (pages[3] < 0 ? 8u : 0u);
+        };
+        auto partial = [&](int u) { return u * UNIT + UNIT - 1 > least; };
+        PromptLoad<D, Q4, FINE> raw;
+        int pages[4];
+        uint32_t lost = 0, lost_next = 0;
+        __syncthreads();                                  // the item before is done with LDS
+        if (threadIdx.x < 6)
+            (&odd[0][0])[threadIdx.x] = 0;
+        __syncthreads();
+        if (unit0 < unit1) {
+            pages_of(unit0, pages);
+            lost = lost_of(pages);
+            raw.load(a, it.kvh, unit0 * UNIT, pages, head_bytes);
+            raw.store(lds[unit0 & 1], lds[unit0 & 1] + PLANE, 2 * PLANE, partial(unit0), odd[unit0 % 3]);
+            if (unit0 + 1 < unit1) {
+                pages_of(unit0 + 1, pages);
+                lost_next = lost_of(pages);
+                raw.load(a, it.kvh, (unit0 + 1) * UNIT, pages, head_bytes);
+            }
+        }
+        __syncthreads();
+        for (int u = unit0; u < unit1; u++) {
+            const char* const plane = lds[u & 1];
+            const int base = u * UNIT;
+            // (read for unit u - 1, next written for unit u + 2)
+            if (threadIdx.x < 2)
+                odd[(u + 2) % 3][threadIdx.x] = 0;
+            f32x16 s[2];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    s[b][e] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < NK; k++) {
+                    const f16x8 kf = *reinterpret_cast<const f16x8*>(plane + key_of[k] + 32 * b * 2 * D);
+                    if constexpr (FINE && Q4) {
+                        const f16x8 kl = *reinterpret_cast<const f16x8*>(plane + key_of[k] + 2 * PLANE + 32 * b * 2 * D);
+                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qf[k], s[b], 0, 0, 0);
+                    }
+                    if constexpr (FINE)
+                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], s[b], 0, 0, 0);
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[k], s[b], 0, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // element e of block b: position base + 32 b + 8 (e / 4) + 4 h + e % 4
+            if (partial(u) || lost) {
+                const uint32_t odd0 = odd[u % 3][0], odd1 = odd[u % 3][1];
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int in = 8 * (e >> 2) + 4 * h + (e & 3);
+                        const bool nan = ((b ? odd1 : odd0) >> in & 1) || (lost >> (2 * b + (e >> 3)) & 1);
+                        s[b][e] = base + 32 * b + in > limit ? -INFINITY : nan ? NAN : s[b][e];
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    top = fmaxf(top, s[b][e]);
+            {
+                auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+            }
+            // (a branch around the rescaling costs more: the accumulators then
+            // live in two places at its end, and registers spill)
+            const float n = fmaxf(ref, top), at = fmaxf(n, -3.4028235e38f);
+            const float fade = __builtin_amdgcn_exp2f(ref - at);
+            ref = n;
+            sum *= fade;
+#pragma unroll
+            for (int n2 = 0; n2 < NC; n2++)
+                acc[n2] *= fade;
+            Frag pf[2][2], pl[2][2];
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const float x = __builtin_amdgcn_exp2f(s[b][e] - at), y = __builtin_amdgcn_exp2f(s[b][e + 1] - at);
+                    sum += x + y;
+                    const f16x2 p = {_Float16(x), _Float16(y)};
+                    pf[b][e >> 3].w[(e & 7) >> 1] = as_u32(p);
+                    if constexpr (FINE)
+                        pl[b][e >> 3].w[(e & 7) >> 1] = as_u32(f16x2{_Float16(x - float(p[0])), _Float16(y - float(p[1]))});
+                }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const char* const at_v = plane + value_of[(2 * b + k) ^ (n & 3)] + 32 * n * 128;
+                        const f16x8 vf = *reinterpret_cast<const f16x8*>(at_v);
+                        if constexpr (FINE && Q4) {
+                            const f16x8 vl = *reinterpret_cast<const f16x8*>(at_v + 2 * PLANE);
+                            acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, pf[b][k].v, acc[n], 0, 0, 0);
+                        }
+                        if constexpr (FINE)
+                            acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[b][k].v, acc[n], 0, 0, 0);
+                        acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[b][k].v, acc[n], 0, 0, 0);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            lost = lost_next;
+            if (u + 1 < unit1) {
+                char* const to = lds[(u + 1) & 1];
+                raw.store(to, to + PLANE, 2 * PLANE, partial(u + 1), odd[(u + 1) % 3]);
+                if (u + 2 < unit1) {
+                    pages_of(u + 2, pages);
+                    lost_next = lost_of(pages);
+                    raw.load(a, it.kvh, (u + 2) * UNIT, pages, head_bytes);
+                }
+            }
+            __syncthreads();
+        }
+        {
+            auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+            sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+        }
+        // (the next item's first barrier is behind everybody's last look at `drawn`)
+        if (!live)
+            continue;
+        // element e of acc[n]: column 32 n + 8 (e / 4) + 4 h + e % 4
+        if (q.parts == 1) {
+            const float inv = wrong ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
+            const int64_t out = (row * a.heads + head) * D + 4 * h;
+#pragma unroll
+            for (int n = 0; n < NC; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    store_out(a, out + 32 * n + 2 * e, acc[n][e] * inv, acc[n][e + 1] * inv, acc[n][e + 2] * inv,
+                              acc[n][e + 3] * inv);
+        } else {
+            float* const slot = a.workspace + prompt_workspace(D) + (it.slot + it.part) * prompt_slot_floats(D);
+            float* const out = slot + (32 * wave + r) * D + 4 * h;
+#pragma unroll
+            for (int n = 0; n < NC; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<f32x4*>(out + 32 * n + 2 * e) = f32x4{acc[n][e], acc[n][e + 1], acc[n][e + 2], acc[n][e + 3]};
+            if (h == 0) {
+                slot[PROMPT_ROWS * D + 32 * wave + r] = wrong ? NAN : ref;
+                slot[PROMPT_ROWS * D + PROMPT_ROWS + 32 * wave + r] = wrong ? NAN : sum;
+            }
+        }
+    }
+}
+
+// Joins the parts of split tiles, 32 rows a workgroup, four values a lane.
+template <int D>
+__global__ void __launch_bounds__(256)
+paged_prompt_merge_kernel(const PagedAttentionArgs a)
+{
+    constexpr int ROWS = 1024 / D;
+    const int kv = a.cache.kv_heads, group = a.heads / kv;
+    Prompt prompt{a.batch, a.cache.page_shift, group, kv, 0};
+    prompt.set_share();
+    PromptItem it;
+    if (!prompt.find<true>(blockIdx.x, &it) || it.q.parts == 1)
+        return;
+    for (int r = int(blockIdx.y) * 32 + int(threadIdx.x) / (D / 4); r < int(blockIdx.y) * 32 + 32; r += ROWS) {
+    const int col = 4 * (int(threadIdx.x) % (D / 4));
+    const int packed = it.tile * PROMPT_ROWS + r, i = packed / group;
+    if (i >= it.q.count)
+        return;
+    float top = -INFINITY, sum = 0.0f;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < it.q.parts; p++) {
+        const float* const slot = a.workspace + prompt_workspace(D) + (it.slot + p) * prompt_slot_floats(D);
+        const float m = slot[PROMPT_ROWS * D + r], l = slot[PROMPT_ROWS * D + PROMPT_ROWS + r];
+        const f32x4 v = *reinterpret_cast<const f32x4*>(slot + r * D + col);
+        const float n = fmaxf(top, m), at = fmaxf(n, -3.4028235e38f);
+        const float f = __builtin_amdgcn_exp2f(top - at), g = __builtin_amdgcn_exp2f(m - at);
+        sum = sum * f + l * g;
+        acc = acc * f + v * g;
+        top = n;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    store_out(a, ((int64_t(it.q.first) + i) * a.heads + it.kvh * group + packed % group) * D + col, acc[0] * inv, acc[1] * inv,
+              acc[2] * inv, acc[3] * inv);
+    }
+}
+
+template <int D, bool Q4, bool FINE>
+hipError_t launch(const PagedAttentionArgs& a, hipStream_t s)
+{
+    const int group = a.heads / a.cache.kv_heads, kv = a.cache.kv_heads;
+    const int64_t packed = int64_t(a.batch.rows) * group;
+    const int some = min(a.batch.rows, a.batch.sequences);                       // sequences with rows, at most
+    paged_attention_kernel<D, Q4, FINE><<<WAVES / 4, 256, 0, s>>>(a);
+    const int tile_rows = int(min(int64_t(TILE_ROWS), int64_t(a.batch.max_rows) * group));
+    paged_merge_kernel<D><<<dim3(unsigned(min(packed / TILE_ROWS + some, int64_t(FEW_ROWS / TILE_ROWS) * some) * kv), unsigned((tile_rows + 256 / D - 1) / (256 / D))),
+                            256, 0, s>>>(a);
+    if (int64_t(a.batch.max_rows) * group > FEW_ROWS) {
+        paged_prompt_kernel<D, Q4, FINE><<<PROMPT_WORKERS, 256, 0, s>>>(a);
+        const int64_t tiles = packed / PROMPT_ROWS + some;
+        paged_prompt_merge_kernel<D><<<dim3(unsigned(tiles * kv), PROMPT_ROWS / 32), 256, 0, s>>>(a);
+    }
+    return hipGetLastError();
+}
+
 template <int D>
 hipError_t launch(const PagedAttentionArgs& a, hipStream_t s)
 {
     const bool fine = a.out_format != PAGED_OUT_BF16;
-    constexpr unsigned grid = WAVES / 4;
-    if (a.cache.q4) {
-        if (fine)
-            paged_attention_kernel<D, true, true><<<grid, 256, 0, s>>>(a);
-        else
-            paged_attention_kernel<D, true, false><<<grid, 256, 0, s>>>(a);
-    } else {
-        if (fine)
-            paged_attention_kernel<D, false, true><<<grid, 256, 0, s>>>(a);
-        else
-            paged_attention_kernel<D, false, false><<<grid, 256, 0, s>>>(a);
-    }
-    const int group = a.heads / a.cache.kv_heads;
-    const int64_t tiles = int64_t(a.batch.rows) * group / TILE_ROWS + min(a.batch.rows, a.batch.sequences);   // at most
-    const int tile_rows = min(TILE_ROWS, int(min(int64_t(TILE_ROWS), int64_t(a.batch.max_rows) * group)));
-    const dim3 merge(unsigned(tiles * a.cache.kv_heads), unsigned((tile_rows + 256 / D - 1) / (256 / D)));
-    paged_merge_kernel<D><<<merge, 256, 0, s>>>(a);
-    return hipGetLastError();
+    if (a.cache.q4)
+        return fine ? launch<D, true, true>(a, s) : launch<D, true, false>(a, s);
+    return fine ? launch<D, false, true>(a, s) : launch<D, false, false>(a, s);
 }
 
 }  // namespace
 
-int64_t paged_attention_workspace_floats(int, int, int head) { return int64_t(WAVES) * 2 * slot_floats(head); }
+int64_t paged_attention_workspace_floats(int, int, int head)
+{
+    return prompt_workspace(head) + int64_t(PROMPT_SLOTS) * prompt_slot_floats(head);
+}
 
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s)
 {
