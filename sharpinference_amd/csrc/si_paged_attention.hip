@@ -44,6 +44,12 @@ __device__ __forceinline__ f16x2 nibbles(uint32_t w)
     return as_f16x2(v) - k;
 }
 
+// Whether one of the word's two FP16 values is infinite or NaN.
+__device__ __forceinline__ bool infinite(uint32_t w)
+{
+    return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
+}
+
 union Frag {
     uint32_t w[4];
     f16x8 v;
@@ -82,10 +88,21 @@ __device__ __forceinline__ Sequence take_sequence(const PagedBatch& b, int page_
     return q;
 }
 
+// a / b for 0 <= a < 2^53, b > 0: a fifth of the code of a 64-bit division.
+// The kernels run their beginnings once, from a cold instruction cache, so
+// what counts there is how many instructions there are.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b)
+{
+    int64_t q = int64_t(double(a) / double(b));
+    const int64_t r = a - q * b;
+    q += r >= b ? 1 : r < 0 ? -1 : 0;
+    return q;
+}
+
 __device__ __forceinline__ int64_t wave_scan(int64_t v)
 {
     const int lane = threadIdx.x & 63;
-#pragma unroll
+#pragma unroll 1
     for (int m = 1; m < 64; m <<= 1) {
         const int64_t o = __shfl_up(v, m);
         v += lane >= m ? o : 0;
@@ -132,48 +149,38 @@ struct Line {
         }
         return false;
     }
-    // The sequence that holds tile x of one KV head, the tile's number in it
-    // and its first unit (of KV head 0).
-    __device__ __forceinline__ bool at_tile(int64_t x, Sequence* q, int64_t* tile, int64_t* start) const
-    {
-        int64_t before = 0, units = 0;
-        for (int base = 0; base < b.sequences; base += 64) {
-            const Sequence mine = take_sequence(b, page_shift, group, base + int(threadIdx.x & 63));
-            const int64_t upto = before + wave_scan(mine.tiles), units_upto = units + wave_scan(units_of(mine));
-            const uint64_t past = __ballot(upto > x);
-            if (past) {
-                const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-                *q = from_lane(mine, at);
-                *tile = x - __shfl(upto - mine.tiles, at);
-                *start = __shfl(units_upto - units_of(mine), at);
-                return true;
-            }
-            before = __shfl(upto, 63);
-            units = __shfl(units_upto, 63);
-        }
-        return false;
-    }
 };
 
-// The waves that share a line of `total` units: wave w of `waves` takes
-// units first(w) .. first(w + 1) - 1, at least MIN_UNITS of them.
+// The waves that share a line of `total` units take equal runs of it.
 constexpr int MIN_UNITS = 2;
 constexpr int WAVES = 2048;
 struct Shares {
-    int64_t total, waves;
-    __device__ __forceinline__ explicit Shares(int64_t t) : total(t), waves(min(int64_t(WAVES), (t + MIN_UNITS - 1) / MIN_UNITS)) {}
-    __device__ __forceinline__ int64_t first(int64_t w) const { return w * total / waves; }
-    __device__ __forceinline__ int64_t wave_of(int64_t unit) const { return ((unit + 1) * waves - 1) / total; }
+    int64_t share;
+    __device__ __forceinline__ explicit Shares(int64_t total) : share(max(int64_t(MIN_UNITS), (total + WAVES - 1) / WAVES)) {}
+    __device__ __forceinline__ int64_t wave_of(int64_t unit) const { return quotient(unit, share); }
+};
+
+// What the merge has to do behind a wave (or worker): join `parts` slots, from
+// the second of this one on, into rows row0 .. of a tile; parts 0: nothing.
+struct Record {
+    int32_t parts;
+    int32_t first;             // the sequence's first batch row
+    int32_t count;             // its rows
+    int32_t row0;              // the tile's first packed row
+    int32_t kvh;
+    int32_t unused[3];
 };
 
 // What a wave leaves of a tile whose units it shares with other waves: the
 // accumulators [TILE_ROWS][D], largest scores and sums [TILE_ROWS] each.
 // Slot 2 w: of the tile that began before wave w's units, slot 2 w + 1: of
 // the one that goes on behind them.
-constexpr int COUNTER_FLOATS = 4;        // a workspace begins with the prompt kernel's counter
 constexpr int slot_floats(int d) { return TILE_ROWS * d + 2 * TILE_ROWS; }
-// where the prompt kernel's slots begin
-constexpr int64_t prompt_workspace(int d) { return COUNTER_FLOATS + int64_t(WAVES) * 2 * slot_floats(d); }
+constexpr int PROMPT_WORKERS = 256;      // workgroups of the prompt kernel, one a CU
+// A workspace: the waves' and the workers' records, their slots.
+constexpr int64_t RECORD_FLOATS = sizeof(Record) / 4 * (WAVES + PROMPT_WORKERS);
+constexpr int64_t prompt_workspace(int d) { return RECORD_FLOATS + int64_t(WAVES) * 2 * slot_floats(d); }
+__device__ __forceinline__ Record* records(float* workspace) { return reinterpret_cast<Record*>(workspace); }
 
 // Running state of a tile: the lane's packed row is lane & 15.
 template <int D>
@@ -457,7 +464,7 @@ struct Attend {
                 } else {
 #pragma unroll
                     for (int k = 0; k < D / 32; k++)
-                        if ((r.v[u][i][k] & 0x7C00u) == 0x7C00u || (r.v[u][i][k] & 0x7C000000u) == 0x7C000000u) {
+                        if (infinite(r.v[u][i][k])) {
                             odd |= 1u << (4 * u + i);
                             r.v[u][i][k] = 0;
                         }
@@ -505,32 +512,26 @@ paged_attention_kernel(const PagedAttentionArgs a)
     constexpr int NV = D / 16;
     const int kv = a.cache.kv_heads, group = a.heads / kv;
     const int64_t wave = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    // (the prompt kernel behind this one draws its items from here)
-    if (blockIdx.x == 0 && threadIdx.x == 0)
-        *reinterpret_cast<int32_t*>(a.workspace) = 0;
     const Line line{a.batch, a.cache.page_shift, group, kv};
     const int64_t total = line.total();
-    if (total == 0)
-        return;
-    const Shares share(total);
-    if (wave >= share.waves)
-        return;
-    const int64_t begin = share.first(wave), end = share.first(wave + 1);
+    const Shares shares(total);
+    const int64_t begin = wave * shares.share, end = min(total, begin + shares.share);
+    Record record{};
     Attend<D, Q4, FINE> w(a);
     Sequence q{};
     int64_t q_start = 0, q_end = 0;
     for (int64_t x = begin; x < end;) {
         if (x >= q_end) {
             if (!line.at_unit(x, &q, &q_start))
-                return;
+                break;
             q_end = q_start + line.units_of(q);
         }
         // unit x: of which KV head, tile and positions
         const int64_t in = x - q_start;
-        const int64_t tile_no = in / q.units;
-        const int kvh = __builtin_amdgcn_readfirstlane(int(tile_no / q.tiles));
-        const int row0 = __builtin_amdgcn_readfirstlane(int(tile_no % q.tiles) * TILE_ROWS);
-        const int unit0 = __builtin_amdgcn_readfirstlane(int(in % q.units));
+        const uint32_t tile_no = uint32_t(quotient(in, q.units));       // at most 4 tiles and 256 heads
+        const int kvh = __builtin_amdgcn_readfirstlane(int(tile_no / uint32_t(q.tiles)));
+        const int row0 = __builtin_amdgcn_readfirstlane(int(tile_no - kvh * q.tiles) * TILE_ROWS);
+        const int unit0 = __builtin_amdgcn_readfirstlane(int(in - int64_t(tile_no) * q.units));
         const int64_t tile_start = x - unit0, tile_end = tile_start + q.units;
         const int unit1 = __builtin_amdgcn_readfirstlane(int(min(tile_end, end) - tile_start));
         x = min(tile_end, end);
@@ -602,7 +603,7 @@ paged_attention_kernel(const PagedAttentionArgs a)
                                   st.acc[n + 3][r] * inv);
             }
         } else if (live) {
-            float* slot = a.workspace + COUNTER_FLOATS + (2 * wave + (tile_start >= begin)) * slot_floats(D);
+            float* slot = a.workspace + RECORD_FLOATS + (2 * wave + (tile_start >= begin)) * slot_floats(D);
             float* at = slot + w.c * D + NV * 4 * w.g;
 #pragma unroll
             for (int r = 0; r < 4; r++)
@@ -615,112 +616,129 @@ paged_attention_kernel(const PagedAttentionArgs a)
                 slot[TILE_ROWS * D + TILE_ROWS + w.c] = sum;
             }
         }
+        if (tile_start >= begin && tile_end > end)
+            record = {int(shares.wave_of(tile_end - 1) - wave) + 1, q.first, q.count, row0, kvh, {}};
     }
+    if (w.lane == 0)
+        records(a.workspace)[wave] = record;
 }
 
-// Joins the tiles that several waves share.  A workgroup takes 256 / D rows
-// of four values a lane in each of its waves, and the waves take the tile's
-// slots in turn.
+// Joins what `parts` slots, `stride` floats apart, hold of four neighbouring
+// values of a row: those of its accumulators at `at`, its largest score and
+// sum at `stats` and `stats` + rows.
+struct Joined {
+    float top = -INFINITY, sum = 0.0f;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    __device__ __forceinline__ void take(float m, float l, f32x4 v)
+    {
+        const float t = fmaxf(top, m), at = fmaxf(t, -3.4028235e38f);
+        const float f = __builtin_amdgcn_exp2f(top - at), g = __builtin_amdgcn_exp2f(m - at);
+        sum = sum * f + l * g;             // (NaN stays NaN)
+        acc = acc * f + v * g;
+        top = t;
+    }
+};
+
+// What the four waves of a workgroup hold, in its first; true there.
+__device__ __forceinline__ bool join_waves(Joined& sum)
+{
+    __shared__ float parts[3][2][64];
+    __shared__ f32x4 parts_acc[3][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (wave) {
+        parts[wave - 1][0][lane] = sum.top;
+        parts[wave - 1][1][lane] = sum.sum;
+        parts_acc[wave - 1][lane] = sum.acc;
+    }
+    __syncthreads();
+    if (wave)
+        return false;
+#pragma unroll
+    for (int k = 0; k < 3; k++)
+        sum.take(parts[k][0][lane], parts[k][1][lane], parts_acc[k][lane]);
+    return true;
+}
+
+// Joins the tiles that several waves share: workgroup x the one that begins
+// in wave x and ends behind it, 256 / D rows of it, four values a lane; its
+// waves take the slots in turn.
 template <int D>
 __global__ void __launch_bounds__(256)
 paged_merge_kernel(const PagedAttentionArgs a)
 {
+    const Record todo = records(a.workspace)[blockIdx.x];
+    if (todo.parts == 0)
+        return;
     constexpr int ROWS = 256 / D;
-    const int kv = a.cache.kv_heads, group = a.heads / kv;
-    const Line line{a.batch, a.cache.page_shift, group, kv};
-    const int64_t total = line.total();
-    Sequence q;
-    int64_t tile, q_start;
-    if (total == 0 || !line.at_tile(blockIdx.x / kv, &q, &tile, &q_start))
-        return;
-    const int kvh = blockIdx.x % kv;
-    const Shares share(total);
-    const int64_t first = q_start + (int64_t(kvh) * q.tiles + tile) * q.units;
-    const int64_t w0 = share.wave_of(first), w1 = share.wave_of(first + q.units - 1);
-    if (w0 == w1)
-        return;
+    const int group = a.heads / a.cache.kv_heads;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int r = int(blockIdx.y) * ROWS + lane / (D / 4), col = 4 * (lane % (D / 4));
-    const int packed = int(tile) * TILE_ROWS + r, i = packed / group;
-    const bool live = i < q.count;
-    float top = -INFINITY, sum = 0.0f;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    bool seen_nan = false;
+    const int packed = todo.row0 + r, i = packed / group;
+    const bool live = i < todo.count;
+    Joined sum;
     if (live) {
-        for (int64_t p = w0 + wave; p <= w1; p += 4) {
-            const float* slot = a.workspace + COUNTER_FLOATS + (2 * p + (p == w0)) * slot_floats(D);
-            const float m = slot[TILE_ROWS * D + r], l = slot[TILE_ROWS * D + TILE_ROWS + r];
-            const f32x4 v = *reinterpret_cast<const f32x4*>(slot + r * D + col);
-            const float t = fmaxf(top, m), at = fmaxf(t, -3.4028235e38f);
-            const float f = __builtin_amdgcn_exp2f(top - at), g = __builtin_amdgcn_exp2f(m - at);
-            seen_nan |= !(l == l);
-            sum = sum * f + l * g;
-            acc = acc * f + v * g;
-            top = t;
+        // (a tile's own wave has it in its second slot, the others in their first)
+        const float* slot = a.workspace + RECORD_FLOATS + 2 * int64_t(blockIdx.x) * slot_floats(D);
+#pragma unroll 2
+        for (int p = wave; p < todo.parts; p += 4) {
+            const float* const at = slot + (2 * p + (p == 0)) * slot_floats(D);
+            sum.take(at[TILE_ROWS * D + r], at[TILE_ROWS * D + TILE_ROWS + r], *reinterpret_cast<const f32x4*>(at + r * D + col));
         }
     }
-    __shared__ float parts[3][64][6];
-    if (wave) {
-        float* t = parts[wave - 1][lane];
-        t[0] = top, t[1] = seen_nan ? NAN : sum, t[2] = acc[0], t[3] = acc[1], t[4] = acc[2], t[5] = acc[3];
-    }
-    __syncthreads();
-    if (wave || !live)
+    if (!join_waves(sum) || !live)
         return;
-#pragma unroll
-    for (int k = 0; k < 3; k++) {
-        const float* t = parts[k][lane];
-        const float n = fmaxf(top, t[0]), at = fmaxf(n, -3.4028235e38f);
-        const float f = __builtin_amdgcn_exp2f(top - at), g = __builtin_amdgcn_exp2f(t[0] - at);
-        seen_nan |= !(t[1] == t[1]);
-        sum = sum * f + t[1] * g;
-        acc = acc * f + f32x4{t[2], t[3], t[4], t[5]} * g;
-        top = n;
-    }
-    const float inv = seen_nan ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
-    store_out(a, ((int64_t(q.first) + i) * a.heads + kvh * group + packed % group) * D + col, acc[0] * inv, acc[1] * inv,
-              acc[2] * inv, acc[3] * inv);
+    const float inv = sum.sum == 0.0f ? 0.0f : 1.0f / sum.sum;
+    store_out(a, ((int64_t(todo.first) + i) * a.heads + todo.kvh * group + packed % group) * D + col, sum.acc[0] * inv,
+              sum.acc[1] * inv, sum.acc[2] * inv, sum.acc[3] * inv);
 }
 
 // ---- many rows of a sequence ------------------------------------------------------------
 
-// A workgroup of four waves takes 128 packed rows of one sequence and KV
+// A workgroup of eight waves takes 256 packed rows of one sequence and KV
 // head, 32 a wave, through units of 64 positions.  The unit's keys and values
-// go through LDS as FP16, dequantized once for the four waves (two waves
-// convert keys, two values), two buffers: the next unit's bytes are loaded
+// go through LDS as FP16, dequantized once for the eight waves (four waves
+// convert keys, four values), two buffers: the next unit's bytes are loaded
 // while this one is multiplied.  Scores stay transposed here too, with
 // v_mfma_f32_32x32x16_f16.
-constexpr int PROMPT_ROWS = 128;
-constexpr int PROMPT_WORKERS = 512;      // two workgroups a CU
-constexpr int PROMPT_SLOTS = 2 * PROMPT_WORKERS;   // see Prompt
-constexpr int PROMPT_MIN = 8;            // units that a workgroup takes at least
+constexpr int PROMPT_ROWS = 256;
+constexpr int PROMPT_THREADS = 512;
+constexpr float REFERENCE_SLACK = 8.0f;
+constexpr int PROMPT_PIECE = 7;          // what a piece of a tile costs besides its units, in units
+constexpr int PROMPT_MIN = 9;            // units that a worker takes at least, with a piece's cost
 
 using f32x16 = float __attribute__((ext_vector_type(16)));
 
 constexpr int prompt_slot_floats(int d) { return PROMPT_ROWS * d + 2 * PROMPT_ROWS; }
 
-// The items of a launch: sequence after sequence, its tiles from the last
-// (which see most) to the first, a tile's `parts` runs of units, the KV
-// heads.  A sequence is split where its units are at least 1.5 times what
-// each worker would take of an equal division; then parts is at most 4/3 of
-// units / share, so no more than 4/3 PROMPT_WORKERS items have slots.
 struct PromptSequence {
-    int index, first, count, length, tiles, units, parts;
-};
-struct PromptItem {
-    PromptSequence q;
-    int tile, part, kvh;
-    int64_t slot;              // of the tile's first part; parts > 1
+    int index, first, count, length, tiles;
+    int64_t a, c;              // weight of the tiles: see PromptLine
 };
 
-struct Prompt {
+// The work of a launch in one line: sequence after sequence, of each its KV
+// heads, of each its tiles.  Tile i of a sequence goes through about (length
+// - count) / 64 + (i + 1/2) 4 / group units (a tile is 256 / group positions
+// long, and each sees all before it), and costs PROMPT_PIECE units more, which its
+// queries and outputs take.  Its weight is group times that: w_i = a + 2 c i + c
+// with c = 2, all of tiles 0 .. t - 1 together a t + c t^2.  Every worker takes an
+// equal run of the line; a border inside a tile is at the same share of its units.
+//
+// Where there are few tiles, a border that every worker meets somewhere in its
+// run costs more than parts that are not quite equal: there all tiles of a
+// sequence are cut into as many parts as its last one needs (c = 0, a = parts *
+// share), and no worker has more than one part.
+struct PromptLine {
     const PagedBatch& b;
     int page_shift, group, kv;
-    int64_t share;             // units of a worker
+    int64_t share;             // of a worker
+    bool cut;                  // into parts
 
+    static __device__ __forceinline__ int64_t before(const PromptSequence& q, int64_t t) { return (q.a + q.c * t) * t; }
+    static __device__ __forceinline__ int64_t tile_weight(const PromptSequence& q, int64_t t) { return q.a + q.c * (2 * t + 1); }
+    __device__ __forceinline__ int64_t weight(const PromptSequence& q) const { return kv * before(q, q.tiles); }
     __device__ __forceinline__ PromptSequence take(int s) const
     {
-        PromptSequence q{s, 0, 0, 0, 0, 0, 1};
+        PromptSequence q{s, 0, 0, 0, 0, 0, 2};
         if (s >= b.sequences)
             return q;
         sequence_rows(b, s, &q.first, &q.count);
@@ -728,51 +746,71 @@ struct Prompt {
         if (q.length < 0 || q.length > int64_t(b.max_pages) << page_shift || q.count > b.max_rows)
             q.length = -1;
         q.tiles = q.count * group > FEW_ROWS ? (q.count * group + PROMPT_ROWS - 1) / PROMPT_ROWS : 0;
-        q.units = max(1, (q.length + UNIT - 1) / UNIT);
-        if (share > 0)
-            q.parts = int((q.units + share - 1) / share);
+        q.a = int64_t(group) * (max(0, q.length - q.count) / UNIT + PROMPT_PIECE);
+        if (cut && q.tiles) {
+            q.a = (quotient(tile_weight(q, q.tiles - 1) - 1, share) + 1) * share;
+            q.c = 0;
+        }
         return q;
     }
-    __device__ __forceinline__ void set_share()
+    __device__ __forceinline__ PromptLine(const PagedBatch& batch, int shift, int heads_per_kv, int kv_heads)
+        : b(batch), page_shift(shift), group(heads_per_kv), kv(kv_heads), share(0), cut(false)
     {
-        share = 0;
-        int64_t sum = 0;
+        // all weight, tiles, and the weight if a sequence's tiles were all like its last
+        int64_t total = 0, tiles = 0, last = 0;
         for (int base = 0; base < b.sequences; base += 64) {
             const PromptSequence q = take(base + int(threadIdx.x & 63));
-            sum += int64_t(kv) * q.tiles * q.units;
+            total += weight(q);
+            tiles += int64_t(kv) * q.tiles;
+            last += q.tiles ? int64_t(kv) * q.tiles * tile_weight(q, q.tiles - 1) : 0;
         }
-        sum = __shfl(wave_scan(sum), 63);
-        share = max(int64_t(PROMPT_MIN), (sum + PROMPT_WORKERS - 1) / PROMPT_WORKERS);
+        total = __shfl(wave_scan(total), 63);
+        tiles = __shfl(wave_scan(tiles), 63);
+        last = __shfl(wave_scan(last), 63);
+        share = max(int64_t(PROMPT_MIN) * group, (total + PROMPT_WORKERS - 1) / PROMPT_WORKERS);
+        if (tiles < PROMPT_WORKERS) {
+            // at most last / parts + tiles <= PROMPT_WORKERS parts
+            const int64_t parts = max(int64_t(PROMPT_MIN) * group, quotient(last, PROMPT_WORKERS - tiles) + 1);
+            cut = parts <= share + PROMPT_PIECE * group;
+            share = cut ? parts : share;
+        }
     }
-    // Item x, or (TILES) the first part of tile x of the launch.
-    template <bool TILES>
-    __device__ __forceinline__ bool find(int64_t x, PromptItem* out) const
+    __device__ __forceinline__ int64_t worker_of(int64_t place) const { return quotient(place, share); }
+    static __device__ __forceinline__ PromptSequence from_lane(const PromptSequence& q, int lane)
     {
-        int64_t before = 0, slots = 0;
+        return {__shfl(q.index, lane), __shfl(q.first, lane), __shfl(q.count, lane), __shfl(q.length, lane),
+                __shfl(q.tiles, lane), __shfl(q.a, lane),     __shfl(q.c, lane)};
+    }
+    // The sequence that holds place x, and the place of its begin.
+    __device__ __forceinline__ bool find(int64_t x, PromptSequence* q, int64_t* start) const
+    {
+        int64_t places = 0;
         for (int base = 0; base < b.sequences; base += 64) {
             const PromptSequence mine = take(base + int(threadIdx.x & 63));
-            const int64_t own = int64_t(kv) * mine.tiles * (TILES ? 1 : mine.parts);
-            const int64_t own_slots = mine.parts > 1 ? int64_t(kv) * mine.tiles * mine.parts : 0;
-            const int64_t upto = before + wave_scan(own), slots_upto = slots + wave_scan(own_slots);
-            const uint64_t past = __ballot(upto > x);
+            const int64_t w = weight(mine);
+            const int64_t places_upto = places + wave_scan(w);
+            const uint64_t past = __ballot(places_upto > x);
             if (past) {
                 const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-                out->q = {__shfl(mine.index, at), __shfl(mine.first, at), __shfl(mine.count, at), __shfl(mine.length, at),
-                          __shfl(mine.tiles, at), __shfl(mine.units, at), __shfl(mine.parts, at)};
-                const int64_t in = x - __shfl(upto - own, at);
-                const int parts = TILES ? 1 : out->q.parts;
-                out->kvh = int(in % kv);
-                out->part = int(in / kv % parts);
-                out->tile = out->q.tiles - 1 - int(in / kv / parts);
-                // a tile's parts and KV heads lie together in the slots
-                out->slot = __shfl(slots_upto - own_slots, at) +
-                            (int64_t(out->q.tiles - 1 - out->tile) * kv + out->kvh) * out->q.parts;
+                *q = from_lane(mine, at);
+                *start = __shfl(places_upto - w, at);
                 return true;
             }
-            before = __shfl(upto, 63);
-            slots = __shfl(slots_upto, 63);
+            places = __shfl(places_upto, 63);
         }
         return false;
+    }
+    // The tile that holds place y of a KV head.
+    static __device__ __forceinline__ int64_t tile_at(const PromptSequence& q, int64_t y)
+    {
+        const double a = double(q.a);
+        int64_t t = q.c ? int64_t((sqrt(a * a + 4.0 * q.c * double(y)) - a) / (2.0 * q.c)) : quotient(y, q.a);
+        t = min(int64_t(q.tiles) - 1, t);
+        while (t > 0 && before(q, t) > y)
+            t--;
+        while (before(q, t + 1) <= y)
+            t++;
+        return t;
     }
 };
 
@@ -786,29 +824,34 @@ __device__ __forceinline__ int value_at(int col, int piece)    // of eight posit
     return col * 128 + ((piece ^ (((col >> 1) ^ (col >> 4)) & 7)) << 4);
 }
 
-// What a thread loads of a unit.  Threads 0..127 take keys: 16-byte pieces of
-// rows; threads 128..255 values: NV columns of eight positions, those that
-// piece q = (thread - 128) / 16 of a column holds: 16 (q / 2) + 4 (q % 2) + {0..3, 8..11}.
+// What a thread loads of a unit.  Threads 0..255 take keys: 16-byte pieces of
+// rows; threads 256..511 values: four columns of the eight positions that
+// piece q of a column holds, 16 (q / 2) + 4 (q % 2) + {0..3, 8..11}.
 template <int D, bool Q4, bool FINE>
 struct PromptLoad {
-    static constexpr int NV = D / 16;
-    static constexpr int KEYS = Q4 ? D / 64 : D / 16;          // 16-byte loads of a key thread
-    static constexpr int PIECES = Q4 ? D / 32 : D / 8;         // of a row
-    uint4 k[KEYS];
-    uint32_t kd[KEYS];
-    uint32_t v[8][Q4 ? 1 : NV / 2];
-    uint32_t vd[4];
+    static constexpr int PIECES = Q4 ? D / 32 : D / 8;         // 16-byte pieces of a row of keys
+    static constexpr int KEYS = (UNIT * PIECES + 255) / 256;   // of a key thread
+    static constexpr int COLS = D / 4;                         // value threads side by side
+    // (one set of registers for both kinds of threads)
+    static constexpr int WORDS = Q4 ? 12 : 16;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ uint32_t& kd(int i) { return w[4 * KEYS + i]; }
+    __device__ __forceinline__ uint32_t& v(int i, int n) { return w[Q4 ? i : 2 * i + n]; }
+    __device__ __forceinline__ uint32_t& vd(int p) { return w[8 + p]; }
 
-    // The thread among its 128, as a new value each time: what follows from it
+    // The thread among its 256, as a new value each time: what follows from it
     // is worked out where it is needed and holds no register through the products.
     static __device__ __forceinline__ int thread()
     {
-        int t = threadIdx.x & 127;
+        int t = threadIdx.x & 255;
         asm volatile("" : "+v"(t));
         return t;
     }
+    // (4-bit rows of 64 values are half as many pieces as there are threads)
+    static __device__ __forceinline__ bool takes_keys(int t) { return threadIdx.x < 256 && (UNIT * PIECES >= 256 || t < UNIT * PIECES); }
+    static __device__ __forceinline__ bool takes_values(int t) { return threadIdx.x >= 256 && (COLS * 8 == 256 || t < COLS * 8); }
     // the row of a key thread's load i, and its piece of it
-    static __device__ __forceinline__ int row(int t, int i) { return t / PIECES + i * (128 / PIECES); }
+    static __device__ __forceinline__ int row(int t, int i) { return t / PIECES + i * (256 / PIECES); }
     static __device__ __forceinline__ int piece(int t) { return t % PIECES; }
 
     // pages: the unit's four pages (a page that is not there: page 0)
@@ -820,76 +863,84 @@ struct PromptLoad {
             const int page = u < 2 ? (u ? pages[1] : pages[0]) : (u == 2 ? pages[2] : pages[3]);
             return (int64_t(max(page, 0)) * a.cache.kv_heads + kvh) * head_bytes;
         };
-        if (threadIdx.x < 128) {
+        if (takes_keys(t)) {
 #pragma unroll
             for (int i = 0; i < KEYS; i++) {
                 const int r = row(t, i), slot = (base + r) & (ps - 1);
                 const char* const p = a.cache.keys + page_at(r >> 4);
-                k[i] = *reinterpret_cast<const uint4*>(p + slot * (Q4 ? D / 2 : 2 * D) + 16 * piece(t));
+                const uint4 x = *reinterpret_cast<const uint4*>(p + slot * (Q4 ? D / 2 : 2 * D) + 16 * piece(t));
+                w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
                 if constexpr (Q4)
-                    kd[i] = reinterpret_cast<const uint16_t*>(p + ps * (D / 2))[piece(t) * ps + slot];
+                    kd(i) = reinterpret_cast<const uint16_t*>(p + ps * (D / 2))[piece(t) * ps + slot];
             }
-        } else {
-            const int c = t & 15, q = t >> 4;
+        } else if (takes_values(t)) {
+            const int c = t % COLS, q = t / COLS;
             const int r = 16 * (q >> 1) + 4 * (q & 1), slot = (base + r) & (ps - 1);
             const char* const p = a.cache.values + page_at(q >> 1);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int s = slot + (i & 3) + 8 * (i >> 2);
                 if constexpr (Q4) {
-                    const char* const at = p + s * (D / 2) + NV / 2 * c;
-                    v[i][0] = D == 128 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at);
-                } else if constexpr (D == 128) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(p + s * (2 * D) + 2 * NV * c);
-                    v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+                    v(i, 0) = *reinterpret_cast<const uint16_t*>(p + s * (D / 2) + 2 * c);
                 } else {
-                    const uint2 x = *reinterpret_cast<const uint2*>(p + s * (2 * D) + 2 * NV * c);
-                    v[i][0] = x.x, v[i][1] = x.y;
+                    const uint2 x = *reinterpret_cast<const uint2*>(p + s * (2 * D) + 8 * c);
+                    v(i, 0) = x.x, v(i, 1) = x.y;
                 }
             }
             if constexpr (Q4) {
-                const uint16_t* const d = reinterpret_cast<const uint16_t*>(p + ps * (D / 2)) + (D == 128 ? c >> 2 : c >> 3) * ps + slot;
+                const uint16_t* const d = reinterpret_cast<const uint16_t*>(p + ps * (D / 2)) + (c >> 3) * ps + slot;
                 const uint2 x = *reinterpret_cast<const uint2*>(d), y = *reinterpret_cast<const uint2*>(d + 8);
-                vd[0] = x.x, vd[1] = x.y, vd[2] = y.x, vd[3] = y.y;
+                vd(0) = x.x, vd(1) = x.y, vd(2) = y.x, vd(3) = y.y;
             }
         }
     }
 
     // Into LDS as FP16 (FINE 4-bit: and what is left of the products beside
-    // it).  `partial`: some row does not see all of the unit; values that are
-    // not finite are then taken out and their positions marked in `odd`.
+    // it).  `partial`: some row does not see all of the unit; keys and values
+    // that are not finite are then taken out and their positions marked in `odd`.
     __device__ __forceinline__ void store(char* keys, char* values, int lo, bool partial, uint32_t* odd)
     {
         const int t = thread();
-        if (threadIdx.x < 128) {
+        if (takes_keys(t)) {
 #pragma unroll
             for (int i = 0; i < KEYS; i++) {
                 const int r = row(t, i);
+                if (partial) {
+                    bool bad;
+                    if constexpr (Q4) {
+                        bad = (kd(i) & 0x7000u) == 0x7000u;
+                        kd(i) = bad ? 0 : kd(i);
+                    } else {
+                        bad = infinite(w[4 * i]) || infinite(w[4 * i + 1]) || infinite(w[4 * i + 2]) || infinite(w[4 * i + 3]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            w[4 * i + j] = bad ? 0 : w[4 * i + j];
+                    }
+                    if (bad)
+                        atomicOr(&odd[r >> 5], 1u << (r & 31));
+                }
                 if constexpr (Q4) {
-                    const f16x2 d = as_f16x2(kd[i] | kd[i] << 16);
-                    const uint32_t w[4] = {k[i].x, k[i].y, k[i].z, k[i].w};
+                    const f16x2 d = as_f16x2(kd(i) | kd(i) << 16);
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        uint4 x, y;
-                        uint32_t* const xs[4] = {&x.x, &x.y, &x.z, &x.w};
-                        uint32_t* const ys[4] = {&y.x, &y.y, &y.z, &y.w};
+                        Frag x, y;
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const f16x2 n = nibbles(w[j] >> (4 * e)), p = n * d;
-                            *xs[e] = as_u32(p);
+                            const f16x2 n = nibbles(w[4 * i + j] >> (4 * e)), p = n * d;
+                            x.w[e] = as_u32(p);
                             if constexpr (FINE)
-                                *ys[e] = as_u32(__builtin_elementwise_fma(n, d, -p));
+                                y.w[e] = as_u32(__builtin_elementwise_fma(n, d, -p));
                         }
-                        *reinterpret_cast<uint4*>(keys + key_at<D>(r, 4 * piece(t) + j)) = x;
+                        *reinterpret_cast<f16x8*>(keys + key_at<D>(r, 4 * piece(t) + j)) = x.v;
                         if constexpr (FINE)
-                            *reinterpret_cast<uint4*>(keys + lo + key_at<D>(r, 4 * piece(t) + j)) = y;
+                            *reinterpret_cast<f16x8*>(keys + lo + key_at<D>(r, 4 * piece(t) + j)) = y.v;
                     }
                 } else {
-                    *reinterpret_cast<uint4*>(keys + key_at<D>(r, piece(t))) = k[i];
+                    *reinterpret_cast<uint4*>(keys + key_at<D>(r, piece(t))) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
                 }
             }
-        } else {
-            const int c = t & 15, q = t >> 4;
+        } else if (takes_values(t)) {
+            const int c = t % COLS, q = t / COLS;
             if (partial) {
                 uint32_t mask = 0;
 #pragma unroll
@@ -897,15 +948,15 @@ struct PromptLoad {
                     bool bad = false;
                     if constexpr (Q4) {
                         const uint32_t e = 0x7000u << (16 * (i & 1));      // (8192 and up, as above)
-                        bad = (vd[i >> 1] & e) == e;
+                        bad = (vd(i >> 1) & e) == e;
                         if (bad)
-                            vd[i >> 1] &= ~(0xFFFFu << (16 * (i & 1)));
+                            vd(i >> 1) &= ~(0xFFFFu << (16 * (i & 1)));
                     } else {
 #pragma unroll
-                        for (int n = 0; n < NV / 2; n++)
-                            if ((v[i][n] & 0x7C00u) == 0x7C00u || (v[i][n] & 0x7C000000u) == 0x7C000000u) {
+                        for (int n = 0; n < 2; n++)
+                            if (infinite(v(i, n))) {
                                 bad = true;
-                                v[i][n] = 0;
+                                v(i, n) = 0;
                             }
                     }
                     const int pos = 16 * (q >> 1) + 4 * (q & 1) + (i & 3) + 8 * (i >> 2);
@@ -914,41 +965,37 @@ struct PromptLoad {
                 if (mask)
                     atomicOr(&odd[q >> 2], mask);
             }
-            uint32_t lo16[4], hi16[4];
+            uint32_t both[4];                              // 4-bit: two positions' four columns
             if constexpr (Q4) {
 #pragma unroll
-                for (int p = 0; p < 4; p++) {
-                    lo16[p] = __builtin_amdgcn_perm(v[2 * p + 1][0], v[2 * p][0], 0x05040100u);
-                    hi16[p] = __builtin_amdgcn_perm(v[2 * p + 1][0], v[2 * p][0], 0x07060302u);
-                }
+                for (int p = 0; p < 4; p++)
+                    both[p] = v(2 * p, 0) | v(2 * p + 1, 0) << 16;
             }
 #pragma unroll
-            for (int n = 0; n < NV; n++) {
-                uint4 x, y;
-                uint32_t* const xs[4] = {&x.x, &x.y, &x.z, &x.w};
-                uint32_t* const ys[4] = {&y.x, &y.y, &y.z, &y.w};
+            for (int n = 0; n < 4; n++) {
+                Frag x, y;
 #pragma unroll
                 for (int p = 0; p < 4; p++) {
                     if constexpr (Q4) {
-                        const f16x2 d = as_f16x2(vd[p]);
-                        const f16x2 m = nibbles((n < 4 ? lo16[p] : hi16[p]) >> (4 * (n & 3))), z = m * d;
-                        *xs[p] = as_u32(z);
+                        const f16x2 d = as_f16x2(vd(p));
+                        const f16x2 m = nibbles(both[p] >> (4 * n)), z = m * d;
+                        x.w[p] = as_u32(z);
                         if constexpr (FINE)
-                            *ys[p] = as_u32(__builtin_elementwise_fma(m, d, -z));
+                            y.w[p] = as_u32(__builtin_elementwise_fma(m, d, -z));
                     } else {
-                        *xs[p] = __builtin_amdgcn_perm(v[2 * p + 1][n >> 1], v[2 * p][n >> 1], n & 1 ? 0x07060302u : 0x05040100u);
+                        x.w[p] = __builtin_amdgcn_perm(v(2 * p + 1, n >> 1), v(2 * p, n >> 1), n & 1 ? 0x07060302u : 0x05040100u);
                     }
                 }
-                *reinterpret_cast<uint4*>(values + value_at(NV * c + n, q)) = x;
+                *reinterpret_cast<f16x8*>(values + value_at(4 * c + n, q)) = x.v;
                 if constexpr (FINE && Q4)
-                    *reinterpret_cast<uint4*>(values + lo + value_at(NV * c + n, q)) = y;
+                    *reinterpret_cast<f16x8*>(values + lo + value_at(4 * c + n, q)) = y.v;
             }
         }
     }
 };
 
 template <int D, bool Q4, bool FINE>
-__global__ void __launch_bounds__(256, FINE && Q4 && D == 128 ? 1 : 2)
+__global__ void __launch_bounds__(PROMPT_THREADS, 2)
 paged_prompt_kernel(const PagedAttentionArgs a)
 {
     constexpr int NK = D / 16, NC = D / 32;
@@ -959,32 +1006,42 @@ paged_prompt_kernel(const PagedAttentionArgs a)
     const int kv = a.cache.kv_heads, group = a.heads / kv;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
     const int64_t head_bytes = paged_head_bytes(Q4, a.cache.page_size, D);
-    Prompt prompt{a.batch, a.cache.page_shift, group, kv, 0};
-    prompt.set_share();
-    PromptItem it;
-    __shared__ int drawn;
-    int32_t* const counter = reinterpret_cast<int32_t*>(a.workspace);
-    for (;;) {
-        // whoever is done takes the next item: long ones first, so the last end together
-        if (threadIdx.x == 0)
-            drawn = atomicAdd(counter, 1);
-        __syncthreads();
-        if (!prompt.find<false>(drawn, &it))
-            return;
-        const PromptSequence& q = it.q;
+    const PromptLine line(a.batch, a.cache.page_shift, group, kv);
+    // neighbours in the line on one die (workgroup b runs on die b % 8): they
+    // go through the same keys and values, and meet in its L2
+    const int64_t worker = int64_t(blockIdx.x % 8) * (PROMPT_WORKERS / 8) + blockIdx.x / 8;
+    const int64_t begin = worker * line.share, end = begin + line.share;
+    Record record{};
+    PromptSequence q{};
+    int64_t q_start = 0, q_end = 0;
+    for (int64_t x = begin; x < end;) {
+        if (x >= q_end) {
+            if (!line.find(x, &q, &q_start))
+                break;
+            q_end = q_start + line.weight(q);
+        }
+        const int64_t head_weight = PromptLine::before(q, q.tiles);
+        const int kvh = __builtin_amdgcn_readfirstlane(int(quotient(x - q_start, head_weight)));
+        const int64_t y = x - q_start - kvh * head_weight;
+        const int tile = __builtin_amdgcn_readfirstlane(int(PromptLine::tile_at(q, y)));
+        const int64_t weight = PromptLine::tile_weight(q, tile), lo = y - PromptLine::before(q, tile);
+        const int64_t hi = min(weight, lo + (end - x));
+        x += hi - lo;
+        if (lo == 0 && hi < weight)
+            record = {int(line.worker_of(x + weight - hi - 1) - worker) + 1, q.first, q.count, tile * PROMPT_ROWS, kvh, {}};
         const bool wrong = q.length < 0;
-        const int row0 = it.tile * PROMPT_ROWS;
+        const int row0 = tile * PROMPT_ROWS;
         const int packed = row0 + 32 * wave + r, i = packed / group;
         const bool live = i < q.count;
         const int64_t row = int64_t(q.first) + i;
-        const int head = it.kvh * group + packed % group;
+        const int head = kvh * group + packed % group;
         const int limit = live && !wrong ? q.length - q.count + i : -1;
         const int last_row = min(q.count - 1, (row0 + PROMPT_ROWS - 1) / group);
         const int most = __builtin_amdgcn_readfirstlane(wrong ? -1 : q.length - q.count + last_row);
         const int least = __builtin_amdgcn_readfirstlane(q.length - q.count + row0 / group);
         const int units = (most + UNIT) / UNIT;           // of this tile, 0 where no row sees anything
-        const int unit0 = __builtin_amdgcn_readfirstlane(int(int64_t(units) * it.part / q.parts));
-        const int unit1 = __builtin_amdgcn_readfirstlane(int(int64_t(units) * (it.part + 1) / q.parts));
+        const int unit0 = __builtin_amdgcn_readfirstlane(int(quotient(units * lo, weight)));
+        const int unit1 = __builtin_amdgcn_readfirstlane(int(quotient(units * hi, weight)));
         const int32_t* const table = a.batch.table + int64_t(q.index) * a.batch.max_pages;
 
         // queries of this lane's row: piece 2 k + h of its values for product k
@@ -1015,7 +1072,7 @@ paged_prompt_kernel(const PagedAttentionArgs a)
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 acc[n][e] = 0.0f;
-        float ref = -INFINITY, sum = 0.0f;
+        float ref = 0.0f, gate = -INFINITY, sum = 0.0f;
         // Places of the lane's fragments: rows 32 apart share their swizzle,
         // columns 32 apart differ in it by 2 n, so eight and four offsets do.
         int key_of[NK], value_of[4];
@@ -1050,55 +1107,105 @@ paged_prompt_kernel(const PagedAttentionArgs a)
         __syncthreads();                                  // the item before is done with LDS
         if (threadIdx.x < 6)
             (&odd[0][0])[threadIdx.x] = 0;
-        __syncthreads();
+        // The loop begins with a unit before the first one, whose scores are
+        // -inf and whose values are zeros: what it does for the next units
+        // (storing, loading, the scores) need not stand here once more.
+#pragma unroll 1
+        for (int p = 1; p < PLANES; p += 2)
+            for (int at = 16 * threadIdx.x; at < PLANE; at += 16 * PROMPT_THREADS)
+                *reinterpret_cast<uint4*>(lds[(unit0 + 1) & 1] + p * PLANE + at) = make_uint4(0, 0, 0, 0);
         if (unit0 < unit1) {
             pages_of(unit0, pages);
-            lost = lost_of(pages);
-            raw.load(a, it.kvh, unit0 * UNIT, pages, head_bytes);
-            raw.store(lds[unit0 & 1], lds[unit0 & 1] + PLANE, 2 * PLANE, partial(unit0), odd[unit0 % 3]);
-            if (unit0 + 1 < unit1) {
-                pages_of(unit0 + 1, pages);
-                lost_next = lost_of(pages);
-                raw.load(a, it.kvh, (unit0 + 1) * UNIT, pages, head_bytes);
-            }
+            lost_next = lost_of(pages);
+            raw.load(a, kvh, unit0 * UNIT, pages, head_bytes);
         }
         __syncthreads();
-        for (int u = unit0; u < unit1; u++) {
-            const char* const plane = lds[u & 1];
-            const int base = u * UNIT;
-            // (read for unit u - 1, next written for unit u + 2)
-            if (threadIdx.x < 2)
-                odd[(u + 2) % 3][threadIdx.x] = 0;
-            f32x16 s[2];
+
+        // Fragments are read two groups ahead of their products; the order is
+        // pinned, or the compiler reads each right before it is used.
+        constexpr int GROUP = FINE ? 1 : 2, SETS = FINE ? 2 : 3;
+        f16x8 f[SETS][GROUP], fl[SETS][FINE && Q4 ? GROUP : 1];
+        f32x16 s[2];
+        Frag pf[2][2], pl[2][2];
+        auto read = [&](const char* at, int set, int i) {
+            f[set][i] = *reinterpret_cast<const f16x8*>(at);
+            if constexpr (FINE && Q4)
+                fl[set][i] = *reinterpret_cast<const f16x8*>(at + 2 * PLANE);
+        };
+        auto column = [](int p) { return 2 * (p >> 3) + (p & 1); };
+        auto read_keys = [&](int u, int g, int set) {
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    s[b][e] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < NK; k++) {
-                    const f16x8 kf = *reinterpret_cast<const f16x8*>(plane + key_of[k] + 32 * b * 2 * D);
-                    if constexpr (FINE && Q4) {
-                        const f16x8 kl = *reinterpret_cast<const f16x8*>(plane + key_of[k] + 2 * PLANE + 32 * b * 2 * D);
-                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qf[k], s[b], 0, 0, 0);
-                    }
-                    if constexpr (FINE)
-                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], s[b], 0, 0, 0);
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[k], s[b], 0, 0, 0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < GROUP; i++) {
+                const int p = g * GROUP + i;
+                read(lds[u & 1] + key_of[p >> 1] + 32 * (p & 1) * 2 * D, set, i);
             }
-            // element e of block b: position base + 32 b + 8 (e / 4) + 4 h + e % 4
-            if (partial(u) || lost) {
-                const uint32_t odd0 = odd[u % 3][0], odd1 = odd[u % 3][1];
+        };
+        auto read_values = [&](int u, int g, int set) {
+#pragma unroll
+            for (int i = 0; i < GROUP; i++) {
+                const int p = g * GROUP + i, n = column(p);
+                read(lds[u & 1] + value_of[(p >> 1 & 3) ^ (n & 3)] + 32 * n * 128, set, i);
+            }
+        };
+        // Two accumulators take turns, so a product does not wait for the one
+        // before it: product p of the scores is of block p % 2 and values p / 2,
+        // of the sums of columns column(p) and positions p / 2 % 4.
+        constexpr int AHEAD = SETS - 1;
+        constexpr int SCORES = 2 * NK / GROUP, SUMS = 4 * NC / GROUP;      // groups of a unit
+        // The scores of unit u, whose first fragments are in sets `set` and on.  They
+        // start from 0, or from -inf where a row does not see the position.
+        // Element e of block b: position base + 32 b + 8 (e / 4) + 4 h + e % 4.
+        auto scores = [&](int u, int set) {
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                s[0][e] = s[1][e] = -ref;
+            if (partial(u)) {
+                // (a new value each time, or 32 positions live through the loop)
+                int first = 4 * h;
+                asm volatile("" : "+v"(first));
+                const int seen = limit - u * UNIT - first;
 #pragma unroll
                 for (int b = 0; b < 2; b++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int in = 8 * (e >> 2) + 4 * h + (e & 3);
-                        const bool nan = ((b ? odd1 : odd0) >> in & 1) || (lost >> (2 * b + (e >> 3)) & 1);
-                        s[b][e] = base + 32 * b + in > limit ? -INFINITY : nan ? NAN : s[b][e];
-                    }
+                    for (int e = 0; e < 16; e++)
+                        s[b][e] = 32 * b + 8 * (e >> 2) + (e & 3) > seen ? -INFINITY : -ref;
+            }
+#pragma unroll
+            for (int g = 0; g < SCORES; g++) {
+                if (g + AHEAD < SCORES)
+                    read_keys(u, g + AHEAD, (set + g + AHEAD) % SETS);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < GROUP; i++) {
+                    const int k = (g * GROUP + i) >> 1, b = (g * GROUP + i) & 1, at = (set + g) % SETS;
+                    if constexpr (FINE && Q4)
+                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[at][i], qf[k], s[b], 0, 0, 0);
+                    if constexpr (FINE)
+                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[at][i], ql[k], s[b], 0, 0, 0);
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[at][i], qf[k], s[b], 0, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // The matrix cores and the vector units take turns: waves 4..7 run half
+        // a unit behind waves 0..3, so each SIMD has one wave at its products
+        // while the other is at its exponentials and conversions.  Every
+        // half ends at a barrier.  Waves 0..3 convert keys, a half before anyone
+        // needs them; waves 4..7 values, which are needed two halves later.
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            s[0][e] = s[1][e] = -INFINITY;
+        for (int u = unit0 - 1; u < unit1; u++) {
+            const int base = u * UNIT;
+            if (u >= unit0 && (partial(u) || lost)) {
+                // a row that sees a position without a page, or with a key or
+                // value that is not finite (0 in LDS), is NaN
+                const uint32_t bad0 = odd[u % 3][0] | (lost & 1 ? 0xFFFFu : 0u) | (lost & 2 ? 0xFFFF0000u : 0u);
+                const uint32_t bad1 = odd[u % 3][1] | (lost & 4 ? 0xFFFFu : 0u) | (lost & 8 ? 0xFFFF0000u : 0u);
+                const int seen = limit - base;
+                const uint32_t see0 = seen >= 31 ? ~0u : seen < 0 ? 0u : (2u << seen) - 1;
+                const uint32_t see1 = seen >= 63 ? ~0u : seen < 32 ? 0u : (2u << (seen - 32)) - 1;
+                sum = (bad0 & see0) | (bad1 & see1) ? NAN : sum;
             }
             float top = -INFINITY;
 #pragma unroll
@@ -1110,44 +1217,49 @@ paged_prompt_kernel(const PagedAttentionArgs a)
                 auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
                 top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
             }
-            // (a branch around the rescaling costs more: the accumulators then
-            // live in two places at its end, and registers spill)
-            const float n = fmaxf(ref, top), at = fmaxf(n, -3.4028235e38f);
-            const float fade = __builtin_amdgcn_exp2f(ref - at);
-            ref = n;
-            sum *= fade;
+            if (__any(top > gate)) {
+                const float by = top > gate ? top : 0.0f, fade = __builtin_amdgcn_exp2f(-by);
+                gate = top > gate ? REFERENCE_SLACK : gate;
+                ref += by;
+                sum *= fade;
 #pragma unroll
-            for (int n2 = 0; n2 < NC; n2++)
-                acc[n2] *= fade;
-            Frag pf[2][2], pl[2][2];
+                for (int n = 0; n < NC; n++)
+                    acc[n] *= fade;
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+                    s[b] -= by;
+            }
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) {
-                    const float x = __builtin_amdgcn_exp2f(s[b][e] - at), y = __builtin_amdgcn_exp2f(s[b][e + 1] - at);
-                    sum += x + y;
+                    const float x = __builtin_amdgcn_exp2f(s[b][e]), y = __builtin_amdgcn_exp2f(s[b][e + 1]);
                     const f16x2 p = {_Float16(x), _Float16(y)};
                     pf[b][e >> 3].w[(e & 7) >> 1] = as_u32(p);
+                    sum = FINE ? sum + (x + y) : __builtin_amdgcn_fdot2(p, f16x2{_Float16(1.0f), _Float16(1.0f)}, sum, false);
                     if constexpr (FINE)
                         pl[b][e >> 3].w[(e & 7) >> 1] = as_u32(f16x2{_Float16(x - float(p[0])), _Float16(y - float(p[1]))});
                 }
-            __builtin_amdgcn_sched_barrier(0);
+            // (last read for unit u - 1, next marked for unit u + 2)
+            if (threadIdx.x < 2)
+                odd[(u + 2) % 3][threadIdx.x] = 0;
+            read_values(u, 0, 0);
+            if constexpr (AHEAD > 1)
+                read_values(u, 1, 1);
 #pragma unroll
-            for (int n = 0; n < NC; n++) {
+            for (int g = 0; g < SUMS; g++) {
+                if (g + AHEAD < SUMS)
+                    read_values(u, g + AHEAD, (g + AHEAD) % SETS);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int b = 0; b < 2; b++)
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const char* const at_v = plane + value_of[(2 * b + k) ^ (n & 3)] + 32 * n * 128;
-                        const f16x8 vf = *reinterpret_cast<const f16x8*>(at_v);
-                        if constexpr (FINE && Q4) {
-                            const f16x8 vl = *reinterpret_cast<const f16x8*>(at_v + 2 * PLANE);
-                            acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, pf[b][k].v, acc[n], 0, 0, 0);
-                        }
-                        if constexpr (FINE)
-                            acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[b][k].v, acc[n], 0, 0, 0);
-                        acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[b][k].v, acc[n], 0, 0, 0);
-                    }
+                for (int i = 0; i < GROUP; i++) {
+                    const int p = g * GROUP + i, n2 = column(p), b = (p >> 2) & 1, k = (p >> 1) & 1;
+                    if constexpr (FINE && Q4)
+                        acc[n2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[g % SETS][i], pf[b][k].v, acc[n2], 0, 0, 0);
+                    if constexpr (FINE)
+                        acc[n2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[g % SETS][i], pl[b][k].v, acc[n2], 0, 0, 0);
+                    acc[n2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[g % SETS][i], pf[b][k].v, acc[n2], 0, 0, 0);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
             lost = lost_next;
@@ -1157,20 +1269,23 @@ paged_prompt_kernel(const PagedAttentionArgs a)
                 if (u + 2 < unit1) {
                     pages_of(u + 2, pages);
                     lost_next = lost_of(pages);
-                    raw.load(a, it.kvh, (u + 2) * UNIT, pages, head_bytes);
+                    raw.load(a, kvh, (u + 2) * UNIT, pages, head_bytes);
                 }
             }
             __syncthreads();
+            read_keys(u + 1, 0, 0);
+            if constexpr (AHEAD > 1)
+                read_keys(u + 1, 1, 1);
+            scores(u + 1, 0);
         }
         {
             auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
             sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
         }
-        // (the next item's first barrier is behind everybody's last look at `drawn`)
-        if (!live)
-            continue;
         // element e of acc[n]: column 32 n + 8 (e / 4) + 4 h + e % 4
-        if (q.parts == 1) {
+        if (lo == 0 && hi == weight) {
+            if (!live)
+                continue;
             const float inv = wrong ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
             const int64_t out = (row * a.heads + head) * D + 4 * h;
 #pragma unroll
@@ -1179,71 +1294,81 @@ paged_prompt_kernel(const PagedAttentionArgs a)
                 for (int e = 0; e < 16; e += 4)
                     store_out(a, out + 32 * n + 2 * e, acc[n][e] * inv, acc[n][e + 1] * inv, acc[n][e + 2] * inv,
                               acc[n][e + 3] * inv);
-        } else {
-            float* const slot = a.workspace + prompt_workspace(D) + (it.slot + it.part) * prompt_slot_floats(D);
-            float* const out = slot + (32 * wave + r) * D + 4 * h;
+        } else if (row0 + 32 * wave < q.count * group) {
+            float* const slot = a.workspace + prompt_workspace(D) + (2 * worker + (lo == 0)) * prompt_slot_floats(D);
+            f32x4* const out = reinterpret_cast<f32x4*>(slot) + wave * (4 * NC * 64) + lane;
 #pragma unroll
             for (int n = 0; n < NC; n++)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4)
-                    *reinterpret_cast<f32x4*>(out + 32 * n + 2 * e) = f32x4{acc[n][e], acc[n][e + 1], acc[n][e + 2], acc[n][e + 3]};
+                    out[(4 * n + e / 4) * 64] = f32x4{acc[n][e], acc[n][e + 1], acc[n][e + 2], acc[n][e + 3]};
             if (h == 0) {
-                slot[PROMPT_ROWS * D + 32 * wave + r] = wrong ? NAN : ref;
+                slot[PROMPT_ROWS * D + 32 * wave + r] = sum == 0.0f ? -INFINITY : ref;
                 slot[PROMPT_ROWS * D + PROMPT_ROWS + 32 * wave + r] = wrong ? NAN : sum;
             }
         }
     }
+    if (threadIdx.x == 0)
+        records(a.workspace)[WAVES + worker] = record;
 }
 
-// Joins the parts of split tiles, 32 rows a workgroup, four values a lane.
+// Joins the tiles that several workers share: workgroups y the one that
+// begins in worker y and ends behind it, each four pieces of 64 lanes' values.
 template <int D>
 __global__ void __launch_bounds__(256)
 paged_prompt_merge_kernel(const PagedAttentionArgs a)
 {
-    constexpr int ROWS = 1024 / D;
-    const int kv = a.cache.kv_heads, group = a.heads / kv;
-    Prompt prompt{a.batch, a.cache.page_shift, group, kv, 0};
-    prompt.set_share();
-    PromptItem it;
-    if (!prompt.find<true>(blockIdx.x, &it) || it.q.parts == 1)
+    const Record todo = records(a.workspace)[WAVES + blockIdx.y];
+    if (todo.parts == 0)
         return;
-    for (int r = int(blockIdx.y) * 32 + int(threadIdx.x) / (D / 4); r < int(blockIdx.y) * 32 + 32; r += ROWS) {
-    const int col = 4 * (int(threadIdx.x) % (D / 4));
-    const int packed = it.tile * PROMPT_ROWS + r, i = packed / group;
-    if (i >= it.q.count)
-        return;
-    float top = -INFINITY, sum = 0.0f;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p = 0; p < it.q.parts; p++) {
-        const float* const slot = a.workspace + prompt_workspace(D) + (it.slot + p) * prompt_slot_floats(D);
-        const float m = slot[PROMPT_ROWS * D + r], l = slot[PROMPT_ROWS * D + PROMPT_ROWS + r];
-        const f32x4 v = *reinterpret_cast<const f32x4*>(slot + r * D + col);
-        const float n = fmaxf(top, m), at = fmaxf(n, -3.4028235e38f);
-        const float f = __builtin_amdgcn_exp2f(top - at), g = __builtin_amdgcn_exp2f(m - at);
-        sum = sum * f + l * g;
-        acc = acc * f + v * g;
-        top = n;
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    store_out(a, ((int64_t(it.q.first) + i) * a.heads + it.kvh * group + packed % group) * D + col, acc[0] * inv, acc[1] * inv,
-              acc[2] * inv, acc[3] * inv);
+    constexpr int PIECES = D / 8;                         // of 32 rows
+    const int group = a.heads / a.cache.kv_heads;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const float* const slot = a.workspace + prompt_workspace(D) + 2 * int64_t(blockIdx.y) * prompt_slot_floats(D);
+    auto take = [&](Joined& sum, int piece, int r, int p) {
+        // (a tile's own worker has it in its second slot, the others in their first)
+        const float* const at = slot + (2 * p + (p == 0)) * int64_t(prompt_slot_floats(D));
+        sum.take(at[PROMPT_ROWS * D + r], at[PROMPT_ROWS * D + PROMPT_ROWS + r], reinterpret_cast<const f32x4*>(at)[piece * 64 + lane]);
+    };
+    auto finish = [&](const Joined& sum, int piece, int r) {
+        const int packed = todo.row0 + r, i = packed / group;
+        if (i >= todo.count)
+            return;
+        const int col = 8 * (piece % PIECES) + 4 * (lane >> 5);
+        const float inv = sum.sum == 0.0f ? 0.0f : 1.0f / sum.sum;
+        store_out(a, ((int64_t(todo.first) + i) * a.heads + todo.kvh * group + packed % group) * D + col, sum.acc[0] * inv,
+                  sum.acc[1] * inv, sum.acc[2] * inv, sum.acc[3] * inv);
+    };
+    // Few slots: a piece a wave.  Many: its waves take them in turn.
+    const bool turns = todo.parts > 4;
+#pragma unroll 1
+    for (int k = 0; k < (turns ? 4 : 1); k++) {
+        const int piece = 4 * int(blockIdx.x) + (turns ? k : wave), r = 32 * (piece / PIECES) + (lane & 31);
+        // (rows that are not in the sequence were not stored)
+        if (todo.row0 + 32 * (piece / PIECES) >= todo.count * group)
+            return;
+        Joined sum;
+#pragma unroll 4
+        for (int p = turns ? wave : 0; p < todo.parts; p += turns ? 4 : 1)
+            take(sum, piece, r, p);
+        if (!turns || join_waves(sum))
+            finish(sum, piece, r);
+        if (turns)
+            __syncthreads();
     }
 }
 
 template <int D, bool Q4, bool FINE>
 hipError_t launch(const PagedAttentionArgs& a, hipStream_t s)
 {
-    const int group = a.heads / a.cache.kv_heads, kv = a.cache.kv_heads;
-    const int64_t packed = int64_t(a.batch.rows) * group;
-    const int some = min(a.batch.rows, a.batch.sequences);                       // sequences with rows, at most
+    const int group = a.heads / a.cache.kv_heads;
+    const int64_t most = int64_t(a.batch.max_rows) * group;       // packed rows of a sequence
+    const unsigned tile_rows = unsigned(min(int64_t(TILE_ROWS), most));
     paged_attention_kernel<D, Q4, FINE><<<WAVES / 4, 256, 0, s>>>(a);
-    const int tile_rows = int(min(int64_t(TILE_ROWS), int64_t(a.batch.max_rows) * group));
-    paged_merge_kernel<D><<<dim3(unsigned(min(packed / TILE_ROWS + some, int64_t(FEW_ROWS / TILE_ROWS) * some) * kv), unsigned((tile_rows + 256 / D - 1) / (256 / D))),
-                            256, 0, s>>>(a);
-    if (int64_t(a.batch.max_rows) * group > FEW_ROWS) {
-        paged_prompt_kernel<D, Q4, FINE><<<PROMPT_WORKERS, 256, 0, s>>>(a);
-        const int64_t tiles = packed / PROMPT_ROWS + some;
-        paged_prompt_merge_kernel<D><<<dim3(unsigned(tiles * kv), PROMPT_ROWS / 32), 256, 0, s>>>(a);
+    paged_merge_kernel<D><<<dim3(WAVES, (tile_rows + 256 / D - 1) / (256 / D)), 256, 0, s>>>(a);
+    if (most > FEW_ROWS) {
+        paged_prompt_kernel<D, Q4, FINE><<<PROMPT_WORKERS, PROMPT_THREADS, 0, s>>>(a);
+        paged_prompt_merge_kernel<D><<<dim3(PROMPT_ROWS * D / 1024, PROMPT_WORKERS), 256, 0, s>>>(a);
     }
     return hipGetLastError();
 }
@@ -1261,7 +1386,7 @@ hipError_t launch(const PagedAttentionArgs& a, hipStream_t s)
 
 int64_t paged_attention_workspace_floats(int, int, int head)
 {
-    return prompt_workspace(head) + int64_t(PROMPT_SLOTS) * prompt_slot_floats(head);
+    return prompt_workspace(head) + int64_t(2 * PROMPT_WORKERS) * prompt_slot_floats(head);
 }
 
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s)
