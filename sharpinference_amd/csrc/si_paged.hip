@@ -2,8 +2,8 @@
 // the way), and rows of the pages back as FP32.
 //
 // A workgroup serves one row of the batch: its waves take the row's heads,
-// two neighbouring values a lane, so a 4-bit block of 32 values is one
-// 16-lane row of the wave and its largest value a DPP reduction.  The
+// four neighbouring values a lane, so a 4-bit block of 32 values is eight
+// lanes of the wave and its largest value a DPP reduction.  The
 // rotation runs in FP64 (angle, cosine, sine, products; rounded to FP32
 // once): positions of any size keep their angle, and a key's codes do not
 // depend on which kernel rotated it.
@@ -60,47 +60,90 @@ __device__ __forceinline__ Place find_place(const PagedBatch& b, const PagedCach
     return r;
 }
 
-// The 4-bit block that 16 lanes hold, two values each: scale = the value of
+// The 4-bit block that eight lanes hold, four values each: scale = the value of
 // largest magnitude (the first of them) / -8 in FP16, code = value / scale
 // rounded to the nearest (ties to even) + 8.  A value that FP16 could not
 // hold makes the whole block NaN.
-__device__ __forceinline__ void block_codes(float v0, float v1, int lane, uint32_t* codes, uint16_t* scale)
+__device__ __forceinline__ void block_codes(const float* v, int lane, uint16_t* codes, uint16_t* scale)
 {
-    const float a0 = fabsf(v0), a1 = fabsf(v1);
-    const float top = row_max<16>(fmaxf(a0, a1));
-    const bool has = a0 == top || a1 == top;
-    const bool odd = !(a0 <= 65504.0f) || !(a1 <= 65504.0f);   // NaN too
-    const uint32_t shift = lane & 48;
-    const uint32_t holders = uint32_t(__ballot(has) >> shift) & 0xFFFFu;
-    const uint32_t bad = uint32_t(__ballot(odd) >> shift) & 0xFFFFu;
-    const float mine = a0 == top ? v0 : v1;
+    float mine = v[0];
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        mine = fabsf(v[j]) > fabsf(mine) ? v[j] : mine;        // (the first of equal ones stays)
+        odd |= !(fabsf(v[j]) <= 65504.0f);                     // NaN too
+    }
+    const float top = row_max<8>(fabsf(mine));
+    const uint32_t shift = lane & 56;
+    const uint32_t holders = uint32_t(__ballot(fabsf(mine) == top) >> shift) & 0xFFu;
+    const uint32_t bad = uint32_t(__ballot(odd) >> shift) & 0xFFu;
     const float first = __shfl(mine, int(shift) + (holders ? __ffs(holders) - 1 : 0));
     uint16_t d = __half_as_ushort(__float2half_rn(first / -8.0f));
     const float df = __half2float(__ushort_as_half(d));
-    uint32_t q0 = 8, q1 = 8;
+    uint32_t q = 0x8888;
     if (bad) {
         d = 0x7E00;
     } else if (df == 0.0f) {
         d = 0;                                                 // a block of zeros, whatever their signs
     } else {
-        q0 = uint32_t(int(fminf(fmaxf(rintf(v0 / df) + 8.0f, 0.0f), 15.0f)));
-        q1 = uint32_t(int(fminf(fmaxf(rintf(v1 / df) + 8.0f, 0.0f), 15.0f)));
+        q = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            q |= uint32_t(int(fminf(fmaxf(rintf(v[j] / df) + 8.0f, 0.0f), 15.0f))) << (4 * j);
     }
-    *codes = q0 | q1 << 4;
+    *codes = uint16_t(q);
     *scale = d;
 }
+
+// Values beside each other (qkv and query are aligned to 4 bytes only).
+typedef float float4_4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// The batch's row of workgroup x: the rows of a page on one die (workgroup b
+// runs on die b % 8), whose L2 joins their 64-byte rows and 2-byte scales to
+// whole lines.
+__device__ __forceinline__ int row_of_workgroup() { return int(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8); }
 
 template <int D, bool Q4>
 __global__ void __launch_bounds__(256)
 paged_append_kernel(const PagedAppendArgs a, int per_group)
 {
-    constexpr int PER = 128 / D;                   // heads a wave serves at once
+    constexpr int PER = 256 / D;                   // heads a wave serves at once
     __shared__ double turn[2][64];                 // cos, sin of the row's pairs
-    const int t = blockIdx.x;
+    const int t = row_of_workgroup();
+    if (t >= a.batch.rows)
+        return;
     const Place at = find_place(a.batch, a.cache, t);
     if (at.page < 0)
         return;                                    // the whole workgroup
     const int half = a.rotary >> 1;
+    const int lane = threadIdx.x & 63;
+    const int kv = a.cache.kv_heads, total = a.heads + 2 * kv;
+    const int i0 = 4 * (lane % (D / 4));           // this lane's values i0 .. i0 + 3 of its head
+    auto partner = [&](int i) { return i < half ? i + half : i < 2 * half ? i - half : i; };
+    const float* row = a.qkv + int64_t(t) * total * D;
+    const int64_t head_bytes = paged_head_bytes(Q4, a.cache.page_size, D);
+    const int end = min(total, (int(blockIdx.y) + 1) * per_group);
+    // A lane's values and their partners; asked for before they are needed.
+    float4_4 own, other;
+    auto load = [&](int h0) {
+        // (a lane without a head works on the last one and stores nothing)
+        const int h = min(h0 + lane / (D / 4), end - 1);
+        const float* const x = row + int64_t(h) * D;
+        own = *reinterpret_cast<const float4_4*>(x + i0);
+        other = own;
+        if (h < a.heads + kv) {
+            if (half & 3) {                        // the four may lie on different sides
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    other[j] = x[partner(i0 + j)];
+            } else {
+                other = *reinterpret_cast<const float4_4*>(x + partner(i0));
+            }
+        }
+    };
+    int h0 = int(blockIdx.y) * per_group + int(threadIdx.x >> 6) * PER;
+    if (h0 < end)
+        load(h0);
     if (int(threadIdx.x) < half) {
         double s, c;
         sincos(double(at.position) * double(a.frequencies[threadIdx.x]), &s, &c);
@@ -108,53 +151,54 @@ paged_append_kernel(const PagedAppendArgs a, int per_group)
         turn[1][threadIdx.x] = s * double(a.rope_scale);
     }
     __syncthreads();
-    const int lane = threadIdx.x & 63;
-    const int kv = a.cache.kv_heads, total = a.heads + 2 * kv;
-    const int i0 = 2 * (lane % (D / 2));           // this lane's values i0, i0 + 1 of its head
-    const float* row = a.qkv + int64_t(t) * total * D;
-    const int64_t head_bytes = paged_head_bytes(Q4, a.cache.page_size, D);
-    const int end = min(total, (int(blockIdx.y) + 1) * per_group);
-    for (int h0 = int(blockIdx.y) * per_group + int(threadIdx.x >> 6) * PER; h0 < end; h0 += 4 * PER) {
-        const int h = h0 + lane / (D / 2);
-        // (a lane without a head works on the last one and stores nothing)
-        const float* x = row + int64_t(min(h, end - 1)) * D;
-        float v[2];
-        const bool turned = h < a.heads + kv;
+    // the lane's turns: the same for every head
+    double c[4] = {}, s[4] = {};
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int i = i0 + j;
-            v[j] = x[i];
-            if (turned && i < 2 * half) {
-                const bool low = i < half;
-                const int pair = low ? i : i - half;
-                const double own = v[j], other = x[low ? i + half : pair];
-                const double c = turn[0][pair], s = turn[1][pair];
-                v[j] = float(low ? own * c - other * s : own * c + other * s);
-            }
+    for (int j = 0; j < 4; j++) {
+        const int i = i0 + j;
+        if (i < 2 * half) {
+            const int pair = i < half ? i : i - half;
+            c[j] = turn[0][pair];
+            s[j] = i < half ? -turn[1][pair] : turn[1][pair];
+        }
+    }
+    for (; h0 < end; h0 += 4 * PER) {
+        const int h = h0 + lane / (D / 4);
+        float4_4 v = own;
+        const float4_4 w = other;
+        if (h0 + 4 * PER < end)
+            load(h0 + 4 * PER);
+        if (h < a.heads + kv) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (i0 + j < 2 * half)
+                    v[j] = float(double(v[j]) * c[j] + double(w[j]) * s[j]);
         }
         if (h >= end)
-            v[0] = v[1] = 0.0f;
-        uint32_t codes = 0;
-        uint16_t scale = 0;
+            v = float4_4{0.0f, 0.0f, 0.0f, 0.0f};
+        uint16_t codes = 0, scale = 0;
         if constexpr (Q4)
-            block_codes(v[0], v[1], lane, &codes, &scale);
+            if (h0 + PER > a.heads) {              // (some lane has a key or value)
+                const float x[4] = {v.x, v.y, v.z, v.w};
+                block_codes(x, lane, &codes, &scale);
+            }
         if (h >= end)
             continue;
         if (h < a.heads) {
-            float* q = a.query + (int64_t(t) * a.heads + h) * D + i0;
-            q[0] = v[0];
-            q[1] = v[1];
+            *reinterpret_cast<float4_4*>(a.query + (int64_t(t) * a.heads + h) * D + i0) = v;
             continue;
         }
         const int kvh = h - a.heads < kv ? h - a.heads : h - a.heads - kv;
         char* page = (h - a.heads < kv ? a.cache.keys : a.cache.values) + (at.page * kv + kvh) * head_bytes;
         if constexpr (Q4) {
-            page[at.slot * (D / 2) + i0 / 2] = char(codes);
-            if ((lane & 15) == 0)
+            reinterpret_cast<uint16_t*>(page)[at.slot * (D / 4) + i0 / 4] = codes;
+            if ((lane & 7) == 0)
                 reinterpret_cast<uint16_t*>(page + a.cache.page_size * (D / 2))[(i0 / 32) * a.cache.page_size + at.slot] = scale;
         } else {
-            reinterpret_cast<__half2*>(page)[at.slot * (D / 2) + i0 / 2] =
-                __halves2half2(__float2half_rn(v[0]), __float2half_rn(v[1]));
+            const __half2 lo = __halves2half2(__float2half_rn(v.x), __float2half_rn(v.y));
+            const __half2 hi = __halves2half2(__float2half_rn(v.z), __float2half_rn(v.w));
+            reinterpret_cast<uint2*>(page)[at.slot * (D / 4) + i0 / 4] =
+                make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
         }
     }
 }
@@ -163,41 +207,48 @@ template <int D, bool Q4>
 __global__ void __launch_bounds__(256)
 paged_read_kernel(const PagedBatch b, const PagedCache c, float* keys, float* values)
 {
-    const int t = blockIdx.x;
+    const int t = row_of_workgroup();
+    if (t >= b.rows)
+        return;
     const Place at = find_place(b, c, t);
     if (!at.live)
         return;
     const int64_t head_bytes = paged_head_bytes(Q4, c.page_size, D);
-    const int pairs = c.kv_heads * (D / 2);
-    for (int i = threadIdx.x; i < 2 * pairs; i += 256) {
-        const int j = i < pairs ? i : i - pairs, h = j / (D / 2), e = j % (D / 2);
-        float2 v = make_float2(NAN, NAN);
+    const int quads = c.kv_heads * (D / 4);
+    for (int i = threadIdx.x; i < 2 * quads; i += 256) {
+        const int j = i < quads ? i : i - quads, h = j / (D / 4), e = j % (D / 4);
+        float4_4 v = {NAN, NAN, NAN, NAN};
         if (at.page >= 0) {
-            const char* page = (i < pairs ? c.keys : c.values) + (at.page * c.kv_heads + h) * head_bytes;
+            const char* page = (i < quads ? c.keys : c.values) + (at.page * c.kv_heads + h) * head_bytes;
             if constexpr (Q4) {
-                const uint32_t q = static_cast<uint8_t>(page[at.slot * (D / 2) + e]);
+                const uint32_t q = reinterpret_cast<const uint16_t*>(page)[at.slot * (D / 4) + e];
                 const float d = __half2float(
-                    reinterpret_cast<const __half*>(page + c.page_size * (D / 2))[(e / 16) * c.page_size + at.slot]);
-                v = make_float2(float(int(q & 15) - 8) * d, float(int(q >> 4) - 8) * d);
+                    reinterpret_cast<const __half*>(page + c.page_size * (D / 2))[(e / 8) * c.page_size + at.slot]);
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+                    v[n] = float(int(q >> (4 * n) & 15) - 8) * d;
             } else {
-                v = __half22float2(reinterpret_cast<const __half2*>(page)[at.slot * (D / 2) + e]);
+                const uint2 q = reinterpret_cast<const uint2*>(page)[at.slot * (D / 4) + e];
+                const float2 lo = __half22float2(__builtin_bit_cast(__half2, q.x)), hi = __half22float2(__builtin_bit_cast(__half2, q.y));
+                v = float4_4{lo.x, lo.y, hi.x, hi.y};
             }
         }
-        float* out = (i < pairs ? keys : values) + (int64_t(t) * pairs + j) * 2;
-        out[0] = v.x;
-        out[1] = v.y;
+        *reinterpret_cast<float4_4*>((i < quads ? keys : values) + (int64_t(t) * quads + j) * 4) = v;
     }
 }
+
+// as many rows for each die
+unsigned workgroups(int rows) { return (unsigned(rows) + 7) / 8 * 8; }
 
 }  // namespace
 
 hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s)
 {
-    // few rows: a row's heads over several workgroups, two for each wave
+    // few rows: a row's heads over several workgroups
     const int total = a.heads + 2 * a.cache.kv_heads;
-    const int two = 2 * 4 * (128 / a.cache.head);
-    const int per_group = a.batch.rows < 512 ? two : (total + two - 1) / two * two;
-    const dim3 grid(unsigned(a.batch.rows), unsigned((total + per_group - 1) / per_group));
+    const int one = 4 * (256 / a.cache.head);
+    const int per_group = a.batch.rows < 512 ? one : (total + one - 1) / one * one;
+    const dim3 grid(workgroups(a.batch.rows), unsigned((total + per_group - 1) / per_group));
     if (a.cache.head == 128) {
         if (a.cache.q4)
             paged_append_kernel<128, true><<<grid, 256, 0, s>>>(a, per_group);
@@ -216,14 +267,14 @@ hipError_t launch_paged_read(const PagedBatch& b, const PagedCache& c, float* ke
 {
     if (c.head == 128) {
         if (c.q4)
-            paged_read_kernel<128, true><<<unsigned(b.rows), 256, 0, s>>>(b, c, keys, values);
+            paged_read_kernel<128, true><<<workgroups(b.rows), 256, 0, s>>>(b, c, keys, values);
         else
-            paged_read_kernel<128, false><<<unsigned(b.rows), 256, 0, s>>>(b, c, keys, values);
+            paged_read_kernel<128, false><<<workgroups(b.rows), 256, 0, s>>>(b, c, keys, values);
     } else {
         if (c.q4)
-            paged_read_kernel<64, true><<<unsigned(b.rows), 256, 0, s>>>(b, c, keys, values);
+            paged_read_kernel<64, true><<<workgroups(b.rows), 256, 0, s>>>(b, c, keys, values);
         else
-            paged_read_kernel<64, false><<<unsigned(b.rows), 256, 0, s>>>(b, c, keys, values);
+            paged_read_kernel<64, false><<<workgroups(b.rows), 256, 0, s>>>(b, c, keys, values);
     }
     return hipGetLastError();
 }
