@@ -99,21 +99,35 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b)
     return q;
 }
 
+__device__ __forceinline__ int64_t of_lane(int64_t v, int lane)
+{
+    const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(v), lane)), hi = uint32_t(__builtin_amdgcn_readlane(int(v >> 32), lane));
+    return int64_t(uint64_t(hi) << 32 | lo);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t dpp_or_zero(int64_t v)
+{
+    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROWS, 0xF, false));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(v >> 32), CTRL, ROWS, 0xF, false));
+    return int64_t(uint64_t(hi) << 32 | lo);
+}
+// Sums of the lanes up to each: within rows of 16, then over them.
 __device__ __forceinline__ int64_t wave_scan(int64_t v)
 {
-    const int lane = threadIdx.x & 63;
-#pragma unroll 1
-    for (int m = 1; m < 64; m <<= 1) {
-        const int64_t o = __shfl_up(v, m);
-        v += lane >= m ? o : 0;
-    }
+    v += dpp_or_zero<0x111, 0xF>(v);       // row_shr:1
+    v += dpp_or_zero<0x112, 0xF>(v);
+    v += dpp_or_zero<0x114, 0xF>(v);
+    v += dpp_or_zero<0x118, 0xF>(v);
+    v += dpp_or_zero<0x142, 0xA>(v);       // row_bcast:15 into rows 1 and 3
+    v += dpp_or_zero<0x143, 0xC>(v);       // row_bcast:31 into rows 2 and 3
     return v;
 }
+__device__ __forceinline__ int64_t wave_total(int64_t v) { return of_lane(wave_scan(v), 63); }
 
 __device__ __forceinline__ Sequence from_lane(const Sequence& q, int lane)
 {
-    return {__shfl(q.index, lane), __shfl(q.first, lane), __shfl(q.count, lane), __shfl(q.length, lane),
-            __shfl(q.tiles, lane), __shfl(q.units, lane)};
+    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, lane); };
+    return {of(q.index), of(q.first), of(q.count), of(q.length), of(q.tiles), of(q.units)};
 }
 
 // The work of a launch in one line: sequence after sequence, of each its KV
@@ -122,32 +136,44 @@ __device__ __forceinline__ Sequence from_lane(const Sequence& q, int lane)
 struct Line {
     const PagedBatch& b;
     int page_shift, group, kv;
+    int64_t total;             // units
+    // up to 64 sequences are looked at once: the lane's, and the units up to it
+    Sequence mine;
+    int64_t upto;
 
     __device__ __forceinline__ int64_t units_of(const Sequence& q) const { return int64_t(kv) * q.tiles * q.units; }
-    __device__ __forceinline__ int64_t total() const
+    __device__ __forceinline__ void look(int base, int64_t before)
     {
-        int64_t sum = 0;
-        for (int base = 0; base < b.sequences; base += 64)
-            sum += units_of(take_sequence(b, page_shift, group, base + int(threadIdx.x & 63)));
-        return __shfl(wave_scan(sum), 63);
+        mine = take_sequence(b, page_shift, group, base + int(threadIdx.x & 63));
+        upto = before + wave_scan(units_of(mine));
+    }
+    __device__ __forceinline__ Line(const PagedBatch& batch, int shift, int heads_per_kv, int kv_heads)
+        : b(batch), page_shift(shift), group(heads_per_kv), kv(kv_heads), total(0)
+    {
+        for (int base = 0; base < b.sequences; base += 64) {
+            look(base, total);
+            total = of_lane(upto, 63);
+        }
     }
     // The sequence that holds unit x, and the number of its first unit.
-    __device__ __forceinline__ bool at_unit(int64_t x, Sequence* q, int64_t* start) const
+    __device__ __forceinline__ bool at_unit(int64_t x, Sequence* q, int64_t* start)
     {
-        int64_t before = 0;
-        for (int base = 0; base < b.sequences; base += 64) {
-            const Sequence mine = take_sequence(b, page_shift, group, base + int(threadIdx.x & 63));
-            const int64_t upto = before + wave_scan(units_of(mine));
-            const uint64_t past = __ballot(upto > x);
-            if (past) {
-                const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-                *q = from_lane(mine, at);
-                *start = __shfl(upto - units_of(mine), at);
-                return true;
+        if (b.sequences > 64) {
+            int64_t before = 0;
+            for (int base = 0; base < b.sequences; base += 64) {
+                look(base, before);
+                before = of_lane(upto, 63);
+                if (before > x)
+                    break;
             }
-            before = __shfl(upto, 63);
         }
-        return false;
+        const uint64_t past = __ballot(upto > x);
+        if (!past)
+            return false;
+        const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+        *q = from_lane(mine, at);
+        *start = of_lane(upto - units_of(mine), at);
+        return true;
     }
 };
 
@@ -505,15 +531,18 @@ __device__ __forceinline__ void store_out(const PagedAttentionArgs& a, int64_t a
 // Every wave takes an equal run of the line's units, whatever sequences they
 // lie in; tiles that are wholly its own are written out, the others left in
 // its slots for the merge.
+// A unit of 128 FP16 values a position is 128 registers a lane: two waves on a
+// SIMD would spill them (64 sequences of 500 to 16000 positions: 5.14 TB/s,
+// with one wave 5.59).
 template <int D, bool Q4, bool FINE>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, !Q4 && D == 128 ? 1 : 2)
 paged_attention_kernel(const PagedAttentionArgs a)
 {
     constexpr int NV = D / 16;
     const int kv = a.cache.kv_heads, group = a.heads / kv;
     const int64_t wave = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const Line line{a.batch, a.cache.page_shift, group, kv};
-    const int64_t total = line.total();
+    Line line(a.batch, a.cache.page_shift, group, kv);
+    const int64_t total = line.total;
     const Shares shares(total);
     const int64_t begin = wave * shares.share, end = min(total, begin + shares.share);
     Record record{};
@@ -764,9 +793,9 @@ struct PromptLine {
             tiles += int64_t(kv) * q.tiles;
             last += q.tiles ? int64_t(kv) * q.tiles * tile_weight(q, q.tiles - 1) : 0;
         }
-        total = __shfl(wave_scan(total), 63);
-        tiles = __shfl(wave_scan(tiles), 63);
-        last = __shfl(wave_scan(last), 63);
+        total = wave_total(total);
+        tiles = wave_total(tiles);
+        last = wave_total(last);
         share = max(int64_t(PROMPT_MIN) * group, (total + PROMPT_WORKERS - 1) / PROMPT_WORKERS);
         if (tiles < PROMPT_WORKERS) {
             // at most last / parts + tiles <= PROMPT_WORKERS parts
@@ -778,8 +807,8 @@ struct PromptLine {
     __device__ __forceinline__ int64_t worker_of(int64_t place) const { return quotient(place, share); }
     static __device__ __forceinline__ PromptSequence from_lane(const PromptSequence& q, int lane)
     {
-        return {__shfl(q.index, lane), __shfl(q.first, lane), __shfl(q.count, lane), __shfl(q.length, lane),
-                __shfl(q.tiles, lane), __shfl(q.a, lane),     __shfl(q.c, lane)};
+        auto of = [&](int v) { return __builtin_amdgcn_readlane(v, lane); };
+        return {of(q.index), of(q.first), of(q.count), of(q.length), of(q.tiles), of_lane(q.a, lane), of_lane(q.c, lane)};
     }
     // The sequence that holds place x, and the place of its begin.
     __device__ __forceinline__ bool find(int64_t x, PromptSequence* q, int64_t* start) const
@@ -793,10 +822,10 @@ struct PromptLine {
             if (past) {
                 const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
                 *q = from_lane(mine, at);
-                *start = __shfl(places_upto - w, at);
+                *start = of_lane(places_upto - w, at);
                 return true;
             }
-            places = __shfl(places_upto, 63);
+            places = of_lane(places_upto, 63);
         }
         return false;
     }
