@@ -853,173 +853,163 @@ __device__ __forceinline__ int value_at(int col, int piece)    // of eight posit
     return col * 128 + ((piece ^ (((col >> 1) ^ (col >> 4)) & 7)) << 4);
 }
 
-// What a thread loads of a unit.  Threads 0..255 take keys: 16-byte pieces of
-// rows; threads 256..511 values: four columns of the eight positions that
-// piece q of a column holds, 16 (q / 2) + 4 (q % 2) + {0..3, 8..11}.
+// What a lane loads of a unit.  Wave w takes eight positions' keys, an eighth of
+// a row a lane, and piece w of the values' columns, two columns a lane: positions
+// 16 (w / 2) + 4 (w % 2) + {0..3, 8..11}.  Both lie in one page, so everything
+// that changes from unit to unit is in scalar registers; the lane keeps its
+// places in the page and in LDS.  (Waves that took keys or values only: the
+// registers of both then met behind the branch, which waited for the loads
+// there and then.)
 template <int D, bool Q4, bool FINE>
 struct PromptLoad {
-    static constexpr int PIECES = Q4 ? D / 32 : D / 8;         // 16-byte pieces of a row of keys
-    static constexpr int KEYS = (UNIT * PIECES + 255) / 256;   // of a key thread
-    static constexpr int COLS = D / 4;                         // value threads side by side
-    // (one set of registers for both kinds of threads)
-    static constexpr int WORDS = Q4 ? 12 : 16;
-    uint32_t w[WORDS];
-    __device__ __forceinline__ uint32_t& kd(int i) { return w[4 * KEYS + i]; }
-    __device__ __forceinline__ uint32_t& v(int i, int n) { return w[Q4 ? i : 2 * i + n]; }
-    __device__ __forceinline__ uint32_t& vd(int p) { return w[8 + p]; }
+    static constexpr int ROW = Q4 ? D / 2 : 2 * D;             // bytes of a row in a page
+    static constexpr int PIECES = D / 64;                      // of the lane's keys: words (4-bit) or 16 bytes, 128 apart
+    static constexpr bool ALL = D == 128;                      // lanes that have values
+    uint32_t k[Q4 ? PIECES : 4 * PIECES], kd;
+    uint32_t v[8], vd[Q4 ? 4 : 1];
+    int key_from, key_scale, key_to, value_from, value_scale, value_to;
+    int key_first, value_first;            // first positions in the unit
+    bool has_values;
 
-    // The thread among its 256, as a new value each time: what follows from it
-    // is worked out where it is needed and holds no register through the products.
-    static __device__ __forceinline__ int thread()
+    __device__ __forceinline__ PromptLoad(int wave, int lane, int page_size, int values_at)
     {
-        int t = threadIdx.x & 255;
-        asm volatile("" : "+v"(t));
-        return t;
+        const int half = wave & 1, row = 8 * half + (lane >> 3), piece = lane & 7;
+        key_first = GRANULE * (wave >> 1) + row;
+        key_from = row * ROW + (Q4 ? 4 * PIECES : 16) * piece;
+        key_scale = 2 * ((PIECES * piece >> 2) * page_size + row);
+        key_to = key_at<D>(key_first, Q4 ? PIECES * piece : piece);
+        has_values = ALL || lane < D / 2;
+        const int c = lane % (D / 2);
+        value_first = GRANULE * (wave >> 1) + 4 * half;
+        value_from = 4 * half * ROW + (Q4 ? 1 : 4) * c;
+        value_scale = 2 * ((c >> 4) * page_size + 4 * half);
+        value_to = values_at + value_at(2 * c, wave);
     }
-    // (4-bit rows of 64 values are half as many pieces as there are threads)
-    static __device__ __forceinline__ bool takes_keys(int t) { return threadIdx.x < 256 && (UNIT * PIECES >= 256 || t < UNIT * PIECES); }
-    static __device__ __forceinline__ bool takes_values(int t) { return threadIdx.x >= 256 && (COLS * 8 == 256 || t < COLS * 8); }
-    // the row of a key thread's load i, and its piece of it
-    static __device__ __forceinline__ int row(int t, int i) { return t / PIECES + i * (256 / PIECES); }
-    static __device__ __forceinline__ int piece(int t) { return t % PIECES; }
 
-    // pages: the unit's four pages (a page that is not there: page 0)
-    __device__ __forceinline__ void load(const PagedAttentionArgs& a, int kvh, int base, const int* pages, int64_t head_bytes)
+    // keys, values: the granule's page of this KV head, slot: the granule's place in it
+    __device__ __forceinline__ void load(const char* keys, const char* values, int slot, int page_size)
     {
-        const int ps = a.cache.page_size, t = thread();
-        // (selects: an array indexed by a lane's value would live in memory)
-        auto page_at = [&](int u) {
-            const int page = u < 2 ? (u ? pages[1] : pages[0]) : (u == 2 ? pages[2] : pages[3]);
-            return (int64_t(max(page, 0)) * a.cache.kv_heads + kvh) * head_bytes;
-        };
-        if (takes_keys(t)) {
+        const char* const kr = keys + slot * ROW;
+        const char* const vr = values + slot * ROW;
+        const int scales = page_size * (D / 2) + 2 * slot;
+        if constexpr (Q4) {
+            if constexpr (PIECES == 2) {
+                const uint2 x = *reinterpret_cast<const uint2*>(kr + key_from);
+                k[0] = x.x, k[1] = x.y;
+            } else {
+                k[0] = *reinterpret_cast<const uint32_t*>(kr + key_from);
+            }
+            kd = *reinterpret_cast<const uint16_t*>(keys + scales + key_scale);
+        } else {
 #pragma unroll
-            for (int i = 0; i < KEYS; i++) {
-                const int r = row(t, i), slot = (base + r) & (ps - 1);
-                const char* const p = a.cache.keys + page_at(r >> 4);
-                const uint4 x = *reinterpret_cast<const uint4*>(p + slot * (Q4 ? D / 2 : 2 * D) + 16 * piece(t));
-                w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
-                if constexpr (Q4)
-                    kd(i) = reinterpret_cast<const uint16_t*>(p + ps * (D / 2))[piece(t) * ps + slot];
+            for (int j = 0; j < PIECES; j++) {
+                const uint4 x = *reinterpret_cast<const uint4*>(kr + key_from + 128 * j);
+                k[4 * j] = x.x, k[4 * j + 1] = x.y, k[4 * j + 2] = x.z, k[4 * j + 3] = x.w;
             }
-        } else if (takes_values(t)) {
-            const int c = t % COLS, q = t / COLS;
-            const int r = 16 * (q >> 1) + 4 * (q & 1), slot = (base + r) & (ps - 1);
-            const char* const p = a.cache.values + page_at(q >> 1);
+        }
+        // (a lane without values reads those of another)
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int s = slot + (i & 3) + 8 * (i >> 2);
-                if constexpr (Q4) {
-                    v(i, 0) = *reinterpret_cast<const uint16_t*>(p + s * (D / 2) + 2 * c);
-                } else {
-                    const uint2 x = *reinterpret_cast<const uint2*>(p + s * (2 * D) + 8 * c);
-                    v(i, 0) = x.x, v(i, 1) = x.y;
-                }
-            }
-            if constexpr (Q4) {
-                const uint16_t* const d = reinterpret_cast<const uint16_t*>(p + ps * (D / 2)) + (c >> 3) * ps + slot;
-                const uint2 x = *reinterpret_cast<const uint2*>(d), y = *reinterpret_cast<const uint2*>(d + 8);
-                vd(0) = x.x, vd(1) = x.y, vd(2) = y.x, vd(3) = y.y;
-            }
+        for (int i = 0; i < 8; i++) {
+            const char* const p = vr + value_from + ((i & 3) + 8 * (i >> 2)) * ROW;
+            v[i] = Q4 ? uint32_t(*reinterpret_cast<const uint8_t*>(p)) : *reinterpret_cast<const uint32_t*>(p);
+        }
+        if constexpr (Q4) {
+            const char* const d = values + scales + value_scale;
+            const uint2 x = *reinterpret_cast<const uint2*>(d), y = *reinterpret_cast<const uint2*>(d + 16);
+            vd[0] = x.x, vd[1] = x.y, vd[2] = y.x, vd[3] = y.y;
         }
     }
 
-    // Into LDS as FP16 (FINE 4-bit: and what is left of the products beside
-    // it).  `partial`: some row does not see all of the unit; keys and values
+    // Into LDS as FP16 (FINE 4-bit: and what is left of the products `lo` bytes
+    // on).  `partial`: some row does not see all of the unit; keys and values
     // that are not finite are then taken out and their positions marked in `odd`.
-    __device__ __forceinline__ void store(char* keys, char* values, int lo, bool partial, uint32_t* odd)
+    __device__ __forceinline__ void store(char* lds, int lo, bool partial, uint32_t* odd)
     {
-        const int t = thread();
-        if (takes_keys(t)) {
+        if (partial)
+            take_out_odd(odd);
+        if constexpr (Q4) {
+            const f16x2 d = as_f16x2(kd | kd << 16);
 #pragma unroll
-            for (int i = 0; i < KEYS; i++) {
-                const int r = row(t, i);
-                if (partial) {
-                    bool bad;
-                    if constexpr (Q4) {
-                        bad = (kd(i) & 0x7000u) == 0x7000u;
-                        kd(i) = bad ? 0 : kd(i);
-                    } else {
-                        bad = infinite(w[4 * i]) || infinite(w[4 * i + 1]) || infinite(w[4 * i + 2]) || infinite(w[4 * i + 3]);
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            w[4 * i + j] = bad ? 0 : w[4 * i + j];
-                    }
-                    if (bad)
-                        atomicOr(&odd[r >> 5], 1u << (r & 31));
-                }
-                if constexpr (Q4) {
-                    const f16x2 d = as_f16x2(kd(i) | kd(i) << 16);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        Frag x, y;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const f16x2 n = nibbles(w[4 * i + j] >> (4 * e)), p = n * d;
-                            x.w[e] = as_u32(p);
-                            if constexpr (FINE)
-                                y.w[e] = as_u32(__builtin_elementwise_fma(n, d, -p));
-                        }
-                        *reinterpret_cast<f16x8*>(keys + key_at<D>(r, 4 * piece(t) + j)) = x.v;
-                        if constexpr (FINE)
-                            *reinterpret_cast<f16x8*>(keys + lo + key_at<D>(r, 4 * piece(t) + j)) = y.v;
-                    }
-                } else {
-                    *reinterpret_cast<uint4*>(keys + key_at<D>(r, piece(t))) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-                }
-            }
-        } else if (takes_values(t)) {
-            const int c = t % COLS, q = t / COLS;
-            if (partial) {
-                uint32_t mask = 0;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    bool bad = false;
-                    if constexpr (Q4) {
-                        const uint32_t e = 0x7000u << (16 * (i & 1));      // (8192 and up, as above)
-                        bad = (vd(i >> 1) & e) == e;
-                        if (bad)
-                            vd(i >> 1) &= ~(0xFFFFu << (16 * (i & 1)));
-                    } else {
-#pragma unroll
-                        for (int n = 0; n < 2; n++)
-                            if (infinite(v(i, n))) {
-                                bad = true;
-                                v(i, n) = 0;
-                            }
-                    }
-                    const int pos = 16 * (q >> 1) + 4 * (q & 1) + (i & 3) + 8 * (i >> 2);
-                    mask |= bad ? 1u << (pos & 31) : 0u;
-                }
-                if (mask)
-                    atomicOr(&odd[q >> 2], mask);
-            }
-            uint32_t both[4];                              // 4-bit: two positions' four columns
-            if constexpr (Q4) {
-#pragma unroll
-                for (int p = 0; p < 4; p++)
-                    both[p] = v(2 * p, 0) | v(2 * p + 1, 0) << 16;
-            }
-#pragma unroll
-            for (int n = 0; n < 4; n++) {
+            for (int j = 0; j < PIECES; j++) {
                 Frag x, y;
 #pragma unroll
-                for (int p = 0; p < 4; p++) {
-                    if constexpr (Q4) {
-                        const f16x2 d = as_f16x2(vd(p));
-                        const f16x2 m = nibbles(both[p] >> (4 * n)), z = m * d;
-                        x.w[p] = as_u32(z);
-                        if constexpr (FINE)
-                            y.w[p] = as_u32(__builtin_elementwise_fma(m, d, -z));
-                    } else {
-                        x.w[p] = __builtin_amdgcn_perm(v(2 * p + 1, n >> 1), v(2 * p, n >> 1), n & 1 ? 0x07060302u : 0x05040100u);
-                    }
+                for (int e = 0; e < 4; e++) {
+                    const f16x2 n = nibbles(k[j] >> (4 * e)), p = n * d;
+                    x.w[e] = as_u32(p);
+                    if constexpr (FINE)
+                        y.w[e] = as_u32(__builtin_elementwise_fma(n, d, -p));
                 }
-                *reinterpret_cast<f16x8*>(values + value_at(4 * c + n, q)) = x.v;
-                if constexpr (FINE && Q4)
-                    *reinterpret_cast<f16x8*>(values + lo + value_at(4 * c + n, q)) = y.v;
+                *reinterpret_cast<f16x8*>(lds + (key_to ^ j << 4)) = x.v;
+                if constexpr (FINE)
+                    *reinterpret_cast<f16x8*>(lds + lo + (key_to ^ j << 4)) = y.v;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < PIECES; j++)
+                *reinterpret_cast<uint4*>(lds + (key_to ^ j << 7)) = make_uint4(k[4 * j], k[4 * j + 1], k[4 * j + 2], k[4 * j + 3]);
+        }
+        if (!has_values)
+            return;
+        uint32_t both[4];                                  // 4-bit: two positions' two columns
+        if constexpr (Q4) {
+#pragma unroll
+            for (int p = 0; p < 4; p++)
+                both[p] = v[2 * p] | v[2 * p + 1] << 16;
+        }
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            Frag x, y;
+#pragma unroll
+            for (int p = 0; p < 4; p++) {
+                if constexpr (Q4) {
+                    const f16x2 d = as_f16x2(vd[p]);
+                    const f16x2 m = nibbles(both[p] >> (4 * n)), z = m * d;
+                    x.w[p] = as_u32(z);
+                    if constexpr (FINE)
+                        y.w[p] = as_u32(__builtin_elementwise_fma(m, d, -z));
+                } else {
+                    x.w[p] = __builtin_amdgcn_perm(v[2 * p + 1], v[2 * p], n & 1 ? 0x07060302u : 0x05040100u);
+                }
+            }
+            *reinterpret_cast<f16x8*>(lds + value_to + n * 128) = x.v;
+            if constexpr (FINE && Q4)
+                *reinterpret_cast<f16x8*>(lds + lo + value_to + n * 128) = y.v;
+        }
+    }
+
+    __device__ __forceinline__ void take_out_odd(uint32_t* odd)
+    {
+        bool bad = false;
+        if constexpr (Q4) {
+            bad = (kd & 0x7000u) == 0x7000u;               // 8192 and up: 8 x it passes FP16's largest value
+            kd = bad ? 0 : kd;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4 * PIECES; j++) {
+                const bool b = infinite(k[j]);
+                bad |= b;
+                k[j] = b ? 0 : k[j];
             }
         }
+        if (bad)
+            atomicOr(&odd[key_first >> 5], 1u << (key_first & 31));
+        uint32_t mask = 0;                                 // positions from value_first on
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            bool b;
+            if constexpr (Q4) {
+                const uint32_t e = 0x7000u << (16 * (i & 1));
+                b = (vd[i >> 1] & e) == e;
+                vd[i >> 1] = b ? vd[i >> 1] & ~(0xFFFFu << (16 * (i & 1))) : vd[i >> 1];
+            } else {
+                b = infinite(v[i]);
+                v[i] = b ? 0 : v[i];
+            }
+            mask |= b ? 1u << ((i & 3) + 8 * (i >> 2)) : 0u;
+        }
+        // (a granule lies in one of the two words)
+        if (mask)
+            atomicOr(&odd[value_first >> 5], mask << (value_first & 31));
     }
 };
 
@@ -1040,6 +1030,7 @@ paged_prompt_kernel(const PagedAttentionArgs a)
     // go through the same keys and values, and meet in its L2
     const int64_t worker = int64_t(blockIdx.x % 8) * (PROMPT_WORKERS / 8) + blockIdx.x / 8;
     const int64_t begin = worker * line.share, end = begin + line.share;
+    PromptLoad<D, Q4, FINE> raw(wave, lane, a.cache.page_size, PLANE);
     Record record{};
     PromptSequence q{};
     int64_t q_start = 0, q_end = 0;
@@ -1112,26 +1103,27 @@ paged_prompt_kernel(const PagedAttentionArgs a)
         for (int k = 0; k < 4; k++)
             value_of[k] = PLANE + value_at(r, 2 * k + h);
 
-        // pages of the 64 granules around a unit, one a lane of every wave
+        // Pages of the 64 granules around a unit, one a lane of every wave; those
+        // that are not there: page 0 is read in their place.
         int held = 0, held_at = -1;
-        auto pages_of = [&](int u, int* pages) {
+        uint64_t held_lost = 0;
+        auto load = [&](int u) -> uint32_t {
             if (u >> 4 != held_at) {
                 held_at = u >> 4;
                 const int pos = (held_at * 64 + lane) * GRANULE;
                 held = pos <= most ? table[pos >> a.cache.page_shift] : 0;
                 if (held >= a.cache.pages)
                     held = -1;
+                held_lost = __ballot(held < 0);
             }
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                pages[k] = __builtin_amdgcn_readlane(held, (u & 15) * 4 + k);
-        };
-        auto lost_of = [](const int* pages) {
-            return (pages[0] < 0 ? 1u : 0u) | (pages[1] < 0 ? 2u : 0u) | (pages[2] < 0 ? 4u : 0u) | (pages[3] < 0 ? 8u : 0u);
+            const int granule = (u & 15) * 4 + (wave >> 1);
+            const int page = max(0, __builtin_amdgcn_readlane(held, granule));
+            const int64_t head = (int64_t(page) * a.cache.kv_heads + kvh) * head_bytes;
+            raw.load(a.cache.keys + head, a.cache.values + head, (u * UNIT + (wave >> 1) * GRANULE) & (a.cache.page_size - 1),
+                     a.cache.page_size);
+            return uint32_t(held_lost >> (u & 15) * 4) & 15;
         };
         auto partial = [&](int u) { return u * UNIT + UNIT - 1 > least; };
-        PromptLoad<D, Q4, FINE> raw;
-        int pages[4];
         uint32_t lost = 0, lost_next = 0;
         __syncthreads();                                  // the item before is done with LDS
         if (threadIdx.x < 6)
@@ -1144,9 +1136,7 @@ paged_prompt_kernel(const PagedAttentionArgs a)
             for (int at = 16 * threadIdx.x; at < PLANE; at += 16 * PROMPT_THREADS)
                 *reinterpret_cast<uint4*>(lds[(unit0 + 1) & 1] + p * PLANE + at) = make_uint4(0, 0, 0, 0);
         if (unit0 < unit1) {
-            pages_of(unit0, pages);
-            lost_next = lost_of(pages);
-            raw.load(a, kvh, unit0 * UNIT, pages, head_bytes);
+            lost_next = load(unit0);
         }
         __syncthreads();
 
@@ -1293,13 +1283,9 @@ paged_prompt_kernel(const PagedAttentionArgs a)
             }
             lost = lost_next;
             if (u + 1 < unit1) {
-                char* const to = lds[(u + 1) & 1];
-                raw.store(to, to + PLANE, 2 * PLANE, partial(u + 1), odd[(u + 1) % 3]);
-                if (u + 2 < unit1) {
-                    pages_of(u + 2, pages);
-                    lost_next = lost_of(pages);
-                    raw.load(a, kvh, (u + 2) * UNIT, pages, head_bytes);
-                }
+                raw.store(lds[(u + 1) & 1], 2 * PLANE, partial(u + 1), odd[(u + 1) % 3]);
+                if (u + 2 < unit1)
+                    lost_next = load(u + 2);
             }
             __syncthreads();
             read_keys(u + 1, 0, 0);
