@@ -866,7 +866,8 @@ struct PromptLoad {
     static constexpr int PIECES = D / 64;                      // of the lane's keys: words (4-bit) or 16 bytes, 128 apart
     static constexpr bool ALL = D == 128;                      // lanes that have values
     uint32_t k[Q4 ? PIECES : 4 * PIECES], kd;
-    uint32_t v[8], vd[Q4 ? 4 : 1];
+    uint32_t v[Q4 ? 2 : 8], vd[Q4 ? 4 : 1];
+    uint32_t byte;                         // of the words of a quad of lanes: this lane's
     int key_from, key_scale, key_to, value_from, value_scale, value_to;
     int key_first, value_first;            // first positions in the unit
     bool has_values;
@@ -881,7 +882,8 @@ struct PromptLoad {
         has_values = ALL || lane < D / 2;
         const int c = lane % (D / 2);
         value_first = GRANULE * (wave >> 1) + 4 * half;
-        value_from = 4 * half * ROW + (Q4 ? 1 : 4) * c;
+        value_from = Q4 ? (4 * half + (c & 3)) * ROW + (c & ~3) : 4 * half * ROW + 4 * c;
+        byte = 0x0C040C00u + 0x00010001u * (c & 3);
         value_scale = 2 * ((c >> 4) * page_size + 4 * half);
         value_to = values_at + value_at(2 * c, wave);
     }
@@ -908,12 +910,14 @@ struct PromptLoad {
             }
         }
         // (a lane without values reads those of another)
+        if constexpr (!Q4) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const char* const p = vr + value_from + ((i & 3) + 8 * (i >> 2)) * ROW;
-            v[i] = Q4 ? uint32_t(*reinterpret_cast<const uint8_t*>(p)) : *reinterpret_cast<const uint32_t*>(p);
-        }
-        if constexpr (Q4) {
+            for (int i = 0; i < 8; i++)
+                v[i] = *reinterpret_cast<const uint32_t*>(vr + value_from + ((i & 3) + 8 * (i >> 2)) * ROW);
+        } else {
+            // four lanes read the words of four positions each, and share them below
+            v[0] = *reinterpret_cast<const uint32_t*>(vr + value_from);
+            v[1] = *reinterpret_cast<const uint32_t*>(vr + value_from + 8 * ROW);
             const char* const d = values + scales + value_scale;
             const uint2 x = *reinterpret_cast<const uint2*>(d), y = *reinterpret_cast<const uint2*>(d + 16);
             vd[0] = x.x, vd[1] = x.y, vd[2] = y.x, vd[3] = y.y;
@@ -953,8 +957,10 @@ struct PromptLoad {
         uint32_t both[4];                                  // 4-bit: two positions' two columns
         if constexpr (Q4) {
 #pragma unroll
-            for (int p = 0; p < 4; p++)
-                both[p] = v[2 * p] | v[2 * p + 1] << 16;
+            for (int p = 0; p < 2; p++) {
+                both[2 * p] = __builtin_amdgcn_perm(of_quad<1>(v[p]), of_quad<0>(v[p]), byte);
+                both[2 * p + 1] = __builtin_amdgcn_perm(of_quad<3>(v[p]), of_quad<2>(v[p]), byte);
+            }
         }
 #pragma unroll
         for (int n = 0; n < 2; n++) {
@@ -975,6 +981,13 @@ struct PromptLoad {
             if constexpr (FINE && Q4)
                 *reinterpret_cast<f16x8*>(lds + lo + value_to + n * 128) = y.v;
         }
+    }
+
+    // v of lane I of the quad
+    template <int I>
+    static __device__ __forceinline__ uint32_t of_quad(uint32_t v)
+    {
+        return uint32_t(__builtin_amdgcn_mov_dpp(int(v), 0x55 * I, 0xF, 0xF, true));
     }
 
     __device__ __forceinline__ void take_out_odd(uint32_t* odd)
