@@ -725,12 +725,22 @@ paged_merge_kernel(const PagedAttentionArgs a)
 
 // A workgroup of eight waves takes 256 packed rows of one sequence and KV
 // head, 32 a wave, through units of 64 positions.  The unit's keys and values
-// go through LDS as FP16, dequantized once for the eight waves (four waves
-// convert keys, four values), two buffers: the next unit's bytes are loaded
-// while this one is multiplied.  Scores stay transposed here too, with
-// v_mfma_f32_32x32x16_f16.
+// go through LDS as FP16, dequantized once for the eight waves, two buffers: the
+// next unit's bytes are loaded while this one is multiplied.  Scores stay
+// transposed here too, with v_mfma_f32_32x32x16_f16.
+//
+// What bounds it: of the 5000 cycles that a unit of 64 positions takes, the two
+// waves of a SIMD spend 2050 in matrix instructions and 2300 in vector ones (a
+// quarter of them the exponentials), which overlap little.  840 TFLOP/s within
+// the units, 0.55 of what a large matrix product reaches.
+// 128 rows in four waves: 252 us where this takes 233 (chunks of up to 2000 rows
+// over up to 6000 positions).
 constexpr int PROMPT_ROWS = 256;
 constexpr int PROMPT_THREADS = 512;
+// What the scores are taken relative to follows their maximum only when that is
+// further above it: the exponentials stay under 2^8, far from FP16's end, and the
+// accumulators are rescaled a few times a row instead of once a unit (440
+// vector instructions a unit then, 300 now).
 constexpr float REFERENCE_SLACK = 8.0f;
 constexpr int PROMPT_PIECE = 7;          // what a piece of a tile costs besides its units, in units
 constexpr int PROMPT_MIN = 9;            // units that a worker takes at least, with a piece's cost
@@ -1148,13 +1158,13 @@ paged_prompt_kernel(const PagedAttentionArgs a)
         for (int p = 1; p < PLANES; p += 2)
             for (int at = 16 * threadIdx.x; at < PLANE; at += 16 * PROMPT_THREADS)
                 *reinterpret_cast<uint4*>(lds[(unit0 + 1) & 1] + p * PLANE + at) = make_uint4(0, 0, 0, 0);
-        if (unit0 < unit1) {
+        if (unit0 < unit1)
             lost_next = load(unit0);
-        }
         __syncthreads();
 
-        // Fragments are read two groups ahead of their products; the order is
-        // pinned, or the compiler reads each right before it is used.
+        // Fragments are read ahead of their products (FINE: by a smaller step, for
+        // want of registers); the order is pinned, or the compiler reads each right
+        // before it is used.
         constexpr int GROUP = FINE ? 1 : 2, SETS = FINE ? 2 : 3;
         f16x8 f[SETS][GROUP], fl[SETS][FINE && Q4 ? GROUP : 1];
         f32x16 s[2];
@@ -1185,23 +1195,12 @@ paged_prompt_kernel(const PagedAttentionArgs a)
         constexpr int AHEAD = SETS - 1;
         constexpr int SCORES = 2 * NK / GROUP, SUMS = 4 * NC / GROUP;      // groups of a unit
         // The scores of unit u, whose first fragments are in sets `set` and on.  They
-        // start from 0, or from -inf where a row does not see the position.
+        // start from what is taken off them, and are -inf where a row does not see the position.
         // Element e of block b: position base + 32 b + 8 (e / 4) + 4 h + e % 4.
         auto scores = [&](int u, int set) {
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 s[0][e] = s[1][e] = -ref;
-            if (partial(u)) {
-                // (a new value each time, or 32 positions live through the loop)
-                int first = 4 * h;
-                asm volatile("" : "+v"(first));
-                const int seen = limit - u * UNIT - first;
-#pragma unroll
-                for (int b = 0; b < 2; b++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        s[b][e] = 32 * b + 8 * (e >> 2) + (e & 3) > seen ? -INFINITY : -ref;
-            }
 #pragma unroll
             for (int g = 0; g < SCORES; g++) {
                 if (g + AHEAD < SCORES)
@@ -1218,12 +1217,25 @@ paged_prompt_kernel(const PagedAttentionArgs a)
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+            if (partial(u)) {
+                // (a new value each time, or 32 positions live through the loop)
+                int first = 4 * h;
+                asm volatile("" : "+v"(first));
+                const int seen = limit - u * UNIT - first;
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        s[b][e] = 32 * b + 8 * (e >> 2) + (e & 3) > seen ? -INFINITY : s[b][e];
+            }
         };
-        // The matrix cores and the vector units take turns: waves 4..7 run half
-        // a unit behind waves 0..3, so each SIMD has one wave at its products
-        // while the other is at its exponentials and conversions.  Every
-        // half ends at a barrier.  Waves 0..3 convert keys, a half before anyone
-        // needs them; waves 4..7 values, which are needed two halves later.
+        // One barrier a unit: between two of them a wave takes the scores of a
+        // unit, its exponentials and sums, and stores its part of the next one.
+        // The two waves of a SIMD come to each step after each other, so one is at
+        // its products while the other is at its exponentials.  (Halves of the
+        // workgroup that take turns behind two barriers a unit were no faster, with
+        // the conversions among the exponentials or among the products: 198 to 219
+        // against 197 us for 137216 positions.)
 #pragma unroll
         for (int e = 0; e < 16; e++)
             s[0][e] = s[1][e] = -INFINITY;
@@ -1250,7 +1262,9 @@ paged_prompt_kernel(const PagedAttentionArgs a)
                 top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
             }
             if (__any(top > gate)) {
-                const float by = top > gate ? top : 0.0f, fade = __builtin_amdgcn_exp2f(-by);
+                // (a row that has seen nothing yet has nothing to rescale, and its
+                // first score may be far below 0)
+                const float by = top > gate ? top : 0.0f, fade = top > gate && gate < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-by);
                 gate = top > gate ? REFERENCE_SLACK : gate;
                 ref += by;
                 sum *= fade;

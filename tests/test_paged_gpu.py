@@ -175,6 +175,32 @@ def test_append_and_read(hip, fmt, head, heads, kv, page, rotary, seqs):
 
 
 @gpu
+@pytest.mark.parametrize("fmt,head,rotary", [(Q4, 128, 96), (F16, 64, 64), (Q4, 64, 6)])
+def test_append_and_read_at_any_word(hip, fmt, head, rotary):
+    """Rows that begin at any multiple of four bytes."""
+    heads, kv = 3, 1
+    st = Setup(hip, fmt, head, kv, 16, [(5, 20), (1, 3)], seed=rotary).upload()
+    qkv = st.rng.standard_normal((st.rows, (heads + 2 * kv) * head)).astype(np.float32)
+    freq = (0.4 ** np.arange(rotary // 2)).astype(np.float32)
+    want = _expect_append(st, heads, rotary, qkv, freq, 1.0)
+    for off in (1, 2, 3):
+        dq = hip.to_device(np.concatenate([np.zeros(off, np.float32), qkv.reshape(-1)]))
+        df = hip.to_device(np.concatenate([np.zeros(off, np.float32), freq]))
+        query, keys = (hip.to_device(np.full((st.rows * n * head + off) * 4, SENTINEL, np.uint8)) for n in (heads, kv))
+        vals = hip.to_device(np.zeros(st.rows * kv * head + off, np.float32))
+        hip.paged_kv_append(native.PagedAppendArgs(st.batch, st.cache, dq.ptr + 4 * off, df.ptr + 4 * off,
+                                                   query.ptr + 4 * off, heads, rotary, 1.0))
+        assert _same(query.readback(np.float32)[off:].reshape(want.shape), want)
+        for b, pool in zip(st.dev[3:], (st.k, st.v)):
+            assert np.array_equal(b.readback(np.uint8), pool.raw.reshape(-1))
+        hip.paged_kv_read(st.batch, st.cache, keys.ptr + 4 * off, vals.ptr + 4 * off)
+        rows = keys.readback(np.float32)[off:].reshape(st.rows, kv, head)
+        for t in range(st.used):
+            _, p, page = ref.place(st.table, st.starts, st.lengths, 16, st.pages, t)
+            assert np.array_equal(rows[t], st.k.load(page, p % 16).astype(np.float32))
+
+
+@gpu
 def test_append_many_rows(hip):
     """Enough rows for whole rows a workgroup, and more sequences than threads."""
     seqs = [(2, 2 + 3 * (i % 5)) for i in range(300)]
@@ -330,6 +356,55 @@ def test_attention_sharp_and_flat(hip, fmt):
                     want, mag, slack = ref.attention(q[t].reshape(6, 128), keys, values, n)
                     bound = np.minimum(np.expm1(4 * 2.0 ** -11 * slack), 2 * 1e3)[:, None] * mag + 2.0 ** -8 * np.abs(want) + 2e-3 * mag
                     assert np.all(np.abs(got[t] - want) <= bound)
+
+
+@gpu
+@pytest.mark.parametrize("course", ["flat", "rising", "falling"])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("fmt,out_fmt", [(F16, F32), (Q4, BF16)])
+def test_attention_far_from_zero(hip, fmt, out_fmt, sign, course):
+    """Scores around -300 or 300, all alike or on their way there: what they are
+    taken relative to starts far from 0, or moves many times."""
+    d, heads, kv = 128, 6, 2
+    st = Setup(hip, fmt, d, kv, 32, [(1, 333), (5, 200), (90, 333), (150, 150)], seed=27)
+    flips = st.rng.choice([-1.0, 1.0], d)
+    for s, (_, length) in enumerate(st.seqs):
+        for p in range(length):
+            part = {"flat": 1.0, "rising": p / length, "falling": 1 - p / length}[course]
+            k = 2 * part * flips + 0.1 * st.rng.standard_normal((kv, d))
+            page = int(st.table[s, p // 32])
+            st.k.store(page, p % 32, k.astype(np.float32))
+            st.v.store(page, p % 32, st.rng.standard_normal((kv, d)).astype(np.float32))
+    st.upload()
+    q = (sign * 13.3 * np.tile(flips, heads) + 0.5 * st.rng.standard_normal((st.rows, heads * d))).astype(np.float32)
+    got = _attend(hip, st, heads, q, out_fmt)
+    # (scores of hundreds: the element bound alone, as their roundings do not average out over few weights)
+    h, half_out = (2.0 ** -11, 2.0 ** -8) if out_fmt == BF16 else (2.0 ** -18, 2.0 ** -24)
+    for s, (new, length) in enumerate(st.seqs):
+        keys, values = st.rows_of(s, length)
+        for i in range(new):
+            t = st.starts[s] + i
+            want, mag, slack = ref.attention(q[t].reshape(heads, d), keys, values, length - new + i + 1)
+            bound = (np.expm1(4 * h * slack)[:, None] + 2 * h + 1e-5) * mag * (1 + half_out) + half_out * np.abs(want)
+            assert np.all(np.abs(got[t] - want) <= bound), (s, i, np.max(np.abs(got[t] - want) / bound))
+
+
+@gpu
+@pytest.mark.parametrize("fmt,out_fmt", [(Q4, BF16), (F16, F32)])
+@pytest.mark.parametrize("head,heads,kv,page,seqs", [
+    (64, 16, 16, 16, [(70 + i, 70 + i + 41 * (i % 3)) for i in range(16)]),     # as many tiles as workgroups
+    (64, 32, 16, 32, [(65, 900), (33, 64), (1, 500), (260, 300), (65, 65), (40, 1000)] * 2),
+    (128, 6, 2, 64, [(90, 3001)]),                                              # one tile in many parts
+    (128, 5, 1, 16, [(120, 130), (1, 2000), (13, 1500)]),
+])
+def test_attention_shared_out(hip, fmt, out_fmt, head, heads, kv, page, seqs):
+    """Tiles that several workgroups share, borders anywhere, decode beside prompts."""
+    st = Setup(hip, fmt, head, kv, page, seqs, seed=len(seqs)).fill().upload()
+    q = st.rng.standard_normal((st.rows, heads * head)).astype(np.float32)
+    got = _attend(hip, st, heads, q, out_fmt)
+    pick = st.rng.choice(st.used, min(st.used, 160), replace=False)
+    _check_rows(st, heads, q, got, out_fmt, set(int(t) for t in pick))
+    assert np.all(np.isfinite(got[:st.used]))
 
 
 @gpu
