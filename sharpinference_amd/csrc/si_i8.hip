@@ -21,10 +21,6 @@ namespace si {
 
 namespace {
 
-// Values of a row that a thread keeps in registers; longer rows are read
-// again (from L2, mostly) for their codes.
-constexpr int KEEP = 32;
-
 enum InKind : int { IN_NORM, IN_NORM_RESIDUAL, IN_F32, IN_F16, IN_BF16 };
 
 struct RowsArgs {
@@ -39,104 +35,150 @@ struct RowsArgs {
     float eps;
 };
 
-template <int VEC>
-struct Values {
-    float v[VEC];
+// Four values beside each other; ODD: at any address that one value may have.
+// (The instructions are the same, but not their order: 4000 rows of 4096 values
+// take 55 us with the aligned types and 64 us with the others; 1900 rows of
+// 8001 took 103 us a value at a time, and take 54.)
+template <bool ODD>
+struct Fours {
+    typedef float f32 __attribute__((ext_vector_type(4)));
+    typedef uint16_t f16 __attribute__((ext_vector_type(4)));
+    typedef uint32_t codes;
+};
+template <>
+struct Fours<true> {
+    typedef float f32 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef uint16_t f16 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef uint32_t codes __attribute__((aligned(1)));
 };
 
-template <int VEC>
-__device__ __forceinline__ Values<VEC> load_f32(const float* p)
+struct Values {
+    float v[4];
+};
+
+// The row's four values from i on, 0 behind its end.  Without a branch: all of a
+// row's loads are asked for before one is waited for.  ODD: rows of a length that
+// four does not divide, or at such addresses; the last four of such a row begin up
+// to three values before the ones that are wanted.
+template <typename T4, typename T>
+__device__ __forceinline__ void load_four(const T* row, int64_t i, int64_t n, bool odd, T* v)
 {
-    Values<VEC> r;
-    if constexpr (VEC == 4) {
-        const float4 t = *reinterpret_cast<const float4*>(p);
-        r.v[0] = t.x, r.v[1] = t.y, r.v[2] = t.z, r.v[3] = t.w;
+    const int past = int(min(max(i - (n - 4), int64_t(0)), int64_t(4)));
+    const T4 t = *reinterpret_cast<const T4*>(row + i - (past < 4 ? past : i - (n - 4)));
+    const T z = T(0);
+    if (odd) {
+        v[0] = past < 2 ? (past ? t.y : t.x) : past < 4 ? (past == 2 ? t.z : t.w) : z;
+        v[1] = past < 2 ? (past ? t.z : t.y) : past == 2 ? t.w : z;
+        v[2] = past < 2 ? (past ? t.w : t.z) : z;
+        v[3] = past ? z : t.w;
     } else {
-        r.v[0] = *p;
+        v[0] = past ? z : t.x, v[1] = past ? z : t.y, v[2] = past ? z : t.z, v[3] = past ? z : t.w;
     }
+}
+template <typename T4, bool ODD, typename T>
+__device__ __forceinline__ void load_row(const T* row, int64_t i, int64_t n, T* v)
+{
+    if (ODD && n < 4) {                    // (the same for all rows)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            v[j] = i + j < n ? row[i + j] : T(0);
+    } else {
+        load_four<T4, T>(row, i, n, ODD, v);
+    }
+}
+
+template <bool ODD>
+__device__ __forceinline__ Values load_f32(const float* row, int64_t i, int64_t n)
+{
+    Values r;
+    load_row<typename Fours<ODD>::f32, ODD>(row, i, n, r.v);
     return r;
 }
 
-// The row's value as the codes are made of it: the input, plus the residual.
-template <int IN, int VEC>
-__device__ __forceinline__ Values<VEC> load_in(const RowsArgs& a, int64_t at)
+// The row's input as FP32.
+template <int IN, bool ODD>
+__device__ __forceinline__ Values load_in(const RowsArgs& a, int64_t base, int64_t i)
 {
     if constexpr (IN == IN_F16 || IN == IN_BF16) {
-        Values<VEC> r;
-        const uint16_t* p = static_cast<const uint16_t*>(a.x) + at;
-        uint16_t h[VEC];
-        if constexpr (VEC == 4) {
-            const uint2 t = *reinterpret_cast<const uint2*>(p);
-            h[0] = t.x & 0xFFFFu, h[1] = t.x >> 16, h[2] = t.y & 0xFFFFu, h[3] = t.y >> 16;
-        } else {
-            h[0] = *p;
-        }
+        Values r;
+        uint16_t h[4];
+        load_row<typename Fours<ODD>::f16, ODD>(static_cast<const uint16_t*>(a.x) + base, i, a.n, h);
 #pragma unroll
-        for (int i = 0; i < VEC; i++)
-            r.v[i] = IN == IN_F16 ? __half2float(__ushort_as_half(h[i])) : __uint_as_float(uint32_t(h[i]) << 16);
+        for (int j = 0; j < 4; j++)
+            r.v[j] = IN == IN_F16 ? __half2float(__ushort_as_half(h[j])) : __uint_as_float(uint32_t(h[j]) << 16);
         return r;
     } else {
-        Values<VEC> r = load_f32<VEC>(static_cast<const float*>(a.x) + at);
-        if constexpr (IN == IN_NORM_RESIDUAL) {
-            const Values<VEC> b = load_f32<VEC>(a.residual + at);
-#pragma unroll
-            for (int i = 0; i < VEC; i++)
-                r.v[i] += b.v[i];
-        }
-        return r;
+        return load_f32<ODD>(static_cast<const float*>(a.x) + base, i, a.n);
     }
 }
 
-__device__ __forceinline__ double wave_sum(double v)
+// over N neighbouring lanes
+template <int N>
+__device__ __forceinline__ double lanes_sum(double v)
 {
 #pragma unroll
-    for (int m = 32; m; m >>= 1)
+    for (int m = N / 2; m; m >>= 1)
         v += __shfl_xor(v, m);
     return v;
 }
-__device__ __forceinline__ double wave_max(double v)
+template <int N>
+__device__ __forceinline__ double lanes_max(double v)
 {
 #pragma unroll
-    for (int m = 32; m; m >>= 1)
+    for (int m = N / 2; m; m >>= 1)
         v = fmax(v, __shfl_xor(v, m));
     return v;
 }
 
-// THREADS threads a row (64: four rows a workgroup of 256).
-template <int IN, int THREADS, int VEC>
-__global__ void __launch_bounds__(THREADS == 64 ? 256 : THREADS)
+// THREADS threads a row (16, 64: 16 or 4 rows a workgroup of 256), STEPS fours of
+// it in a thread's registers; longer rows are read again (from L2, mostly) for
+// their codes.
+template <int IN, int THREADS, int STEPS, bool ODD>
+__global__ void __launch_bounds__(THREADS <= 64 ? 256 : THREADS)
 rows_i8_kernel(const RowsArgs a)
 {
     constexpr bool NORM = IN == IN_NORM || IN == IN_NORM_RESIDUAL;
-    constexpr int STEPS = KEEP / VEC;
+    constexpr bool RESIDUAL = IN == IN_NORM_RESIDUAL;
+    constexpr int LANES = THREADS < 64 ? THREADS : 64;
     const int lane = threadIdx.x % THREADS;
-    const int64_t row = THREADS == 64 ? int64_t(blockIdx.x) * 4 + threadIdx.x / 64 : blockIdx.x;
+    const int64_t row = THREADS <= 64 ? int64_t(blockIdx.x) * (256 / THREADS) + threadIdx.x / THREADS : blockIdx.x;
     if (row >= a.rows)
-        return;   // whole waves, and no barrier follows where THREADS is 64
+        return;   // all lanes of a row, and no barrier follows where THREADS is at most 64
     const int64_t base = row * a.n;
-    const int64_t stride = int64_t(THREADS) * VEC;
+    const int64_t stride = int64_t(THREADS) * 4;
 
-    Values<VEC> kept[STEPS], w[NORM ? STEPS : 1];
+    Values kept[STEPS], add[RESIDUAL ? STEPS : 1], w[NORM ? STEPS : 1];
 #pragma unroll
     for (int k = 0; k < STEPS; k++) {
-        const int64_t i = k * stride + lane * VEC;
-        if (i < a.n) {
-            kept[k] = load_in<IN, VEC>(a, base + i);
-            if constexpr (NORM)
-                w[k] = load_f32<VEC>(a.weight + i);
-        }
+        const int64_t i = k * stride + lane * 4;
+        kept[k] = load_in<IN, ODD>(a, base, i);
+        if constexpr (RESIDUAL)
+            add[k] = load_f32<ODD>(a.residual + base, i, a.n);
+        if constexpr (NORM)
+            w[k] = load_f32<ODD>(a.weight, i, a.n);
+    }
+    if constexpr (RESIDUAL) {
+#pragma unroll
+        for (int k = 0; k < STEPS; k++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                kept[k].v[j] += add[k].v[j];
     }
     double sum = 0.0, top = 0.0;
     bool bad = false;
-    auto take = [&](const Values<VEC>& u, const Values<VEC>& wt, int64_t i) {
-        if constexpr (IN == IN_NORM_RESIDUAL) {
-            if constexpr (VEC == 4)
-                *reinterpret_cast<float4*>(a.updated + base + i) = make_float4(u.v[0], u.v[1], u.v[2], u.v[3]);
-            else
-                a.updated[base + i] = u.v[0];
+    auto take = [&](const Values& u, const Values& wt, int64_t i) {
+        if constexpr (RESIDUAL) {
+            if (ODD && a.n - i < 4) {
+#pragma unroll
+                for (int j = 0; j < 3; j++)
+                    if (j < a.n - i)
+                        a.updated[base + i + j] = u.v[j];
+            } else if (i < a.n) {
+                *reinterpret_cast<typename Fours<ODD>::f32*>(a.updated + base + i) = typename Fours<ODD>::f32{u.v[0], u.v[1], u.v[2], u.v[3]};
+            }
         }
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
+        for (int j = 0; j < 4; j++) {
             const double x = u.v[j];
             double y = x;
             if constexpr (NORM) {
@@ -149,21 +191,31 @@ rows_i8_kernel(const RowsArgs a)
     };
 #pragma unroll
     for (int k = 0; k < STEPS; k++) {
-        const int64_t i = k * stride + lane * VEC;
-        if (i < a.n)
-            take(kept[k], w[NORM ? k : 0], i);
+        take(kept[k], w[NORM ? k : 0], k * stride + lane * 4);
     }
-    for (int64_t i = STEPS * stride + lane * VEC; i < a.n; i += stride) {
-        Values<VEC> wt{};
+    auto again = [&](int64_t i, Values* wt) {
+        Values u = load_in<IN, ODD>(a, base, i);
+        if constexpr (RESIDUAL) {
+            const Values b = load_f32<ODD>(a.residual + base, i, a.n);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                u.v[j] += b.v[j];
+        }
+        *wt = Values{};
         if constexpr (NORM)
-            wt = load_f32<VEC>(a.weight + i);
-        take(load_in<IN, VEC>(a, base + i), wt, i);
+            *wt = load_f32<ODD>(a.weight, i, a.n);
+        return u;
+    };
+    for (int64_t i = STEPS * stride + lane * 4; i < a.n; i += stride) {
+        Values wt;
+        const Values u = again(i, &wt);
+        take(u, wt, i);
     }
     // the reduction: a value that is not finite travels as a NaN sum
     if (bad)
         sum = NAN;
-    sum = wave_sum(sum);
-    top = wave_max(top);
+    sum = lanes_sum<LANES>(sum);
+    top = lanes_max<LANES>(top);
     if constexpr (THREADS > 64) {
         __shared__ double parts[2][THREADS / 64];
         if ((threadIdx.x & 63) == 0) {
@@ -187,43 +239,54 @@ rows_i8_kernel(const RowsArgs a)
         a.scale[row] = scale;
     // no scale, no codes: a row of zeros, or one that holds something infinite or NaN
     const double c = scale > 0.0f ? inv / double(scale) : 0.0;
-    auto give = [&](const Values<VEC>& u, const Values<VEC>& wt, int64_t i) {
-        int q[VEC];
+    auto give = [&](const Values& u, const Values& wt, int64_t i) {
+        int q[4];
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
+        for (int j = 0; j < 4; j++) {
             const double y = NORM ? double(u.v[j]) * double(wt.v[j]) : double(u.v[j]);
             // (a scale among the subnormals is coarse enough to pass 127)
             q[j] = scale > 0.0f ? int(fmin(fmax(rint(y * c), -127.0), 127.0)) : 0;
         }
-        if constexpr (VEC == 4)
-            *reinterpret_cast<uint32_t*>(a.codes + base + i) =
+        if (ODD && a.n - i < 4) {
+#pragma unroll
+            for (int j = 0; j < 3; j++)
+                if (j < a.n - i)
+                    a.codes[base + i + j] = static_cast<int8_t>(q[j]);
+        } else {
+            *reinterpret_cast<typename Fours<ODD>::codes*>(a.codes + base + i) =
                 (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | uint32_t(q[3]) << 24;
-        else
-            a.codes[base + i] = static_cast<int8_t>(q[0]);
+        }
     };
 #pragma unroll
     for (int k = 0; k < STEPS; k++) {
-        const int64_t i = k * stride + lane * VEC;
+        const int64_t i = k * stride + lane * 4;
         if (i < a.n)
             give(kept[k], w[NORM ? k : 0], i);
     }
-    for (int64_t i = STEPS * stride + lane * VEC; i < a.n; i += stride) {
-        Values<VEC> wt{};
-        if constexpr (NORM)
-            wt = load_f32<VEC>(a.weight + i);
-        give(load_in<IN, VEC>(a, base + i), wt, i);
+    for (int64_t i = STEPS * stride + lane * 4; i < a.n; i += stride) {
+        Values wt;
+        const Values u = again(i, &wt);
+        give(u, wt, i);
     }
 }
 
-template <int IN, int VEC>
+template <int IN, bool ODD>
 hipError_t launch_rows(const RowsArgs& a, hipStream_t s)
 {
-    if (a.n <= 64 * KEEP && a.rows >= 1024)
-        rows_i8_kernel<IN, 64, VEC><<<unsigned((a.rows + 3) / 4), 256, 0, s>>>(a);
-    else if (a.n <= 256 * KEEP)
-        rows_i8_kernel<IN, 256, VEC><<<unsigned(a.rows), 256, 0, s>>>(a);
+    // the fewest threads a row that keep it in registers, but for few rows, which
+    // the whole chip has to share
+    if (a.n <= 16 * 16 && a.rows >= 1024)
+        rows_i8_kernel<IN, 16, 4, ODD><<<unsigned((a.rows + 15) / 16), 256, 0, s>>>(a);
+    else if (a.n <= 64 * 16 && a.rows >= 1024)
+        rows_i8_kernel<IN, 64, 4, ODD><<<unsigned((a.rows + 3) / 4), 256, 0, s>>>(a);
+    else if (a.n <= 64 * 32 && a.rows >= 1024)
+        rows_i8_kernel<IN, 64, 8, ODD><<<unsigned((a.rows + 3) / 4), 256, 0, s>>>(a);
+    else if (a.n <= 256 * 16)
+        rows_i8_kernel<IN, 256, 4, ODD><<<unsigned(a.rows), 256, 0, s>>>(a);
+    else if (a.n <= 256 * 32)
+        rows_i8_kernel<IN, 256, 8, ODD><<<unsigned(a.rows), 256, 0, s>>>(a);
     else
-        rows_i8_kernel<IN, 1024, VEC><<<unsigned(a.rows), 1024, 0, s>>>(a);
+        rows_i8_kernel<IN, 1024, 4, ODD><<<unsigned(a.rows), 1024, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -233,30 +296,32 @@ template <int IN>
 hipError_t launch_rows(const RowsArgs& a, hipStream_t s)
 {
     const uintptr_t in = IN == IN_F16 || IN == IN_BF16 ? 8 : 16;
-    const bool wide = a.n % 4 == 0 && on(a.x, in) && on(a.residual, 16) && on(a.weight, 16) && on(a.updated, 16) &&
-                      on(a.codes, 4);
-    return wide ? launch_rows<IN, 4>(a, s) : launch_rows<IN, 1>(a, s);
+    const bool fours = a.n % 4 == 0 && on(a.x, in) && on(a.residual, 16) && on(a.weight, 16) && on(a.updated, 16) &&
+                       on(a.codes, 4);
+    return fours ? launch_rows<IN, false>(a, s) : launch_rows<IN, true>(a, s);
 }
 
-template <int VEC>
+// a workgroup takes 1024 columns of one row at a time
+template <bool ODD>
 __global__ void __launch_bounds__(256)
 dequant_i8_kernel(const int8_t* codes, const float* scale, float* out, int64_t rows, int64_t n)
 {
-    // a workgroup takes 256 * VEC columns of one row at a time
-    const int64_t per_row = (n + 256 * VEC - 1) / (256 * VEC);
+    const int64_t per_row = (n + 1023) / 1024;
     for (int64_t b = blockIdx.x; b < rows * per_row; b += gridDim.x) {
         const int64_t row = b / per_row;
-        const int64_t i = (b - row * per_row) * (256 * VEC) + threadIdx.x * VEC;
+        const int64_t i = (b - row * per_row) * 1024 + threadIdx.x * 4;
         if (i >= n)
             continue;
         const float d = scale[row];
-        if constexpr (VEC == 4) {
-            const uint32_t q = *reinterpret_cast<const uint32_t*>(codes + row * n + i);
-            *reinterpret_cast<float4*>(out + row * n + i) =
-                make_float4(float(int8_t(q)) * d, float(int8_t(q >> 8)) * d, float(int8_t(q >> 16)) * d,
-                            float(int8_t(q >> 24)) * d);
+        const int8_t* const from = codes + row * n + i;
+        float* const to = out + row * n + i;
+        if (ODD && n - i < 4) {
+            for (int j = 0; j < n - i; j++)
+                to[j] = float(from[j]) * d;
         } else {
-            out[row * n + i] = float(codes[row * n + i]) * d;
+            const uint32_t q = *reinterpret_cast<const typename Fours<ODD>::codes*>(from);
+            *reinterpret_cast<typename Fours<ODD>::f32*>(to) = typename Fours<ODD>::f32{
+                float(int8_t(q)) * d, float(int8_t(q >> 8)) * d, float(int8_t(q >> 16)) * d, float(int8_t(q >> 24)) * d};
         }
     }
 }
@@ -281,13 +346,12 @@ hipError_t launch_quantize_i8(int fmt, const void* x, int8_t* codes, float* scal
 hipError_t launch_dequant_i8(const int8_t* codes, const float* scale, float* out, int64_t rows, int64_t n,
                              hipStream_t s)
 {
-    const bool wide = n % 4 == 0 && on(codes, 4) && on(out, 16);
-    const int64_t blocks = rows * ((n + (wide ? 1023 : 255)) / (wide ? 1024 : 256));
+    const int64_t blocks = rows * ((n + 1023) / 1024);
     const unsigned grid = unsigned(blocks < (1 << 20) ? blocks : 1 << 20);
-    if (wide)
-        dequant_i8_kernel<4><<<grid, 256, 0, s>>>(codes, scale, out, rows, n);
+    if (n % 4 == 0 && on(codes, 4) && on(out, 16))
+        dequant_i8_kernel<false><<<grid, 256, 0, s>>>(codes, scale, out, rows, n);
     else
-        dequant_i8_kernel<1><<<grid, 256, 0, s>>>(codes, scale, out, rows, n);
+        dequant_i8_kernel<true><<<grid, 256, 0, s>>>(codes, scale, out, rows, n);
     return hipGetLastError();
 }
 
