@@ -71,6 +71,45 @@ def test_norm_codes(hip, rows, n, residual):
         _spare_untouched(b, nb)
 
 
+@pytest.mark.parametrize("rows,n", [(1024, 3), (1500, 2), (1024, 255), (1100, 256), (1030, 1003), (1024, 1024), (2, 4097),
+                                    (1, 6002), (2, 8190), (3, 16385)])
+@pytest.mark.parametrize("shift", [0, 1, 2])
+@pytest.mark.parametrize("fmt", [None, native.F32, native.F16, native.BF16])
+def test_rows_of_any_length_at_any_address(hip, fmt, rows, n, shift):
+    """Ends inside a four, one place of the type off its alignment; None: the norm with a residual."""
+    rng = np.random.default_rng(rows * n + shift)
+    x = (_rows(rng, rows, n) / 50).astype(np.float32)
+    size = 2 if fmt in (native.F16, native.BF16) else 4
+    raw = x.astype(np.float16) if fmt == native.F16 else (x.view(np.uint32) >> 16).astype(np.uint16) if fmt == native.BF16 else x
+    exact = (raw.astype(np.uint32) << 16).view(np.float32).astype(np.float64) if fmt == native.BF16 else raw.astype(np.float64)
+
+    def at(a, step):
+        b = hip.alloc(a.nbytes + 64)
+        b.upload(np.ascontiguousarray(a), step * shift)
+        return b, b.ptr + step * shift
+    held, dx = at(raw, size)
+    q, s = hip.to_device(np.full(rows * n + 64, 0x5A, np.uint8)), hip.alloc(rows * 4)
+    if fmt is None:
+        r, w = rng.standard_normal((rows, n)).astype(np.float32), (1 + 0.2 * rng.standard_normal(n)).astype(np.float32)
+        (hr, dr), (hw, dw) = at(r, 4), at(w, 4)
+        up = hip.to_device(np.full(rows * n * 4 + 64, 0x5A, np.uint8))
+        hip.residual_rms_norm_i8(dx, dr, dw, up.ptr + 4 * shift, q.ptr + shift, s.ptr, rows, n, 1e-5)
+        u = x + r
+        assert np.array_equal(up.readback(np.float32, rows * n, 4 * shift).reshape(rows, n), u)
+        assert np.all(up.readback(np.uint8, 64 - 4 * shift, rows * n * 4 + 4 * shift) == 0x5A)
+        u = u.astype(np.float64)
+        exact = u / np.sqrt((u * u).mean(1, keepdims=True) + float(np.float32(1e-5))) * w.astype(np.float64)
+    else:
+        hip.quantize_i8(fmt, dx, q.ptr + shift, s.ptr, rows, n)
+    codes, scale = q.readback(np.int8, rows * n, shift).reshape(rows, n), s.readback(np.float32, rows)
+    _check_codes(exact, codes, scale)
+    assert np.all(q.readback(np.uint8, 64 - shift, rows * n + shift) == 0x5A)
+    back = hip.to_device(np.full(rows * n * 4 + 64, 0x5A, np.uint8))
+    hip.dequant_i8(q.ptr + shift, s.ptr, back.ptr + 4 * shift, rows, n)
+    assert np.array_equal(back.readback(np.float32, rows * n, 4 * shift).reshape(rows, n), codes * scale[:, None])
+    assert np.all(back.readback(np.uint8, 64 - 4 * shift, rows * n * 4 + 4 * shift) == 0x5A)
+
+
 def test_norm_codes_at_odd_addresses(hip):
     rng = np.random.default_rng(5)
     rows, n = 3, 1024
