@@ -130,6 +130,8 @@ __device__ __forceinline__ Sequence from_lane(const Sequence& q, int lane)
     return {of(q.index), of(q.first), of(q.count), of(q.length), of(q.tiles), of(q.units)};
 }
 
+constexpr int LONG = 128;                // units: see Shares
+
 // The work of a launch in one line: sequence after sequence, of each its KV
 // heads, of each its tiles, of each its units.  A wave searches together,
 // one sequence a lane.
@@ -137,6 +139,7 @@ struct Line {
     const PagedBatch& b;
     int page_shift, group, kv;
     int64_t total;             // units
+    bool some_long;            // a tile is more than LONG units
     // up to 64 sequences are looked at once: the lane's, and the units up to it
     Sequence mine;
     int64_t upto;
@@ -148,10 +151,11 @@ struct Line {
         upto = before + wave_scan(units_of(mine));
     }
     __device__ __forceinline__ Line(const PagedBatch& batch, int shift, int heads_per_kv, int kv_heads)
-        : b(batch), page_shift(shift), group(heads_per_kv), kv(kv_heads), total(0)
+        : b(batch), page_shift(shift), group(heads_per_kv), kv(kv_heads), total(0), some_long(false)
     {
         for (int base = 0; base < b.sequences; base += 64) {
             look(base, total);
+            some_long |= __any(mine.tiles && mine.units > LONG);
             total = of_lane(upto, 63);
         }
     }
@@ -177,12 +181,17 @@ struct Line {
     }
 };
 
-// The waves that share a line of `total` units take equal runs of it.
-constexpr int MIN_UNITS = 2;
+// The waves that share a line take equal runs of it.  Two units at least where a
+// tile is more than LONG units: there its many slots take longer to join than a
+// second unit does.  (One unit against two: 4 sequences of up to 500 positions 10.1
+// and 12.8 us, one of 8000 14.6 and 14.3, one of 60000 with one KV head 33 and 24.)
 constexpr int WAVES = 2048;
 struct Shares {
     int64_t share;
-    __device__ __forceinline__ explicit Shares(int64_t total) : share(max(int64_t(MIN_UNITS), (total + WAVES - 1) / WAVES)) {}
+    __device__ __forceinline__ explicit Shares(const Line& line)
+        : share(max(int64_t(line.some_long ? 2 : 1), (line.total + WAVES - 1) / WAVES))
+    {
+    }
     __device__ __forceinline__ int64_t wave_of(int64_t unit) const { return quotient(unit, share); }
 };
 
@@ -543,7 +552,7 @@ paged_attention_kernel(const PagedAttentionArgs a)
     const int64_t wave = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
     Line line(a.batch, a.cache.page_shift, group, kv);
     const int64_t total = line.total;
-    const Shares shares(total);
+    const Shares shares(line);
     const int64_t begin = wave * shares.share, end = min(total, begin + shares.share);
     Record record{};
     Attend<D, Q4, FINE> w(a);
@@ -708,7 +717,7 @@ paged_merge_kernel(const PagedAttentionArgs a)
     if (live) {
         // (a tile's own wave has it in its second slot, the others in their first)
         const float* slot = a.workspace + RECORD_FLOATS + 2 * int64_t(blockIdx.x) * slot_floats(D);
-#pragma unroll 2
+#pragma unroll 8
         for (int p = wave; p < todo.parts; p += 4) {
             const float* const at = slot + (2 * p + (p == 0)) * slot_floats(D);
             sum.take(at[TILE_ROWS * D + r], at[TILE_ROWS * D + TILE_ROWS + r], *reinterpret_cast<const f32x4*>(at + r * D + col));
