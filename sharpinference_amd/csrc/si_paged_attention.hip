@@ -83,7 +83,9 @@ __device__ __forceinline__ Sequence take_sequence(const PagedBatch& b, int page_
     q.length = b.lengths[s];
     if (q.length < 0 || q.length > int64_t(b.max_pages) << page_shift || q.count > b.max_rows)
         q.length = -1;
-    q.tiles = q.count * group > FEW_ROWS ? 0 : (q.count * group + TILE_ROWS - 1) / TILE_ROWS;
+    // (more rows than the call said: NaN from here, the prompt kernel may not run)
+    const bool prompt = q.count * group > FEW_ROWS && q.count <= b.max_rows;
+    q.tiles = prompt ? 0 : (q.count * group + TILE_ROWS - 1) / TILE_ROWS;
     q.units = max(1, (q.length + UNIT - 1) / UNIT);
     return q;
 }
@@ -566,7 +568,7 @@ paged_attention_kernel(const PagedAttentionArgs a)
         }
         // unit x: of which KV head, tile and positions
         const int64_t in = x - q_start;
-        const uint32_t tile_no = uint32_t(quotient(in, q.units));       // at most 4 tiles and 256 heads
+        const uint32_t tile_no = uint32_t(quotient(in, q.units));       // at most 2^20 tiles and 256 heads
         const int kvh = __builtin_amdgcn_readfirstlane(int(tile_no / uint32_t(q.tiles)));
         const int row0 = __builtin_amdgcn_readfirstlane(int(tile_no - kvh * q.tiles) * TILE_ROWS);
         const int unit0 = __builtin_amdgcn_readfirstlane(int(in - int64_t(tile_no) * q.units));
@@ -791,9 +793,10 @@ struct PromptLine {
             return q;
         sequence_rows(b, s, &q.first, &q.count);
         q.length = b.lengths[s];
-        if (q.length < 0 || q.length > int64_t(b.max_pages) << page_shift || q.count > b.max_rows)
+        if (q.length < 0 || q.length > int64_t(b.max_pages) << page_shift)
             q.length = -1;
-        q.tiles = q.count * group > FEW_ROWS ? (q.count * group + PROMPT_ROWS - 1) / PROMPT_ROWS : 0;
+        const bool prompt = q.count * group > FEW_ROWS && q.count <= b.max_rows;
+        q.tiles = prompt ? (q.count * group + PROMPT_ROWS - 1) / PROMPT_ROWS : 0;
         q.a = int64_t(group) * (max(0, q.length - q.count) / UNIT + PROMPT_PIECE);
         if (cut && q.tiles) {
             q.a = (quotient(tile_weight(q, q.tiles - 1) - 1, share) + 1) * share;

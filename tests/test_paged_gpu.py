@@ -487,6 +487,22 @@ def test_sequences_that_do_not_fit(hip):
     assert np.all(u[6:8] == SENTINEL * 0x0101)
 
 
+@gpu
+@pytest.mark.parametrize("most", [1, 3, 90])
+@pytest.mark.parametrize("out_fmt", [BF16, F32])
+def test_more_rows_than_said(hip, most, out_fmt):
+    """Sequences of more rows than max_rows are NaN, however many they are; the others are right."""
+    st = Setup(hip, Q4, 128, 2, 16, [(1, 40), (100, 300), (1, 20), (4, 4), (200, 150)], seed=31).fill()
+    st.most = most
+    st.upload()
+    q = st.rng.standard_normal((st.rows, 4 * 128)).astype(np.float32)
+    got = _attend(hip, st, 4, q, out_fmt)
+    good = [t for s, (new, _) in enumerate(st.seqs) if new <= most for t in range(st.starts[s], st.starts[s + 1])]
+    bad = [t for t in range(st.used) if t not in good]
+    assert np.all(np.isnan(got[bad])) and len(bad) == {1: 304, 3: 304, 90: 300}[most]
+    _check_rows(st, 4, q, got, out_fmt, good)
+
+
 def _attend_raw(hip, st, heads, q):
     out = hip.to_device(np.full(st.rows * heads * st.d * 2, SENTINEL, np.uint8))
     ws = hip.alloc(native.paged_attention_workspace_bytes(heads, st.kv, st.d))
