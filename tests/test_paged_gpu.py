@@ -591,6 +591,37 @@ def test_two_contexts_on_one_cache(hip):
             assert np.array_equal((u.astype(np.uint32) << 16).view(np.float32).astype(np.float64), want[:st.used])
 
 
+@gpu
+@pytest.mark.parametrize("fmt", [F16, Q4])
+def test_pages_far_into_a_pool(hip, fmt):
+    """Pages more than 4 GiB into their pools: append, read, attention of few and of many rows."""
+    heads, kv, d = 4, 2, 128
+    st = Setup(hip, fmt, d, kv, 256, [(1, 300), (40, 270), (3, 5)], seed=33).fill().upload()
+    page = kv * native.paged_page_bytes(fmt, 256, d)
+    shift = 2 ** 32 // page + 3
+    pools = [hip.alloc((shift + st.pages) * page) for _ in range(2)]
+    for b, pool in zip(pools, (st.k, st.v)):
+        b.upload(pool.raw, shift * page)
+    held = (st.table >= 0) & (st.table < st.pages)
+    st.dev[0].upload(np.where(held, st.table + shift, st.table).astype(np.int32))
+    st.cache = native.PagedCache(pools[0].ptr, pools[1].ptr, shift + st.pages, 256, kv, d, fmt)
+    qkv = st.rng.standard_normal((st.rows, (heads + 2 * kv) * d)).astype(np.float32)
+    freq = (0.7 ** np.arange(d // 2)).astype(np.float32)
+    query = _append(hip, st, heads, d, qkv, freq, 1.0)
+    want = _expect_append(st, heads, d, qkv, freq, 1.0)
+    q = query.readback(np.float32).reshape(want.shape)
+    assert _same(q, want)
+    for b, pool in zip(pools, (st.k, st.v)):
+        assert np.array_equal(b.readback(np.uint8, pool.raw.size, shift * page), pool.raw.reshape(-1))
+    keys, vals = (hip.alloc(st.rows * kv * d * 4) for _ in range(2))
+    hip.paged_kv_read(st.batch, st.cache, keys.ptr, vals.ptr)
+    rows = vals.readback(np.float32).reshape(st.rows, kv, d)
+    for t in range(st.used):
+        _, p, at = ref.place(st.table, st.starts, st.lengths, 256, st.pages, t)
+        assert np.array_equal(rows[t], st.v.load(at, p % 256).astype(np.float32))
+    _check_rows(st, heads, q, _attend(hip, st, heads, q, BF16), BF16)
+
+
 # ---- an attention block of a step ------------------------------------------------------------
 
 @gpu
