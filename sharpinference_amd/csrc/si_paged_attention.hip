@@ -530,14 +530,17 @@ __device__ __forceinline__ uint32_t pack_out(float x, float y, bool bf16)
 }
 
 // Four neighbouring values of an output row, at value index `at`.
-__device__ __forceinline__ void store_out(const PagedAttentionArgs& a, int64_t at, float x, float y, float z, float w)
+__device__ __forceinline__ void store_out(const PagedAttentionArgs& a, int format, int64_t at, float x, float y, float z, float w)
 {
-    if (a.out_format == PAGED_OUT_F32)
+    if (format == PAGED_OUT_F32)
         *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(x, y, z, w);
     else
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
-            make_uint2(pack_out(x, y, a.out_format == PAGED_OUT_BF16), pack_out(z, w, a.out_format == PAGED_OUT_BF16));
+            make_uint2(pack_out(x, y, format == PAGED_OUT_BF16), pack_out(z, w, format == PAGED_OUT_BF16));
 }
+// (what is not FINE is BF16)
+template <bool FINE>
+__device__ __forceinline__ int format_of(const PagedAttentionArgs& a) { return FINE ? a.out_format : PAGED_OUT_BF16; }
 
 // Every wave takes an equal run of the line's units, whatever sequences they
 // lie in; tiles that are wholly its own are written out, the others left in
@@ -644,7 +647,7 @@ paged_attention_kernel(const PagedAttentionArgs a)
                 for (int r = 0; r < 4; r++)
 #pragma unroll
                     for (int n = 0; n < NV; n += 4)
-                        store_out(a, at + NV * r + n, st.acc[n][r] * inv, st.acc[n + 1][r] * inv, st.acc[n + 2][r] * inv,
+                        store_out(a, format_of<FINE>(a), at + NV * r + n, st.acc[n][r] * inv, st.acc[n + 1][r] * inv, st.acc[n + 2][r] * inv,
                                   st.acc[n + 3][r] * inv);
             }
         } else if (live) {
@@ -733,7 +736,7 @@ paged_merge_kernel(const PagedAttentionArgs a)
     if (!join_waves(sum) || !live)
         return;
     const float inv = sum.sum == 0.0f ? 0.0f : 1.0f / sum.sum;
-    store_out(a, ((int64_t(todo.first) + i) * a.heads + todo.kvh * group + packed % group) * D + col, sum.acc[0] * inv,
+    store_out(a, a.out_format, ((int64_t(todo.first) + i) * a.heads + todo.kvh * group + packed % group) * D + col, sum.acc[0] * inv,
               sum.acc[1] * inv, sum.acc[2] * inv, sum.acc[3] * inv);
 }
 
@@ -1351,7 +1354,7 @@ paged_prompt_kernel(const PagedAttentionArgs a)
             for (int n = 0; n < NC; n++)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4)
-                    store_out(a, out + 32 * n + 2 * e, acc[n][e] * inv, acc[n][e + 1] * inv, acc[n][e + 2] * inv,
+                    store_out(a, format_of<FINE>(a), out + 32 * n + 2 * e, acc[n][e] * inv, acc[n][e + 1] * inv, acc[n][e + 2] * inv,
                               acc[n][e + 3] * inv);
         } else if (row0 + 32 * wave < q.count * group) {
             float* const slot = a.workspace + prompt_workspace(D) + (2 * worker + (lo == 0)) * prompt_slot_floats(D);
@@ -1395,7 +1398,7 @@ paged_prompt_merge_kernel(const PagedAttentionArgs a)
             return;
         const int col = 8 * (piece % PIECES) + 4 * (lane >> 5);
         const float inv = sum.sum == 0.0f ? 0.0f : 1.0f / sum.sum;
-        store_out(a, ((int64_t(todo.first) + i) * a.heads + todo.kvh * group + packed % group) * D + col, sum.acc[0] * inv,
+        store_out(a, a.out_format, ((int64_t(todo.first) + i) * a.heads + todo.kvh * group + packed % group) * D + col, sum.acc[0] * inv,
                   sum.acc[1] * inv, sum.acc[2] * inv, sum.acc[3] * inv);
     };
     // Few slots: a piece a wave.  Many: its waves take them in turn.
