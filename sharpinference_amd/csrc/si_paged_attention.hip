@@ -1150,6 +1150,9 @@ paged_prompt_kernel(const PagedAttentionArgs a)
         // that are not there: page 0 is read in their place.
         int held = 0, held_at = -1;
         uint64_t held_lost = 0;
+        const char* const keys = a.cache.keys + kvh * head_bytes;
+        const char* const values = a.cache.values + kvh * head_bytes;
+        const uint32_t page_bytes = uint32_t(a.cache.kv_heads * head_bytes);       // at most 16 MiB
         auto load = [&](int u) -> uint32_t {
             if (u >> 4 != held_at) {
                 held_at = u >> 4;
@@ -1161,9 +1164,8 @@ paged_prompt_kernel(const PagedAttentionArgs a)
             }
             const int granule = (u & 15) * 4 + (wave >> 1);
             const int page = max(0, __builtin_amdgcn_readlane(held, granule));
-            const int64_t head = (int64_t(page) * a.cache.kv_heads + kvh) * head_bytes;
-            raw.load(a.cache.keys + head, a.cache.values + head, (u * UNIT + (wave >> 1) * GRANULE) & (a.cache.page_size - 1),
-                     a.cache.page_size);
+            const uint64_t at = uint64_t(uint32_t(page)) * page_bytes;
+            raw.load(keys + at, values + at, (u * UNIT + (wave >> 1) * GRANULE) & (a.cache.page_size - 1), a.cache.page_size);
             return uint32_t(held_lost >> (u & 15) * 4) & 15;
         };
         auto partial = [&](int u) { return u * UNIT + UNIT - 1 > least; };
@@ -1306,8 +1308,9 @@ paged_prompt_kernel(const PagedAttentionArgs a)
                     if constexpr (FINE)
                         pl[b][e >> 3].w[(e & 7) >> 1] = as_u32(f16x2{_Float16(x - float(p[0])), _Float16(y - float(p[1]))});
                 }
-            // (last read for unit u - 1, next marked for unit u + 2)
-            if (threadIdx.x < 2)
+            // (last read for unit u - 1, next marked for unit u + 2; marked for
+            // partial units alone, which are the last ones)
+            if (partial(u + 2) && threadIdx.x < 2)
                 odd[(u + 2) % 3][threadIdx.x] = 0;
             read_values(u, 0, 0);
             if constexpr (AHEAD > 1)
