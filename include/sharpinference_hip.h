@@ -581,6 +581,7 @@ typedef struct si_hip_paged_attention_args {
     int32_t output_format;     /* SI_HIP_F32, SI_HIP_F16 or SI_HIP_BF16 */
 } si_hip_paged_attention_args;
 
+/* Whatever the batch: about 98 MiB for heads of 128 values, 50 MiB for 64. */
 int si_hip_paged_attention_workspace_bytes(int query_heads, int kv_heads, int head_size, uint64_t* bytes);
 
 /* output_t,h = softmax(q_t,h . K^T / sqrt(head_size)) . V over the positions

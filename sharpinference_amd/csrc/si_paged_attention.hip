@@ -748,11 +748,12 @@ paged_merge_kernel(const PagedAttentionArgs a)
 // next unit's bytes are loaded while this one is multiplied.  Scores stay
 // transposed here too, with v_mfma_f32_32x32x16_f16.
 //
-// What bounds it: of the 5000 cycles that a unit of 64 positions takes, the two
-// waves of a SIMD spend 2050 in matrix instructions and 2300 in vector ones (a
-// quarter of them the exponentials), which overlap little.  840 TFLOP/s within
-// the units, 0.55 of what a large matrix product reaches.
-// 128 rows in four waves: 252 us where this takes 233 (chunks of up to 2000 rows
+// What bounds it: of the 4880 cycles that a unit of 64 positions takes, the two
+// waves of a SIMD spend 2050 in matrix instructions and 2100 in vector ones (580
+// of them the exponentials), which overlap little.  840 TFLOP/s within the units
+// at the 1.95 GHz that the card then runs at, 0.55 of what a large matrix product
+// reaches.
+// 128 rows in four waves: 252 us where this takes 229 (chunks of up to 2000 rows
 // over up to 6000 positions).
 constexpr int PROMPT_ROWS = 256;
 constexpr int PROMPT_THREADS = 512;
