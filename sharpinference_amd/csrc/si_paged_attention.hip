@@ -559,10 +559,14 @@ paged_attention_kernel(const PagedAttentionArgs a)
 {
     constexpr int NV = D / 16;
     const int kv = a.cache.kv_heads, group = a.heads / kv;
-    const int64_t wave = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
     Line line(a.batch, a.cache.page_shift, group, kv);
     const int64_t total = line.total;
     const Shares shares(line);
+    // Neighbours in the line on one die (workgroup b runs on die b % 8): the tiles
+    // of a sequence's rows go through the same pages, and meet in its L2.
+    const int per = int(quotient(total + 32 * shares.share - 1, 32 * shares.share));       // workgroups of a die
+    const int block = int(blockIdx.x) / 8 < per ? int(blockIdx.x) % 8 * per + int(blockIdx.x) / 8 : int(blockIdx.x);
+    const int64_t wave = int64_t(block) * 4 + (threadIdx.x >> 6);
     const int64_t begin = wave * shares.share, end = min(total, begin + shares.share);
     Record record{};
     Attend<D, Q4, FINE> w(a);
