@@ -64,6 +64,7 @@ struct PagedAttentionArgs {
     float* workspace;
     int heads;
     int out_format;            // PagedOut
+    int few_rows;              // set by the launch
 };
 
 int64_t paged_attention_workspace_floats(int heads, int kv_heads, int head);

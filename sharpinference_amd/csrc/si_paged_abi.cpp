@@ -237,7 +237,8 @@ int si_hip_paged_attention(si_hip_context* ctx, const si_hip_paged_attention_arg
                                    args->query_heads,
                                    args->output_format == SI_HIP_F32   ? si::PAGED_OUT_F32
                                    : args->output_format == SI_HIP_F16 ? si::PAGED_OUT_F16
-                                                                       : si::PAGED_OUT_BF16};
+                                                                       : si::PAGED_OUT_BF16,
+                                   0};
     return launched(ctx, si::launch_paged_attention(a, ctx->stream), op);
 }
 

@@ -24,7 +24,6 @@ using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
 using f32x4 = float __attribute__((ext_vector_type(4)));
 
 constexpr int TILE_ROWS = 16;            // packed query rows (position, head of the group) of a tile
-constexpr int FEW_ROWS = 64;             // sequences of more packed rows go to the prompt kernel
 constexpr int UNIT = 64;                 // positions of a step: four granules of 16
 constexpr int GRANULE = 16;              // positions that always lie in one page
 
@@ -74,7 +73,8 @@ struct Sequence {
     int units;
 };
 
-__device__ __forceinline__ Sequence take_sequence(const PagedBatch& b, int page_shift, int group, int s)
+// few: sequences of more packed rows are the prompt kernel's
+__device__ __forceinline__ Sequence take_sequence(const PagedBatch& b, int page_shift, int group, int few, int s)
 {
     Sequence q{s, 0, 0, 0, 0, 0};
     if (s >= b.sequences)
@@ -84,7 +84,7 @@ __device__ __forceinline__ Sequence take_sequence(const PagedBatch& b, int page_
     if (q.length < 0 || q.length > int64_t(b.max_pages) << page_shift || q.count > b.max_rows)
         q.length = -1;
     // (more rows than the call said: NaN from here, the prompt kernel may not run)
-    const bool prompt = q.count * group > FEW_ROWS && q.count <= b.max_rows;
+    const bool prompt = q.count * group > few && q.count <= b.max_rows;
     q.tiles = prompt ? 0 : (q.count * group + TILE_ROWS - 1) / TILE_ROWS;
     q.units = max(1, (q.length + UNIT - 1) / UNIT);
     return q;
@@ -139,7 +139,7 @@ constexpr int LONG = 128;                // units: see Shares
 // one sequence a lane.
 struct Line {
     const PagedBatch& b;
-    int page_shift, group, kv;
+    int page_shift, group, kv, few;
     int64_t total;             // units
     bool some_long;            // a tile is more than LONG units
     // up to 64 sequences are looked at once: the lane's, and the units up to it
@@ -149,11 +149,12 @@ struct Line {
     __device__ __forceinline__ int64_t units_of(const Sequence& q) const { return int64_t(kv) * q.tiles * q.units; }
     __device__ __forceinline__ void look(int base, int64_t before)
     {
-        mine = take_sequence(b, page_shift, group, base + int(threadIdx.x & 63));
+        mine = take_sequence(b, page_shift, group, few, base + int(threadIdx.x & 63));
         upto = before + wave_scan(units_of(mine));
     }
-    __device__ __forceinline__ Line(const PagedBatch& batch, int shift, int heads_per_kv, int kv_heads)
-        : b(batch), page_shift(shift), group(heads_per_kv), kv(kv_heads), total(0), some_long(false)
+    __device__ __forceinline__ explicit Line(const PagedAttentionArgs& a)
+        : b(a.batch), page_shift(a.cache.page_shift), group(a.heads / a.cache.kv_heads), kv(a.cache.kv_heads),
+          few(a.few_rows), total(0), some_long(false)
     {
         for (int base = 0; base < b.sequences; base += 64) {
             look(base, total);
@@ -559,7 +560,7 @@ paged_attention_kernel(const PagedAttentionArgs a)
 {
     constexpr int NV = D / 16;
     const int kv = a.cache.kv_heads, group = a.heads / kv;
-    Line line(a.batch, a.cache.page_shift, group, kv);
+    Line line(a);
     const int64_t total = line.total;
     const Shares shares(line);
     // Neighbours in the line on one die (workgroup b runs on die b % 8): the tiles
@@ -792,7 +793,7 @@ struct PromptSequence {
 // share), and no worker has more than one part.
 struct PromptLine {
     const PagedBatch& b;
-    int page_shift, group, kv;
+    int page_shift, group, kv, few;
     int64_t share;             // of a worker
     bool cut;                  // into parts
 
@@ -808,7 +809,7 @@ struct PromptLine {
         q.length = b.lengths[s];
         if (q.length < 0 || q.length > int64_t(b.max_pages) << page_shift)
             q.length = -1;
-        const bool prompt = q.count * group > FEW_ROWS && q.count <= b.max_rows;
+        const bool prompt = q.count * group > few && q.count <= b.max_rows;
         q.tiles = prompt ? (q.count * group + PROMPT_ROWS - 1) / PROMPT_ROWS : 0;
         q.a = int64_t(group) * (max(0, q.length - q.count) / UNIT + PROMPT_PIECE);
         if (cut && q.tiles) {
@@ -817,8 +818,9 @@ struct PromptLine {
         }
         return q;
     }
-    __device__ __forceinline__ PromptLine(const PagedBatch& batch, int shift, int heads_per_kv, int kv_heads)
-        : b(batch), page_shift(shift), group(heads_per_kv), kv(kv_heads), share(0), cut(false)
+    __device__ __forceinline__ explicit PromptLine(const PagedAttentionArgs& a)
+        : b(a.batch), page_shift(a.cache.page_shift), group(a.heads / a.cache.kv_heads), kv(a.cache.kv_heads),
+          few(a.few_rows), share(0), cut(false)
     {
         // all weight, tiles, and the weight if a sequence's tiles were all like its last
         int64_t total = 0, tiles = 0, last = 0;
@@ -1073,7 +1075,7 @@ paged_prompt_kernel(const PagedAttentionArgs a)
     const int kv = a.cache.kv_heads, group = a.heads / kv;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
     const int64_t head_bytes = paged_head_bytes(Q4, a.cache.page_size, D);
-    const PromptLine line(a.batch, a.cache.page_shift, group, kv);
+    const PromptLine line(a);
     // neighbours in the line on one die (workgroup b runs on die b % 8): they
     // go through the same keys and values, and meet in its L2
     const int64_t worker = int64_t(blockIdx.x % 8) * (PROMPT_WORKERS / 8) + blockIdx.x / 8;
@@ -1436,7 +1438,7 @@ hipError_t launch(const PagedAttentionArgs& a, hipStream_t s)
     const unsigned tile_rows = unsigned(min(int64_t(TILE_ROWS), most));
     paged_attention_kernel<D, Q4, FINE><<<WAVES / 4, 256, 0, s>>>(a);
     paged_merge_kernel<D><<<dim3(WAVES, (tile_rows + 256 / D - 1) / (256 / D)), 256, 0, s>>>(a);
-    if (most > FEW_ROWS) {
+    if (most > a.few_rows) {
         paged_prompt_kernel<D, Q4, FINE><<<PROMPT_WORKERS, PROMPT_THREADS, 0, s>>>(a);
         paged_prompt_merge_kernel<D><<<dim3(PROMPT_ROWS * D / 1024, PROMPT_WORKERS), 256, 0, s>>>(a);
     }
@@ -1461,7 +1463,17 @@ int64_t paged_attention_workspace_floats(int, int, int head)
 
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s)
 {
-    return a.cache.head == 128 ? launch<128>(a, s) : launch<64>(a, s);
+    // Sequences of how many packed rows go to the prompt kernel.  It turns a unit
+    // into FP16 once for 256 rows and the other does for 16, but a launch of both
+    // costs 20 us more, and few tiles do not fill its workgroups.  Rows a sequence,
+    // us with 128 and 64 here: 4 sequences of 126 rows and up to 300 positions 20 and
+    // 31, one of 126 and 9000 37 and 49, 8 of 72 to 128 and 2000 to 6000 34 and 48;
+    // but 16 of 126 and 3000 to 9000 183 and 143 (of 96: 145 and 140, of 72: 134 and
+    // 144).
+    const int64_t group = a.heads / a.cache.kv_heads, most = a.batch.max_rows * group, all = a.batch.rows * group;
+    PagedAttentionArgs b = a;
+    b.few_rows = most <= 96 || (most <= 128 && all <= 1024) ? 128 : 64;
+    return a.cache.head == 128 ? launch<128>(b, s) : launch<64>(b, s);
 }
 
 }  // namespace si

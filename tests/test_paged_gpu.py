@@ -488,6 +488,17 @@ def test_sequences_that_do_not_fit(hip):
 
 
 @gpu
+@pytest.mark.parametrize("fmt,out_fmt", [(Q4, BF16), (F16, F16), (Q4, F32)])
+@pytest.mark.parametrize("head,more", [(128, []), (64, []), (128, [(60, 100)]), (64, [(43, 43)]), (128, [(33, 70)] * 9)])
+def test_attention_between_few_and_many(hip, fmt, out_fmt, head, more):
+    """Sequences of 48 to 128 packed rows, alone, beside one of more, and in a larger batch."""
+    seqs = [(22, 300), (40, 40), (1, 9), (16, 130), (42, 501), (21, 21)] + more
+    st = Setup(hip, fmt, head, 2, 64, seqs, seed=35).fill().upload()
+    q = st.rng.standard_normal((st.rows, 6 * head)).astype(np.float32)
+    _check_rows(st, 6, q, _attend(hip, st, 6, q, out_fmt), out_fmt)
+
+
+@gpu
 @pytest.mark.parametrize("most", [1, 3, 90])
 @pytest.mark.parametrize("out_fmt", [BF16, F32])
 def test_more_rows_than_said(hip, most, out_fmt):
