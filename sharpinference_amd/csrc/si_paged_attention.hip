@@ -712,26 +712,21 @@ __device__ __forceinline__ bool join_waves(Joined& sum)
     return true;
 }
 
-// Joins the tiles that several waves share: workgroup x the one that begins
-// in wave x and ends behind it, 256 / D rows of it, four values a lane; its
-// waves take the slots in turn.
+// Joins the tile that begins in wave `owner` and ends behind it: rows 256 / D x
+// `piece` and on, four values a lane; the workgroup's waves take the slots in turn.
 template <int D>
-__global__ void __launch_bounds__(256)
-paged_merge_kernel(const PagedAttentionArgs a)
+__device__ __forceinline__ void join_tile(const PagedAttentionArgs& a, const Record& todo, int owner, int piece)
 {
-    const Record todo = records(a.workspace)[blockIdx.x];
-    if (todo.parts == 0)
-        return;
     constexpr int ROWS = 256 / D;
     const int group = a.heads / a.cache.kv_heads;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int r = int(blockIdx.y) * ROWS + lane / (D / 4), col = 4 * (lane % (D / 4));
+    const int r = piece * ROWS + lane / (D / 4), col = 4 * (lane % (D / 4));
     const int packed = todo.row0 + r, i = packed / group;
     const bool live = i < todo.count;
     Joined sum;
     if (live) {
         // (a tile's own wave has it in its second slot, the others in their first)
-        const float* slot = a.workspace + RECORD_FLOATS + 2 * int64_t(blockIdx.x) * slot_floats(D);
+        const float* slot = a.workspace + RECORD_FLOATS + 2 * int64_t(owner) * slot_floats(D);
 #pragma unroll 8
         for (int p = wave; p < todo.parts; p += 4) {
             const float* const at = slot + (2 * p + (p == 0)) * slot_floats(D);
@@ -743,6 +738,16 @@ paged_merge_kernel(const PagedAttentionArgs a)
     const float inv = sum.sum == 0.0f ? 0.0f : 1.0f / sum.sum;
     store_out(a, a.out_format, ((int64_t(todo.first) + i) * a.heads + todo.kvh * group + packed % group) * D + col, sum.acc[0] * inv,
               sum.acc[1] * inv, sum.acc[2] * inv, sum.acc[3] * inv);
+}
+
+// Joins the tiles that several waves share: workgroup x the one that begins in wave x.
+template <int D>
+__global__ void __launch_bounds__(256)
+paged_merge_kernel(const PagedAttentionArgs a)
+{
+    const Record todo = records(a.workspace)[blockIdx.x];
+    if (todo.parts)
+        join_tile<D>(a, todo, blockIdx.x, blockIdx.y);
 }
 
 // ---- many rows of a sequence ------------------------------------------------------------
@@ -1384,19 +1389,33 @@ paged_prompt_kernel(const PagedAttentionArgs a)
         records(a.workspace)[WAVES + worker] = record;
 }
 
-// Joins the tiles that several workers share: workgroups y the one that
-// begins in worker y and ends behind it, each four pieces of 64 lanes' values.
+// Joins the tiles that several workers share, the one that begins in worker y and
+// ends behind it by as many workgroups as x has, each four pieces of 64 lanes'
+// values; and, in two workgroups each before those, the tiles that several waves of
+// the other kernel share (one launch less: 3 to 5 us).
+constexpr int prompt_merge_parts(int d) { return PROMPT_ROWS * d / 1024; }
 template <int D>
 __global__ void __launch_bounds__(256)
 paged_prompt_merge_kernel(const PagedAttentionArgs a)
 {
-    const Record todo = records(a.workspace)[WAVES + blockIdx.y];
+    if (blockIdx.x < WAVES * 2) {
+        const int wave = int(blockIdx.x) % WAVES, half = int(blockIdx.x) / WAVES;
+        const Record todo = records(a.workspace)[wave];
+        if (todo.parts)
+            for (int k = 0; k < TILE_ROWS * D / 512; k++) {
+                join_tile<D>(a, todo, wave, half * (TILE_ROWS * D / 512) + k);
+                __syncthreads();
+            }
+        return;
+    }
+    const int block = int(blockIdx.x) - WAVES * 2, worker = block / prompt_merge_parts(D), part = block % prompt_merge_parts(D);
+    const Record todo = records(a.workspace)[WAVES + worker];
     if (todo.parts == 0)
         return;
     constexpr int PIECES = D / 8;                         // of 32 rows
     const int group = a.heads / a.cache.kv_heads;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const float* const slot = a.workspace + prompt_workspace(D) + 2 * int64_t(blockIdx.y) * prompt_slot_floats(D);
+    const float* const slot = a.workspace + prompt_workspace(D) + 2 * int64_t(worker) * prompt_slot_floats(D);
     auto take = [&](Joined& sum, int piece, int r, int p) {
         // (a tile's own worker has it in its second slot, the others in their first)
         const float* const at = slot + (2 * p + (p == 0)) * int64_t(prompt_slot_floats(D));
@@ -1415,7 +1434,7 @@ paged_prompt_merge_kernel(const PagedAttentionArgs a)
     const bool turns = todo.parts > 4;
 #pragma unroll 1
     for (int k = 0; k < (turns ? 4 : 1); k++) {
-        const int piece = 4 * int(blockIdx.x) + (turns ? k : wave), r = 32 * (piece / PIECES) + (lane & 31);
+        const int piece = 4 * part + (turns ? k : wave), r = 32 * (piece / PIECES) + (lane & 31);
         // (rows that are not in the sequence were not stored)
         if (todo.row0 + 32 * (piece / PIECES) >= todo.count * group)
             return;
@@ -1437,10 +1456,11 @@ hipError_t launch(const PagedAttentionArgs& a, hipStream_t s)
     const int64_t most = int64_t(a.batch.max_rows) * group;       // packed rows of a sequence
     const unsigned tile_rows = unsigned(min(int64_t(TILE_ROWS), most));
     paged_attention_kernel<D, Q4, FINE><<<WAVES / 4, 256, 0, s>>>(a);
-    paged_merge_kernel<D><<<dim3(WAVES, (tile_rows + 256 / D - 1) / (256 / D)), 256, 0, s>>>(a);
     if (most > a.few_rows) {
         paged_prompt_kernel<D, Q4, FINE><<<PROMPT_WORKERS, PROMPT_THREADS, 0, s>>>(a);
-        paged_prompt_merge_kernel<D><<<dim3(PROMPT_ROWS * D / 1024, PROMPT_WORKERS), 256, 0, s>>>(a);
+        paged_prompt_merge_kernel<D><<<2 * WAVES + PROMPT_WORKERS * prompt_merge_parts(D), 256, 0, s>>>(a);
+    } else {
+        paged_merge_kernel<D><<<dim3(WAVES, (tile_rows + 256 / D - 1) / (256 / D)), 256, 0, s>>>(a);
     }
     return hipGetLastError();
 }
