@@ -584,6 +584,39 @@ def test_plan_serves_growing_sequences(hip):
 
 
 @gpu
+@pytest.mark.parametrize("fmt,out_fmt", [(Q4, BF16), (F16, F32)])
+def test_plan_serves_changing_batches(hip, fmt, out_fmt):
+    """One recorded call over batches whose rows move between prompts, drafts and single
+    tokens; eager calls in between, the workspace never cleared."""
+    heads, kv, d = 6, 2, 128
+    st = Setup(hip, fmt, d, kv, 32, [(100, 420), (100, 420), (1, 420)], seed=37, spare_rows=0).fill().upload()
+    out = hip.alloc(st.rows * heads * d * (4 if out_fmt == F32 else 2))
+    ws = hip.alloc(native.paged_attention_workspace_bytes(heads, kv, d))
+    q = st.rng.standard_normal((st.rows, heads * d)).astype(np.float32)
+    dq = hip.to_device(q)
+    att = native.PagedAttentionArgs(st.batch, st.cache, dq.ptr, out.ptr, ws.ptr, heads, out_fmt)
+    # (twice: a plan of more than four kernels is a graph)
+    plan = hip.record(lambda: [hip.paged_attention(att) for _ in range(2)])
+    for seqs in ([(100, 420), (90, 90), (1, 33)], [(1, 400), (1, 7), (1, 64)], [(30, 30), (3, 420), (70, 300)],
+                 [(0, 5), (100, 100), (0, 0)], [(1, 1), (40, 411), (100, 420)]):
+        st.seqs = seqs
+        st.starts = np.concatenate([[0], np.cumsum([n for n, _ in seqs])]).astype(np.int32)
+        st.used = int(st.starts[-1])
+        st.dev[1].upload(st.starts)
+        st.dev[2].upload(np.array([l for _, l in seqs], np.int32))
+        raws = []
+        for call in (plan.launch, lambda: hip.paged_attention(att), plan.launch):
+            hip.fill_u32(out.ptr, 0xFFFFFFFF, out.nbytes // 4)
+            call()
+            raws.append(out.readback(np.uint32 if out_fmt == F32 else np.uint16).reshape(st.rows, heads, d))
+        assert all(np.array_equal(raws[0], r) for r in raws[1:])
+        assert np.all(raws[0][st.used:] == raws[0].dtype.type(-1 & 0xFFFFFFFF if out_fmt == F32 else 0xFFFF))
+        got = raws[0].view(np.float32) if out_fmt == F32 else (raws[0].astype(np.uint32) << 16).view(np.float32)
+        _check_rows(st, heads, q, got.astype(np.float64), out_fmt)
+    plan.destroy()
+
+
+@gpu
 def test_two_contexts_on_one_cache(hip):
     """Another context's stream, workspaces of their own."""
     st = Setup(hip, F16, 128, 2, 32, [(1, 500), (30, 200)], seed=16).fill().upload()
