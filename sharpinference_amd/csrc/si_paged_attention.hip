@@ -1114,7 +1114,8 @@ paged_prompt_kernel(const PagedAttentionArgs a)
         const int last_row = min(q.count - 1, (row0 + PROMPT_ROWS - 1) / group);
         const int most = __builtin_amdgcn_readfirstlane(wrong ? -1 : q.length - q.count + last_row);
         const int least = __builtin_amdgcn_readfirstlane(q.length - q.count + row0 / group);
-        const int units = (most + UNIT) / UNIT;           // of this tile, 0 where no row sees anything
+        // of this tile; 0 where no row sees anything, however far before position 0 its rows lie
+        const int units = max(0, (most + UNIT) / UNIT);
         const int unit0 = __builtin_amdgcn_readfirstlane(int(quotient(units * lo, weight)));
         const int unit1 = __builtin_amdgcn_readfirstlane(int(quotient(units * hi, weight)));
         const int32_t* const table = a.batch.table + int64_t(q.index) * a.batch.max_pages;

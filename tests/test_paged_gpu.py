@@ -514,6 +514,25 @@ def test_more_rows_than_said(hip, most, out_fmt):
     _check_rows(st, 4, q, got, out_fmt, good)
 
 
+@gpu
+@pytest.mark.parametrize("head,heads,kv,seqs", [
+    (64, 1, 1, [(4096, 500)]),                             # sixteen tiles in eight parts each, fourteen of them see nothing
+    (64, 4, 2, [(900, 130), (1, 70), (700, 0)]),
+    (128, 3, 1, [(1000, 1000), (1000, 64), (1000, 63)]),
+])
+@pytest.mark.parametrize("fmt,out_fmt", [(Q4, BF16), (F16, F32)])
+def test_prompts_with_more_rows_than_positions(hip, fmt, out_fmt, head, heads, kv, seqs):
+    """Whole tiles of rows far before position 0, shared between workgroups: 0, and the rows behind them are right."""
+    st = Setup(hip, fmt, head, kv, 16, seqs, seed=41).fill().upload()
+    q = st.rng.standard_normal((st.rows, heads * head)).astype(np.float32)
+    got = _attend(hip, st, heads, q, out_fmt)
+    for s, (new, length) in enumerate(seqs):
+        assert np.all(got[st.starts[s]:st.starts[s] + max(0, new - length)] == 0)
+    seen = [t for s, (new, length) in enumerate(seqs) for t in range(st.starts[s] + max(0, new - length), st.starts[s + 1])]
+    pick = set(int(t) for t in st.rng.choice(seen, min(len(seen), 300), replace=False))
+    _check_rows(st, heads, q, got, out_fmt, pick)
+
+
 def _attend_raw(hip, st, heads, q):
     out = hip.to_device(np.full(st.rows * heads * st.d * 2, SENTINEL, np.uint8))
     ws = hip.alloc(native.paged_attention_workspace_bytes(heads, st.kv, st.d))
