@@ -590,7 +590,8 @@ int si_hip_paged_attention_workspace_bytes(int query_heads, int kv_heads, int he
  * cores, statistics and sums in FP32: for BF16 outputs of FP16 operands
  * (queries / sqrt(head_size) times log2(e), cached values and exponentials
  * rounded to fp16 once), for F16 and F32 outputs of operands in two fp16
- * terms (22 bits; cached values exact).  A row before
+ * terms (22 bits; cached values exact); an exponential is off by that much or
+ * by 2^-32 (F16 and F32 outputs: 2^-38) of its row's largest.  A row before
  * position 0 (a sequence with fewer positions than rows) sees nothing and
  * is 0.  A row that sees a page outside 0..pages - 1, a cached infinity or
  * NaN or a 4-bit scale beyond +-8188 (values that fp16 cannot hold; append

@@ -54,6 +54,19 @@ union Frag {
     f16x8 v;
 };
 
+// The weights 2^(s - at) go into the second product as FP16, whose smallest step is
+// 2^-24 (of their second terms too): relative to the largest score itself, a weight
+// below 2^-14 of the largest would lose bits and one below 2^-25 be nothing, however
+// many there are.  So `at` lies `room` below that score; sums and accumulators carry
+// the factor 2^room, and the division takes it out.  Weights stay under 2^15, half of
+// FP16's range.
+constexpr float WEIGHTS_UNDER = 15.0f;
+__device__ __forceinline__ float reference(float top, float room)
+{
+    const float at = fmaxf(top, -3.4028235e38f), low = at - room;      // (a row that has seen nothing yet)
+    return at - low <= WEIGHTS_UNDER ? low : at;   // (beyond 2^27 the difference may round to 16 and more)
+}
+
 // Rows of sequence s, as far as the batch's buffers hold them.
 __device__ __forceinline__ void sequence_rows(const PagedBatch& b, int s, int* first, int* count)
 {
@@ -210,7 +223,7 @@ struct Record {
 };
 
 // What a wave leaves of a tile whose units it shares with other waves: the
-// accumulators [TILE_ROWS][D], largest scores and sums [TILE_ROWS] each.
+// accumulators [TILE_ROWS][D], what they are relative to and sums [TILE_ROWS] each.
 // Slot 2 w: of the tile that began before wave w's units, slot 2 w + 1: of
 // the one that goes on behind them.
 constexpr int slot_floats(int d) { return TILE_ROWS * d + 2 * TILE_ROWS; }
@@ -226,6 +239,7 @@ struct State {
     static constexpr int NV = D / 16;
     f32x4 acc[NV];             // acc[n][i]: column NV * (4 * (lane >> 4) + i) + n
     float top;                 // largest score so far (in units of log 2)
+    float at;                  // what the weights are relative to
     float sum;                 // of this lane's positions
 };
 
@@ -247,6 +261,7 @@ template <int D, bool Q4, bool FINE>
 struct Attend {
     static constexpr int NJ = D / 32;    // products of 32 values that a score takes
     static constexpr int NV = D / 16;    // column sets of a row of values
+    static constexpr float ROOM = 14.0f; // weights of up to 2^14
     const PagedAttentionArgs& a;
     int lane, g, c;
     int64_t head_bytes;
@@ -418,33 +433,41 @@ struct Attend {
             for (int i = 0; i < 4; i++)
                 top = fmaxf(top, s[u][i]);
         top = rows_max(top);
-        const float at = fmaxf(top, -3.4028235e38f);      // (a row that has seen nothing yet)
         if (__any(top > st.top)) {
-            const float fade = __builtin_amdgcn_exp2f(st.top - at);
+            const float at = reference(top, ROOM), fade = __builtin_amdgcn_exp2f(st.at - at);
             st.sum *= fade;
 #pragma unroll
             for (int n = 0; n < NV; n++)
                 st.acc[n] *= fade;
             st.top = top;
+            st.at = at;
         }
+        // (a unit's weights are summed by themselves: added one by one to a sum that
+        // one weight dominates, ten thousand of them would lose 2^-11 of it)
         Frag pf[2], pl[2];
+        float sum = 0.0f;
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             float p[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                p[i] = __builtin_amdgcn_exp2f(s[u][i] - at);
-                st.sum += p[i];
+                p[i] = __builtin_amdgcn_exp2f(s[u][i] - st.at);
+                if constexpr (FINE)
+                    sum += p[i];
             }
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const f16x2 h = {_Float16(p[2 * k]), _Float16(p[2 * k + 1])};
                 pf[u >> 1].w[2 * (u & 1) + k] = as_u32(h);
+                // (the sum of what the product takes: their roundings cancel in the division)
+                if constexpr (!FINE)
+                    sum = __builtin_amdgcn_fdot2(h, f16x2{_Float16(1.0f), _Float16(1.0f)}, sum, false);
                 if constexpr (FINE)
                     pl[u >> 1].w[2 * (u & 1) + k] =
                         as_u32(f16x2{_Float16(p[2 * k] - float(h[0])), _Float16(p[2 * k + 1] - float(h[1]))});
             }
         }
+        st.sum += sum;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             uint32_t lo[4], hi[4];                         // 4-bit: words of two positions by halves
@@ -601,6 +624,7 @@ paged_attention_kernel(const PagedAttentionArgs a)
         for (int n = 0; n < NV; n++)
             st.acc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         st.top = -INFINITY;
+        st.at = reference(st.top, 0.0f);
         st.sum = 0.0f;
         // the last position that a row of the tile sees, and that all of them see
         const int last_row = min(q.count - 1, (row0 + TILE_ROWS - 1) / group);
@@ -665,7 +689,7 @@ paged_attention_kernel(const PagedAttentionArgs a)
                     *reinterpret_cast<f32x4*>(at + NV * r + n) =
                         f32x4{st.acc[n][r], st.acc[n + 1][r], st.acc[n + 2][r], st.acc[n + 3][r]};
             if (w.g == 0) {
-                slot[TILE_ROWS * D + w.c] = st.top;
+                slot[TILE_ROWS * D + w.c] = st.at;
                 slot[TILE_ROWS * D + TILE_ROWS + w.c] = sum;
             }
         }
@@ -677,8 +701,8 @@ paged_attention_kernel(const PagedAttentionArgs a)
 }
 
 // Joins what `parts` slots, `stride` floats apart, hold of four neighbouring
-// values of a row: those of its accumulators at `at`, its largest score and
-// sum at `stats` and `stats` + rows.
+// values of a row: those of its accumulators at `at`, what it is relative to and
+// its sum at `stats` and `stats` + rows.
 struct Joined {
     float top = -INFINITY, sum = 0.0f;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -767,11 +791,12 @@ paged_merge_kernel(const PagedAttentionArgs a)
 // over up to 6000 positions).
 constexpr int PROMPT_ROWS = 256;
 constexpr int PROMPT_THREADS = 512;
-// What the scores are taken relative to follows their maximum only when that is
-// further above it: the exponentials stay under 2^8, far from FP16's end, and the
-// accumulators are rescaled a few times a row instead of once a unit (440
-// vector instructions a unit then, 300 now).
-constexpr float REFERENCE_SLACK = 8.0f;
+// What the scores are taken relative to follows their maximum only when the weights
+// would pass 2^15 (WEIGHTS_UNDER): the accumulators are rescaled a few times a row
+// instead of once a unit (440 vector instructions a unit then, 300 now).  It then lies
+// this far below the maximum: a maximum that grows by 8, or (two-term operands,
+// whose weights are to keep their bits further down) by 2, moves it again.
+constexpr float prompt_room(bool fine) { return fine ? 13.0f : 7.0f; }
 constexpr int PROMPT_PIECE = 7;          // what a piece of a tile costs besides its units, in units
 constexpr int PROMPT_MIN = 9;            // units that a worker takes at least, with a piece's cost
 
@@ -1299,8 +1324,9 @@ paged_prompt_kernel(const PagedAttentionArgs a)
             if (__any(top > gate)) {
                 // (a row that has seen nothing yet has nothing to rescale, and its
                 // first score may be far below 0)
-                const float by = top > gate ? top : 0.0f, fade = top > gate && gate < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-by);
-                gate = top > gate ? REFERENCE_SLACK : gate;
+                const float by = top > gate ? reference(top, prompt_room(FINE)) : 0.0f;
+                const float fade = top > gate && gate < 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-by);
+                gate = top > gate ? WEIGHTS_UNDER : gate;
                 ref += by;
                 sum *= fade;
 #pragma unroll
@@ -1310,6 +1336,7 @@ paged_prompt_kernel(const PagedAttentionArgs a)
                 for (int b = 0; b < 2; b++)
                     s[b] -= by;
             }
+            float more = 0.0f;
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -1317,10 +1344,11 @@ paged_prompt_kernel(const PagedAttentionArgs a)
                     const float x = __builtin_amdgcn_exp2f(s[b][e]), y = __builtin_amdgcn_exp2f(s[b][e + 1]);
                     const f16x2 p = {_Float16(x), _Float16(y)};
                     pf[b][e >> 3].w[(e & 7) >> 1] = as_u32(p);
-                    sum = FINE ? sum + (x + y) : __builtin_amdgcn_fdot2(p, f16x2{_Float16(1.0f), _Float16(1.0f)}, sum, false);
+                    more = FINE ? more + (x + y) : __builtin_amdgcn_fdot2(p, f16x2{_Float16(1.0f), _Float16(1.0f)}, more, false);
                     if constexpr (FINE)
                         pl[b][e >> 3].w[(e & 7) >> 1] = as_u32(f16x2{_Float16(x - float(p[0])), _Float16(y - float(p[1]))});
                 }
+            sum += more;
             // (last read for unit u - 1, next marked for unit u + 2; marked for
             // partial units alone, which are the last ones)
             if (partial(u + 2) && threadIdx.x < 2)

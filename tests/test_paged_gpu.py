@@ -390,6 +390,98 @@ def test_attention_far_from_zero(hip, fmt, out_fmt, sign, course):
 
 
 @gpu
+@pytest.mark.parametrize("new,at,count", [(1, 0, 1), (1, 0, 64), (1, -1, 64), (9, 4321, 64), (100, 0, 1), (100, 0, 32),
+                                          (100, -1, 32)])
+@pytest.mark.parametrize("fmt,out_fmt", [(Q4, BF16), (F16, BF16), (F16, F32), (Q4, F32)])
+@pytest.mark.parametrize("head", [64, 128])
+def test_weights_far_below_the_largest(hip, fmt, out_fmt, head, new, at, count):
+    """One position far above 40000 alike ones, which hold a share of the sum all the
+    same; one sequence, cut into short runs, and many (of the same pages), whose runs are long.
+
+    Every operand is exact in FP16: the query times log2(e) / sqrt(d) is a number
+    of at most ten bits (to FP32's two roundings), keys are 0 or 1 and values whole.
+    What is left are the weights: half an FP16 step of themselves (twice, in
+    numerator and sum; 2^-22 in two terms) and half FP16's smallest step, which
+    is at most 2^-32 of the row's largest (2^-38 in two terms); FP32 sums; and the
+    output's.  An FP32 sum is off by half a step, 2^-24 of the sum, for each addition
+    that it is a chain of: at most 625 units' weights and as many joined runs, and in an
+    accumulator 625 units' products, four each (of 16 positions) for one, two or three
+    pairs of terms.
+    """
+    heads, kv, length, page = 16, 8, 40000 + new, 256
+    st = Setup(hip, fmt, head, kv, page, [(new, length)], seed=43, spare_rows=0)
+    columns = np.arange(head) % 13 - 6
+    top = at if at >= 0 else length - new                  # seen by all rows
+    top_page, slot = int(st.table[0, top // page]), top % page
+    for pool, rest, one in ((st.k, np.zeros(head, np.int64), np.ones(head, np.int64)),
+                            (st.v, columns, np.zeros(head, np.int64))):
+        if fmt == F16:
+            pool.values_view()[:], pool.values_view()[top_page, :, slot] = rest, one
+        else:
+            pool.raw[:, :, page * head // 2:] = np.tile(np.frombuffer(np.float16(1).tobytes(), np.uint8), page * head // 32)
+            pool.nibble_view()[:] = (rest + 8)[0::2] | (rest + 8)[1::2] << 4
+            pool.nibble_view()[top_page, :, slot] = (one + 8)[0::2] | (one + 8)[1::2] << 4
+    st.seqs, st.table, st.lengths = st.seqs * count, np.repeat(st.table, count, 0), np.repeat(st.lengths, count)
+    st.starts = (new * np.arange(count + 1)).astype(np.int32)
+    st.used = st.rows = new * count
+    st.upload()
+    half_out, weight, floor = (2.0 ** -8, 2.0 ** -11, 2.0 ** -32) if out_fmt == BF16 else (2.0 ** -24, 2.0 ** -22, 2.0 ** -38)
+    chain = 2 * 625 + 625 * 4 * (1 if out_fmt == BF16 else 3 if fmt == Q4 else 2)
+    others = np.tile(length - new + np.arange(new), count)
+    for far in (14.03125, 20.03125, 22.6875, 25.1875):      # in units of log 2
+        q = np.full((st.rows, heads * head), far / head * np.sqrt(head) * np.log(2), np.float32)
+        w = np.exp(-q[0, 0].astype(np.float64) * np.sqrt(head))
+        share = others * w / (1 + others * w)
+        want = share[:, None, None] * columns
+        rel = np.expm1(far * 2.0 ** -21) + 2 * weight + chain * 2.0 ** -24
+        bound = rel * np.abs(want) + (2 * floor * others / (1 + others * w))[:, None, None] * np.abs(columns)
+        bound = bound * (1 + half_out) + half_out * np.abs(want)
+        off = np.abs(_attend(hip, st, heads, q, out_fmt) - want)
+        worst = float(np.max((off / share[:, None, None])[..., columns != 0] / np.abs(columns[columns != 0])))
+        inside = bool(np.all(off <= bound))
+        assert inside, (far, worst)
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("fmt,out_fmt", [(Q4, BF16), (F16, BF16), (F16, F32), (Q4, F32)])
+def test_scores_with_coarse_steps(hip, fmt, out_fmt, new):
+    """Scores of 2^25 to 2^28, whose FP32 steps are 2 to 16: what lies a little below the
+    largest rounds to it, or to a whole step further down.  Two positions of the same
+    key share the sum, all else is nothing beside them: their values' mean (whole and
+    half numbers), 2^-20 for exponentials, the reciprocal and its product."""
+    head, heads, length, page = 64, 2, 300 + new, 64
+    st = Setup(hip, fmt, head, 1, page, [(new, length)], seed=47, spare_rows=0)
+    for p in (37, 290):
+        assert p < length - new
+    values = np.stack([np.arange(head) % 15 - 7, np.arange(head) % 11 - 5])
+    half_out = 2.0 ** -8 if out_fmt == BF16 else 2.0 ** -24
+    for size, odd in itertools.product((64, 128, 256, 512), (1, 3, 5, 7)):
+        key = np.ones(head, np.int64)
+        key[63] = odd
+        for pool, rows, scale in ((st.k, [key, key], size), (st.v, values, 1)):
+            if fmt == F16:
+                pool.values_view()[:] = 0
+            else:
+                pool.nibble_view()[:] = 0x88
+                pool.raw[:, :, page * head // 2:] = np.tile(np.frombuffer(np.float16(scale).tobytes(), np.uint8), page * head // 32)
+            for p, row in zip((37, 290), rows):
+                at = int(st.table[0, p // page]), slice(None), p % page
+                if fmt == F16:
+                    pool.values_view()[at] = row * scale
+                else:
+                    pool.nibble_view()[at] = (row + 8)[0::2] | (row + 8)[1::2] << 4
+        st.upload()
+        t = np.full(head, 8192.0)
+        t[63] = 2.0 ** -5
+        q = np.tile((t * np.sqrt(head) * np.log(2)).astype(np.float32), (st.rows, heads))
+        got = _attend(hip, st, heads, q, out_fmt)
+        want = values.mean(0)
+        off = np.abs(got - want)
+        assert np.all(off <= (2.0 ** -20 + half_out * (1 + 2.0 ** -20)) * np.abs(want)), (size, odd)
+
+
+@gpu
 @pytest.mark.parametrize("fmt,out_fmt", [(Q4, BF16), (F16, F32)])
 @pytest.mark.parametrize("head,heads,kv,page,seqs", [
     (64, 16, 16, 16, [(70 + i, 70 + i + 41 * (i % 3)) for i in range(16)]),     # as many tiles as workgroups
