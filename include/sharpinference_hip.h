@@ -594,9 +594,11 @@ int si_hip_paged_attention_workspace_bytes(int query_heads, int kv_heads, int he
  * by 2^-32 (F16 and F32 outputs: 2^-38) of its row's largest.  A row before
  * position 0 (a sequence with fewer positions than rows) sees nothing and
  * is 0.  A row that sees a page outside 0..pages - 1, a cached infinity or
- * NaN or a 4-bit scale beyond +-8188 (values that fp16 cannot hold; append
- * writes none) holds NaN or infinities; all rows of a sequence with a negative length,
- * one beyond max_pages * page_size, or more than max_rows rows hold NaN.  What a row
+ * NaN (what append is given beyond fp16 is infinite in FP16 pages, NaN in
+ * 4-bit ones) holds NaN or infinities, and may where it sees a 4-bit scale
+ * beyond +-8188, which append never writes; all rows of a sequence with a
+ * negative length, one beyond max_pages * page_size, or more than max_rows
+ * rows hold NaN.  What a row
  * does not see (later positions, the rest of the last page) changes nothing
  * of it, whatever it holds.  Replaces: transformer.batch-gqa-scores,
  * batch-causal-softmax and batch-gqa-values (GpuBatchTransformerInstructions.cs:

@@ -410,6 +410,23 @@ struct Attend {
     __device__ __forceinline__ void unit(State<D>& st, Raw<D, Q4>& r, f32x4* s, uint32_t lost, int base, int limit,
                                          bool full) const
     {
+        if constexpr (!Q4) {
+            // An infinite key (FP16 pages hold what they were given; finite ones do not
+            // score so) may make a score -inf: not a position of no weight, but NaN.
+            float low = INFINITY;
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    low = fminf(low, s[u][i]);
+            if (__any(low == -INFINITY)) {
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        s[u][i] = s[u][i] == -INFINITY && base + GRANULE * u + 4 * g + i <= limit ? NAN : s[u][i];
+            }
+        }
         if (!full) {
             // what a row does not see scores -inf
 #pragma unroll
@@ -1276,6 +1293,23 @@ paged_prompt_kernel(const PagedAttentionArgs a)
                     s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[at][i], qf[k], s[b], 0, 0, 0);
                 }
                 __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (!Q4) {
+                // an infinite key's -inf is NaN to those that see it (all of them, or the
+                // key was taken out)
+                float low = INFINITY;
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        low = fminf(low, s[b][e]);
+                if (__any(low == -INFINITY)) {
+#pragma unroll
+                    for (int b = 0; b < 2; b++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            s[b][e] = s[b][e] == -INFINITY ? NAN : s[b][e];
+                }
             }
             if (partial(u)) {
                 // (a new value each time, or 32 positions live through the loop)

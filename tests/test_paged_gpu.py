@@ -546,6 +546,32 @@ def test_values_that_are_not_finite(hip, fmt, new):
 
 
 @gpu
+@pytest.mark.parametrize("out_fmt", [BF16, F32])
+@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("new", [1, 3, 90])
+def test_keys_that_are_not_finite(hip, out_fmt, head, value, new):
+    """A row that sees an infinite or NaN key is NaN whichever way its score goes, in units that
+    every row sees as in those that only some do; the other rows and sequences are right."""
+    seqs = [(new, 300)] * 5 + [(new, 90)]
+    st = Setup(hip, F16, head, 1, 16, seqs, seed=49).fill()
+    # positions in the first unit, in the last one, the last that the first row sees, one that only the last row sees
+    holes = [3, 300 - new, 300 - new - 1, 299]
+    for s, p in enumerate(holes):
+        st.k.values_view()[int(st.table[s, p // 16]), 0, p % 16, 5] = value
+    # and behind the end: seen by none
+    st.k.values_view()[int(st.table[4, 300 // 16]), 0, 300 % 16] = value
+    st.upload()
+    q = st.rng.standard_normal((st.rows, 2 * head)).astype(np.float32)
+    q[:, 5], q[:, head + 5] = np.abs(q[:, 5]) + 0.1, -np.abs(q[:, head + 5]) - 0.1       # scores of both signs
+    got = _attend(hip, st, 2, q, out_fmt)
+    bad = [t for s, p in enumerate(holes) for t in range(st.starts[s] + max(0, p - (300 - new)), st.starts[s + 1])]
+    assert np.all(np.isnan(got[bad]))
+    _check_rows(st, 2, q, got, out_fmt, set(range(st.used)) - set(bad)) if new > 1 else \
+        _check_rows(st, 2, q, got, out_fmt, {4, 5})
+
+
+@gpu
 def test_pages_outside_the_pool(hip):
     """A row that sees a bad page is NaN, earlier rows and other sequences are right."""
     st = Setup(hip, Q4, 128, 2, 16, [(40, 100), (2, 50), (1, 20), (30, 300), (1, 64)], seed=6).fill()
