@@ -591,7 +591,9 @@ int si_hip_paged_attention_workspace_bytes(int query_heads, int kv_heads, int he
  * (queries / sqrt(head_size) times log2(e), cached values and exponentials
  * rounded to fp16 once), for F16 and F32 outputs of operands in two fp16
  * terms (22 bits; cached values exact); an exponential is off by that much or
- * by 2^-32 (F16 and F32 outputs: 2^-38) of its row's largest.  A row before
+ * by 2^-32 (F16 and F32 outputs: 2^-38) of its row's largest.  A query head
+ * with a value that passes fp16 so scaled (beyond +-363000 for heads of 64
+ * values, +-513000 for 128), or that is not finite, gives NaN.  A row before
  * position 0 (a sequence with fewer positions than rows) sees nothing and
  * is 0.  A row that sees a page outside 0..pages - 1, a cached infinity or
  * NaN (what append is given beyond fp16 is infinite in FP16 pages, NaN in

@@ -684,7 +684,10 @@ paged_attention_kernel(const PagedAttentionArgs a)
             if (u + 1 < stop)
                 w.load_values(raw, kvh, (u + 1) * UNIT, pages);
         }
-        const float sum = rows_sum(st.sum);
+        // (a row that sees some position here has a weight of 1 and more, but for a query
+        // beyond FP16 whose keys all have the other sign: every score is -inf)
+        float sum = rows_sum(st.sum);
+        sum = sum == 0.0f && limit >= unit0 * UNIT ? NAN : sum;
         if (tile_start >= begin && tile_end <= end) {
             const float inv = wrong ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
             if (live) {
@@ -1421,6 +1424,8 @@ paged_prompt_kernel(const PagedAttentionArgs a)
         {
             auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
             sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+            // (scores that are all -inf: a query beyond FP16)
+            sum = sum == 0.0f && unit0 < unit1 && limit >= unit0 * UNIT ? NAN : sum;
         }
         // element e of acc[n]: column 32 n + 8 (e / 4) + 4 h + e % 4
         if (lo == 0 && hi == weight) {

@@ -572,6 +572,29 @@ def test_keys_that_are_not_finite(hip, out_fmt, head, value, new):
 
 
 @gpu
+@pytest.mark.parametrize("fmt,out_fmt", [(Q4, BF16), (F16, BF16), (F16, F32), (Q4, F32)])
+@pytest.mark.parametrize("head,limit", [(64, 363000.0), (128, 513000.0)])
+@pytest.mark.parametrize("new", [1, 90])
+def test_queries_beyond_fp16(hip, fmt, out_fmt, head, limit, new):
+    """A query that passes FP16 once it is scaled makes its head's row NaN, whatever the keys'
+    signs; just below that it counts, and a row that sees nothing stays 0."""
+    seqs = [(new, 200), (new, new), (1, 0)]
+    st = Setup(hip, fmt, head, 1, 16, seqs, seed=51).fill()
+    key = -np.ones((1, head), np.float32)                   # scores of one sign
+    for s, (_, length) in enumerate(seqs):
+        for p in range(length):
+            st.k.store(int(st.table[s, p // 16]), p % 16, key)
+    st.upload()
+    for value, nan in ((limit, False), (-limit, False), (1.01 * limit, True), (-1.01 * limit, True), (1e30, True),
+                       (np.inf, True), (-np.inf, True), (np.nan, True)):
+        q = np.zeros((st.rows, 2 * head), np.float32)
+        q[:, 7] = value
+        got = _attend(hip, st, 2, q, out_fmt)
+        assert np.all(np.isnan(got[:2 * new, 0])) if nan else np.all(np.isfinite(got[:2 * new, 0]))
+        assert np.all(np.isfinite(got[:2 * new, 1])) and np.all(got[2 * new] == 0)
+
+
+@gpu
 def test_pages_outside_the_pool(hip):
     """A row that sees a bad page is NaN, earlier rows and other sequences are right."""
     st = Setup(hip, Q4, 128, 2, 16, [(40, 100), (2, 50), (1, 20), (30, 300), (1, 64)], seed=6).fill()
