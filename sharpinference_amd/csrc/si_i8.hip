@@ -3,9 +3,10 @@
 // codes' values.
 //
 // The codes are decided in FP64: u * weight is exact there, so
-//   q = rint(u * weight * c),  c = (1 / sqrt(mean(u^2) + eps)) / scale
-// carries one rounding of 2^-53 before its own, and the sum's order, the
-// thread count and the row's neighbours change no code.  FP64 runs at half
+//   q = rint(y / scale),  y = u * weight * (1 / sqrt(mean(u^2) + eps))
+// carries three roundings of 2^-53 before its own (rows as they are: none that
+// could move a half), and the sum's order, the thread count and the row's
+// neighbours change no code.  FP64 runs at half
 // the FP32 rate here, and the row's bytes (13 a value with a residual) are
 // what bounds the kernel, so the wider type costs nothing.  One pass over
 // memory: the row stays in registers between the reduction (sum of squares
@@ -241,14 +242,19 @@ rows_i8_kernel(const RowsArgs a)
     if (lane == 0)
         a.scale[row] = scale;
     // no scale, no codes: a row of zeros, or one that holds something infinite or NaN
-    const double c = scale > 0.0f ? inv / double(scale) : 0.0;
+    const double c = scale > 0.0f ? 1.0 / double(scale) : 0.0;
     auto give = [&](const Values& u, const Values& wt, int64_t i) {
         int q[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const double y = NORM ? double(u.v[j]) * double(wt.v[j]) : double(u.v[j]);
+            const double y = NORM ? double(u.v[j]) * double(wt.v[j]) * inv : double(u.v[j]);
+            // The quotient y / scale: y * c may miss a half by its last bit (9487.5 / 75
+            // gave 127 and not the even 126); what is left of y, exact for a scale of 24
+            // bits, puts it right.
+            double t = y * c;
+            t = fma(fma(-t, double(scale), y), c, t);
             // (a scale among the subnormals is coarse enough to pass 127)
-            q[j] = scale > 0.0f ? int(fmin(fmax(rint(y * c), -127.0), 127.0)) : 0;
+            q[j] = scale > 0.0f ? int(fmin(fmax(rint(t), -127.0), 127.0)) : 0;
         }
         if (ODD && a.n - i < 4) {
 #pragma unroll

@@ -156,6 +156,36 @@ def test_norm_special_rows(hip, n):
         assert np.all(v[0] == 0) and np.all(np.isnan(v[1:3])) and np.array_equal(v[3:], codes[3:] * scale[3:, None])
 
 
+@pytest.mark.parametrize("fmt", [None, native.F32, native.F16, native.BF16])
+@pytest.mark.parametrize("rows,n", [(1000, 255), (1100, 256), (2, 4097), (1, 9001)])
+def test_codes_between_two_steps(hip, fmt, rows, n):
+    """Whole numbers over a whole scale: many quotients are halves exactly, and go to the even
+    code.  (None: the norm of rows of -1 and 1 with such weights, whose mean square is 1.)"""
+    rng = np.random.default_rng(n)
+    # 127 times the scale has to be exact in the format, and every half of it
+    most = {native.F16: 8, native.BF16: 1}.get(fmt, 16000)
+    step = rng.integers(1, most + 1, 1 if fmt is None else rows) * 2.0
+    half = rng.integers(-253, 254, (len(step), n))
+    half[:, n // 2] = 254
+    x = half * (step[:, None] / 2)
+    want = np.rint(half / 2).astype(np.int8)                   # (ties to even)
+    codes, scale = hip.alloc(rows * n), hip.alloc(rows * 4)
+    if fmt is None:
+        signs = rng.choice([-1.0, 1.0], (rows, n)).astype(np.float32)
+        hip.residual_rms_norm_i8(hip.to_device(signs).ptr, 0, hip.to_device(x[0].astype(np.float32)).ptr, 0, codes.ptr,
+                                 scale.ptr, rows, n, 0.0)
+        step, want = np.repeat(step, rows), (want * signs).astype(np.int8)
+    else:
+        raw = x.astype({native.F32: np.float32, native.F16: np.float16, native.BF16: np.float32}[fmt])
+        assert np.array_equal(raw.astype(np.float64), x)
+        if fmt == native.BF16:
+            assert not np.any(raw.view(np.uint32) & 0xFFFF)
+            raw = (raw.view(np.uint32) >> 16).astype(np.uint16)
+        hip.quantize_i8(fmt, hip.to_device(raw).ptr, codes.ptr, scale.ptr, rows, n)
+    assert np.array_equal(scale.readback(np.float32), step.astype(np.float32))
+    assert np.array_equal(codes.readback(np.int8).reshape(rows, n), want)
+
+
 @pytest.mark.parametrize("fmt", [native.F32, native.F16, native.BF16])
 @pytest.mark.parametrize("rows,n", [(1, 16), (3, 33), (1024, 96), (2, 8192), (1, 40000)])
 def test_quantize_and_back(hip, fmt, rows, n):
