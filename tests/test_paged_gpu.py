@@ -389,6 +389,95 @@ def test_attention_far_from_zero(hip, fmt, out_fmt, sign, course):
             assert np.all(np.abs(got[t] - want) <= bound), (s, i, np.max(np.abs(got[t] - want) / bound))
 
 
+COURSES = ["flat", "rising", "falling", "steps"]
+
+
+def _exact_operands(hip, fmt, course, sign):
+    """A batch whose operands are exact in FP16: scores around +-300 (in units of log 2), all alike
+    or on their way there.  Queries times log2(e) / sqrt(d) are +-1 or +-1/2, to FP32's two
+    roundings; three quarters of a key are a multiple of 1/64 whose sign follows the query's, the
+    last one small random multiples of 1/64; values are whole."""
+    d, heads, kv, page = 128, 6, 2, 32
+    st = Setup(hip, fmt, d, kv, page, [(1, 333), (5, 200), (90, 333), (150, 150)], seed=53)
+    rng = st.rng
+    flips = rng.choice([-1, 1], d)
+    for s, (_, length) in enumerate(st.seqs):
+        for p in range(length):
+            share = {"flat": 1.0, "rising": p / length, "falling": 1 - p / length, "steps": 0.5 + 0.05 * (p // 23 % 10)}[course]
+            codes = np.tile(flips, (kv, 1))
+            codes[:, 96:] = rng.integers(-7, 8, (kv, 32))
+            scales = np.full(4, round(200 * share) / 64.0)       # 96 products of up to 3.125: 300
+            scales[3] = 1 / 64
+            values = rng.integers(-7, 8, (kv, d))
+            at, slot = int(st.table[s, p // page]), p % page
+            for pool, c, b in ((st.k, codes, scales), (st.v, values, np.ones(4))):
+                if fmt == F16:
+                    pool.values_view()[at, :, slot] = c * np.repeat(b, 32)
+                    continue
+                pool.nibble_view()[at, :, slot] = (c + 8)[:, 0::2] | (c + 8)[:, 1::2] << 4
+                for h, i in itertools.product(range(kv), range(4)):
+                    pool.put_scale(at, h, i, slot, b[i])
+    q = np.tile(sign * flips, (st.rows, heads, 1)).astype(np.float64)
+    q[:, :, 96:] = rng.choice([-1, -0.5, 0.5, 1], (st.rows, heads, 32))
+    return st, heads, (q * np.sqrt(d) * np.log(2)).astype(np.float32).reshape(st.rows, -1)
+
+
+def _exact_rows(st, heads, q, out_fmt, rescaled=True):
+    """(want, bound) of all rows.  What is left of the errors where the operands are exact: the
+    query's two FP32 roundings and a score's (2^-22 of sum |q| |k| / sqrt(d)), in numerator and
+    sum; the weights' half step of FP16 (2^-22 in two terms), twice; FP32 sums of chains of less
+    than 100; the output's half step.  Not `rescaled`: as if sums and accumulators stayed as they
+    are when a later unit of 64 positions brings a larger maximum."""
+    half_out, weight = (2.0 ** -8, 2.0 ** -11) if out_fmt == BF16 else (2.0 ** -24, 2.0 ** -22)
+    wants, bounds = np.zeros((st.used, heads, st.d)), np.zeros((st.used, heads, st.d))
+    for s, (new, length) in enumerate(st.seqs):
+        keys, values = st.rows_of(s, length)
+        for i in range(new):
+            t, n = st.starts[s] + i, length - new + i + 1
+            x = q[t].reshape(heads, st.d)
+            want, mag, slack = ref.attention(x, keys, values, n)
+            rel = np.expm1(2 * 2.0 ** -22 * slack)[:, None] + 2 * weight + 100 * 2.0 ** -24
+            bounds[t] = rel * mag * (1 + half_out) + half_out * np.abs(want)
+            if not rescaled:
+                for h in range(heads):
+                    score = keys[:n, h * st.kv // heads] @ x[h].astype(np.float64) / np.sqrt(st.d)
+                    top = np.maximum.accumulate([score[u:u + 64].max() for u in range(0, n, 64)])
+                    p = np.exp(score - np.repeat(top, 64)[:n])
+                    want[h] = p @ values[:n, h * st.kv // heads] / p.sum()
+            wants[t] = want
+    return wants, bounds
+
+
+@pytest.mark.parametrize("course", COURSES)
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_bounds_of_exact_operands_hold_what_they_say(course, sign):
+    """The bound of the next test passes neither zeros nor outputs whose rescaling was left out."""
+    st, heads, q = _exact_operands(None, Q4, course, sign)
+    want, bound = _exact_rows(st, heads, q, BF16)
+    assert np.mean(np.abs(want) <= bound) < 0.02
+    if (course, sign) in (("steps", 1), ("rising", 1), ("falling", -1)):      # maxima that grow a lot
+        wrong = _exact_rows(st, heads, q, BF16, rescaled=False)[0]
+        for s, (new, length) in enumerate(st.seqs):
+            rows = slice(st.starts[s + 1] - 1, st.starts[s + 1])      # its last row: sees every unit
+            assert np.mean(np.abs(wrong[rows] - want[rows]) > bound[rows]) > 0.1
+
+
+@gpu
+@pytest.mark.parametrize("course", COURSES)
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("fmt,out_fmt", [(Q4, BF16), (F16, BF16), (F16, F32), (Q4, F32)])
+def test_attention_of_exact_operands(hip, fmt, out_fmt, sign, course):
+    """Scores far from 0 whose reference starts there or moves many times, within a few steps of the output."""
+    st, heads, q = _exact_operands(hip, fmt, course, sign)
+    st.upload()
+    want, bound = _exact_rows(st, heads, q, out_fmt)
+    off = np.abs(_attend(hip, st, heads, q, out_fmt)[:st.used] - want)
+    assert np.all(off <= bound), np.max(off / bound)
+    # over the whole output the roundings average out
+    half_out, weight = (2.0 ** -8, 2.0 ** -11) if out_fmt == BF16 else (2.0 ** -24, 2.0 ** -18)
+    assert np.linalg.norm(off) <= (half_out + 6 * weight) * np.linalg.norm(want)
+
+
 @gpu
 @pytest.mark.parametrize("new,at,count", [(1, 0, 1), (1, 0, 64), (1, -1, 64), (9, 4321, 64), (100, 0, 1), (100, 0, 32),
                                           (100, -1, 32)])
