@@ -223,11 +223,33 @@ def _context():
     return _hip
 
 
+class _Owner:
+    """Keeps a state's device memory until the context's stream is done with it."""
+
+    def __init__(self, *held):
+        self.held = held
+
+    def __del__(self):
+        if _hip is not None:   # (None as the interpreter ends)
+            _hip.sync()
+
+
 def _program(state):
-    """What a program sets up once for its buffers: the calls with their arguments."""
+    """What a program sets up once for its buffers: the calls with their arguments.
+
+    The context has a stream of its own, which torch's does not wait for, nor it for torch's.  So
+    what torch fills is waited for here, once; whoever reads outputs waits for the context
+    (or the device) first; and the memory goes back to torch only behind the context's work.
+    """
     from sharpinference_amd import native
     hip, case, inp, bufs = _context(), state["case"], state["inp"], state["bufs"]
     p = lambda t: 0 if t is None else t.data_ptr()
+    workspace = None
+    if case["kind"] == "attend":
+        workspace = torch.empty(native.paged_attention_workspace_bytes(case["heads"], case["kv_heads"], case["head"]),
+                                dtype=torch.uint8, device="cuda")
+    state["owner"] = _Owner(inp, bufs, workspace)
+    torch.cuda.synchronize()
     if case["kind"] == "norm":
         updated = bufs["updated"] if case["residual"] else None
         args = (p(inp["hidden"]), p(inp["residual"]), p(inp["weight"]), p(updated), p(bufs["q"]), p(bufs["scale"]),
@@ -266,11 +288,8 @@ def _program(state):
             hip.paged_kv_read(batch, cache, p(bufs["keys"]), p(bufs["values"]))
             return [bufs["query"], bufs["keys"], bufs["values"]]
         return call
-    workspace = torch.empty(native.paged_attention_workspace_bytes(case["heads"], case["kv_heads"], case["head"]),
-                            dtype=torch.uint8, device="cuda")
     args = native.PagedAttentionArgs(batch, cache, p(inp["q"]), p(bufs["out"]), p(workspace), case["heads"],
                                      FORMATS[case["out"]])
-    state["workspace"] = workspace
 
     def call():
         hip.paged_attention(args)
