@@ -490,7 +490,8 @@ int si_hip_dequant_i8(si_hip_context* ctx, const int8_t* codes, const float* sca
 /* y[t][o] = x_scale[t] * w_scale[o] * sum_k x[t][k] w[o][k] (+
  * residual[t][o], which may be y), x [m, cols] and w [rows, cols] codes,
  * 16-byte aligned, cols a multiple of 16 in 16..65536: exact int32 sums on
- * the matrix cores, one FP32 rounding for each scale and for the residual.
+ * the matrix cores, one FP32 rounding for the sum (beyond 2^24), for each scale
+ * and for the residual.
  * A call allocates nothing.
  * Replaces: transformer.batch-shared-matvec (GpuBatchTransformerInstructions.cs:
  * 224-279) for weights kept in 8 bits. */
@@ -521,7 +522,9 @@ typedef struct si_hip_paged_cache {
 /* The newest positions of `sequences` sequences, row after row: rows
  * row_starts[s] .. row_starts[s + 1] - 1 are the last positions of sequence
  * s, whose cache holds lengths[s] positions with them, so row t is position
- * lengths[s] - row_starts[s + 1] + t.  A sequence may bring no row.  Rows
+ * lengths[s] - row_starts[s + 1] + t.  A sequence may bring no row.  The starts
+ * may not fall and lie in 0..rows; the attention takes a sequence whose starts
+ * do not as one without rows (its output is left as it was).  Rows
  * from row_starts[sequences] on belong to none and are neither read nor
  * written.  The arrays are read on the GPU when the call runs there, so a
  * recorded plan serves whatever they hold at each replay. */
@@ -554,8 +557,8 @@ typedef struct si_hip_paged_append_args {
  * rotary_size values of each q and k head (in FP64, rounded to FP32), q to
  * `query`, k and v to the row's place in the pages, rounded to fp16 or to
  * blocks of 32 4-bit values: scale = the block's value of largest magnitude
- * (the first of equals) / -8 in fp16, nibble = value / scale rounded to the
- * nearest + 8, at most 15.  A 4-bit block with a value beyond +-65504 or
+ * (the first of equals) / -8 in fp16, nibble = value / scale (in FP32) rounded
+ * to the nearest + 8, at most 15.  A 4-bit block with a value beyond +-65504 or
  * NaN reads back as NaN.  A row whose position lies outside 0..max_pages *
  * page_size - 1, or in a page outside 0..pages - 1, writes nothing.  Two
  * rows of one call may not share a place.  Replaces: transformer.
@@ -590,7 +593,8 @@ int si_hip_paged_attention_workspace_bytes(int query_heads, int kv_heads, int he
  * cores, statistics and sums in FP32: for BF16 outputs of FP16 operands
  * (queries / sqrt(head_size) times log2(e), cached values and exponentials
  * rounded to fp16 once), for F16 and F32 outputs of operands in two fp16
- * terms (22 bits; cached values exact); an exponential is off by that much or
+ * terms (22 bits, of scaled queries no finer than 2^-25; cached values exact);
+ * an exponential is off by that much or
  * by 2^-32 (F16 and F32 outputs: 2^-38) of its row's largest.  A query head
  * with a value that passes fp16 so scaled (beyond +-363000 for heads of 64
  * values, +-513000 for 128), or that is not finite, gives NaN.  A row before
@@ -602,7 +606,9 @@ int si_hip_paged_attention_workspace_bytes(int query_heads, int kv_heads, int he
  * negative length, one beyond max_pages * page_size, or more than max_rows
  * rows hold NaN.  What a row
  * does not see (later positions, the rest of the last page) changes nothing
- * of it, whatever it holds.  Replaces: transformer.batch-gqa-scores,
+ * of it, whatever it holds.  Where the sums of a row are cut follows the whole
+ * batch: the same batch gives the same bits, but beside other sequences a row
+ * may differ in its last ones.  Replaces: transformer.batch-gqa-scores,
  * batch-causal-softmax and batch-gqa-values (GpuBatchTransformerInstructions.cs:
  * 415-598) for many sequences over pages. */
 int si_hip_paged_attention(si_hip_context* ctx, const si_hip_paged_attention_args* args);

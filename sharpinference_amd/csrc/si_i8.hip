@@ -11,9 +11,10 @@
 // what bounds the kernel, so the wider type costs nothing.  One pass over
 // memory: the row stays in registers between the reduction (sum of squares
 // and largest |u * weight|, both in the first pass) and the codes.  4093 rows of
-// 4096 values with a residual take 36 us, 6.0 TB/s (again and again over
-// the same buffers, of which the cache before HBM holds a part); one row takes 3.2
-// us, a launch and two round trips.
+// 4096 values with a residual take 34 us again and again over the same buffers, of
+// which the cache before HBM holds a part, and 43 us (5.1 TB/s) over others each
+// time; without it 22.  Rows as they are (F32 or 16 bits) take 16 to 19 us.
+// One row takes 3.2 us, a launch and two round trips.
 #include "si_i8.hpp"
 #include "si_internal.hpp"
 
@@ -41,8 +42,8 @@ struct RowsArgs {
 
 // Four values beside each other; ODD: at any address that one value may have.
 // (The instructions are the same, but not their order: 4000 rows of 4096 values
-// take 55 us with the aligned types and 64 us with the others; 1900 rows of
-// 8001 took 103 us a value at a time, and take 54.)
+// and their codes read back took 55 us with the aligned types and 64 us with the others;
+// 1900 rows of 8001 took 103 us a value at a time, and take 64, 43 without the read-back.)
 template <bool ODD>
 struct Fours {
     typedef float f32 __attribute__((ext_vector_type(4)));

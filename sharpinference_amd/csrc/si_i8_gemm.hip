@@ -150,7 +150,7 @@ __device__ __forceinline__ void store_blocks(const GemmI8Args& a, const i32x16 (
 // for the piece that belongs where its bytes land, still 128 whole bytes of a
 // row to eight lanes.
 //
-// 4093 x 8192 x 4096 takes 143 us (1.92 POP/s), 4096 x 16384 x 8192 519 us
+// 4093 x 8192 x 4096 takes 136 us (2.0 POP/s), 4096 x 16384 x 8192 519 us
 // (2.12); the vendor's plain product of 8-bit integers, int32 out and no
 // scales, reaches 2.18 and 2.10 on such shapes.  In a single workgroup a step
 // of the 256 x 256 tile takes 1.2 us, near the LDS traffic of its fragments;

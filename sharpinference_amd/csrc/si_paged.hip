@@ -9,8 +9,10 @@
 // depend on which kernel rotated it.
 //
 // Bound by bytes: five prompts of up to 1500 rows (24 + 2 x 8 heads of 128, 4-bit
-// pages) take 30 us, 4.7 TB/s, with one row a workgroup (two values a lane, loads
-// behind the turns, neighbouring rows on different dies: 46); 64 single rows take
+// pages) take 30 us over the same buffers again and again, 4.7 TB/s with the help of
+// the cache before HBM, and 40 over others each time, with one row a workgroup (two
+// values a lane, loads behind the turns, neighbouring rows on different dies: 46 where
+// this takes 30); 64 single rows take
 // 4.6 us, five workgroups a row, of which the search for the row's sequence, its
 // page and the turns are three round trips.
 #include "si_paged.hpp"

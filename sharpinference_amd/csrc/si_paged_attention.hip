@@ -587,10 +587,12 @@ __device__ __forceinline__ int format_of(const PagedAttentionArgs& a) { return F
 // lie in; tiles that are wholly its own are written out, the others left in
 // its slots for the merge.  (A workgroup a tile, with the longest sequence of 64 the
 // last to end: 1080 us where this takes 80.)
-// Bound by the pages' bytes where there are enough of them: 64 sequences of 500 to
-// 16000 positions, 4-bit pages, 80 us with the merge, 4.4 TB/s.  A unit takes a
-// wave 2.7 us by itself, 500 vector instructions and a round trip that they hide
-// half of: short batches are a launch, the search, one unit and the merge, 10 us.
+// FP16 pages are bound by their bytes where there are enough of them; 4-bit ones by
+// the 650 vector instructions of a unit, which run for two thirds of the time, and the
+// round trips that two waves a SIMD leave open: 64 sequences of 500 to 16000
+// positions take 80 us with the merge, 4.4 TB/s, where FP16 pages reach 5.6.  A unit
+// takes a wave 2.7 us by itself: short batches are a launch, the search, one unit and the
+// merge, 10 us.
 // A unit of 128 FP16 values a position is 128 registers a lane: two waves on a
 // SIMD would spill them (64 sequences of 500 to 16000 positions: 5.14 TB/s,
 // with one wave 5.59).
@@ -807,8 +809,8 @@ paged_merge_kernel(const PagedAttentionArgs a)
 // of them the exponentials), which overlap little.  840 TFLOP/s within the units
 // at the 1.95 GHz that the card then runs at, 0.55 of what a large matrix product
 // reaches.
-// 128 rows in four waves: 252 us where this takes 229 (chunks of up to 2000 rows
-// over up to 6000 positions).
+// Chunks of up to 2000 rows over up to 6000 positions take 210 us, joins included; when
+// this form took 229, one of 128 rows in four waves took 252.
 constexpr int PROMPT_ROWS = 256;
 constexpr int PROMPT_THREADS = 512;
 // What the scores are taken relative to follows their maximum only when the weights
@@ -1553,11 +1555,13 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s)
 {
     // Sequences of how many packed rows go to the prompt kernel.  It turns a unit
     // into FP16 once for 256 rows and the other does for 16, but a launch of both
-    // costs 20 us more, and few tiles do not fill its workgroups.  Rows a sequence,
-    // us with 128 and 64 here: 4 sequences of 126 rows and up to 300 positions 20 and
-    // 31, one of 126 and 9000 37 and 49, 8 of 72 to 128 and 2000 to 6000 34 and 48;
-    // but 16 of 126 and 3000 to 9000 183 and 143 (of 96: 145 and 140, of 72: 134 and
-    // 144).
+    // costs 10 us more, and few tiles do not fill its workgroups.  Rows a sequence,
+    // us with 128 and 64 here (4-bit pages, heads of 128): 4 sequences of 126 rows and
+    // up to 300 positions 19 and 28, one of 126 and 9000 37 and 46, 8 of 72 to 126 and
+    // 2000 to 6000 64 and 68, 40 of 66 to 96 and 300 to 2000 71 and 84; but 16 of 126
+    // and 3000 to 9000 175 and 131.  Lengths, which the host does not know, would move
+    // the border: 16 of 96 and 3000 to 9000 135 and 124 (of 72: 116 and 124), 4 of 96
+    // and 2000 47 and 40, 3 of 126 and 30000 159 and 117.
     const int64_t group = a.heads / a.cache.kv_heads, most = a.batch.max_rows * group, all = a.batch.rows * group;
     PagedAttentionArgs b = a;
     b.few_rows = most <= 96 || (most <= 128 && all <= 1024) ? 128 : 64;
