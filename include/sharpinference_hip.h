@@ -469,7 +469,7 @@ int si_hip_batch_select_last(si_hip_context* ctx, const float* input, const int3
 /* u = hidden + residual, updated = u (residual and updated both NULL: u =
  * hidden), y = u * (1 / sqrt(sum(u^2) / n + eps)) * weight, scale[r] =
  * max |y| / 127, codes[r][i] = y_i / scale[r] rounded to the nearest (ties
- * to even), decided in FP64: the same codes in any batch.  eps finite and
+ * to even), decided in FP64, whose last bits alone hang on the number of rows.  eps finite and
  * >= 0; outputs may not overlap any input.  Replaces: transformer.
  * batch-residual-rms-norm (GpuBatchTransformerInstructions.cs:158-222) in
  * front of products in 8 bits, which the reference does not have. */

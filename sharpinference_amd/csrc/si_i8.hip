@@ -4,9 +4,9 @@
 //
 // The codes are decided in FP64: u * weight is exact there, so
 //   q = rint(y / scale),  y = u * weight * (1 / sqrt(mean(u^2) + eps))
-// carries three roundings of 2^-53 before its own (rows as they are: none that
-// could move a half), and the sum's order, the thread count and the row's
-// neighbours change no code.  FP64 runs at half
+// carries a few roundings of 2^-53 before its own (rows as they are: none that
+// could move a half); the sum's order, which the thread count and so the number of
+// rows decide, reaches a code or scale by no more than those.  FP64 runs at half
 // the FP32 rate here, and the row's bytes (13 a value with a residual) are
 // what bounds the kernel, so the wider type costs nothing.  One pass over
 // memory: the row stays in registers between the reduction (sum of squares
