@@ -613,6 +613,131 @@ int si_hip_paged_attention_workspace_bytes(int query_heads, int kv_heads, int he
  * 415-598) for many sequences over pages. */
 int si_hip_paged_attention(si_hip_context* ctx, const si_hip_paged_attention_args* args);
 
+/* ---- many sequences at once: a recurrent model's step, and a search over beams ---------- */
+
+/* The newest rows of `sequences` sequences, row after row, and where their
+ * recurrent states lie: rows row_starts[s] .. row_starts[s + 1] - 1 are
+ * sequence s, which goes on from slot from[s] of a state array (-1: from a
+ * state of zeros) and leaves its state in slot to[s] (-1: nowhere).  A sequence may
+ * bring no row: its state is then not touched.  The starts may not fall and lie in
+ * 0..rows; a sequence whose starts do not is taken as one without rows.  Rows in no
+ * sequence are neither read nor written.  from and to of a sequence may be equal, and
+ * several sequences may go on from one slot; a slot that one sequence writes may not be
+ * another's of the same call.  A sequence whose `from` is neither -1 nor
+ * a slot goes on from a state of NaN; a `to` outside the slots is taken as -1.  The arrays
+ * are read on the GPU when the call runs there, so a recorded plan serves whatever they hold
+ * at each replay. */
+typedef struct si_hip_row_batch {
+    const int32_t* row_starts; /* device [sequences + 1], from 0 up */
+    const int32_t* from;       /* device [sequences] */
+    const int32_t* to;         /* device [sequences]; may be `from` */
+    int32_t sequences;         /* 1..4096 */
+    int32_t slots;             /* of the state arrays, at least 1 */
+    int32_t rows;              /* rows of the batch's buffers, 1..1048576 */
+    int32_t max_rows;          /* most rows that one sequence brings, 1..rows: the launch goes by it; a sequence
+                                  with more is right but may be slow */
+} si_hip_row_batch;
+
+typedef struct si_hip_layernorm_mix_rows_args {
+    si_hip_row_batch batch;
+    const float* x;            /* [rows][n] */
+    const float* residual;     /* optional [rows][n] */
+    const float* weight, *bias;   /* [n] */
+    const float* mix;          /* [mixes][n] */
+    float* state;              /* [slots][n]: the normalised row before a sequence's first one */
+    float* updated;            /* [rows][n], with a residual only: x + residual */
+    void* output;              /* [mixes][rows][n] of output_format; mixes = 0: [rows][n] */
+    int32_t n;                 /* 1..8192 */
+    int32_t mixes;             /* 0..8; 0: output = norm, without mix and state */
+    int32_t output_format;     /* SI_HIP_F32, SI_HIP_F16 or SI_HIP_BF16 */
+    float eps;                 /* finite, >= 0 */
+} si_hip_layernorm_mix_rows_args;
+
+/* Every row of the batch: u = x (+ residual), norm = ((u - mean) * (1 /
+ * sqrt(var + eps))) * weight + bias, output_m = norm + (before - norm) *
+ * mix_m, with `before` the norm of the row before in the same sequence, for its first
+ * row what the state's slot holds; the state keeps the norm of its last row.  FP32
+ * throughout, outputs rounded once.  Outputs may not overlap inputs or one another.
+ * Replaces: the Normalize + Affine + Mix node chains of the RWKV-7 graph and
+ * its att / ffn previous states (PortableRwkv7GraphProvider.cs:163-170,
+ * 180-184, 202-210, 278-288) for many rows. */
+int si_hip_layernorm_mix_rows(si_hip_context* ctx, const si_hip_layernorm_mix_rows_args* args);
+
+typedef struct si_hip_rwkv7_wkv_rows_args {
+    si_hip_row_batch batch;
+    int32_t heads;             /* 1..1024; head size is 64 */
+    int32_t first_layer;
+    const float* r, *k, *v;    /* [rows][heads * 64] */
+    const float* w_lora, *a_lora, *gate, *v_lora;   /* the same; v_lora unused when first_layer */
+    const float* w0, *a0, *v0, *k_k, *k_a, *r_k, *lnx_weight, *lnx_bias;   /* [heads * 64] */
+    float* v_first;            /* [rows][heads * 64]: written when first_layer, else read */
+    float* state;              /* FP32 [slots][heads][64][64] */
+    void* output;              /* [rows][heads * 64] of output_format */
+    void* workspace;           /* si_hip_rwkv7_wkv_rows_workspace_bytes; any contents on entry; calls sharing one
+                                  workspace must not overlap on the GPU */
+    int32_t output_format;     /* SI_HIP_F32, SI_HIP_F16 or SI_HIP_BF16 */
+} si_hip_rwkv7_wkv_rows_args;
+
+int si_hip_rwkv7_wkv_rows_workspace_bytes(int heads, uint64_t* bytes);
+
+/* si_hip_rwkv7_wkv (its formulas, in FP32) for every row of the batch, row after row of
+ * each sequence through the sequence's state; output rounded once.  [rows] arrays, state and
+ * workspace 16-byte aligned.  A value that is not finite changes nothing of rows before its own.
+ * Replaces: the WKV node chain (PortableRwkv7GraphProvider.cs:224-276), run token after
+ * token there. */
+int si_hip_rwkv7_wkv_rows(si_hip_context* ctx, const si_hip_rwkv7_wkv_rows_args* args);
+
+typedef struct si_hip_beam_select_args {
+    const void* logits;        /* [sequences * beams] rows of vocab values of logits_format, `stride` values apart */
+    const float* scores;       /* [sequences * beams]: each beam's log-probability so far; not finite: no beam */
+    const int32_t* done;       /* optional [sequences * beams]: not 0: the beam has ended */
+    const int32_t* slots;      /* optional [sequences * beams]: the slot of each beam's state */
+    int32_t* parents;          /* [sequences][candidates]: the beam, 0..beams - 1, that the candidate continues */
+    int32_t* tokens;           /* [sequences][candidates] */
+    float* new_scores;         /* [sequences][candidates]; may be `scores` when candidates = beams */
+    int32_t* new_done;         /* optional [sequences][candidates]; may be `done` when candidates = beams */
+    int32_t* from;             /* with slots: [sequences][beams]: the slot that the candidate goes on from */
+    int32_t* to;               /* with slots: [sequences][beams]: the slot it takes over; may be `slots` */
+    void* workspace;           /* si_hip_beam_select_workspace_bytes, 16-byte aligned; any contents on entry; calls
+                                  sharing one workspace must not overlap on the GPU */
+    int64_t vocab;             /* 1..2097152 */
+    int64_t stride;            /* >= vocab */
+    int32_t sequences;         /* sequences * beams at most 65536 */
+    int32_t beams;             /* 1..16 */
+    int32_t candidates;        /* 1..32; with slots: beams */
+    int32_t logits_format;     /* SI_HIP_F32, SI_HIP_F16 or SI_HIP_BF16 */
+    int32_t end_token;         /* the token that ends a beam; -1: none (then without done and new_done) */
+} si_hip_beam_select_args;
+
+int si_hip_beam_select_workspace_bytes(int sequences, int beams, int candidates, int64_t vocab, uint64_t* bytes);
+
+/* For each sequence the `candidates` pairs (beam b, token t) of largest score
+ * scores[b] + log softmax(logits[b])[t], from the largest down; of equal
+ * ones the lower beam first, then the lower token.  An ended beam has one candidate: itself
+ * under end_token with its score as it is.  A pair whose score is not finite is no candidate (a masked
+ * logit of -infinity; every token of a beam whose logits hold NaN or +infinity); where there are
+ * fewer candidates than asked for, the rest have parent and token -1 and score -infinity.
+ * new_done is 1 where the token is end_token.  With slots, from is the parent's slot (-1 without a parent) and
+ * `to` hands the beams' slots on: a beam's first candidate keeps its slot, every other candidate takes, in order, the
+ * slot of the next beam without candidates; si_hip_copy_slots then moves the states.  Logits are compared
+ * exactly, scores in FP64 (exponentials in FP32).  No counterpart in the reference, which takes the argmax
+ * (transformer.argmax, GpuTransformerInstructionCollection.cs:697-748). */
+int si_hip_beam_select(si_hip_context* ctx, const si_hip_beam_select_args* args);
+
+typedef struct si_hip_slot_array {
+    void* base;                /* [slots] of slot_bytes */
+    uint64_t slot_bytes;       /* at least 1 */
+} si_hip_slot_array;
+
+/* In each of `count` arrays (1..4096, not overlapping) slot to[i] becomes slot from[i], for i <
+ * moves with 0 <= from[i], to[i] < slots and from[i] != to[i]; from and to are device arrays, read when the call
+ * runs on the GPU (the list of arrays is read here).  A slot written by one move may be neither read nor
+ * written by another.  Moves the states of beams after si_hip_beam_select, and copies pages of a
+ * paged cache that two sequences share before one writes them (slots are pages then).  No counterpart in the
+ * reference, whose state bindings belong to one sequence. */
+int si_hip_copy_slots(si_hip_context* ctx, const si_hip_slot_array* arrays, int count, int64_t slots,
+                      const int32_t* from, const int32_t* to, int moves);
+
 /* ---- Phi-4 decode step ------------------------------------------------------------ */
 
 typedef struct si_hip_phi4_layer {

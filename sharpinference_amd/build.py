@@ -50,6 +50,10 @@ SOURCES = [
     "si_paged.hip",
     "si_paged_attention.hip",
     "si_paged_abi.cpp",
+    "si_mix_rows.hip",
+    "si_wkv_rows.hip",
+    "si_beam.hip",
+    "si_sequences_abi.cpp",
 ]
 
 

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from typing import Iterable, Optional, Sequence
+from typing import Iterable, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -141,6 +141,37 @@ class PagedAttentionArgs(ctypes.Structure):
                 ("query_heads", _i32), ("output_format", _i32)]
 
 
+class RowBatch(ctypes.Structure):
+    """si_hip_row_batch (`from_`: the slots that the sequences go on from)."""
+    _fields_ = [("row_starts", _vp), ("from_", _vp), ("to", _vp), ("sequences", _i32), ("slots", _i32),
+                ("rows", _i32), ("max_rows", _i32)]
+
+
+class LayernormMixRowsArgs(ctypes.Structure):
+    """si_hip_layernorm_mix_rows_args."""
+    _fields_ = [("batch", RowBatch)] + [(n, _vp) for n in ("x", "residual", "weight", "bias", "mix", "state", "updated",
+                                                           "output")] + \
+        [("n", _i32), ("mixes", _i32), ("output_format", _i32), ("eps", ctypes.c_float)]
+
+
+class BeamSelectArgs(ctypes.Structure):
+    """si_hip_beam_select_args."""
+    _fields_ = [(n, _vp) for n in ("logits", "scores", "done", "slots", "parents", "tokens", "new_scores", "new_done",
+                                   "from_", "to", "workspace")] + \
+        [("vocab", _i64), ("stride", _i64)] + [(n, _i32) for n in ("sequences", "beams", "candidates", "logits_format",
+                                                                   "end_token")]
+
+
+class SlotArray(ctypes.Structure):
+    """si_hip_slot_array."""
+    _fields_ = [("base", _vp), ("slot_bytes", _u64)]
+
+
+def slot_arrays(arrays: Sequence[Tuple[int, int]]):
+    """(device address, bytes of a slot) pairs as HipContext.copy_slots takes them."""
+    return (SlotArray * len(arrays))(*[SlotArray(int(base) or None, int(size)) for base, size in arrays])
+
+
 class Phi4Layer(ctypes.Structure):
     """si_hip_phi4_layer."""
     _fields_ = [("attn_norm", _vp), ("qkv", _vp), ("o", _vp), ("ffn_norm", _vp), ("up", _vp), ("down", _vp),
@@ -166,6 +197,12 @@ class Rwkv7WkvArgs(ctypes.Structure):
     """si_hip_rwkv7_wkv_args."""
     _fields_ = [("heads", _i32), ("first_layer", _i32)] + [(n, _vp) for n in RWKV7_WKV_VECTORS] + \
         [("v_first", _vp), ("state", _vp), ("out", _vp)]
+
+
+class Rwkv7WkvRowsArgs(ctypes.Structure):
+    """si_hip_rwkv7_wkv_rows_args."""
+    _fields_ = [("batch", RowBatch), ("heads", _i32), ("first_layer", _i32)] + [(n, _vp) for n in RWKV7_WKV_VECTORS] + \
+        [("v_first", _vp), ("state", _vp), ("output", _vp), ("workspace", _vp), ("output_format", _i32)]
 
 
 RWKV7_LAYER_FIELDS = ("ln1_weight", "ln1_bias", "ln2_weight", "ln2_bias", "mix", "receptance", "key", "value",
@@ -254,6 +291,12 @@ SIGNATURES.update({
     "si_hip_paged_kv_read": ([_vp, ctypes.POINTER(PagedBatch), ctypes.POINTER(PagedCache), _vp, _vp], _i32),
     "si_hip_paged_attention_workspace_bytes": ([_i32, _i32, _i32, ctypes.POINTER(_u64)], _i32),
     "si_hip_paged_attention": ([_vp, ctypes.POINTER(PagedAttentionArgs)], _i32),
+    "si_hip_layernorm_mix_rows": ([_vp, ctypes.POINTER(LayernormMixRowsArgs)], _i32),
+    "si_hip_rwkv7_wkv_rows_workspace_bytes": ([_i32, ctypes.POINTER(_u64)], _i32),
+    "si_hip_rwkv7_wkv_rows": ([_vp, ctypes.POINTER(Rwkv7WkvRowsArgs)], _i32),
+    "si_hip_beam_select_workspace_bytes": ([_i32, _i32, _i32, _i64, ctypes.POINTER(_u64)], _i32),
+    "si_hip_beam_select": ([_vp, ctypes.POINTER(BeamSelectArgs)], _i32),
+    "si_hip_copy_slots": ([_vp, ctypes.POINTER(SlotArray), _i32, _i64, _vp, _vp, _i32], _i32),
     "si_hip_phi4_workspace_bytes": ([ctypes.POINTER(Phi4Model), ctypes.POINTER(_u64)], _i32),
     "si_hip_phi4_decode": ([_vp, ctypes.POINTER(Phi4Model)], _i32),
     "si_hip_phi4_decode_bounded": ([_vp, ctypes.POINTER(Phi4Model), _i32], _i32),
@@ -563,6 +606,19 @@ class HipContext:
     def paged_attention(self, args: PagedAttentionArgs) -> None:
         self._call(lib().si_hip_paged_attention, ctypes.byref(args))
 
+    def layernorm_mix_rows(self, args: LayernormMixRowsArgs) -> None:
+        self._call(lib().si_hip_layernorm_mix_rows, ctypes.byref(args))
+
+    def rwkv7_wkv_rows(self, args: Rwkv7WkvRowsArgs) -> None:
+        self._call(lib().si_hip_rwkv7_wkv_rows, ctypes.byref(args))
+
+    def beam_select(self, args: BeamSelectArgs) -> None:
+        self._call(lib().si_hip_beam_select, ctypes.byref(args))
+
+    def copy_slots(self, arrays, slots: int, from_: int, to: int, moves: int) -> None:
+        """arrays: slot_arrays(...)."""
+        self._call(lib().si_hip_copy_slots, arrays, len(arrays), int(slots), _p(from_), _p(to), int(moves))
+
     def phi4_decode(self, model: Phi4Model) -> None:
         self._call(lib().si_hip_phi4_decode, ctypes.byref(model))
 
@@ -677,6 +733,18 @@ def paged_page_bytes(fmt: int, page_size: int, head_size: int) -> int:
 def paged_attention_workspace_bytes(query_heads: int, kv_heads: int, head_size: int) -> int:
     n = ctypes.c_uint64(0)
     _check(lib().si_hip_paged_attention_workspace_bytes(query_heads, kv_heads, head_size, ctypes.byref(n)))
+    return n.value
+
+
+def rwkv7_wkv_rows_workspace_bytes(heads: int) -> int:
+    n = ctypes.c_uint64(0)
+    _check(lib().si_hip_rwkv7_wkv_rows_workspace_bytes(heads, ctypes.byref(n)))
+    return n.value
+
+
+def beam_select_workspace_bytes(sequences: int, beams: int, candidates: int, vocab: int) -> int:
+    n = ctypes.c_uint64(0)
+    _check(lib().si_hip_beam_select_workspace_bytes(sequences, beams, candidates, vocab, ctypes.byref(n)))
     return n.value
 
 
