@@ -20,12 +20,6 @@ constexpr int SCAN_WAVES = 4, MERGE_WAVES = 8;
 
 typedef unsigned long long Key;   // order of a logit (high word: 0 for none) and of its token, lowest last
 
-__device__ __forceinline__ void wave_sync()
-{
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // Order of a logit: larger for larger values, 0 for -infinity and NaN; -0 as 0.
 __device__ __forceinline__ uint32_t order_of(float v)
 {

@@ -111,6 +111,31 @@ __device__ __forceinline__ void store_row_value(void* out, int format, int64_t a
     else
         static_cast<__bf16*>(out)[at] = static_cast<__bf16>(v);
 }
+
+// LDS written by other lanes of the wave is read behind this.
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Four neighbours at a multiple of four.
+template <typename V>
+__device__ __forceinline__ void store_row4(void* out, int format, int64_t at, V v)
+{
+    if (format == ROWS_OUT_F32) {
+        typedef float W __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<W*>(static_cast<float*>(out) + at) = W{v[0], v[1], v[2], v[3]};
+    } else if (format == ROWS_OUT_F16) {
+        typedef _Float16 W __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<W*>(static_cast<_Float16*>(out) + at) =
+            W{static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]), static_cast<_Float16>(v[3])};
+    } else {
+        typedef __bf16 W __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<W*>(static_cast<__bf16*>(out) + at) =
+            W{static_cast<__bf16>(v[0]), static_cast<__bf16>(v[1]), static_cast<__bf16>(v[2]), static_cast<__bf16>(v[3])};
+    }
+}
 #endif
 
 }  // namespace si

@@ -9,6 +9,7 @@ from sharpinference_amd import native
 
 U = 2.0 ** -24
 HEAD = 64
+RHO = 1 - 1 / 512
 GROUP_EPS = float(np.float32(64e-5))
 STEP = {native.F32: 2.0 ** -24, native.F16: 2.0 ** -11, native.BF16: 2.0 ** -8}
 TINY = {native.F32: 2.0 ** -149, native.F16: 2.0 ** -24, native.BF16: 2.0 ** -133}
@@ -91,11 +92,13 @@ def _sigmoid(x):
 def wkv_rows(inp, heads, first, starts, source, to):
     """(out, bound, state, bound per head, v_first): the recurrence in 64 bits, and how far FP32 may be off.
 
-    A step's state S' = S (diag(w) - kn (kn a)^T) + v k^T comes from its factors with at most C
+    A step's state S' = S G + v k^T, G = diag(w) - kn (kn a)^T, comes from its factors with at most C
     roundings a term (sums of 64 products, then of up to 16 rows; exponentials and quotients a few
-    each), and an error of the state before it passes on with the norm of the matrix: both
-    in Frobenius norm, a head at a time.  A readout adds C roundings of |S| |r|; the GroupNorm divides by
-    the root of its variance; the output is rounded once.
+    each): an error D_t with |D_t| <= d_t in Frobenius norm, a head at a time.  After T steps the state is off by
+    sum_t D_t P_t, P_t = G_(t+1) .. G_T; by Cauchy and Schwarz, with weights rho^(T - t), a readout of it by r is off by at
+    most sqrt(sum rho^(T - t)) sqrt(r^T M r), M = sum_t d_t^2 rho^(t - T) P_t^T P_t, and the state by the root of
+    M's largest eigenvalue in place of r^T M r.  A readout adds C roundings of |S| |r|; the GroupNorm divides by the
+    root of its variance; the output is rounded once.
     """
     rows = len(inp["r"])
     d = {k: v.astype(np.float64) for k, v in inp.items() if v is not None and v.dtype == np.float32}
@@ -115,18 +118,18 @@ def wkv_rows(inp, heads, first, starts, source, to):
     lw, lb, rk, gate = per(d["lnx_weight"][None])[0], per(d["lnx_bias"][None])[0], per(d["r_k"][None])[0], per(d["gate"])
     norm = lambda x: np.linalg.norm(x, axis=-1)
     for s, first_row, last_row in spans(starts, rows):
-        S, E = taken(d["state"], source[s]).copy(), np.zeros(heads)
+        S, M, weights = taken(d["state"], source[s]).copy(), np.zeros((heads, HEAD, HEAD)), 0.0
         for t in range(first_row, last_row):
             G = np.zeros((heads, HEAD, HEAD))
             G[:, np.arange(HEAD), np.arange(HEAD)] = decay[t]
             G -= kn[t][:, :, None] * ak[t][:, None, :]
             size = np.linalg.norm(S, axis=(1, 2))
-            finite = np.isfinite(G).all((1, 2))
-            grow = np.where(finite, np.linalg.norm(np.where(finite[:, None, None], G, 0), 2, axis=(1, 2)), np.nan)
-            E = grow * E + C * (size * (1 + norm(ak[t])) + norm(value[t]) * norm(key[t]))
+            step = C * (size * (1 + norm(ak[t])) + norm(value[t]) * norm(key[t]))
+            weights = weights * RHO + 1
+            M = G.transpose(0, 2, 1) @ M @ G / RHO + step[:, None, None] ** 2 * np.eye(HEAD)
             S = S @ G + value[t][:, :, None] * key[t][:, None, :]
             y = (S @ r[t][:, :, None])[..., 0]
-            y_off = (E + C * np.linalg.norm(S, axis=(1, 2))) * norm(r[t])
+            y_off = np.sqrt(weights * np.einsum("hi,hij,hj->h", r[t], M, r[t])) + C * np.linalg.norm(S, axis=(1, 2)) * norm(r[t])
             mean = y.mean(-1, keepdims=True)
             inv = 1 / np.sqrt(((y - mean) ** 2).mean(-1, keepdims=True) + GROUP_EPS)
             ln = (y - mean) * inv
@@ -138,7 +141,8 @@ def wkv_rows(inp, heads, first, starts, source, to):
             bound[t] = (ln_off * np.abs(lw) + 100 * U * (np.abs(lb) + size_b) + 4 * U * np.abs(ln * lw)) * np.abs(gate[t]) + \
                 4 * U * np.abs(out[t])
         if 0 <= to[s] < len(state):
-            state[to[s]], off[to[s]] = S, E
+            state[to[s]] = S
+            off[to[s]] = np.sqrt(weights * np.linalg.eigvalsh(np.where(np.isfinite(M), M, 0))[:, -1])
     return out.reshape(rows, -1), bound.reshape(rows, -1), state, off
 
 
