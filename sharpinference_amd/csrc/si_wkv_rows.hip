@@ -26,6 +26,9 @@ struct RowIn {
     float r, k, v, wl, al, gate, vl, vf;
 };
 
+struct Plan;
+__device__ void make_plan(const WkvRowsArgs& a, int over, int stretch, int room, Plan* plan);
+
 // Sequences of few rows: a workgroup takes one head of one sequence, the state
 // in registers (a thread holds 8 columns of two state rows: 8 lanes a state
 // row, whose sums take three DPP steps, and half the LDS reads of 16 columns
@@ -34,11 +37,14 @@ struct RowIn {
 // Bound by reading and writing the state (32 KiB a head) where a sequence
 // brings one row; by vector instructions (92 a row and wave) and LDS reads
 // (10 b128 a lane and row) where it brings many.
-__global__ __launch_bounds__(256) void wkv_few_kernel(WkvRowsArgs a, int most)
+// With a plan to make, the last workgroup makes it.
+__global__ __launch_bounds__(256) void wkv_few_kernel(WkvRowsArgs a, int most, int stretch, int room, Plan* plan)
 {
     __shared__ float4 s_vec[4][5][N / 4];   // decay, key, kn, kn * a, r of the four rows
     __shared__ float s_value[4][N], s_y[4][N];
     const int s = blockIdx.x / a.heads, h = blockIdx.x - s * a.heads;
+    if (s == a.batch.sequences)
+        return make_plan(a, most, stretch, room, plan);
     const RowSpan span = rows_of(a.batch, s);
     const int from = a.batch.from[s], to = a.batch.to[s];
     if (span.last - span.first < 1 || span.last - span.first > most)
@@ -201,23 +207,21 @@ __device__ __forceinline__ f4 mfma4(f4 a, f4 b, f4 c)
     return c;
 }
 
-template <int SHIFT>
-__device__ __forceinline__ float row_shr(float v)   // the value SHIFT lanes before in the row of 16, or 0
-{
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x110 + SHIFT, 0xF, 0xF, true));
-}
-
-// The value of the lane before in the row of 16; 1 in the first.
-__device__ __forceinline__ float row_shr_or_one(float v)
-{
-    return __int_as_float(__builtin_amdgcn_update_dpp(0x3f800000, __float_as_int(v), 0x111, 0xF, 0xF, false));
-}
-
 // The value that lane I of the row of 16 holds.
 template <int I>
 __device__ __forceinline__ float row_lane(float v)
 {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + I, 0xF, 0xF, true));
+}
+
+// Sum of the values in this lane's column of the rows of 16 lanes before its own.
+__device__ __forceinline__ float rows_before(float v)
+{
+    const int g = (threadIdx.x >> 4) & 3;
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const float even = __uint_as_float(a[0]), pair = even + __uint_as_float(a[1]);   // rows 0 0 2 2; 0+1 0+1 2+3 2+3
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(pair), __float_as_uint(pair), false, false);
+    return (g & 1 ? even : 0.0f) + (g & 2 ? __uint_as_float(b[0]) : 0.0f);
 }
 
 // max(top, |x|, |y|), NaN if any is
@@ -227,46 +231,48 @@ __device__ __forceinline__ float largest(float top, float x, float y)
     return top;
 }
 
-// z + sum of the values that lanes S .. S + TERMS - 1 of the row of 16 hold in l, times x[S] ..: one instruction a term (the
-// compiler forms two).  The wait in front keeps the two instructions' distance that a lane-crossing read of a register just
-// written needs; nothing here writes l.
-template <int S, int TERMS>
-__device__ __forceinline__ float add_terms(float z, float l, const float* x)
-{
-    if constexpr (TERMS == 4)
-        asm("s_nop 1\n\t"
-            "v_fmac_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n\t"
-            "v_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n\t"
-            "v_fmac_f32_dpp %0, %1, %4 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n\t"
-            "v_fmac_f32_dpp %0, %1, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf"
-            : "+&v"(z)
-            : "v"(l), "v"(x[S]), "v"(x[S + 1]), "v"(x[S + 2]), "v"(x[S + 3]), "n"(S), "n"(S + 1), "n"(S + 2), "n"(S + 3));
-    else
-        asm("s_nop 1\n\t"
-            "v_fmac_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf"
-            : "+&v"(z)
-            : "v"(l), "v"(x[S]), "n"(S));
-    return z;
-}
-// z_i = n_i (z_i + sum over s < i of l_i[s] z_s) row after row; l_i[s] lies in lane s of each row of 16, as n does.
-template <int I, int S>
-__device__ __forceinline__ void add_rows(float (&z)[C], const float (&l)[C])
-{
-    if constexpr (S < I) {
-        constexpr int TERMS = I - S >= 4 ? 4 : 1;
-        z[I] = add_terms<S, TERMS>(z[I], l[I], z);
-        add_rows<I, S + TERMS>(z, l);
-    }
-}
-template <int I>
+// The solution z_i = n_i (z_i + sum over s < i of l_i[s] z_s) of 16 rows, column by column: l_i[s] lies in lane s
+// of each row of 16 lanes, n_i in lane i.  One instruction a term reads its lane and multiplies (the compiler forms
+// two); as soon as a z_s is known it goes into all later rows, so that the terms are independent.  A first
+// half of 8 rows, its terms in the second half, the second half.  The wait in front keeps the distance that a
+// lane-crossing read needs from what wrote the register; nothing inside writes l or n.
+#define SI_TERM(i, l, s, x) "v_fmac_f32_dpp %" #i ", %" #l ", %" #x " row_newbcast:" #s " row_mask:0xf bank_mask:0xf\n\t"
+#define SI_LENGTH(i, s) "v_mul_f32_dpp %" #i ", %15, %" #i " row_newbcast:" #s " row_mask:0xf bank_mask:0xf\n\t"
+// operands: z_0 .. z_7 = %0 .. %7, l_1 .. l_7 = %8 .. %14, n = %15; B: the half's first lane
+#define SI_HALF(B0, B1, B2, B3, B4, B5, B6, B7)                                                                            \
+    "s_nop 1\n\t" SI_LENGTH(0, B0)                                                                                         \
+    SI_TERM(1, 8, B0, 0) SI_TERM(2, 9, B0, 0) SI_TERM(3, 10, B0, 0) SI_LENGTH(1, B1)                                        \
+    SI_TERM(4, 11, B0, 0) SI_TERM(5, 12, B0, 0) SI_TERM(6, 13, B0, 0) SI_TERM(7, 14, B0, 0)                                 \
+    SI_TERM(2, 9, B1, 1) SI_TERM(3, 10, B1, 1) SI_TERM(4, 11, B1, 1) SI_LENGTH(2, B2)                                       \
+    SI_TERM(5, 12, B1, 1) SI_TERM(6, 13, B1, 1) SI_TERM(7, 14, B1, 1)                                                       \
+    SI_TERM(3, 10, B2, 2) SI_TERM(4, 11, B2, 2) SI_TERM(5, 12, B2, 2) SI_LENGTH(3, B3)                                      \
+    SI_TERM(6, 13, B2, 2) SI_TERM(7, 14, B2, 2)                                                                             \
+    SI_TERM(4, 11, B3, 3) SI_TERM(5, 12, B3, 3) SI_TERM(6, 13, B3, 3) SI_LENGTH(4, B4) SI_TERM(7, 14, B3, 3)                \
+    SI_TERM(5, 12, B4, 4) SI_TERM(6, 13, B4, 4) SI_TERM(7, 14, B4, 4) SI_LENGTH(5, B5)                                      \
+    SI_TERM(6, 13, B5, 5) SI_TERM(7, 14, B5, 5) SI_LENGTH(6, B6)                                                            \
+    SI_TERM(7, 14, B6, 6) SI_LENGTH(7, B7)
+// operands: z_8 .. z_15 = %0 .. %7, l_8 .. l_15 = %8 .. %15, z_0 .. z_7 = %16 .. %23
+#define SI_ACROSS(s, x)                                                                                                     \
+    SI_TERM(0, 8, s, x) SI_TERM(1, 9, s, x) SI_TERM(2, 10, s, x) SI_TERM(3, 11, s, x) SI_TERM(4, 12, s, x)                  \
+    SI_TERM(5, 13, s, x) SI_TERM(6, 14, s, x) SI_TERM(7, 15, s, x)
 __device__ __forceinline__ void solve_rows(float (&z)[C], const float (&l)[C], float n)
 {
-    if constexpr (I < C) {
-        add_rows<I, 0>(z, l);
-        z[I] *= row_lane<I>(n);
-        solve_rows<I + 1>(z, l, n);
-    }
+    asm(SI_HALF(0, 1, 2, 3, 4, 5, 6, 7)
+        : "+&v"(z[0]), "+&v"(z[1]), "+&v"(z[2]), "+&v"(z[3]), "+&v"(z[4]), "+&v"(z[5]), "+&v"(z[6]), "+&v"(z[7])
+        : "v"(l[1]), "v"(l[2]), "v"(l[3]), "v"(l[4]), "v"(l[5]), "v"(l[6]), "v"(l[7]), "v"(n));
+    asm("s_nop 1\n\t" SI_ACROSS(0, 16) SI_ACROSS(1, 17) SI_ACROSS(2, 18) SI_ACROSS(3, 19) SI_ACROSS(4, 20) SI_ACROSS(5, 21)
+            SI_ACROSS(6, 22) SI_ACROSS(7, 23)
+        : "+&v"(z[8]), "+&v"(z[9]), "+&v"(z[10]), "+&v"(z[11]), "+&v"(z[12]), "+&v"(z[13]), "+&v"(z[14]), "+&v"(z[15])
+        : "v"(l[8]), "v"(l[9]), "v"(l[10]), "v"(l[11]), "v"(l[12]), "v"(l[13]), "v"(l[14]), "v"(l[15]), "v"(z[0]), "v"(z[1]),
+          "v"(z[2]), "v"(z[3]), "v"(z[4]), "v"(z[5]), "v"(z[6]), "v"(z[7]));
+    asm(SI_HALF(8, 9, 10, 11, 12, 13, 14, 15)
+        : "+&v"(z[8]), "+&v"(z[9]), "+&v"(z[10]), "+&v"(z[11]), "+&v"(z[12]), "+&v"(z[13]), "+&v"(z[14]), "+&v"(z[15])
+        : "v"(l[9]), "v"(l[10]), "v"(l[11]), "v"(l[12]), "v"(l[13]), "v"(l[14]), "v"(l[15]), "v"(n));
 }
+#undef SI_TERM
+#undef SI_LENGTH
+#undef SI_HALF
+#undef SI_ACROSS
 template <int I>
 __device__ __forceinline__ void scale_rows(float* to, const float (&z)[C], float n)
 {
@@ -291,7 +297,6 @@ struct ChunkLds {
     float m[C][LD];                    // A, B, D, E beside one another
     float w[C][LD];                    // W in the columns that A has in m
     float y[C][LD];
-    float params[6][N];                // of the head: w0, a0, v0 (times -log2(e)), k_k, k_a, r_k
 };
 
 __device__ __forceinline__ f4 row4(const float (&m)[C][LD], int row, int col) { return *reinterpret_cast<const f4*>(&m[row][col]); }
@@ -319,6 +324,13 @@ struct Blocks {
     }
 };
 
+__device__ __forceinline__ void put_column4(float (&m)[C][LD], int row, int col, f4 v)
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        m[row + i][col] = v[i];
+}
+
 __device__ __forceinline__ f4 load4(const float* p)   // at a multiple of 4 bytes
 {
     f4 v;
@@ -326,9 +338,9 @@ __device__ __forceinline__ f4 load4(const float* p)   // at a multiple of 4 byte
     return v;
 }
 
-__device__ __forceinline__ f4 load_at(const float* uniform, uint32_t bytes)
+__device__ __forceinline__ float load_at(const float* uniform, uint32_t bytes)
 {
-    return *reinterpret_cast<const f4*>(reinterpret_cast<const char*>(uniform) + bytes);
+    return *reinterpret_cast<const float*>(reinterpret_cast<const char*>(uniform) + bytes);
 }
 
 // 1 / (1 + exp(-(x + bias))), shift = -LOG2E * bias
@@ -337,32 +349,48 @@ __device__ __forceinline__ float sigmoid_shifted(float x, float shift)
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(fmaf(x, -LOG2E, shift)));
 }
 
+// TRANSFER: only what a stretch's transfer needs (no readout).
+template <bool TRANSFER>
 __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks blocks)
 {
     const int lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
     const int q = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3);
     const int64_t width = static_cast<int64_t>(a.heads) * N;
-    const int ch = 16 * q + 4 * g;                       // this lane's four channels, of row t
+    const int ch = 16 * q + t;
     const bool first = a.first_layer != 0;
     const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int e = h * N + ch;
+    const float w0 = -LOG2E * a.w0[e], a0 = -LOG2E * a.a0[e], v0 = first ? 0.0f : -LOG2E * a.v0[e], kkk = a.k_k[e], kka = a.k_a[e],
+                rk = a.r_k[e];
     struct {
         f4 r, k, v, wl, al, vl, vf;
     } x;
-    // (a row behind the block's last reads the last again, and is masked where it counts)
-    auto load = [&](int at, int last) {
-        const int64_t from = at * width + h * N;
-        const uint32_t lane_at = 4u * (min(t, last - 1 - at) * static_cast<uint32_t>(width) + ch);
-        x.r = load_at(a.r + from, lane_at);
-        x.k = load_at(a.k + from, lane_at);
-        x.v = load_at(a.v + from, lane_at);
-        x.wl = load_at(a.w_lora + from, lane_at);
-        x.al = load_at(a.a_lora + from, lane_at);
+    uint32_t full[4];   // bytes from a block's first value of the head to this lane's
+#pragma unroll
+    for (int v = 0; v < 4; v++)
+        full[v] = 4u * ((4 * g + v) * static_cast<uint32_t>(width) + ch);
+    auto load = [&](int first_row, int last) {
+        const int64_t from = first_row * width + h * N;
+        uint32_t at[4];
+#pragma unroll
+        for (int v = 0; v < 4; v++)   // (a row behind the block's last reads the last again, and is masked where it counts)
+            at[v] = last - first_row == C ? full[v] : 4u * (min(4 * g + v, last - first_row - 1) * static_cast<uint32_t>(width) + ch);
+        auto rows = [&](const float* p) {
+            p += from;
+            return f4{load_at(p, at[0]), load_at(p, at[1]), load_at(p, at[2]), load_at(p, at[3])};
+        };
+        if (!TRANSFER)
+            x.r = rows(a.r);
+        x.k = rows(a.k);
+        x.v = rows(a.v);
+        x.wl = rows(a.w_lora);
+        x.al = rows(a.a_lora);
         if (!first) {
-            x.vl = load_at(a.v_lora + from, lane_at);
-            x.vf = load_at(a.v_first + from, lane_at);
+            x.vl = rows(a.v_lora);
+            x.vf = rows(a.v_first);
         }
     };
-    x.vl = x.vf = zero;
+    x.r = x.vl = x.vf = zero;
     load(blocks.at, blocks.last());
     for (int stage = 0; blocks.at < blocks.end; stage++) {
         BlockLds& b = lds.block[stage & 1];
@@ -370,57 +398,68 @@ __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks
         // 1: the rows' factors
         if (rows < C) {   // a decay of 1, the rest 0
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool in = t < rows;
-                x.wl[j] = in ? x.wl[j] : -3e38f;
-                x.al[j] = in ? x.al[j] : 0.0f;
-                x.vl[j] = in ? x.vl[j] : 0.0f;
-                x.vf[j] = in ? x.vf[j] : 0.0f;
-                x.k[j] = in ? x.k[j] : 0.0f;
-                x.v[j] = in ? x.v[j] : 0.0f;
-                x.r[j] = in ? x.r[j] : 0.0f;
+            for (int v = 0; v < 4; v++) {
+                const bool in = 4 * g + v < rows;
+                x.wl[v] = in ? x.wl[v] : -3e38f;
+                x.al[v] = in ? x.al[v] : 0.0f;
+                x.vl[v] = in ? x.vl[v] : 0.0f;
+                x.vf[v] = in ? x.vf[v] : 0.0f;
+                x.k[v] = in ? x.k[v] : 0.0f;
+                x.v[v] = in ? x.v[v] : 0.0f;
+                x.r[v] = in ? x.r[v] : 0.0f;
             }
         }
-        f4 al, rh, be, kh, va, decay;
-        auto par = [&](int i) { return *reinterpret_cast<const f4*>(&lds.params[i][ch]); };
-        const f4 w0 = par(0), a0 = par(1), v0 = par(2), kkk = par(3), kka = par(4), rk = par(5);
-        float squares = 0.0f, bonus = 0.0f, top = 0.0f;
+        f4 al, rh, be, kh, va, cum, squares, bonus;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            float c = -0.606531f * LOG2E * sigmoid_shifted(x.wl[j], w0[j]);
-            c += row_shr<1>(c);
-            c += row_shr<2>(c);
-            c += row_shr<4>(c);
-            c += row_shr<8>(c);
-            decay[j] = __builtin_amdgcn_exp2f(c);
+        for (int v = 0; v < 4; v++)
+            cum[v] = -0.606531f * LOG2E * sigmoid_shifted(x.wl[v], w0);
+        cum[1] += cum[0];
+        cum[2] += cum[1];
+        cum[3] += cum[2];
+        const float earlier = rows_before(cum[3]);
+        float decay = __builtin_amdgcn_exp2f(earlier), top = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const float c = earlier + cum[v];
+            const float ad = sigmoid_shifted(x.al[v], a0);
+            const float sk = x.k[v] * kkk;
+            const float key = fmaf(x.k[v] * kka, ad - 1.0f, x.k[v]);
+            va[v] = first ? x.v[v] : fmaf(x.vf[v] - x.v[v], sigmoid_shifted(x.vl[v], v0), x.v[v]);
+            al[v] = sk * decay;
+            decay = __builtin_amdgcn_exp2f(c);
             const float shrink = __builtin_amdgcn_exp2f(-c);
-            const float ad = sigmoid_shifted(x.al[j], a0[j]);
-            const float sk = x.k[j] * kkk[j];
-            const float key = fmaf(x.k[j] * kka[j], ad - 1.0f, x.k[j]);
-            va[j] = first ? x.v[j] : fmaf(x.vf[j] - x.v[j], sigmoid_shifted(x.vl[j], v0[j]), x.v[j]);
-            al[j] = sk * row_shr_or_one(decay[j]);
-            be[j] = (sk * ad) * shrink;
-            kh[j] = key * shrink;
-            rh[j] = x.r[j] * decay[j];
-            squares = fmaf(sk, sk, squares);
-            bonus = fmaf(key * x.r[j], rk[j], bonus);
-            top = largest(largest(top, al[j], kh[j]), rh[j], va[j]);   // (beta is at most alpha / decay)
+            be[v] = (sk * ad) * shrink;
+            kh[v] = key * shrink;
+            rh[v] = x.r[v] * decay;
+            squares[v] = sk * sk;
+            bonus[v] = key * x.r[v] * rk;
+            top = largest(largest(top, al[v], kh[v]), rh[v], va[v]);   // (beta is at most alpha / decay)
         }
-        *reinterpret_cast<f4*>(&b.alpha[t][ch]) = al;
-        *reinterpret_cast<f4*>(&b.rho[t][ch]) = rh;
-        *reinterpret_cast<f4*>(&b.beta[t][ch]) = be;
-        *reinterpret_cast<f4*>(&b.khat[t][ch]) = kh;
-        *reinterpret_cast<f4*>(&b.value[t][ch]) = va;
-        squares = rows_sum(squares);
-        bonus = rows_sum(bonus);
-        if (g == 0) {
-            b.squares[q][t] = squares;
-            b.bonus[q][t] = bonus;
+        put_column4(b.alpha, 4 * g, ch, al);
+        if (!TRANSFER)
+            put_column4(b.rho, 4 * g, ch, rh);
+        put_column4(b.beta, 4 * g, ch, be);
+        put_column4(b.khat, 4 * g, ch, kh);
+        put_column4(b.value, 4 * g, ch, va);
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            squares[v] = row_sum<16>(squares[v]);
+            if (!TRANSFER)
+                bonus[v] = row_sum<16>(bonus[v]);
         }
-        if (t == C - 1)
-            *reinterpret_cast<f4*>(&b.decay[ch]) = decay;
-        if (first && t < rows)
-            *reinterpret_cast<f4*>(a.v_first + (at + t) * width + h * N + ch) = x.v;
+        if (t == 0) {
+            *reinterpret_cast<f4*>(&b.squares[q][4 * g]) = squares;
+            if (!TRANSFER)
+                *reinterpret_cast<f4*>(&b.bonus[q][4 * g]) = bonus;
+        }
+        if (g == 3)
+            b.decay[ch] = decay;
+        if (first && !TRANSFER) {
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+                if (4 * g + v < rows)
+                    a.v_first[(at + 4 * g + v) * width + e] = x.v[v];
+        }
         if (!(top < 0x1p50f))
             b.odd = 1;
         __syncthreads();
@@ -430,7 +469,7 @@ __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks
             load(blocks.at, blocks.last());
         float length = b.squares[0][t] + b.squares[1][t] + b.squares[2][t] + b.squares[3][t];
         length = __builtin_amdgcn_rsqf(length > 1e-24f ? length : 1e-24f);   // 1 / |sk| of row t
-        {
+        if (!TRANSFER || q < 2) {
             const auto& left = q < 2 ? b.alpha : b.rho;
             const auto& right = q & 1 ? b.khat : b.beta;
             f4 l[4], r[4], m0 = zero, m1 = zero;
@@ -439,6 +478,7 @@ __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks
                 l[j] = row4(left, t, 16 * j + 4 * g);
                 r[j] = row4(right, t, 16 * j + 4 * g);
             }
+            __builtin_amdgcn_sched_barrier(0);   // all reads before the first product
             m0 = mfma4(l[0], r[0], m0);
             m1 = mfma4(l[1], r[1], m1);
             m0 = mfma4(l[2], r[2], m0);
@@ -449,7 +489,7 @@ __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks
             for (int v = 0; v < 4; v++) {
                 const int i = 4 * g + v;
                 const int keep = -static_cast<int>(i < rows && t < (q < 2 ? i : i + 1));   // (as bits: a choice branches)
-                lds.m[i][16 * q + t] = __int_as_float(__float_as_int((m0[v] + m1[v]) * f) & keep);
+                lds.m[i][ch] = __int_as_float(__float_as_int((m0[v] + m1[v]) * f) & keep);
             }
         }
         __syncthreads();
@@ -465,20 +505,22 @@ __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks
                 l[i] = lds.m[i][t];
                 z[i] = column[i * LD];
             }
-            solve_rows<0>(z, l, length);
+            solve_rows(z, l, length);
             float* const solved = of_b ? &lds.w[0][t] : &b.alpha[0][16 * q + t];   // (w: the same from all four waves)
             if (lane < 32)
                 scale_rows<0>(solved, z, length);
             wave_sync();
             const f4 v_tile = column4(b.value, 4 * g, 16 * q + t);
             b.v_part[q][lane] = mfma4(row4(lds.w, t, 4 * g), v_tile, zero);
-            const f4 d = -row4(lds.m, t, 32 + 4 * g);
-            const f4 rho = mfma4(d, column4(b.alpha, 4 * g, 16 * q + t), column4(b.rho, 4 * g, 16 * q + t));
-            const f4 zt = mfma4(column4(lds.w, 4 * g, t), d, row4(lds.m, t, 48 + 4 * g));   // Z^T
+            if (!TRANSFER) {
+                const f4 d = -row4(lds.m, t, 32 + 4 * g);
+                const f4 rho = mfma4(d, column4(b.alpha, 4 * g, 16 * q + t), column4(b.rho, 4 * g, 16 * q + t));
+                const f4 zt = mfma4(column4(lds.w, 4 * g, t), d, row4(lds.m, t, 48 + 4 * g));   // Z^T
 #pragma unroll
-            for (int v = 0; v < 4; v++)
-                b.rho[4 * g + v][16 * q + t] = rho[v];
-            b.y_part[q][lane] = mfma4(zt, v_tile, zero);
+                for (int v = 0; v < 4; v++)
+                    b.rho[4 * g + v][16 * q + t] = rho[v];
+                b.y_part[q][lane] = mfma4(zt, v_tile, zero);
+            }
         }
         if (threadIdx.x == CHUNK_THREADS - 1)
             lds.block[(stage & 1) ^ 1].odd = 0;
@@ -490,26 +532,33 @@ __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks
     __syncthreads();
 }
 
-__device__ void chunk_advance(const WkvRowsArgs& a, ChunkLds& lds, int h, int from, int to, Blocks blocks)
+// Where a workgroup's state comes from and goes to.
+struct StateEnds {
+    const f4* start;   // S^T tiles as the matrix instructions hold them, or null: from `from`
+    const float* from; // [64][64], or null: all `fill`
+    float fill;
+    float* to;         // [64][64], or null
+};
+
+__device__ __forceinline__ void load_state(const StateEnds& ends, int w, f4 (&S)[4])
+{
+    const int lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        S[j] = ends.start ? ends.start[(4 * w + j) * 64 + lane]
+               : ends.from ? *reinterpret_cast<const f4*>(ends.from + (16 * w + t) * N + 16 * j + 4 * g)
+                           : f4{ends.fill, ends.fill, ends.fill, ends.fill};
+}
+
+__device__ void chunk_advance(const WkvRowsArgs& a, ChunkLds& lds, int h, const StateEnds& ends, Blocks blocks)
 {
     const int lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t width = static_cast<int64_t>(a.heads) * N;
     const int tn = 4 * w + g, cn = 4 * t;   // row and four channels in the normalisation
     const f4 lw = load4(a.lnx_weight + h * N + cn), lb = load4(a.lnx_bias + h * N + cn);
-    // S^T tiles: keys 16 j + 4 g + v, value 16 w + t
-    f4 S[4];
-    if (from >= 0 && from < a.batch.slots) {
-        const float* p = a.state + ((static_cast<int64_t>(from) * a.heads + h) * N + 16 * w + t) * N + 4 * g;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            S[j] = *reinterpret_cast<const f4*>(p + 16 * j);
-    } else {
-        const float z = from == -1 ? 0.0f : __builtin_nanf("");
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            S[j] = f4{z, z, z, z};
-    }
+    f4 S[4];   // S^T tiles: keys 16 j + 4 g + v, value 16 w + t
+    load_state(ends, w, S);
     // while the first block is prepared
     int at = blocks.at, rows = blocks.last() - at;
     __syncthreads();
@@ -526,7 +575,7 @@ __device__ void chunk_advance(const WkvRowsArgs& a, ChunkLds& lds, int h, int fr
             xr = mfma4(row4(b.rho, t, 16 * j + 4 * g), S[j], xr);
         };
         if (have) {
-            gate = load_at(a.gate + at * width + h * N, 4u * (min(tn, rows - 1) * static_cast<uint32_t>(width) + cn));
+            gate = load4(a.gate + (at + min(tn, rows - 1)) * width + h * N + cn);
             xa = b.v_part[w][lane];
             xr = b.y_part[w][lane];
             part(0);
@@ -572,59 +621,309 @@ __device__ void chunk_advance(const WkvRowsArgs& a, ChunkLds& lds, int h, int fr
         if (!more)
             break;
     }
-    if (to >= 0 && to < a.batch.slots) {
-        float* p = a.state + ((static_cast<int64_t>(to) * a.heads + h) * N + 16 * w + t) * N + 4 * g;
+    if (ends.to) {
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            *reinterpret_cast<f4*>(p + 16 * j) = S[j];
+            *reinterpret_cast<f4*>(ends.to + (16 * w + t) * N + 16 * j + 4 * g) = S[j];
     }
 }
 
-// One head of one sequence, block after block.  While the state's waves take block i
+// A stretch's transfer: the state behind it is S M + (S's start at zero), and M's rows are 64 more states that start as
+// the unit matrix and take no values.
+__device__ void chunk_transfer(ChunkLds& lds, float* record, Blocks blocks)
+{
+    const int lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    f4 S[4], M[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            S[j][v] = 0.0f;
+            M[j][v] = 16 * j + 4 * g + v == 16 * w + t ? 1.0f : 0.0f;
+        }
+    __syncthreads();
+    bool counts = blocks.next(lds.block[0].odd != 0);
+    __syncthreads();
+    __syncthreads();
+    for (int stage = 1;; stage++) {
+        const BlockLds& b = lds.block[(stage & 1) ^ 1];
+        const bool have = counts, more = blocks.at < blocks.end;
+        f4 xs, xm;
+        auto part = [&](int j) {
+            const f4 al = row4(b.alpha, t, 16 * j + 4 * g);
+            xs = mfma4(al, S[j], xs);
+            xm = mfma4(al, M[j], xm);
+        };
+        if (have) {
+            xs = b.v_part[w][lane];
+            xm = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            part(0);
+            part(1);
+        }
+        __syncthreads();
+        counts = more && blocks.next(lds.block[stage & 1].odd != 0);
+        if (have) {
+            part(2);
+            part(3);
+        }
+        __syncthreads();
+        if (have) {
+            const f4 us = -xs, um = -xm, v_tile = column4(b.value, 4 * g, 16 * w + t);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const f4 beta = column4(b.beta, 4 * g, 16 * j + t), decay = *reinterpret_cast<const f4*>(&b.decay[16 * j + 4 * g]);
+                M[j] = mfma4(beta, um, M[j]) * decay;
+                S[j] = mfma4(beta, us, S[j]);
+                S[j] = mfma4(column4(b.khat, 4 * g, 16 * j + t), v_tile, S[j]) * decay;
+            }
+        }
+        __syncthreads();
+        if (!more)
+            break;
+    }
+    f4* const start = reinterpret_cast<f4*>(record + N * N);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        start[(4 * w + j) * 64 + lane] = S[j];
+#pragma unroll
+        for (int v = 0; v < 4; v++)   // M^T, row after row
+            record[(16 * j + 4 * g + v) * N + 16 * w + t] = M[j][v];
+    }
+}
+
+// ---- long sequences in stretches ---------------------------------------------------------------
+//
+// Where the heads of all sequences are too few for the card, long sequences are cut: (1) each stretch's transfer
+// (M, N), all stretches at once; (2) the states between them, S_(i+1) = S_i M_i + N_i; (3) every stretch as a
+// sequence of its own.  (1) costs about 0.8 of (3).
+
+constexpr int RECORD = 2 * N * N;        // floats of a stretch and head: M^T; N, later the next stretch's start
+constexpr int HEAD_STRETCHES = 512;      // stretches times heads: two workgroups a compute unit
+constexpr int LEAST_STRETCH = 64;        // rows
+
+struct Stretch {
+    int sequence, first, last;   // rows
+    int record;                  // of the sequence's first stretch, or -1: the sequence is whole
+    int index, count;            // of the sequence's stretches
+};
+struct Plan {
+    int stretches, cut;          // in list, and sequences that are cut
+    int pad[2];
+    Stretch list[1];             // every stretch of the sequences that go by blocks; cut sequences' first ones again behind `room`
+};
+
+__device__ __forceinline__ StateEnds state_ends(const WkvRowsArgs& a, int s, int h)
+{
+    const int from = a.batch.from[s], to = a.batch.to[s];
+    auto at = [&](int slot) { return a.state + (static_cast<int64_t>(slot) * a.heads + h) * N * N; };
+    return {nullptr, from >= 0 && from < a.batch.slots ? at(from) : nullptr, from == -1 ? 0.0f : __builtin_nanf(""),
+            to >= 0 && to < a.batch.slots ? at(to) : nullptr};
+}
+
+// One head of one sequence or stretch, block after block.  While the state's waves take block i
 // (64 matrix instructions each), the others prepare block i + 1 (32 each, and the
-// exponentials), in three phases between barriers.
-__global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs a, int over)
+// exponentials), in three phases between barriers.  FP32 matrix instructions take the vector units' place (32 and 5 cycles side by
+// side on a SIMD take 50 in all): a block costs 3072 cycles of them and about 800 vector instructions a SIMD.
+enum ChunkPass { CHUNK_SEQUENCES, CHUNK_STRETCHES, CHUNK_TRANSFERS };
+
+template <int PASS>
+__global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs a, int over, const Plan* plan, float* records)
 {
     __shared__ ChunkLds lds;
     const int s = blockIdx.x / a.heads, h = blockIdx.x - s * a.heads;
-    RowSpan span = rows_of(a.batch, s);
+    RowSpan span;
+    StateEnds ends;
+    float* record = nullptr;
+    if constexpr (PASS == CHUNK_SEQUENCES) {
+        span = rows_of(a.batch, s);
+        if (span.last - span.first <= over)
+            return;
+        ends = state_ends(a, s, h);
+    } else {
+        if (s >= plan->stretches)
+            return;
+        const Stretch part = plan->list[s];
+        span = {part.first, part.last};
+        auto record_of = [&](int i) { return records + (static_cast<int64_t>(part.record + i) * a.heads + h) * RECORD; };
+        if (PASS == CHUNK_TRANSFERS) {
+            if (part.record < 0 || part.index == part.count - 1)
+                return;
+            record = record_of(part.index);
+        } else {
+            ends = state_ends(a, part.sequence, h);
+            if (part.record >= 0) {   // (the first stretch's start lies in the last one's record)
+                ends.start = reinterpret_cast<const f4*>(record_of(part.index ? part.index - 1 : part.count - 1) + N * N);
+                ends.to = part.index == part.count - 1 ? ends.to : nullptr;
+            }
+        }
+    }
     span.first = __builtin_amdgcn_readfirstlane(span.first);
     span.last = __builtin_amdgcn_readfirstlane(span.last);
-    if (span.last - span.first <= over)
-        return;
     if (threadIdx.x < 2)
         lds.block[threadIdx.x].odd = 0;
-    if (threadIdx.x < N) {
-        const int t = threadIdx.x, e = h * N + t;
-        lds.params[0][t] = -LOG2E * a.w0[e];
-        lds.params[1][t] = -LOG2E * a.a0[e];
-        lds.params[2][t] = a.first_layer ? 0.0f : -LOG2E * a.v0[e];
-        lds.params[3][t] = a.k_k[e];
-        lds.params[4][t] = a.k_a[e];
-        lds.params[5][t] = a.r_k[e];
-    }
     __syncthreads();
     const Blocks blocks{span.first, span.last, span.first};
-    if (threadIdx.x < CHUNK_THREADS / 2)
-        chunk_advance(a, lds, h, a.batch.from[s], a.batch.to[s], blocks);
+    if (threadIdx.x >= CHUNK_THREADS / 2)
+        chunk_prepare<PASS == CHUNK_TRANSFERS>(a, lds, h, blocks);
+    else if (PASS == CHUNK_TRANSFERS)
+        chunk_transfer(lds, record, blocks);
     else
-        chunk_prepare(a, lds, h, blocks);
+        chunk_advance(a, lds, h, ends, blocks);
+}
+
+// The states between a cut sequence's stretches.  A workgroup takes 16 values of one head, each of its waves 16 keys:
+// a stretch costs it 16 matrix instructions a wave, an exchange of the state's tiles through LDS, and M's 16 KiB,
+// requested a stretch ahead.
+__global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, const Plan* plan, int room, float* records)
+{
+    __shared__ f4 s_tile[2][4][64];
+    const int c = blockIdx.x / (4 * a.heads), rest = blockIdx.x - c * 4 * a.heads, h = rest >> 2, i = rest & 3;
+    if (c >= plan->cut)
+        return;
+    const Stretch part = plan->list[room + c];
+    const int lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto record_of = [&](int k) { return records + (static_cast<int64_t>(part.record + k) * a.heads + h) * RECORD; };
+    auto tile_of = [&](int k) { return reinterpret_cast<f4*>(record_of(k) + N * N) + (4 * i + w) * 64 + lane; };
+    f4 S[4], m[4], next[4], add, add_next;
+    load_state(state_ends(a, part.sequence, h), i, S);
+    auto load = [&](int k, f4(&rows)[4], f4& n) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            rows[j] = *reinterpret_cast<const f4*>(record_of(k) + (16 * w + t) * N + 16 * j + 4 * g);
+        n = *tile_of(k);
+    };
+    load(0, next, add_next);
+    *tile_of(part.count - 1) = w == 0 ? S[0] : w == 1 ? S[1] : w == 2 ? S[2] : S[3];
+    for (int k = 0; k + 1 < part.count; k++) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            m[j] = next[j];
+        add = add_next;
+        if (k + 2 < part.count)
+            load(k + 1, next, add_next);
+        f4 other = {0.0f, 0.0f, 0.0f, 0.0f};
+        add = mfma4(m[0], S[0], add);
+        other = mfma4(m[1], S[1], other);
+        add = mfma4(m[2], S[2], add);
+        other = mfma4(m[3], S[3], other);
+        add += other;
+        *tile_of(k) = add;
+        s_tile[k & 1][w][lane] = add;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            S[j] = s_tile[k & 1][j][lane];
+    }
+}
+
+// How a launch cuts its sequences: into stretches of at least this many rows, or 0: not at all.
+int stretch_rows(const WkvRowsArgs& a)
+{
+    const int64_t each = (static_cast<int64_t>(a.batch.rows) * a.heads + HEAD_STRETCHES - 1) / HEAD_STRETCHES;
+    const int64_t rows = (each > LEAST_STRETCH ? each + C - 1 : LEAST_STRETCH) / C * C;
+    return a.batch.max_rows >= 3 * rows ? static_cast<int>(rows) : 0;
+}
+
+// The list of stretches of all sequences over `over` rows, by one workgroup: 4096 sequences in turns of 256.
+__device__ void make_plan(const WkvRowsArgs& a, int over, int stretch, int room, Plan* plan)
+{
+    __shared__ int s_count[3][256];
+    const int t = threadIdx.x;
+    int stretches = 0, cut = 0, records = 0;
+    // where starts fall, sequences may share rows, and the list's room is for rows that are one sequence's
+    int64_t all = 0;
+    for (int i = t; i < a.batch.sequences; i += 256) {
+        const RowSpan span = rows_of(a.batch, i);
+        all += span.last - span.first;
+    }
+    s_count[0][t] = static_cast<int>(min(all, static_cast<int64_t>(a.batch.rows) + 1));
+    __syncthreads();
+    all = 0;
+    for (int i = 0; i < 256; i++)
+        all += s_count[0][i];
+    if (all > a.batch.rows) {
+        if (t == 0)
+            plan->stretches = plan->cut = 0;
+        return;
+    }
+    for (int base = 0; base < a.batch.sequences; base += 256) {
+        RowSpan span{0, 0};
+        if (base + t < a.batch.sequences)
+            span = rows_of(a.batch, base + t);
+        const int rows = span.last - span.first;
+        const int most = rows >= 2 * stretch ? rows / stretch : 1;
+        const int each = ((rows + most - 1) / most + C - 1) / C * C;
+        const int parts = rows <= over ? 0 : most > 1 ? (rows + each - 1) / each : 1;   // (none of them empty)
+        const int own[3] = {parts, parts > 1, parts > 1 ? parts : 0};
+        int before[3], sum[3];
+        __syncthreads();
+        for (int i = 0; i < 3; i++)
+            s_count[i][t] = own[i];
+        __syncthreads();
+        for (int step = 1; step < 256; step *= 2) {
+            for (int i = 0; i < 3; i++)
+                before[i] = t >= step ? s_count[i][t - step] : 0;
+            __syncthreads();
+            for (int i = 0; i < 3; i++)
+                s_count[i][t] += before[i];
+            __syncthreads();
+        }
+        for (int i = 0; i < 3; i++) {
+            sum[i] = s_count[i][255];
+            before[i] = s_count[i][t] - own[i];
+        }
+        for (int k = 0; k < parts; k++) {
+            const Stretch part{base + t, span.first + k * each, k + 1 < parts ? span.first + (k + 1) * each : span.last,
+                               parts > 1 ? records + before[2] : -1, k, parts};
+            plan->list[stretches + before[0] + k] = part;
+            if (parts > 1 && k == 0)
+                plan->list[room + cut + before[1]] = part;
+        }
+        stretches += sum[0];
+        cut += sum[1];
+        records += sum[2];
+    }
+    if (t == 0) {
+        plan->stretches = stretches;
+        plan->cut = cut;
+    }
 }
 
 }  // namespace
 
-int64_t wkv_rows_workspace_bytes(int) { return 16; }
+// Stretches: at most one for every `over` + 1 rows that is a sequence's only one, and HEAD_STRETCHES / heads of cut ones.
+constexpr int FEW_ROWS = 8;              // sequences of up to this many rows go row by row
+constexpr int WHOLE_ROOM = ROW_SEQUENCES_MAX;
 
-// Sequences of up to this many rows go row by row.
-constexpr int FEW_ROWS = 8;
+constexpr int64_t PLAN_BYTES = (sizeof(Plan) + (WHOLE_ROOM + 2 * HEAD_STRETCHES) * sizeof(Stretch) + 255) / 256 * 256;
+
+int64_t wkv_rows_workspace_bytes(int) { return PLAN_BYTES + static_cast<int64_t>(HEAD_STRETCHES) * RECORD * 4; }
 
 hipError_t launch_wkv_rows(const WkvRowsArgs& a, hipStream_t s)
 {
     const unsigned grid = static_cast<unsigned>(a.batch.sequences) * a.heads;
-    const bool long_ones = a.batch.max_rows > FEW_ROWS;
-    hipLaunchKernelGGL(wkv_few_kernel, dim3(grid), dim3(256), 0, s, a, long_ones ? FEW_ROWS : INT32_MAX);
-    if (long_ones)
-        hipLaunchKernelGGL(wkv_chunk_kernel, dim3(grid), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS);
+    Plan* const plan = reinterpret_cast<Plan*>(a.workspace);
+    float* const records = a.workspace + PLAN_BYTES / 4;
+    if (a.batch.max_rows <= FEW_ROWS) {
+        hipLaunchKernelGGL(wkv_few_kernel, dim3(grid), dim3(256), 0, s, a, INT32_MAX, 0, 0, nullptr);
+        return hipGetLastError();
+    }
+    const int stretch = stretch_rows(a);
+    if (stretch == 0) {
+        hipLaunchKernelGGL(wkv_few_kernel, dim3(grid), dim3(256), 0, s, a, FEW_ROWS, 0, 0, nullptr);
+        hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_SEQUENCES>, dim3(grid), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, nullptr, nullptr);
+        return hipGetLastError();
+    }
+    // what the host knows of the list's length
+    const int whole = a.batch.rows / (FEW_ROWS + 1) < a.batch.sequences ? a.batch.rows / (FEW_ROWS + 1) : a.batch.sequences;
+    const int cut_parts = a.batch.rows / stretch, room = whole + cut_parts;
+    const unsigned heads = static_cast<unsigned>(a.heads);
+    hipLaunchKernelGGL(wkv_few_kernel, dim3(grid + 1), dim3(256), 0, s, a, FEW_ROWS, stretch, room, plan);
+    hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_TRANSFERS>, dim3(room * heads), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, plan, records);
+    hipLaunchKernelGGL(wkv_join_kernel, dim3((cut_parts / 2) * heads * 4), dim3(256), 0, s, a, plan, room, records);
+    hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_STRETCHES>, dim3(room * heads), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, plan, records);
     return hipGetLastError();
 }
 
