@@ -621,7 +621,7 @@ int si_hip_paged_attention(si_hip_context* ctx, const si_hip_paged_attention_arg
  * state of zeros) and leaves its state in slot to[s] (-1: nowhere).  A sequence may
  * bring no row: its state is then not touched.  The starts may not fall and lie in
  * 0..rows; where they do not, outputs and states may hold anything (nothing outside them is
- * touched).  Rows in no sequence are neither read nor written.  from and to of a sequence may be equal, and
+ * touched).  Rows in no sequence are not written, and what they hold changes nothing.  from and to of a sequence may be equal, and
  * several sequences may go on from one slot; a slot that one sequence writes may not be
  * another's of the same call.  A sequence whose `from` is neither -1 nor
  * a slot goes on from a state of NaN; a `to` outside the slots is taken as -1.  The arrays

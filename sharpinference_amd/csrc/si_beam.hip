@@ -15,8 +15,11 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896f;
 constexpr int TILE = 2048, PER = TILE / 64;   // values of a wave's tile, and of a lane's
-constexpr int KEPT = 256;                     // values over a tile's bound that are ranked together
+constexpr int KEPT = 256;                     // values that are ranked together
 constexpr int SCAN_WAVES = 4, MERGE_WAVES = 8;
+constexpr float INF = __builtin_inff();
+
+typedef uint32_t Sixteen __attribute__((ext_vector_type(4), aligned(1)));   // bytes at any address, in one load or store
 
 typedef unsigned long long Key;   // order of a logit (high word: 0 for none) and of its token, lowest last
 
@@ -24,100 +27,36 @@ typedef unsigned long long Key;   // order of a logit (high word: 0 for none) an
 __device__ __forceinline__ uint32_t order_of(float v)
 {
     const uint32_t u = __float_as_uint(v + 0.0f);
-    return v > -__builtin_inff() ? u ^ (static_cast<int32_t>(u) < 0 ? 0xffffffffu : 0x80000000u) : 0u;
+    return v > -INF ? u ^ (static_cast<int32_t>(u) < 0 ? 0xffffffffu : 0x80000000u) : 0u;
 }
 __device__ __forceinline__ float logit_of(uint32_t order)
 {
     return __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
 }
 
-__device__ __forceinline__ uint32_t row_max_u32(uint32_t v, int width)
+// The smallest over groups of lanes of the groups' largest values: with k groups or more, so many values lie at or over it.
+__device__ __forceinline__ float group_bound(float best, int k)
 {
-    auto max_of = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
-    v = max_of(v, dpp_row<0xB1>(static_cast<int>(v)));
-    if (width >= 4) v = max_of(v, dpp_row<0x4E>(static_cast<int>(v)));
-    if (width >= 8) v = max_of(v, dpp_row<0x141>(static_cast<int>(v)));
-    if (width >= 16) v = max_of(v, dpp_row<0x140>(static_cast<int>(v)));
-    return v;
-}
-template <typename F>
-__device__ __forceinline__ uint32_t wave_reduce_u32(uint32_t v, F f)
-{
-    v = f(v, static_cast<uint32_t>(dpp_row<0xB1>(static_cast<int>(v))));
-    v = f(v, static_cast<uint32_t>(dpp_row<0x4E>(static_cast<int>(v))));
-    v = f(v, static_cast<uint32_t>(dpp_row<0x141>(static_cast<int>(v))));
-    v = f(v, static_cast<uint32_t>(dpp_row<0x140>(static_cast<int>(v))));
-    auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    v = f(a[0], a[1]);
-    auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return f(b[0], b[1]);
+    best = fmaxf(best, dpp_row<0xB1>(best));
+    if (k <= 16) best = fmaxf(best, dpp_row<0x4E>(best));
+    if (k <= 8) best = fmaxf(best, dpp_row<0x141>(best));
+    if (k <= 4) best = fmaxf(best, dpp_row<0x140>(best));
+    return -rows_max(row_max<16>(-best));
 }
 
-// Merges a tile's values (PERL a lane: value(j) gives order and token's key) into
-// the sorted list of the best k so far.  A bound first: the lanes fall into at least k
-// groups, and the smallest of the groups' largest values has k values at or over it, so only
-// values at or over the bound (and over the list's last) can be among the best k: some
-// dozens of 2048 of spread values, which are ranked by counting.  Where more than
-// KEPT remain (long runs of equal or masked logits), the k best are taken out one by one.
-template <int PERL, typename F>
-__device__ __forceinline__ void merge_tile(const uint32_t (&order)[PERL], F key_of, int k, Key* kept, Key* list)
+// Puts `count` kept keys and the list's own (k of them, sorted, 0 for none) in order: a key's place is the number of larger ones.
+__device__ __forceinline__ void rank_kept(int count, int k, Key* kept, Key* list)
 {
     const int lane = threadIdx.x & 63;
-    uint32_t best = 0;
-#pragma unroll
-    for (int j = 0; j < PERL; j++)
-        best = best > order[j] ? best : order[j];
-    const int width = k <= 4 ? 16 : k <= 8 ? 8 : k <= 16 ? 4 : 2;
-    const uint32_t low = wave_reduce_u32(row_max_u32(best, width), [](uint32_t a, uint32_t b) { return a < b ? a : b; });
-    const uint32_t last = static_cast<uint32_t>(list[k - 1] >> 32);
-    // (a value equal to the list's last has a higher token: tiles come in order)
-    const uint32_t bound = low > last + 1 ? low : last + 1;
-    int count = 0;
-#pragma unroll
-    for (int j = 0; j < PERL; j++) {
-        const uint64_t mask = __ballot(order[j] >= bound);
-        if (mask) {
-            const int at = count + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
-                                                             __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
-            if (order[j] >= bound && at < KEPT)
-                kept[at] = key_of(j);
-            count += __popcll(mask);
-        }
-    }
-    if (count == 0)
-        return;
-    if (count > KEPT) {
-        uint32_t out[(PERL + 31) / 32] = {};   // bit j: value j is taken out already
-        count = 0;
-        for (; count < k; count++) {
-            Key mine = 0;
-#pragma unroll
-            for (int j = 0; j < PERL; j++) {
-                const Key x = order[j] >= bound && !(out[j / 32] >> (j % 32) & 1) ? key_of(j) : 0;
-                mine = x > mine ? x : mine;
-            }
-            const uint32_t high = wave_reduce_u32(static_cast<uint32_t>(mine >> 32), [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-            const uint32_t token = wave_reduce_u32(static_cast<uint32_t>(mine >> 32) == high ? static_cast<uint32_t>(mine) : 0u,
-                                                   [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-            if (high == 0)
-                break;
-            const Key top = static_cast<Key>(high) << 32 | token;
-#pragma unroll
-            for (int j = 0; j < PERL; j++)
-                out[j / 32] |= static_cast<uint32_t>(order[j] >= bound && key_of(j) == top) << (j % 32);
-            if (lane == 0)
-                kept[count] = top;
-        }
-    }
-    // the list's own values behind the kept ones, and each one's place by counting
-    if (lane < k && list[lane] != 0)
-        kept[count + lane] = list[lane];
-    const uint64_t held = __ballot(lane < k && list[lane] != 0);   // a prefix of the lanes: the list is sorted
-    count += __popcll(held);
+    const Key own = lane < k ? list[lane] : 0;
+    if (own != 0)
+        kept[count + lane] = own;
+    count += __popcll(__ballot(own != 0));   // (a prefix of the lanes)
     wave_sync();
     for (int i = lane; i < count; i += 64) {
         const Key mine = kept[i];
         int rank = 0;
+#pragma unroll 4
         for (int j = 0; j < count; j++)
             rank += kept[j] > mine;
         if (rank < k)
@@ -126,16 +65,66 @@ __device__ __forceinline__ void merge_tile(const uint32_t (&order)[PERL], F key_
     wave_sync();
 }
 
+// Merges a tile's values (PERL a lane) into the sorted list of the best k so far.  Only values at or over the groups' bound, and over
+// the list's last (one equal to it has a higher token: tiles come in order), can be among the best k: some dozens of 2048 spread
+// ones.  Where more remain than are ranked together (long runs of equal logits, or so many masked that a group has none), they go
+// a few a lane at a time, each time against the list as it then is.
+template <int PERL, typename F>
+__device__ __forceinline__ void merge_tile(const float (&v)[PERL], float best, F key_of, int k, Key* kept, Key* list)
+{
+    auto least = [&] {   // smallest value that may still enter
+        const uint32_t last = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(list[k - 1] >> 32));
+        return last == 0 ? -INF : logit_of(last);
+    };
+    auto take = [&](int first, int last, float over, float bound, bool equal) {
+        int count = 0;
+#pragma unroll
+        for (int j = 0; j < PERL; j++) {
+            if (j < first || j >= last)
+                continue;
+            const bool in = v[j] >= bound && (v[j] > over || (equal && v[j] == over && over > -INF));
+            const uint64_t mask = __ballot(in);
+            if (mask) {
+                const int at = count + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                                                 __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+                if (in && at < KEPT)
+                    kept[at] = key_of(j);
+                count += __popcll(mask);
+            }
+        }
+        return count;
+    };
+    float over = least();
+    const float bound = group_bound(best, k);
+    const int count = take(0, PERL, over, bound, false);
+    if (count == 0)
+        return;
+    if (count <= KEPT) {
+        rank_kept(count, k, kept, list);
+        return;
+    }
+    constexpr int STEP = KEPT / 64;
+#pragma unroll
+    for (int j = 0; j < PERL; j += STEP) {
+        const int some = take(j, j + STEP, over, bound, true);   // (the list's may be of this tile, with a higher token)
+        if (some > 0) {
+            rank_kept(some, k, kept, list);
+            over = least();
+        }
+    }
+}
+
 // How a row is cut: tiles a part, parts a row.  A wave takes a part; where there are
-// more tiles than some waves for every SIMD, it takes several one after another.
+// more tiles than the card holds waves of this kernel, it takes several one after another.
 struct Cut {
     int tiles, parts;
 };
 Cut cut_of(int rows, int vocab)
 {
+    constexpr int WAVES = 4096;
     const int all = (vocab + TILE - 1) / TILE;
     const int64_t waves = static_cast<int64_t>(rows) * all;
-    const int tiles = static_cast<int>(waves <= 4096 ? 1 : (waves + 4095) / 4096);
+    const int tiles = static_cast<int>(waves <= WAVES ? 1 : (waves + WAVES - 1) / WAVES);
     return {tiles, (all + tiles - 1) / tiles};
 }
 
@@ -154,72 +143,74 @@ __device__ __forceinline__ float value_at(const void* p, int64_t i)
         return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i]) << 16);
 }
 
-// One wave a part of a row.  Bound by HBM (the logits, read once); in small calls by
-// the launch and one tile's latency.
+// One wave a part of a row; the next tile is requested while one is taken.  Bound by vector instructions (about
+// ten a value, the exponential among them) where the logits are 16 bits, in small calls by the launch and one tile's latency.
 template <int FMT>
-__global__ __launch_bounds__(64 * SCAN_WAVES) void beam_scan_kernel(BeamArgs a, int rows, int tiles, int parts, Part* part, Key* keys)
+__global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs a, int rows, int tiles, int parts, Part* part, Key* keys)
 {
     __shared__ Key s_kept[SCAN_WAVES][KEPT + CANDIDATES_MAX], s_list[SCAN_WAVES][CANDIDATES_MAX];
+    constexpr int SIZE = FMT == ROWS_OUT_F32 ? 4 : 2, VEC = 16 / SIZE, LOADS = PER / VEC;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t unit = static_cast<int64_t>(blockIdx.x) * SCAN_WAVES + wave;
     if (unit >= static_cast<int64_t>(rows) * parts)
         return;
     const int row = static_cast<int>(unit / parts), p = static_cast<int>(unit - static_cast<int64_t>(row) * parts);
+    const int first = p * tiles * TILE, last = min(first + tiles * TILE, a.vocab);
+    const char* const x = static_cast<const char*>(a.logits) + row * a.stride * SIZE;
+    Sixteen next[LOADS];
+    auto request = [&](int base) {   // a whole tile
+#pragma unroll
+        for (int j = 0; j < LOADS; j++)
+            next[j] = *reinterpret_cast<const Sixteen*>(x + (static_cast<int64_t>(base) + VEC * (lane + 64 * j)) * SIZE);
+    };
+    if (first + TILE <= last)
+        request(first);
     if (a.done && a.done[row] != 0)
-        return;   // its logits are not looked at
+        return;   // its logits do not count
     const int k = a.candidates;
     Key* const list = s_list[wave];
     if (lane < CANDIDATES_MAX)
         list[lane] = 0;
     wave_sync();
-    constexpr int SIZE = FMT == ROWS_OUT_F32 ? 4 : 2;
-    const char* const x = static_cast<const char*>(a.logits) + row * a.stride * SIZE;
-    float most = -__builtin_inff(), sum = 0.0f;
-    const int64_t first = static_cast<int64_t>(p) * tiles * TILE;
-    for (int i = 0; i < tiles; i++) {
-        const int64_t base = first + static_cast<int64_t>(i) * TILE;
-        if (base >= a.vocab)
-            break;
-        constexpr int VEC = 16 / SIZE;
+    float most = -INF, sum = 0.0f;
+    for (int base = first; base < last; base += TILE) {
         float v[PER];
-        const bool full = base + TILE <= a.vocab;
+        const bool full = base + TILE <= last;
         // token of value j: neighbours in a 16-byte load, or (a row's last tile) every 64th
-        auto token = [&](int j) {
-            return static_cast<uint32_t>(base) + (full ? VEC * (lane + 64 * (j / VEC)) + j % VEC : lane + 64 * j);
-        };
+        auto token = [&](int j) { return static_cast<uint32_t>(base + (full ? VEC * (lane + 64 * (j / VEC)) + j % VEC : lane + 64 * j)); };
         if (full) {
-            uint4 w[PER / VEC];
+            Sixteen w[LOADS];
 #pragma unroll
-            for (int j = 0; j < PER / VEC; j++)
-                __builtin_memcpy(&w[j], x + (base + VEC * (lane + 64 * j)) * SIZE, 16);
+            for (int j = 0; j < LOADS; j++)
+                w[j] = next[j];
+            if (base + 2 * TILE <= last)
+                request(base + TILE);
 #pragma unroll
             for (int j = 0; j < PER; j++)
                 v[j] = value_at<FMT>(&w[j / VEC], j % VEC);
         } else {
 #pragma unroll
-            for (int j = 0; j < PER; j++) {
-                const int64_t at = base + lane + 64 * j;
-                v[j] = value_at<FMT>(x, at < a.vocab ? at : a.vocab - 1);
-                v[j] = at < a.vocab ? v[j] : -__builtin_inff();
-            }
+            for (int j = 0; j < PER; j++)
+                v[j] = value_at<FMT>(x, min(base + lane + 64 * j, last - 1));
+#pragma unroll
+            for (int j = 0; j < PER; j++)
+                v[j] = base + lane + 64 * j < last ? v[j] : -INF;
         }
-        float top = -__builtin_inff();
+        float best = -INF;
 #pragma unroll
         for (int j = 0; j < PER; j++)
-            top = fmaxf(top, v[j]);
-        top = fmaxf(rows_max(row_max<16>(top)), most);
-        const float shift = top == -__builtin_inff() ? 0.0f : top;
-        float add = 0.0f;
+            best = fmaxf(best, v[j]);
+        const float top = fmaxf(rows_max(row_max<16>(best)), most);
+        const float shift = top == -INF ? 0.0f : top;
+        float add = 0.0f, more = 0.0f;
 #pragma unroll
-        for (int j = 0; j < PER; j++)
+        for (int j = 0; j < PER; j += 2) {
             add += __builtin_amdgcn_exp2f((v[j] - shift) * LOG2E);
-        sum = sum * (most == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((most - top) * LOG2E)) + add;
+            more += __builtin_amdgcn_exp2f((v[j + 1] - shift) * LOG2E);
+        }
+        sum = sum * (most == -INF ? 0.0f : __builtin_amdgcn_exp2f((most - top) * LOG2E)) + (add + more);
         most = top;
-        uint32_t order[PER];
-#pragma unroll
-        for (int j = 0; j < PER; j++)
-            order[j] = order_of(v[j]);
-        merge_tile<PER>(order, [&](int j) { return static_cast<Key>(order[j]) << 32 | (0xffffffffu - token(j)); }, k,
+        merge_tile<PER>(v, best, [&](int j) { return static_cast<Key>(order_of(v[j])) << 32 | (0xffffffffu - token(j)); }, k,
                         s_kept[wave], list);
     }
     sum = rows_sum(row_sum<16>(sum));
@@ -230,7 +221,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void beam_scan_kernel(BeamArgs a, 
 }
 
 // One workgroup a sequence: each wave joins rows' parts, then all candidates of the rows are
-// ranked by score.
+// ranked by score.  A chain of round trips: what does not hang on another load is requested first.
 __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a, int parts, const Part* part, const Key* keys)
 {
     constexpr int LANE_KEYS = 8;
@@ -247,52 +238,64 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
         s_slot[t] = a.slots ? a.slots[static_cast<int64_t>(s) * beams + t] : 0;
     for (int b = wave; b < beams; b += MERGE_WAVES) {
         const int64_t row = static_cast<int64_t>(s) * beams + b;
+        const Part* const mine = part + row * parts;
+        const Key* const from = keys + row * parts * k;
+        const int total = parts * k;
+        Key key[LANE_KEYS];
+        auto request = [&](int base) {
+#pragma unroll
+            for (int j = 0; j < LANE_KEYS; j++)
+                key[j] = from[min(base + 64 * j + lane, total - 1)];
+        };
         const double given = a.scores[row];
+        const bool ended = a.done && a.done[row] != 0;
+        Part held = mine[min(lane, parts - 1)];
+        request(0);
         Key* const list = s_list[b];
         if (lane < CANDIDATES_MAX)
             list[lane] = 0;
         wave_sync();
-        if (a.done && a.done[row] != 0) {
+        if (ended) {
             if (lane < k)
                 s_score[b * k + lane] = lane == 0 ? given : -__builtin_inf();
             if (lane == 0)
                 list[0] = 0xffffffffu - static_cast<uint32_t>(a.end_token);
             continue;
         }
-        const Part* const mine = part + row * parts;
-        float most = -__builtin_inff();
-        for (int i = lane; i < parts; i += 64)
+        if (lane >= parts)
+            held = {-INF, 0.0f};
+        float most = held.most;
+        for (int i = lane + 64; i < parts; i += 64)
             most = fmaxf(most, mine[i].most);
         most = rows_max(row_max<16>(most));
-        double sum = 0.0;
-        for (int i = lane; i < parts; i += 64) {
-            const Part q = mine[i];
-            // (a part without a finite logit has the sum 0, or NaN)
-            sum += q.most == -__builtin_inff() ? static_cast<double>(q.sum)
-                                               : static_cast<double>(q.sum) * exp(static_cast<double>(q.most) - static_cast<double>(most));
-        }
+        // (a part without a finite logit has the sum 0, or NaN)
+        auto scaled = [&](Part q) {
+            return static_cast<double>(q.sum) * (q.most == -INF ? 1.0f : __builtin_amdgcn_exp2f((q.most - most) * LOG2E));
+        };
+        double sum = scaled(held);
+        for (int i = lane + 64; i < parts; i += 64)
+            sum += scaled(mine[i]);
 #pragma unroll
         for (int m = 32; m >= 1; m >>= 1)
             sum += __shfl_xor(sum, m);
         const double log_sum = log(sum);
-        const Key* const from = keys + row * parts * k;
-        const int64_t total = static_cast<int64_t>(parts) * k;
-        for (int64_t base = 0; base < total; base += 64 * LANE_KEYS) {
-            Key key[LANE_KEYS];
-            uint32_t order[LANE_KEYS];
+        for (int base = 0; base < total; base += 64 * LANE_KEYS) {
+            if (base > 0)
+                request(base);
+            float v[LANE_KEYS], best = -INF;
 #pragma unroll
             for (int j = 0; j < LANE_KEYS; j++) {
-                const int64_t at = base + 64 * j + lane;
-                key[j] = at < total ? from[at] : 0;
-                order[j] = static_cast<uint32_t>(key[j] >> 32);
+                const uint32_t order = base + 64 * j + lane < total ? static_cast<uint32_t>(key[j] >> 32) : 0u;
+                v[j] = order == 0 ? -INF : logit_of(order);
+                best = fmaxf(best, v[j]);
             }
-            merge_tile<LANE_KEYS>(order, [&](int j) { return key[j]; }, k, s_kept[wave], list);
+            merge_tile<LANE_KEYS>(v, best, [&](int j) { return key[j]; }, k, s_kept[wave], list);
         }
         if (lane < k) {
-            const Key key = list[lane];
-            const double x = static_cast<double>(logit_of(static_cast<uint32_t>(key >> 32)));
+            const Key got = list[lane];
+            const double x = static_cast<double>(logit_of(static_cast<uint32_t>(got >> 32)));
             const double score = given + ((x - static_cast<double>(most)) - log_sum);
-            s_score[b * k + lane] = key != 0 && fabs(score) < __builtin_inf() ? score : -__builtin_inf();
+            s_score[b * k + lane] = got != 0 && fabs(score) < __builtin_inf() ? score : -__builtin_inf();
         }
     }
     __syncthreads();
@@ -302,6 +305,7 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
         const double mine = s_score[i];
         if (fabs(mine) < __builtin_inf()) {
             int rank = 0;
+#pragma unroll 8
             for (int j = 0; j < beams * k; j++) {
                 const double other = s_score[j];
                 rank += other > mine || (other == mine && j < i);
@@ -324,7 +328,7 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
     if (t >= count && t < k) {
         a.parents[out + t] = -1;
         a.tokens[out + t] = -1;
-        a.new_scores[out + t] = -__builtin_inff();
+        a.new_scores[out + t] = -INF;
         if (a.new_done)
             a.new_done[out + t] = 0;
         s_parent[t] = -1;
@@ -363,9 +367,11 @@ struct SlotArrays {
     si_hip_slot_array at[SLOT_ARRAYS_PER_LAUNCH];
 };
 
-constexpr int COPY_THREADS = 256, COPY_BYTES = COPY_THREADS * 16 * 4;   // of a workgroup
+constexpr int COPY_THREADS = 256, COPY_BYTES = COPY_THREADS * 16 * 2;   // of a workgroup
 
-// A workgroup copies 16 KiB of one slot of one array.  Bound by HBM.
+// A workgroup copies 8 KiB of one slot of one array, past the L2s (24 arrays, 12 slots of 540 KB each moved: 43 us;
+// through them 47; 4 or 16 KiB a workgroup 56 and 45; a plain copy of the bytes 65).  Bound by HBM, small moves
+// by the launch.
 __global__ __launch_bounds__(COPY_THREADS) void copy_slots_kernel(SlotArrays arrays, int64_t slots, const int32_t* from, const int32_t* to,
                                                                   int moves)
 {
@@ -381,20 +387,17 @@ __global__ __launch_bounds__(COPY_THREADS) void copy_slots_kernel(SlotArrays arr
         const char* const src = static_cast<char*>(a.base) + source * a.slot_bytes;
         char* const dst = static_cast<char*>(a.base) + target * a.slot_bytes;
         if (last - first == COPY_BYTES) {
-            uint4 v[4];
+            Sixteen v[2];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                __builtin_memcpy(&v[j], src + first + (threadIdx.x + COPY_THREADS * j) * 16, 16);
+            for (int j = 0; j < 2; j++)
+                v[j] = *reinterpret_cast<const Sixteen*>(src + first + (threadIdx.x + COPY_THREADS * j) * 16);
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                __builtin_memcpy(dst + first + (threadIdx.x + COPY_THREADS * j) * 16, &v[j], 16);
+            for (int j = 0; j < 2; j++)
+                __builtin_nontemporal_store(v[j], reinterpret_cast<Sixteen*>(dst + first + (threadIdx.x + COPY_THREADS * j) * 16));
         } else {
             const uint64_t whole = first + (last - first) / 16 * 16;
-            for (uint64_t at = first + threadIdx.x * 16; at < whole; at += COPY_THREADS * 16) {
-                uint4 v;
-                __builtin_memcpy(&v, src + at, 16);
-                __builtin_memcpy(dst + at, &v, 16);
-            }
+            for (uint64_t at = first + threadIdx.x * 16; at < whole; at += COPY_THREADS * 16)
+                *reinterpret_cast<Sixteen*>(dst + at) = *reinterpret_cast<const Sixteen*>(src + at);
             if (whole + threadIdx.x < last)
                 dst[whole + threadIdx.x] = src[whole + threadIdx.x];
         }

@@ -8,53 +8,36 @@
 namespace si {
 namespace {
 
-constexpr int THREADS = 256, WAVES = THREADS / 64;
+constexpr int PER = 8;   // values of a row a thread
 
-template <typename T>
-struct alignas(4 * sizeof(T)) Four {
-    T x, y, z, w;
-};
-
-// A workgroup takes `run` rows one after another, PER values of a row a
-// thread (four neighbours each where FOURS, else every 256th).  The row before
-// stays in registers, so only a run's first row is normalised twice; the
-// sequence's state is read by the workgroup of its first row, which also
-// normalises the last row for the state's slot: the slot has one reader and
-// writer, whatever the other workgroups have done by then.
-// Bound by HBM: 4 bytes in (8 with a residual, 4 more out) and 2 or 4 out a mix.
-template <int PER, bool FOURS, typename OUT>
+// A workgroup of THREADS takes `run` rows one after another, eight values of a row a thread (neighbours where
+// EIGHTS, else every THREADS-th).  Weights and mixes stay in registers, and so does the row before: only a run's
+// first row is normalised twice.  The next row is requested while this one is normalised.  The sequence's
+// state is read by the workgroup of its first row, which also normalises the last row for the state's slot:
+// the slot has one reader and writer, whatever the other workgroups have done by then.
+// Bound by HBM: 4 bytes in (8 with a residual, 4 more out) and 2 or 4 out a mix; a single row by its
+// round trips.
+// HELD: mixes that registers hold (0: they are loaded with every row: 1024 threads leave no room for more than one).
+// PAST: outputs go past the L2s.
+template <int THREADS, bool EIGHTS, int HELD, bool PAST, typename OUT>
 __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int run)
 {
+    constexpr int WAVES = THREADS / 64;
     __shared__ float s_sum[WAVES], s_squares[WAVES];
     __shared__ int s_at[WAVES];
     const int t = threadIdx.x, wave = t >> 6, n = a.n;
     const RowBatch& b = a.batch;
-    auto place = [&](int j) { return FOURS ? 4 * (t + THREADS * (j >> 2)) + (j & 3) : t + THREADS * j; };
-
-    // the sequence of the run's first row: as many as end at or before it
-    int row = blockIdx.x * run;
-    const int end = min(row + run, b.rows);
-    int at = 0;
-    for (int i = t; i < b.sequences; i += THREADS)
-        at += b.starts[i + 1] <= row;
-    at = static_cast<int>(rows_sum(row_sum<16>(static_cast<float>(at))));   // at most 4096: exact
-    if ((t & 63) == 0)
-        s_at[wave] = at;
-    __syncthreads();
-    int s = 0;
-    for (int w = 0; w < WAVES; w++)
-        s += s_at[w];
-    s = __builtin_amdgcn_readfirstlane(s);
-
+    auto place = [&](int j) { return EIGHTS ? PER * t + j : t + THREADS * j; };
     auto load = [&](const float* p, float* v) {
-        if constexpr (FOURS) {
-#pragma unroll
-            for (int j = 0; j < PER; j += 4) {
-                float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (place(j) < n)
-                    f = *reinterpret_cast<const float4*>(p + place(j));
-                v[j] = f.x, v[j + 1] = f.y, v[j + 2] = f.z, v[j + 3] = f.w;
+        if constexpr (EIGHTS) {
+            float4 f[2] = {};
+            if (PER * t < n) {
+                f[0] = *reinterpret_cast<const float4*>(p + PER * t);
+                f[1] = *reinterpret_cast<const float4*>(p + PER * t + 4);
             }
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                v[4 * j] = f[j].x, v[4 * j + 1] = f[j].y, v[4 * j + 2] = f[j].z, v[4 * j + 3] = f[j].w;
         } else {
 #pragma unroll
             for (int j = 0; j < PER; j++)
@@ -63,12 +46,16 @@ __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int ru
     };
     auto store = [&](auto* p, const float* v) {
         using T = std::remove_reference_t<decltype(*p)>;
-        if constexpr (FOURS) {
-#pragma unroll
-            for (int j = 0; j < PER; j += 4)
-                if (place(j) < n)
-                    *reinterpret_cast<Four<T>*>(p + place(j)) =
-                        Four<T>{static_cast<T>(v[j]), static_cast<T>(v[j + 1]), static_cast<T>(v[j + 2]), static_cast<T>(v[j + 3])};
+        if constexpr (EIGHTS) {
+            typedef T Eight __attribute__((ext_vector_type(PER)));
+            const Eight e = {static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3]),
+                             static_cast<T>(v[4]), static_cast<T>(v[5]), static_cast<T>(v[6]), static_cast<T>(v[7])};
+            if (PER * t < n) {
+                if constexpr (PAST)   // (a choice at run time is merged into one ordinary store)
+                    __builtin_nontemporal_store(e, reinterpret_cast<Eight*>(p + PER * t));
+                else
+                    *reinterpret_cast<Eight*>(p + PER * t) = e;
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < PER; j++)
@@ -87,25 +74,49 @@ __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int ru
             sum += part[w];
         return sum;
     };
-    float weight[PER], bias[PER];
+
+    // what the first row needs, requested before its sequence is known
+    int row = blockIdx.x * run;
+    const int end = min(row + run, b.rows);
+    const int64_t width = n;
+    float x[PER], add[PER], weight[PER], bias[PER], mix[HELD ? HELD : 1][PER];
+    auto request = [&](int r) {
+        load(a.x + r * width, x);
+        if (a.residual)
+            load(a.residual + r * width, add);
+    };
+    request(row);
+    int at = 0;
+    for (int i = t; i < b.sequences; i += THREADS)
+        at += b.starts[i + 1] <= row;
     load(a.weight, weight);
     load(a.bias, bias);
-    // the norm of a row, and (its own workgroup's row) the residual sum's store
-    auto norm = [&](int r, float* v, bool keep) {
-        load(a.x + static_cast<int64_t>(r) * n, v);
-        if (a.residual) {
-            float add[PER];
-            load(a.residual + static_cast<int64_t>(r) * n, add);
 #pragma unroll
-            for (int j = 0; j < PER; j++)
-                v[j] += add[j];
-            if (keep)
-                store(a.updated + static_cast<int64_t>(r) * n, v);
-        }
+    for (int m = 0; m < HELD; m++)
+        if (m < a.mixes)
+            load(a.mix + m * width, mix[m]);
+    // the sequence of the run's first row: as many as end at or before it
+    at = static_cast<int>(rows_sum(row_sum<16>(static_cast<float>(at))));   // at most 4096: exact
+    if ((t & 63) == 0)
+        s_at[wave] = at;
+    __syncthreads();
+    int s = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++)
+        s += s_at[w];
+    s = __builtin_amdgcn_readfirstlane(s);
+
+    // the norm of the requested row
+    auto norm = [&](float* v) {
         float sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < PER; j++)
+        for (int j = 0; j < PER; j++) {
+            v[j] = a.residual ? x[j] + add[j] : x[j];
             sum += v[j];
+        }
+        return sum;
+    };
+    auto normalise = [&](float* v, float sum) {
         const float mean = block_sum(sum, s_sum) / static_cast<float>(n);
         float squares = 0.0f;
 #pragma unroll
@@ -118,9 +129,14 @@ __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int ru
         for (int j = 0; j < PER; j++)
             v[j] = fmaf(v[j] * inv, weight[j], bias[j]);
     };
+    auto other_row = [&](int r, float* v) {
+        request(r);
+        normalise(v, norm(v));
+    };
 
     float before[PER], now[PER];
-    bool have = false;   // `before` is the row before
+    bool have = false;        // `before` is the row before
+    bool requested = true;    // x and add are this row's
     OUT* const out = static_cast<OUT*>(a.out);
     for (; row < end; row++) {
         while (s < b.sequences && row >= b.starts[s + 1]) {
@@ -131,43 +147,62 @@ __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int ru
             break;
         const RowSpan span = rows_of(b, s);
         if (row < span.first || row >= span.last) {
-            have = false;
+            have = requested = false;
             continue;
         }
-        if (a.mixes == 0) {
-            norm(row, now, true);
-            store(out + static_cast<int64_t>(row) * n, now);
-            continue;
-        }
-        if (row == span.first) {
+        if (a.mixes > 0 && row == span.first) {
             const int from = b.from[s];
             if (from >= 0 && from < b.slots) {
-                load(a.state + static_cast<int64_t>(from) * n, before);
+                load(a.state + from * width, before);
             } else {
 #pragma unroll
                 for (int j = 0; j < PER; j++)
                     before[j] = from == -1 ? 0.0f : __builtin_nanf("");
             }
-        } else if (!have) {
-            norm(row - 1, before, false);
+        } else if (a.mixes > 0 && !have) {
+            other_row(row - 1, before);
+            requested = false;
         }
-        norm(row, now, true);
-        for (int m = 0; m < a.mixes; m++) {
-            float mix[PER];
-            load(a.mix + static_cast<int64_t>(m) * n, mix);
+        if (!requested)
+            request(row);
+        const float sum = norm(now);
+        if (a.residual)
+            store(a.updated + row * width, now);
+        requested = row + 1 < end;
+        if (requested)
+            request(row + 1);
+        normalise(now, sum);
+        if (a.mixes == 0) {
+            store(out + row * width, now);
+            continue;
+        }
+        auto mixed = [&](int m, const float* held) {
+            float v[PER];
 #pragma unroll
             for (int j = 0; j < PER; j++)
-                mix[j] = fmaf(before[j] - now[j], mix[j], now[j]);
-            store(out + (static_cast<int64_t>(m) * b.rows + row) * n, mix);
+                v[j] = fmaf(before[j] - now[j], held[j], now[j]);
+            store(out + (static_cast<int64_t>(m) * b.rows + row) * width, v);
+        };
+        if constexpr (HELD > 0) {
+#pragma unroll
+            for (int m = 0; m < HELD; m++)
+                if (m < a.mixes)
+                    mixed(m, mix[m]);
+        } else {
+            for (int m = 0; m < a.mixes; m++) {
+                load(a.mix + m * width, mix[0]);
+                mixed(m, mix[0]);
+            }
         }
         if (row == span.first) {
             const int to = b.to[s];
             if (to >= 0 && to < b.slots) {
                 if (span.last - 1 == row) {
-                    store(a.state + static_cast<int64_t>(to) * n, now);
+                    store(a.state + to * width, now);
                 } else {
-                    norm(span.last - 1, before, false);
-                    store(a.state + static_cast<int64_t>(to) * n, before);
+                    other_row(span.last - 1, before);
+                    requested = false;
+                    store(a.state + to * width, before);
                 }
             }
         }
@@ -178,30 +213,61 @@ __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int ru
     }
 }
 
-template <int PER, bool FOURS>
+template <int THREADS, bool EIGHTS, int HELD, bool PAST>
 void launch(const MixRowsArgs& a, int run, hipStream_t s)
 {
     const dim3 grid((a.batch.rows + run - 1) / run);
     if (a.out_format == ROWS_OUT_F32)
-        hipLaunchKernelGGL((mix_rows_kernel<PER, FOURS, float>), grid, dim3(THREADS), 0, s, a, run);
+        hipLaunchKernelGGL((mix_rows_kernel<THREADS, EIGHTS, HELD, PAST, float>), grid, dim3(THREADS), 0, s, a, run);
     else if (a.out_format == ROWS_OUT_F16)
-        hipLaunchKernelGGL((mix_rows_kernel<PER, FOURS, _Float16>), grid, dim3(THREADS), 0, s, a, run);
+        hipLaunchKernelGGL((mix_rows_kernel<THREADS, EIGHTS, HELD, PAST, _Float16>), grid, dim3(THREADS), 0, s, a, run);
     else
-        hipLaunchKernelGGL((mix_rows_kernel<PER, FOURS, __bf16>), grid, dim3(THREADS), 0, s, a, run);
+        hipLaunchKernelGGL((mix_rows_kernel<THREADS, EIGHTS, HELD, PAST, __bf16>), grid, dim3(THREADS), 0, s, a, run);
+}
+
+template <int THREADS, int HELD>
+void launch(const MixRowsArgs& a, bool eights, bool past, int run, hipStream_t s)
+{
+    if (eights && past)
+        launch<THREADS, true, HELD, true>(a, run, s);
+    else if (eights)
+        launch<THREADS, true, HELD, false>(a, run, s);
+    else
+        launch<THREADS, false, HELD, false>(a, run, s);
+}
+
+template <int THREADS>
+void launch(const MixRowsArgs& a, hipStream_t s)
+{
+    constexpr int MANY = THREADS == 1024 ? 0 : MIX_MAX;
+    auto aligned16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+    const bool eights = a.n % 8 == 0 && aligned16(a.x) && aligned16(a.residual) && aligned16(a.weight) && aligned16(a.bias) &&
+                        aligned16(a.mix) && aligned16(a.state) && aligned16(a.updated) && aligned16(a.out);
+    // Outputs that the L2s (32 MiB) cannot keep for the next kernel go past them: 4000 rows of 2048 values in six mixes
+    // take 43 us instead of 66.  Smaller ones stay there for the products that read them.
+    const int64_t out = static_cast<int64_t>(a.batch.rows) * a.n *
+                        ((a.out_format == ROWS_OUT_F32 ? 4 : 2) * (a.mixes > 0 ? a.mixes : 1) + (a.residual ? 4 : 0));
+    const bool past = out > (16 << 20);
+    // Runs such that so many waves a compute unit have one each; few rows one a workgroup.  Odd ones: at 4 or 8 rows a
+    // run the workgroups' rows lie a power of two apart, and 4000 rows take 48 and 55 us, at 3, 5 and 9 rows 43, 41 and 36.
+    const int waves = a.mixes <= 1 ? 20 : 7, resident = 256 * waves * 64 / THREADS, rows = a.batch.rows;
+    const int run = rows <= 2 * resident ? 1 : rows < 15 * resident ? ((rows + resident - 1) / resident) | 1 : 15;
+    if (a.mixes <= 1)
+        launch<THREADS, 1>(a, eights, past, run, s);
+    else
+        launch<THREADS, MANY>(a, eights, past, run, s);
 }
 
 }  // namespace
 
 hipError_t launch_layernorm_mix_rows(const MixRowsArgs& a, hipStream_t s)
 {
-    auto aligned16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
-    const bool fours = a.n % 4 == 0 && aligned16(a.x) && aligned16(a.residual) && aligned16(a.weight) && aligned16(a.bias) &&
-                       aligned16(a.mix) && aligned16(a.state) && aligned16(a.updated) && aligned16(a.out);
-    const int run = a.batch.rows <= 1024 ? 1 : a.batch.rows <= 4096 ? 4 : 8;
-    if (a.n <= 8 * THREADS)
-        fours ? launch<8, true>(a, run, s) : launch<8, false>(a, run, s);
+    if (a.n <= 256 * PER)
+        launch<256>(a, s);
+    else if (a.n <= 512 * PER)
+        launch<512>(a, s);
     else
-        fours ? launch<32, true>(a, run, s) : launch<32, false>(a, run, s);
+        launch<1024>(a, s);
     return hipGetLastError();
 }
 
