@@ -16,6 +16,8 @@ namespace {
 constexpr float LOG2E = 1.44269504088896f;
 constexpr int TILE = 2048, PER = TILE / 64;   // values of a wave's tile, and of a lane's
 constexpr int KEPT = 256;                     // values that are ranked together
+constexpr int ROOM = KEPT + CANDIDATES_MAX + 8;
+constexpr int SHOWN = 24;                     // lanes of a tile whose values are looked at one by one
 constexpr int SCAN_WAVES = 4, MERGE_WAVES = 8;
 constexpr float INF = __builtin_inff();
 
@@ -52,66 +54,89 @@ __device__ __forceinline__ void rank_kept(int count, int k, Key* kept, Key* list
     if (own != 0)
         kept[count + lane] = own;
     count += __popcll(__ballot(own != 0));   // (a prefix of the lanes)
+    if (lane < 8)
+        kept[count + lane] = 0;
     wave_sync();
     for (int i = lane; i < count; i += 64) {
         const Key mine = kept[i];
         int rank = 0;
-#pragma unroll 4
-        for (int j = 0; j < count; j++)
-            rank += kept[j] > mine;
+        for (int j = 0; j < count; j += 8) {   // eight at a time: a chain of LDS reads else
+            Key other[8];
+#pragma unroll
+            for (int m = 0; m < 8; m++)
+                other[m] = kept[j + m];
+#pragma unroll
+            for (int m = 0; m < 8; m++)
+                rank += other[m] > mine;
+        }
         if (rank < k)
             list[rank] = mine;
     }
     wave_sync();
 }
 
-// Merges a tile's values (PERL a lane) into the sorted list of the best k so far.  Only values at or over the groups' bound, and over
-// the list's last (one equal to it has a higher token: tiles come in order), can be among the best k: some dozens of 2048 spread
-// ones.  Where more remain than are ranked together (long runs of equal logits, or so many masked that a group has none), they go
-// a few a lane at a time, each time against the list as it then is.
-template <int PERL, typename F>
-__device__ __forceinline__ void merge_tile(const float (&v)[PERL], float best, F key_of, int k, Key* kept, Key* list)
+// The smallest value that may enter a sorted list of k.
+__device__ __forceinline__ float least_of(const Key* list, int k)
 {
-    auto least = [&] {   // smallest value that may still enter
-        const uint32_t last = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(list[k - 1] >> 32));
-        return last == 0 ? -INF : logit_of(last);
-    };
-    auto take = [&](int first, int last, float over, float bound, bool equal) {
-        int count = 0;
-#pragma unroll
-        for (int j = 0; j < PERL; j++) {
-            if (j < first || j >= last)
-                continue;
-            const bool in = v[j] >= bound && (v[j] > over || (equal && v[j] == over && over > -INF));
-            const uint64_t mask = __ballot(in);
-            if (mask) {
-                const int at = count + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
-                                                                 __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
-                if (in && at < KEPT)
-                    kept[at] = key_of(j);
-                count += __popcll(mask);
-            }
-        }
+    const uint32_t last = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(list[k - 1] >> 32));
+    return last == 0 ? -INF : logit_of(last);
+}
+
+// Appends what `in` marks behind the `count` kept ones (as many as there is room for); returns how many there would be.
+template <typename F>
+__device__ __forceinline__ int append(bool in, F key, int count, Key* kept)
+{
+    const uint64_t mask = __ballot(in);
+    if (mask == 0)
         return count;
-    };
-    float over = least();
-    const float bound = group_bound(best, k);
-    const int count = take(0, PERL, over, bound, false);
-    if (count == 0)
-        return;
-    if (count <= KEPT) {
-        rank_kept(count, k, kept, list);
-        return;
-    }
+    const int at = count + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                                     __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+    if (in && at < KEPT)
+        kept[at] = key();
+    return count + __popcll(mask);
+}
+
+// Merges a tile's values (PERL a lane) into the sorted list of the best k so far, a few a lane at a time.  Only values over
+// the groups' bound, and over the list's last, can be among the best k.  (One equal to the last may have a lower token
+// where it is of the same tile.)
+template <int PERL, typename F>
+__device__ __forceinline__ void merge_tile(const float (&v)[PERL], float bound, F key_of, int k, Key* kept, Key* list)
+{
     constexpr int STEP = KEPT / 64;
+    float over = least_of(list, k);
 #pragma unroll
     for (int j = 0; j < PERL; j += STEP) {
-        const int some = take(j, j + STEP, over, bound, true);   // (the list's may be of this tile, with a higher token)
-        if (some > 0) {
-            rank_kept(some, k, kept, list);
-            over = least();
+        int count = 0;
+#pragma unroll
+        for (int i = j; i < j + STEP; i++)
+            count = append(v[i] >= bound && v[i] >= over && v[i] > -INF, [&] { return key_of(i); }, count, kept);
+        if (count > 0) {
+            rank_kept(count, k, kept, list);
+            over = least_of(list, k);
         }
     }
+}
+
+// Sum over the wave, in every lane, with moves inside rows of lanes and swaps between them.
+template <int CTRL>
+__device__ __forceinline__ double moved(double v)
+{
+    return __hiloint2double(dpp_row<CTRL>(__double2hiint(v)), dpp_row<CTRL>(__double2loint(v)));
+}
+__device__ __forceinline__ double wave_sum(double v)
+{
+    v += moved<0xB1>(v);
+    v += moved<0x4E>(v);
+    v += moved<0x141>(v);
+    v += moved<0x140>(v);
+    auto swapped = [&](auto swap) {
+        const auto high = swap(static_cast<uint32_t>(__double2hiint(v))), low = swap(static_cast<uint32_t>(__double2loint(v)));
+        v = __hiloint2double(static_cast<int>(high[0]), static_cast<int>(low[0])) +
+            __hiloint2double(static_cast<int>(high[1]), static_cast<int>(low[1]));
+    };
+    swapped([](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
+    swapped([](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+    return v;
 }
 
 // How a row is cut: tiles a part, parts a row.  A wave takes a part; where there are
@@ -143,12 +168,14 @@ __device__ __forceinline__ float value_at(const void* p, int64_t i)
         return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i]) << 16);
 }
 
-// One wave a part of a row; the next tile is requested while one is taken.  Bound by vector instructions (about
+// One wave a part of a row.  Bound by vector instructions (about
 // ten a value, the exponential among them) where the logits are 16 bits, in small calls by the launch and one tile's latency.
 template <int FMT>
 __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs a, int rows, int tiles, int parts, Part* part, Key* keys)
 {
-    __shared__ Key s_kept[SCAN_WAVES][KEPT + CANDIDATES_MAX], s_list[SCAN_WAVES][CANDIDATES_MAX];
+    __shared__ Key s_kept[SCAN_WAVES][ROOM], s_list[SCAN_WAVES][CANDIDATES_MAX];
+    __shared__ float4 s_shown[SCAN_WAVES][SHOWN][PER / 4];
+    __shared__ int s_lane[SCAN_WAVES][SHOWN];
     constexpr int SIZE = FMT == ROWS_OUT_F32 ? 4 : 2, VEC = 16 / SIZE, LOADS = PER / VEC;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t unit = static_cast<int64_t>(blockIdx.x) * SCAN_WAVES + wave;
@@ -157,11 +184,11 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
     const int row = static_cast<int>(unit / parts), p = static_cast<int>(unit - static_cast<int64_t>(row) * parts);
     const int first = p * tiles * TILE, last = min(first + tiles * TILE, a.vocab);
     const char* const x = static_cast<const char*>(a.logits) + row * a.stride * SIZE;
-    Sixteen next[LOADS];
+    Sixteen raw[LOADS];
     auto request = [&](int base) {   // a whole tile
 #pragma unroll
         for (int j = 0; j < LOADS; j++)
-            next[j] = *reinterpret_cast<const Sixteen*>(x + (static_cast<int64_t>(base) + VEC * (lane + 64 * j)) * SIZE);
+            raw[j] = *reinterpret_cast<const Sixteen*>(x + (static_cast<int64_t>(base) + VEC * (lane + 64 * j)) * SIZE);
     };
     if (first + TILE <= last)
         request(first);
@@ -172,22 +199,23 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
     if (lane < CANDIDATES_MAX)
         list[lane] = 0;
     wave_sync();
-    float most = -INF, sum = 0.0f;
+    Key* const kept = s_kept[wave];
+    float most = -INF, sum = 0.0f, over = -INF;
+    int pending = 0;   // kept ones that are not in the list yet
     for (int base = first; base < last; base += TILE) {
         float v[PER];
         const bool full = base + TILE <= last;
         // token of value j: neighbours in a 16-byte load, or (a row's last tile) every 64th
-        auto token = [&](int j) { return static_cast<uint32_t>(base + (full ? VEC * (lane + 64 * (j / VEC)) + j % VEC : lane + 64 * j)); };
+        auto token = [&](int lane, int j) {
+            return static_cast<uint32_t>(base + (full ? VEC * (lane + 64 * (j / VEC)) + j % VEC : lane + 64 * j));
+        };
+        auto key_of = [&](float x, int lane, int j) { return static_cast<Key>(order_of(x)) << 32 | (0xffffffffu - token(lane, j)); };
         if (full) {
-            Sixteen w[LOADS];
-#pragma unroll
-            for (int j = 0; j < LOADS; j++)
-                w[j] = next[j];
-            if (base + 2 * TILE <= last)
-                request(base + TILE);
+            if (base > first)
+                request(base);
 #pragma unroll
             for (int j = 0; j < PER; j++)
-                v[j] = value_at<FMT>(&w[j / VEC], j % VEC);
+                v[j] = value_at<FMT>(&raw[j / VEC], j % VEC);
         } else {
 #pragma unroll
             for (int j = 0; j < PER; j++)
@@ -198,8 +226,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
         }
         float best = -INF;
 #pragma unroll
-        for (int j = 0; j < PER; j++)
-            best = fmaxf(best, v[j]);
+        for (int j = 0; j < PER; j += 4)
+            best = fmaxf(best, fmaxf(fmaxf(v[j], v[j + 1]), fmaxf(v[j + 2], v[j + 3])));
         const float top = fmaxf(rows_max(row_max<16>(best)), most);
         const float shift = top == -INF ? 0.0f : top;
         float add = 0.0f, more = 0.0f;
@@ -210,9 +238,58 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
         }
         sum = sum * (most == -INF ? 0.0f : __builtin_amdgcn_exp2f((most - top) * LOG2E)) + (add + more);
         most = top;
-        merge_tile<PER>(v, best, [&](int j) { return static_cast<Key>(order_of(v[j])) << 32 | (0xffffffffu - token(j)); }, k,
-                        s_kept[wave], list);
+        // Only values over the list's last so far (one equal to it has a higher token: tiles come in order), and over the groups'
+        // bound, can be among the best k: some dozens of 2048 spread ones, in as many lanes or fewer.  Those
+        // lanes show all their values, and the wave looks at them together.
+        if (__ballot(best > over) == 0)
+            continue;
+        const float bound = group_bound(best, k);
+        const bool shows = best > over && best >= bound;
+        const uint64_t lanes = __ballot(shows);
+        const int shown = __popcll(lanes);
+        if (shown <= SHOWN) {
+            if (shows) {
+                const int at = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32),
+                                                         __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0));
+                s_lane[wave][at] = lane;
+#pragma unroll
+                for (int j = 0; j < PER; j += 4)
+                    s_shown[wave][at][j / 4] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            }
+            wave_sync();
+            int count = pending;
+            constexpr int TURN = 4;   // values a lane at a time
+            for (int i = 0; i < shown * PER; i += 64 * TURN) {
+                float x[TURN];
+#pragma unroll
+                for (int m = 0; m < TURN; m++)   // (rows behind the shown ones: whatever they hold is passed over)
+                    x[m] = reinterpret_cast<const float*>(s_shown[wave])[min(i + 64 * m, (SHOWN - 2) * PER) + lane];
+#pragma unroll
+                for (int m = 0; m < TURN; m++) {
+                    const int at = (i + 64 * m + lane) / PER, j = (i + 64 * m + lane) % PER;
+                    count = append(at < shown && x[m] > over && x[m] >= bound, [&] { return key_of(x[m], s_lane[wave][at], j); },
+                                   count, kept);
+                }
+            }
+            if (count <= KEPT) {
+                pending = count;
+                if (over == -INF || pending > 64) {
+                    rank_kept(pending, k, kept, list);
+                    over = least_of(list, k);
+                    pending = 0;
+                }
+                continue;
+            }
+            // (more than there is room for: the kept ones of earlier tiles are in place, this tile's go a few at a time)
+        }
+        if (pending > 0)
+            rank_kept(pending, k, kept, list);
+        pending = 0;
+        merge_tile<PER>(v, bound, [&](int j) { return key_of(v[j], lane, j); }, k, kept, list);
+        over = least_of(list, k);
     }
+    if (pending > 0)
+        rank_kept(pending, k, kept, list);
     sum = rows_sum(row_sum<16>(sum));
     if (lane == 0)
         part[unit] = {most, sum};
@@ -225,7 +302,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
 __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a, int parts, const Part* part, const Key* keys)
 {
     constexpr int LANE_KEYS = 8;
-    __shared__ Key s_kept[MERGE_WAVES][KEPT + CANDIDATES_MAX];
+    __shared__ Key s_kept[MERGE_WAVES][ROOM];
     __shared__ Key s_list[BEAMS_MAX][CANDIDATES_MAX];
     __shared__ double s_score[BEAMS_MAX * CANDIDATES_MAX];
     __shared__ int s_parent[CANDIDATES_MAX], s_slot[BEAMS_MAX], s_count;
@@ -275,10 +352,7 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
         double sum = scaled(held);
         for (int i = lane + 64; i < parts; i += 64)
             sum += scaled(mine[i]);
-#pragma unroll
-        for (int m = 32; m >= 1; m >>= 1)
-            sum += __shfl_xor(sum, m);
-        const double log_sum = log(sum);
+        const double log_sum = log(wave_sum(sum));
         for (int base = 0; base < total; base += 64 * LANE_KEYS) {
             if (base > 0)
                 request(base);
@@ -289,7 +363,7 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
                 v[j] = order == 0 ? -INF : logit_of(order);
                 best = fmaxf(best, v[j]);
             }
-            merge_tile<LANE_KEYS>(v, best, [&](int j) { return key[j]; }, k, s_kept[wave], list);
+            merge_tile<LANE_KEYS>(v, group_bound(best, k), [&](int j) { return key[j]; }, k, s_kept[wave], list);
         }
         if (lane < k) {
             const Key got = list[lane];
@@ -336,30 +410,35 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
     if (!a.slots)
         return;
     __syncthreads();
-    if (t < beams) {   // candidates = beams
-        const int parent = s_parent[t];
-        auto keeps = [&](int c) {
-            const int p = s_parent[c];
-            bool first = p >= 0;
-            for (int d = 0; d < c; d++)
-                first = first && s_parent[d] != p;
-            return first;
-        };
-        int slot = parent >= 0 ? s_slot[parent] : -1;
-        a.from[out + t] = slot;
-        if (!keeps(t)) {
-            int turn = 0;   // candidates before this one that take over a slot
-            for (int c = 0; c < t; c++)
-                turn += !keeps(c);
-            for (int b = 0; b < beams; b++) {
-                bool childless = true;
-                for (int c = 0; c < beams; c++)
-                    childless = childless && s_parent[c] != b;
-                if (childless && turn-- == 0)
-                    slot = s_slot[b];
-            }
+    if (t >= 64)
+        return;
+    // candidates = beams, one a lane
+    const int parent = t < beams ? s_parent[t] : -1, own = t < beams ? s_slot[t] : 0;
+    uint32_t childless = 0;
+    bool keeps = false;
+    for (int b = 0; b < beams; b++) {
+        const uint64_t children = __ballot(parent == b);
+        if (children == 0)
+            childless |= 1u << b;
+        else
+            keeps = keeps || t == __builtin_ctzll(children);
+    }
+    const uint64_t take_over = __ballot(t < beams && !keeps);
+    const int turn = __popcll(take_over & ((1ull << t) - 1));   // of the candidates that take over a slot
+    int slot = 0, source = -1, free = 0;
+    for (int b = 0; b < beams; b++) {
+        const int of_b = __builtin_amdgcn_readlane(own, b);
+        if (parent == b)
+            source = of_b;
+        if (childless >> b & 1) {
+            if (free == turn)
+                slot = of_b;
+            free++;
         }
-        a.to[out + t] = slot;
+    }
+    if (t < beams) {
+        a.from[out + t] = source;
+        a.to[out + t] = keeps ? source : slot;
     }
 }
 
