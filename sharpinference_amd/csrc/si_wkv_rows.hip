@@ -773,10 +773,11 @@ __global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs
 }
 
 // The states between a cut sequence's stretches.  A workgroup takes 16 values of one head, each of its waves 16 keys:
-// a stretch costs it 16 matrix instructions a wave, an exchange of the state's tiles through LDS, and M's 16 KiB,
-// requested a stretch ahead.
+// a stretch costs it 16 matrix instructions a wave, an exchange of the state's tiles through LDS, and 4 KiB of M a wave,
+// requested AHEAD stretches before (their round trip takes longer than the products: 0.5 us a stretch, one ahead 1.2).
 __global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, const Plan* plan, int room, float* records)
 {
+    constexpr int AHEAD = 4;
     __shared__ f4 s_tile[2][4][64];
     const int c = blockIdx.x / (4 * a.heads), rest = blockIdx.x - c * 4 * a.heads, h = rest >> 2, i = rest & 3;
     if (c >= plan->cut)
@@ -786,35 +787,39 @@ __global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, const Plan
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     auto record_of = [&](int k) { return records + (static_cast<int64_t>(part.record + k) * a.heads + h) * RECORD; };
     auto tile_of = [&](int k) { return reinterpret_cast<f4*>(record_of(k) + N * N) + (4 * i + w) * 64 + lane; };
-    f4 S[4], m[4], next[4], add, add_next;
-    load_state(state_ends(a, part.sequence, h), i, S);
+    f4 S[4], m[AHEAD][4], add[AHEAD];
+    const int steps = part.count - 1;
     auto load = [&](int k, f4(&rows)[4], f4& n) {
+        const int at = min(k, steps - 1);   // (behind the last step: read again, not used)
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            rows[j] = *reinterpret_cast<const f4*>(record_of(k) + (16 * w + t) * N + 16 * j + 4 * g);
-        n = *tile_of(k);
+            rows[j] = *reinterpret_cast<const f4*>(record_of(at) + (16 * w + t) * N + 16 * j + 4 * g);
+        n = *tile_of(at);
     };
-    load(0, next, add_next);
-    *tile_of(part.count - 1) = w == 0 ? S[0] : w == 1 ? S[1] : w == 2 ? S[2] : S[3];
-    for (int k = 0; k + 1 < part.count; k++) {
+    load_state(state_ends(a, part.sequence, h), i, S);
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            m[j] = next[j];
-        add = add_next;
-        if (k + 2 < part.count)
-            load(k + 1, next, add_next);
-        f4 other = {0.0f, 0.0f, 0.0f, 0.0f};
-        add = mfma4(m[0], S[0], add);
-        other = mfma4(m[1], S[1], other);
-        add = mfma4(m[2], S[2], add);
-        other = mfma4(m[3], S[3], other);
-        add += other;
-        *tile_of(k) = add;
-        s_tile[k & 1][w][lane] = add;
-        __syncthreads();
+    for (int k = 0; k < AHEAD; k++)
+        load(k, m[k], add[k]);
+    *tile_of(steps) = w == 0 ? S[0] : w == 1 ? S[1] : w == 2 ? S[2] : S[3];
+    for (int base = 0; base < steps; base += AHEAD) {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            S[j] = s_tile[k & 1][j][lane];
+        for (int k = 0; k < AHEAD; k++) {
+            if (base + k >= steps)
+                break;
+            f4 other = {0.0f, 0.0f, 0.0f, 0.0f}, sum = add[k];
+            sum = mfma4(m[k][0], S[0], sum);
+            other = mfma4(m[k][1], S[1], other);
+            sum = mfma4(m[k][2], S[2], sum);
+            other = mfma4(m[k][3], S[3], other);
+            sum += other;
+            load(base + k + AHEAD, m[k], add[k]);
+            *tile_of(base + k) = sum;   // the next stretch's start, in N's place
+            s_tile[k & 1][w][lane] = sum;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                S[j] = s_tile[k & 1][j][lane];
+        }
     }
 }
 
@@ -829,25 +834,27 @@ int stretch_rows(const WkvRowsArgs& a)
 // The list of stretches of all sequences over `over` rows, by one workgroup: 4096 sequences in turns of 256.
 __device__ void make_plan(const WkvRowsArgs& a, int over, int stretch, int room, Plan* plan)
 {
-    __shared__ int s_count[3][256];
+    __shared__ int64_t s_count[256];
     const int t = threadIdx.x;
-    int stretches = 0, cut = 0, records = 0;
     // where starts fall, sequences may share rows, and the list's room is for rows that are one sequence's
-    int64_t all = 0;
+    float all = 0.0f;   // (whether it passes 2^20: a sum that does cannot round below it)
     for (int i = t; i < a.batch.sequences; i += 256) {
         const RowSpan span = rows_of(a.batch, i);
-        all += span.last - span.first;
+        all += static_cast<float>(span.last - span.first);
     }
-    s_count[0][t] = static_cast<int>(min(all, static_cast<int64_t>(a.batch.rows) + 1));
+    all = wave_sum(all);
+    if ((t & 63) == 0)
+        s_count[t >> 6] = static_cast<int64_t>(all);
     __syncthreads();
-    all = 0;
-    for (int i = 0; i < 256; i++)
-        all += s_count[0][i];
-    if (all > a.batch.rows) {
+    const int64_t rows_in_all = s_count[0] + s_count[1] + s_count[2] + s_count[3];
+    __syncthreads();
+    if (rows_in_all > a.batch.rows) {
         if (t == 0)
             plan->stretches = plan->cut = 0;
         return;
     }
+    // stretches, cut sequences and their stretches in one number, 20 bits each
+    int64_t total = 0;
     for (int base = 0; base < a.batch.sequences; base += 256) {
         RowSpan span{0, 0};
         if (base + t < a.batch.sequences)
@@ -856,38 +863,30 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int stretch, int room,
         const int most = rows >= 2 * stretch ? rows / stretch : 1;
         const int each = ((rows + most - 1) / most + C - 1) / C * C;
         const int parts = rows <= over ? 0 : most > 1 ? (rows + each - 1) / each : 1;   // (none of them empty)
-        const int own[3] = {parts, parts > 1, parts > 1 ? parts : 0};
-        int before[3], sum[3];
+        const int64_t own = parts | (parts > 1 ? (1ll << 20 | static_cast<int64_t>(parts) << 40) : 0);
+        s_count[t] = own;
         __syncthreads();
-        for (int i = 0; i < 3; i++)
-            s_count[i][t] = own[i];
-        __syncthreads();
-        for (int step = 1; step < 256; step *= 2) {
-            for (int i = 0; i < 3; i++)
-                before[i] = t >= step ? s_count[i][t - step] : 0;
+        for (int step = 1; step < min(256, a.batch.sequences - base); step *= 2) {
+            const int64_t before = t >= step ? s_count[t - step] : 0;
             __syncthreads();
-            for (int i = 0; i < 3; i++)
-                s_count[i][t] += before[i];
+            s_count[t] += before;
             __syncthreads();
         }
-        for (int i = 0; i < 3; i++) {
-            sum[i] = s_count[i][255];
-            before[i] = s_count[i][t] - own[i];
-        }
+        const int64_t before = total + s_count[t] - own;
+        const int at = before & 0xfffff, cut = before >> 20 & 0xfffff, record = static_cast<int>(before >> 40);
         for (int k = 0; k < parts; k++) {
             const Stretch part{base + t, span.first + k * each, k + 1 < parts ? span.first + (k + 1) * each : span.last,
-                               parts > 1 ? records + before[2] : -1, k, parts};
-            plan->list[stretches + before[0] + k] = part;
+                               parts > 1 ? record : -1, k, parts};
+            plan->list[at + k] = part;
             if (parts > 1 && k == 0)
-                plan->list[room + cut + before[1]] = part;
+                plan->list[room + cut] = part;
         }
-        stretches += sum[0];
-        cut += sum[1];
-        records += sum[2];
+        total += s_count[min(255, a.batch.sequences - base - 1)];
+        __syncthreads();
     }
     if (t == 0) {
-        plan->stretches = stretches;
-        plan->cut = cut;
+        plan->stretches = total & 0xfffff;
+        plan->cut = total >> 20 & 0xfffff;
     }
 }
 
