@@ -893,7 +893,8 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int stretch, int room,
 }  // namespace
 
 // Stretches: at most one for every `over` + 1 rows that is a sequence's only one, and HEAD_STRETCHES / heads of cut ones.
-constexpr int FEW_ROWS = 8;              // sequences of up to this many rows go row by row
+constexpr int FEW_ROWS = 12;             // sequences of up to this many rows go row by row: 12 rows of 8 x 32 heads 10.4 us (by
+                                         // blocks 10.9), of 64 x 32 36 (47); 16 rows 12.9 (11.4) and 43 (50)
 constexpr int WHOLE_ROOM = ROW_SEQUENCES_MAX;
 
 constexpr int64_t PLAN_BYTES = (sizeof(Plan) + (WHOLE_ROOM + 2 * HEAD_STRETCHES) * sizeof(Stretch) + 255) / 256 * 256;

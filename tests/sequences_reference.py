@@ -28,7 +28,8 @@ def values(raw, fmt):
 def encode(x, fmt):
     """FP32 values as the bytes of a type (BF16: truncated, so exact in what it decodes to)."""
     x = np.ascontiguousarray(x, np.float32)
-    return x if fmt == native.F32 else x.astype(np.float16) if fmt == native.F16 else (x.view(np.uint32) >> 16).astype(np.uint16)
+    with np.errstate(over="ignore"):
+        return x if fmt == native.F32 else x.astype(np.float16) if fmt == native.F16 else (x.view(np.uint32) >> 16).astype(np.uint16)
 
 
 def taken(state, slot):

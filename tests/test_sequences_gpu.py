@@ -468,3 +468,200 @@ def test_copy_slots(hip, sizes, shift):
         if shift:
             assert np.all(b.readback(np.uint8, shift) == FILL)
         b.free()
+
+
+# ---- recorded, far and beside one another ---------------------------------------------------------------
+
+def test_recorded_calls_read_their_arrays_at_each_replay(hip):
+    """A plan of all four operators, replayed with other row starts, slots and values, beside eager work."""
+    rng = np.random.default_rng(12)
+    heads, rows, slots, n = 2, 300, 6, 128
+    plans, held = [], []
+
+    def new(x):
+        held.append(hip.to_device(x))
+        return held[-1]
+    inp = _wkv_inputs(rng, rows, heads, False, slots)
+    dev = {k: new(v) for k, v in inp.items()}
+    starts, source, to = new(np.zeros(4, np.int32)), new(np.zeros(3, np.int32)), new(np.zeros(3, np.int32))
+    batch = native.RowBatch(starts.ptr, source.ptr, to.ptr, 3, slots, rows, rows)
+    x = _mix_inputs(rng, rows, n, 2, False, slots)
+    mix = {k: new(v) for k, v in x.items() if v is not None}
+    mixed, out = hip.alloc(2 * rows * n * 4), hip.alloc(rows * n * 4)
+    ws = hip.alloc(native.rwkv7_wkv_rows_workspace_bytes(heads))
+    beam_ws = hip.alloc(native.beam_select_workspace_bytes(1, 4, 4, n))
+    scores, slot = new(np.zeros(4, np.float32)), new(np.arange(4, dtype=np.int32))
+    picked = {k: new(np.zeros(4, np.int32)) for k in ("parents", "tokens", "from")}
+
+    def body():
+        hip.layernorm_mix_rows(native.LayernormMixRowsArgs(batch, mix["x"].ptr, 0, mix["weight"].ptr, mix["bias"].ptr, mix["mix"].ptr,
+                                                           mix["state"].ptr, 0, mixed.ptr, n, 2, native.F32, 1e-5))
+        hip.rwkv7_wkv_rows(native.Rwkv7WkvRowsArgs(batch, heads, 0, *[dev[k].ptr for k in native.RWKV7_WKV_VECTORS],
+                                                   dev["v_first"].ptr, dev["state"].ptr, out.ptr, ws.ptr, native.F32))
+        # the first rows of the mixed ones as logits; the slots of beams move in place
+        hip.beam_select(native.BeamSelectArgs(mixed.ptr, scores.ptr, 0, slot.ptr, picked["parents"].ptr, picked["tokens"].ptr,
+                                              scores.ptr, 0, picked["from"].ptr, slot.ptr, beam_ws.ptr, n, n, 1, 4, 4, native.F32, -1))
+        hip.copy_slots(native.slot_arrays([(mix["state"].ptr, 4 * n)]), slots, picked["from"].ptr, slot.ptr, 4)
+    plan = hip.record(body)
+    state, shift = inp["state"].copy(), x["state"].copy()
+    given, beam_slots = np.zeros(4, np.float32), np.arange(4)
+    for turn, (at, a, b) in enumerate((([0, 40, 40, 300], [0, 1, 2], [0, 1, 2]), ([0, 250, 255, 270], [3, -1, 4], [5, 0, 4]),
+                                       ([0, 0, 290, 300], [1, 2, 5], [1, 2, 3]), ([0, 1, 2, 6], [4, 4, 4], [0, 1, 2]))):
+        starts.upload(np.asarray(at, np.int32))
+        source.upload(np.asarray(a, np.int32))
+        to.upload(np.asarray(b, np.int32))
+        scale = np.float32(1 + turn)
+        dev["r"].upload(inp["r"] * scale)
+        plan.launch()
+        now = {**inp, "r": inp["r"] * scale, "state": state}
+        want, bound, after, off = ref.wkv_rows(now, heads, False, at, a, b)
+        live = np.isfinite(want)
+        got = out.readback(np.float32).reshape(rows, n)
+        assert np.all(np.abs(got - want)[live] <= bound[live] + 1e-30)
+        new_state = dev["state"].readback(np.float32).reshape(inp["state"].shape)
+        assert np.all(np.linalg.norm(new_state.astype(np.float64) - after, axis=(2, 3)) <= off + 1e-30)
+        state = new_state
+        _, mixes, mix_off, rows_kept, kept_off, _ = ref.mix_rows(x["x"], None, x["weight"], x["bias"], x["mix"], shift, at, a, b, 1e-5)
+        got = mixed.readback(np.float32).reshape(2, rows, n)
+        live = np.isfinite(mixes)
+        assert np.all(np.abs(got - mixes)[live] <= mix_off[live] + 1e-30)
+        if at[-1] >= 4 and at[0] == 0:
+            best = ref.beam_select(got[0, :4].astype(np.float64), given, None, beam_slots, 4, 4, -1)
+            assert np.array_equal(picked["parents"].readback(np.int32), best["parents"])
+            assert np.array_equal(picked["tokens"].readback(np.int32), best["tokens"])
+            beam_slots = slot.readback(np.int32)
+            assert np.array_equal(beam_slots, best["to"])
+            given = scores.readback(np.float32)
+            for f, t in zip(best["from"], best["to"]):
+                rows_kept[t], kept_off[t] = rows_kept[f].copy(), kept_off[f].copy()
+        shift = mix["state"].readback(np.float32).reshape(slots, n)
+        assert np.all(np.abs(shift - rows_kept) <= kept_off + 1e-30)
+    plan.destroy()
+    for b in [*held, mixed, out, ws, beam_ws]:
+        b.free()
+
+
+def test_rows_and_slots_far_into_their_arrays(hip):
+    """Rows, slots and logits more than 4 GiB into their buffers."""
+    rng = np.random.default_rng(13)
+    # 540000 rows of 32 heads: 4.4 GB an array; only the last 43 are sequences' rows, and slot 8600 is 4.5 GB into the states
+    heads, rows, slots, tail = 32, 540000, 8601, 43
+    width = heads * 64
+    inp = _wkv_inputs(rng, tail, heads, False, 1)
+    dev, held = {}, []
+    for k, v in inp.items():
+        in_rows = v.ndim == 2
+        b = hip.alloc(rows * width * 4 if in_rows else slots * v.nbytes if k == "state" else v.nbytes)
+        b.upload(v, (rows - tail) * width * 4 if in_rows else (slots - 1) * v.nbytes if k == "state" else 0)
+        dev[k] = b
+    starts = np.array([rows - tail, rows - 40, rows], np.int32)
+    batch, held = _batch(hip, starts, [slots - 1, slots - 1], [slots - 2, slots - 3], slots, rows, 40)
+    out, ws = hip.alloc(rows * width * 4), hip.alloc(native.rwkv7_wkv_rows_workspace_bytes(heads))
+    hip.rwkv7_wkv_rows(native.Rwkv7WkvRowsArgs(batch, heads, 0, *[dev[k].ptr for k in native.RWKV7_WKV_VECTORS],
+                                               dev["v_first"].ptr, dev["state"].ptr, out.ptr, ws.ptr, native.F32))
+    want, bound, state, off = ref.wkv_rows({**inp, "state": np.repeat(inp["state"], 3, 0)}, heads, False, [0, 3, tail], [0, 0], [1, 2])
+    got = out.readback(np.float32, tail * width, (rows - tail) * width * 4).reshape(tail, width)
+    _near(got, want, bound)
+    size = width * 64
+    for i, slot in ((1, slots - 2), (2, slots - 3)):
+        s = dev["state"].readback(np.float32, size, slot * size * 4).reshape(heads, 64, 64)
+        assert np.all(np.linalg.norm(s - state[i], axis=(1, 2)) <= off[i])
+    # the same rows, mixed (their state 8600 slots in, too)
+    x = _mix_inputs(rng, tail, width, 1, False, 1)
+    small = [hip.to_device(x[k]) for k in ("weight", "bias", "mix")]
+    dev["r"].upload(x["x"], (rows - tail) * width * 4)
+    shift = hip.alloc(slots * width * 4)
+    shift.upload(x["state"], (slots - 1) * width * 4)
+    hip.layernorm_mix_rows(native.LayernormMixRowsArgs(batch, dev["r"].ptr, 0, *[b.ptr for b in small], shift.ptr, 0, out.ptr, width,
+                                                       1, native.F32, 1e-5))
+    want, bound = ref.mix_rows(x["x"], None, x["weight"], x["bias"], x["mix"], np.repeat(x["state"], 3, 0), [0, 3, tail], [0, 0],
+                               [1, 2], 1e-5)[1:3]
+    _near(out.readback(np.float32, tail * width, (rows - tail) * width * 4).reshape(1, tail, width), want, bound)
+    # logits: four rows 1.2 GB apart
+    logits = (2 * rng.standard_normal((4, 3000))).astype(np.float32)
+    stride = 300_000_000
+    for i in range(4):
+        out.upload(logits[i], 4 * stride * i) if 4 * (stride * i + 3000) <= out.nbytes else None
+    assert 4 * (3 * stride + 3000) <= out.nbytes and 4 * 3 * stride > 1 << 31
+    scores, ids = hip.to_device(np.zeros(4, np.float32)), [hip.alloc(16) for _ in range(3)]
+    hip.beam_select(native.BeamSelectArgs(out.ptr, scores.ptr, 0, 0, ids[0].ptr, ids[1].ptr, ids[2].ptr, 0, 0, 0, ws.ptr, 3000, stride,
+                                          1, 4, 4, native.F32, -1))
+    best = ref.beam_select(logits.astype(np.float64), np.zeros(4), None, None, 4, 4, -1)
+    assert np.array_equal(ids[0].readback(np.int32), best["parents"]) and np.array_equal(ids[1].readback(np.int32), best["tokens"])
+    # a slot 4.5 GB into the states onto the first one
+    pair = [_i32(hip, [slots - 2]), _i32(hip, [0])]
+    hip.copy_slots(native.slot_arrays([(dev["state"].ptr, size * 4)]), slots, pair[0].ptr, pair[1].ptr, 1)
+    assert np.array_equal(dev["state"].readback(np.uint8, size * 4), dev["state"].readback(np.uint8, size * 4, (slots - 2) * size * 4))
+    for b in [*dev.values(), *held, out, ws, shift, scores, *ids, *pair, *small]:
+        b.free()
+
+
+def test_refusals(hip):
+    """Everything that a call refuses, before anything is launched."""
+    b = hip.alloc(1 << 20)
+    far = [hip.alloc(1 << 16) for _ in range(24)]
+    f = [x.ptr for x in far]
+    A, U = native.ERR_ARGUMENT, native.ERR_UNSUPPORTED
+
+    def refused(call, args, status):
+        with pytest.raises(native.HipError) as e:
+            call(args)
+        assert e.value.status == status, e.value
+
+    def changed(make, base, changes):
+        for change, status in changes:
+            yield make({**base, **change}), status, change
+    rows = dict(row_starts=f[0], from_=f[1], to=f[2], sequences=2, slots=3, rows=4, max_rows=4)
+    batches = [(dict(row_starts=0), A), (dict(row_starts=f[0] + 2), A), (dict(from_=0), A), (dict(to=0), A), (dict(sequences=0), A),
+               (dict(sequences=4097), A), (dict(slots=0), A), (dict(rows=0), A), (dict(rows=(1 << 20) + 1), A), (dict(max_rows=0), A),
+               (dict(max_rows=5), A)]
+    mix = dict(batch=native.RowBatch(**rows), x=f[3], residual=0, weight=f[4], bias=f[5], mix=f[6], state=f[7], updated=0, output=f[8],
+               n=64, mixes=2, output_format=native.BF16, eps=1e-5)
+    make_mix = lambda a: native.LayernormMixRowsArgs(**a)
+    for change, status in batches:
+        refused(hip.layernorm_mix_rows, make_mix({**mix, "batch": native.RowBatch(**{**rows, **change})}), status)
+    for args, status, _ in changed(make_mix, mix, [
+            (dict(x=0), A), (dict(x=f[3] + 1), A), (dict(weight=0), A), (dict(bias=0), A), (dict(mix=0), A), (dict(state=0), A),
+            (dict(output=0), A), (dict(output=f[8] + 1), A), (dict(n=0), A), (dict(n=8193), A), (dict(mixes=-1), A), (dict(mixes=9), A),
+            (dict(eps=-1.0), A), (dict(eps=float("nan")), A), (dict(eps=float("inf")), A), (dict(output_format=native.Q8_0), U),
+            (dict(residual=f[9]), A), (dict(updated=f[9]), A), (dict(output=f[3]), A), (dict(state=f[3]), A), (dict(state=f[8]), A),
+            (dict(residual=f[9], updated=f[3]), A), (dict(residual=f[9], updated=f[9]), A), (dict(output=f[0]), A)]):
+        refused(hip.layernorm_mix_rows, args, status)
+    names = native.RWKV7_WKV_VECTORS
+    big = hip.alloc(native.rwkv7_wkv_rows_workspace_bytes(1))
+    wkv = dict(batch=native.RowBatch(**rows), heads=1, first_layer=0, **{n: f[3 + i] for i, n in enumerate(names)}, v_first=f[18],
+               state=f[19], output=f[20], workspace=big.ptr, output_format=native.F32)
+    make_wkv = lambda a: native.Rwkv7WkvRowsArgs(**a)
+    for change, status in batches:
+        refused(hip.rwkv7_wkv_rows, make_wkv({**wkv, "batch": native.RowBatch(**{**rows, **change})}), status)
+    for args, status, _ in changed(make_wkv, wkv, [(dict(heads=0), A), (dict(heads=1025), A), (dict(output_format=native.Q4_0), U),
+                                                   (dict(output=f[20] + 4), A), (dict(state=f[19] + 8), A), (dict(workspace=0), A),
+                                                   (dict(workspace=big.ptr + 8), A), (dict(v_first=0), A), (dict(output=f[3]), A),
+                                                   (dict(state=f[18]), A), (dict(workspace=f[3]), A), (dict(output=f[18]), A),
+                                                   (dict(first_layer=1, v_first=f[5]), A)] +
+                                   [(dict([(n, 0)]), A) for n in names] + [(dict([(n, f[3 + i] + 2)]), A) for i, n in enumerate(names)]):
+        refused(hip.rwkv7_wkv_rows, args, status)
+    beam = dict(logits=f[0], scores=f[1], done=f[2], slots=f[3], parents=f[4], tokens=f[5], new_scores=f[6], new_done=f[7], from_=f[8],
+                to=f[9], workspace=b.ptr, vocab=100, stride=100, sequences=2, beams=4, candidates=4, logits_format=native.F16, end_token=3)
+    for args, status, _ in changed(lambda a: native.BeamSelectArgs(**a), beam, [
+            (dict(vocab=0), A), (dict(vocab=(1 << 21) + 1, stride=1 << 22), A), (dict(stride=99), A), (dict(stride=(1 << 32) + 1), A),
+            (dict(sequences=0), A), (dict(sequences=16385), A), (dict(beams=0), A), (dict(beams=17), A), (dict(candidates=0), A),
+            (dict(candidates=33), A), (dict(candidates=5), A), (dict(logits_format=native.Q8_0), U), (dict(end_token=-2), A),
+            (dict(end_token=100), A), (dict(end_token=-1), A), (dict(slots=0), A), (dict(logits=0), A), (dict(logits=f[0] + 1), A),
+            (dict(scores=0), A), (dict(done=f[2] + 1), A), (dict(parents=0), A), (dict(tokens=0), A), (dict(new_scores=0), A),
+            (dict(from_=0), A), (dict(to=0), A), (dict(workspace=0), A), (dict(workspace=b.ptr + 4), A), (dict(parents=f[4], tokens=f[4]), A),
+            (dict(tokens=f[0]), A), (dict(from_=f[3]), A), (dict(new_scores=f[1] + 4), A), (dict(new_done=f[1]), A),
+            (dict(workspace=f[0]), A)]):
+        refused(hip.beam_select, args, status)
+    for arrays, slots, source, to, moves in (([], 3, f[1], f[2], 1), ([(0, 4)], 3, f[1], f[2], 1), ([(f[0], 0)], 3, f[1], f[2], 1),
+                                             ([(f[0], (1 << 36) + 1)], 3, f[1], f[2], 1), ([(f[0], 4)], 0, f[1], f[2], 1),
+                                             ([(f[0], 4)], 1 << 31, f[1], f[2], 1), ([(f[0], 4)], 3, 0, f[2], 1),
+                                             ([(f[0], 4)], 3, f[1], f[2] + 1, 1), ([(f[0], 4)], 3, f[1], f[2], 0),
+                                             ([(f[0], 4)], 3, f[1], f[2], (1 << 20) + 1), ([(f[0], 4), (f[0] + 8, 4)], 3, f[1], f[2], 1),
+                                             ([(f[0], 4)], 3, f[0] + 8, f[2], 1), ([(f[0], 4)], 3, f[1], f[0], 1),
+                                             ([(f[0], 1)] * 4097, 3, f[1], f[2], 1)):
+        with pytest.raises(native.HipError) as e:
+            hip.copy_slots(native.slot_arrays(arrays), slots, source, to, moves)
+        assert e.value.status == A
+    for x in [b, big, *far]:
+        x.free()
