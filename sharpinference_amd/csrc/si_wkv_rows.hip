@@ -177,9 +177,8 @@ __global__ __launch_bounds__(256) void wkv_few_kernel(WkvRowsArgs a, int most, i
 // Then with u_t = -(S_(t-1) kn_t) the block's state is S_0 + sum_s (u_s beta_s^T + v_s khat_s^T), times L_C, and
 //   (I + A) U = -(alpha S_0^T + B V),   A_ts = alpha_t . beta_s, B_ts = alpha_t . khat_s  (s < t)
 //   Y = rho S_0^T + D U + E V,          D_ts = rho_t . beta_s,   E_ts = rho_t . khat_s    (s <= t).
-// What does not need S_0 is formed beforehand: alpha' = (I + A)^-1 alpha, W = (I + A)^-1 B,
-// rho' = rho - D alpha', Z = E - D W, V' = W V, Y' = Z V, so that a block costs the state
-//   U = -(alpha' S_0^T + V'),  Y = rho' S_0^T + Y',  S = (S_0 + U^T beta + V^T khat) diag(L_C).
+// What does not need S_0 is formed beforehand, alpha' = (I + A)^-1 alpha and V' = (I + A)^-1 B V, so that a
+// block costs the state U = -(alpha' S_0^T + V'), Y as above, S = (S_0 + U^T beta + V^T khat) diag(L_C).
 // (I + A) is solved row by row: rows of like keys make A all ones, where a product of powers of A
 // loses every digit.  The decays are at least exp(-0.606531), so 1 / L grows to 2^14 at most and the
 // factors stay far from FP32's ends; all products are FP32 (v_mfma_f32_16x16x4_f32).
@@ -285,7 +284,8 @@ __device__ __forceinline__ void scale_rows(float* to, const float (&z)[C], float
 // What the preparing waves hand to the state's waves for one block.
 struct BlockLds {
     float alpha[C][LD], rho[C][LD], beta[C][LD], khat[C][LD], value[C][LD];
-    f4 v_part[4][64], y_part[4][64];   // V', Y' tiles as the matrix instructions hold them
+    f4 v_part[4][64];                  // V' tiles as the matrix instructions hold them
+    float m[C][LD];                    // A, B, D, E beside one another
     float decay[N];                    // L_C
     float bonus[4][C];                 // parts of sum(key r r_k)
     float squares[4][C];
@@ -294,8 +294,7 @@ struct BlockLds {
 
 struct ChunkLds {
     BlockLds block[2];
-    float m[C][LD];                    // A, B, D, E beside one another
-    float w[C][LD];                    // W in the columns that A has in m
+    float w[C][LD];                    // (I + A)^-1 B in the columns that A has in m
     float y[C][LD];
 };
 
@@ -489,7 +488,7 @@ __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks
             for (int v = 0; v < 4; v++) {
                 const int i = 4 * g + v;
                 const int keep = -static_cast<int>(i < rows && t < (q < 2 ? i : i + 1));   // (as bits: a choice branches)
-                lds.m[i][ch] = __int_as_float(__float_as_int((m0[v] + m1[v]) * f) & keep);
+                b.m[i][ch] = __int_as_float(__float_as_int((m0[v] + m1[v]) * f) & keep);
             }
         }
         __syncthreads();
@@ -498,11 +497,11 @@ __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks
             // column t of alpha (lanes 0..15 of a half) or of B (16..31), solved row by row:
             // z_i = n_i (r_i + sum_s -A_is n_s z_s), every lane with row i's sums from the row of 16 lanes that holds it
             const bool of_b = (lane & 16) != 0;
-            const float* const column = of_b ? &lds.m[0][16 + t] : &b.alpha[0][16 * q + t];
+            const float* const column = of_b ? &b.m[0][16 + t] : &b.alpha[0][16 * q + t];
             float z[C], l[C];
 #pragma unroll
             for (int i = 0; i < C; i++) {
-                l[i] = lds.m[i][t];
+                l[i] = b.m[i][t];
                 z[i] = column[i * LD];
             }
             solve_rows(z, l, length);
@@ -512,15 +511,6 @@ __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks
             wave_sync();
             const f4 v_tile = column4(b.value, 4 * g, 16 * q + t);
             b.v_part[q][lane] = mfma4(row4(lds.w, t, 4 * g), v_tile, zero);
-            if (!TRANSFER) {
-                const f4 d = -row4(lds.m, t, 32 + 4 * g);
-                const f4 rho = mfma4(d, column4(b.alpha, 4 * g, 16 * q + t), column4(b.rho, 4 * g, 16 * q + t));
-                const f4 zt = mfma4(column4(lds.w, 4 * g, t), d, row4(lds.m, t, 48 + 4 * g));   // Z^T
-#pragma unroll
-                for (int v = 0; v < 4; v++)
-                    b.rho[4 * g + v][16 * q + t] = rho[v];
-                b.y_part[q][lane] = mfma4(zt, v_tile, zero);
-            }
         }
         if (threadIdx.x == CHUNK_THREADS - 1)
             lds.block[(stage & 1) ^ 1].odd = 0;
@@ -569,7 +559,7 @@ __device__ void chunk_advance(const WkvRowsArgs& a, ChunkLds& lds, int h, const 
         const BlockLds& b = lds.block[(stage & 1) ^ 1];
         const bool have = counts, more = blocks.at < blocks.end;
         const int next_at = blocks.at, next_rows = more ? blocks.last() - next_at : 0;
-        f4 gate, xa, xr;
+        f4 gate, xa, xr, v_tile;
         auto part = [&](int j) {
             xa = mfma4(row4(b.alpha, t, 16 * j + 4 * g), S[j], xa);
             xr = mfma4(row4(b.rho, t, 16 * j + 4 * g), S[j], xr);
@@ -577,7 +567,7 @@ __device__ void chunk_advance(const WkvRowsArgs& a, ChunkLds& lds, int h, const 
         if (have) {
             gate = load4(a.gate + (at + min(tn, rows - 1)) * width + h * N + cn);
             xa = b.v_part[w][lane];
-            xr = b.y_part[w][lane];
+            xr = mfma4(row4(b.m, t, 48 + 4 * g), v_tile = column4(b.value, 4 * g, 16 * w + t), f4{0.0f, 0.0f, 0.0f, 0.0f});
             part(0);
             part(1);
         }
@@ -586,6 +576,8 @@ __device__ void chunk_advance(const WkvRowsArgs& a, ChunkLds& lds, int h, const 
         if (have) {
             part(2);
             part(3);
+            xa = -xa;   // U
+            xr = mfma4(row4(b.m, t, 32 + 4 * g), xa, xr);
 #pragma unroll
             for (int v = 0; v < 4; v++)
                 lds.y[4 * g + v][16 * w + t] = xr[v];
@@ -594,10 +586,9 @@ __device__ void chunk_advance(const WkvRowsArgs& a, ChunkLds& lds, int h, const 
         if (have) {
             const f4 y = row4(lds.y, tn, cn), value = row4(b.value, tn, cn);
             const float bonus = b.bonus[0][tn] + b.bonus[1][tn] + b.bonus[2][tn] + b.bonus[3][tn];
-            const f4 u = -xa, v_tile = column4(b.value, 4 * g, 16 * w + t);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                S[j] = mfma4(column4(b.beta, 4 * g, 16 * j + t), u, S[j]);
+                S[j] = mfma4(column4(b.beta, 4 * g, 16 * j + t), xa, S[j]);
                 S[j] = mfma4(column4(b.khat, 4 * g, 16 * j + t), v_tile, S[j]);
             }
             const float mean = row_sum<16>(y[0] + y[1] + y[2] + y[3]) * (1.0f / N);
