@@ -27,7 +27,7 @@ struct RowIn {
 };
 
 struct Plan;
-__device__ void make_plan(const WkvRowsArgs& a, int over, int stretch, int room, Plan* plan);
+__device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Plan* plan);
 
 // Sequences of few rows: a workgroup takes one head of one sequence, the state
 // in registers (a thread holds 8 columns of two state rows: 8 lanes a state
@@ -38,13 +38,13 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int stretch, int room,
 // brings one row; by vector instructions (92 a row and wave) and LDS reads
 // (10 b128 a lane and row) where it brings many.
 // With a plan to make, the last workgroup makes it.
-__global__ __launch_bounds__(256) void wkv_few_kernel(WkvRowsArgs a, int most, int stretch, int room, Plan* plan)
+__global__ __launch_bounds__(256) void wkv_few_kernel(WkvRowsArgs a, int most, int cut, int room, Plan* plan)
 {
     __shared__ float4 s_vec[4][5][N / 4];   // decay, key, kn, kn * a, r of the four rows
     __shared__ float s_value[4][N], s_y[4][N];
     const int s = blockIdx.x / a.heads, h = blockIdx.x - s * a.heads;
     if (s == a.batch.sequences)
-        return make_plan(a, most, stretch, room, plan);
+        return make_plan(a, most, cut, room, plan);
     const RowSpan span = rows_of(a.batch, s);
     const int from = a.batch.from[s], to = a.batch.to[s];
     if (span.last - span.first < 1 || span.last - span.first > most)
@@ -690,7 +690,9 @@ __device__ void chunk_transfer(ChunkLds& lds, float* record, Blocks blocks)
 // sequence of its own.  (1) costs about 0.8 of (3).
 
 constexpr int RECORD = 2 * N * N;        // floats of a stretch and head: M^T; N, later the next stretch's start
-constexpr int HEAD_STRETCHES = 512;      // stretches times heads: two workgroups a compute unit
+constexpr int CARD = 512;                // workgroups of wkv_chunk_kernel that the card holds: two a compute unit
+constexpr int HEAD_STRETCHES = 2 * CARD; // stretches times heads, at most
+constexpr int LONG_STRETCH = 256;
 constexpr int LEAST_STRETCH = 64;        // rows
 
 struct Stretch {
@@ -814,47 +816,72 @@ __global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, const Plan
     }
 }
 
-// How a launch cuts its sequences: into stretches of at least this many rows, or 0: not at all.
-int stretch_rows(const WkvRowsArgs& a)
+// Rows of a stretch where so many rows are cut: the card's workgroups share them with their heads; where that gives each more
+// than LONG_STRETCH, twice as many workgroups do, which even out better beside whole sequences (eight prompts of 500 to 3000
+// rows of 32 heads 560 us, by CARD 648; one of 4001 225, by twice CARD 246).
+__host__ __device__ inline int stretch_rows(int64_t rows, int heads)
 {
-    const int64_t each = (static_cast<int64_t>(a.batch.rows) * a.heads + HEAD_STRETCHES - 1) / HEAD_STRETCHES;
-    const int64_t rows = (each > LEAST_STRETCH ? each + C - 1 : LEAST_STRETCH) / C * C;
-    return a.batch.max_rows >= 3 * rows ? static_cast<int>(rows) : 0;
+    const int64_t each = (rows * heads + CARD - 1) / CARD, half = (each + 1) / 2;
+    const int64_t least = each < LONG_STRETCH ? each : half > LONG_STRETCH ? half : LONG_STRETCH;
+    return static_cast<int>((least > LEAST_STRETCH ? least + C - 1 : LEAST_STRETCH) / C * C);
+}
+
+// From how many rows on a launch cuts its sequences, or 0: none.  Cutting costs the transfers and the join, and pays where the
+// longest sequence has 2.5 times the rows that all, shared out evenly, give a workgroup (eight of 1000 rows of 32 heads, at 2:
+// 230 us whole, 342 cut; sixteen of 100 to 3000, at 3.2: 862 and 624), and for the sequences that become three stretches or
+// more (thirty of 16 to 4000: 880 us, from two on 905).
+int cut_from(const WkvRowsArgs& a)
+{
+    const int64_t each = (static_cast<int64_t>(a.batch.rows) * a.heads + CARD - 1) / CARD;
+    const int from = 3 * stretch_rows(a.batch.rows, a.heads);
+    return a.batch.max_rows >= from && 2ll * a.batch.max_rows >= 5 * each ? from : 0;
 }
 
 // The list of stretches of all sequences over `over` rows, by one workgroup: 4096 sequences in turns of 256.
-__device__ void make_plan(const WkvRowsArgs& a, int over, int stretch, int room, Plan* plan)
+// Whole sequences come first in it: the longest pieces of the last pass.
+__device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Plan* plan)
 {
     __shared__ int64_t s_count[256];
     const int t = threadIdx.x;
-    // where starts fall, sequences may share rows, and the list's room is for rows that are one sequence's
-    float all = 0.0f;   // (whether it passes 2^20: a sum that does cannot round below it)
+    // Rows in all, rows in sequences that are cut, sequences that are not.  Where starts fall, sequences may share rows, and the
+    // list's room is for rows that are one sequence's.
+    float sums[3] = {};   // (exact to 2^24; whether the first passes 2^20: a sum that does cannot round below it)
     for (int i = t; i < a.batch.sequences; i += 256) {
         const RowSpan span = rows_of(a.batch, i);
-        all += static_cast<float>(span.last - span.first);
+        const int rows = span.last - span.first;
+        sums[0] += static_cast<float>(rows);
+        sums[1] += rows >= from ? static_cast<float>(rows) : 0.0f;
+        sums[2] += rows > over && rows < from ? 1.0f : 0.0f;
     }
-    all = wave_sum(all);
-    if ((t & 63) == 0)
-        s_count[t >> 6] = static_cast<int64_t>(all);
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        sums[i] = wave_sum(sums[i]);
+        if ((t & 63) == 0)
+            s_count[4 * i + (t >> 6)] = static_cast<int64_t>(sums[i]);
+    }
     __syncthreads();
-    const int64_t rows_in_all = s_count[0] + s_count[1] + s_count[2] + s_count[3];
+    auto sum_of = [&](int i) { return s_count[4 * i] + s_count[4 * i + 1] + s_count[4 * i + 2] + s_count[4 * i + 3]; };
+    const int64_t rows_in_all = sum_of(0), rows_in_cut = sum_of(1);
+    const int whole = static_cast<int>(sum_of(2));
     __syncthreads();
     if (rows_in_all > a.batch.rows) {
         if (t == 0)
             plan->stretches = plan->cut = 0;
         return;
     }
-    // stretches, cut sequences and their stretches in one number, 20 bits each
+    const int stretch = stretch_rows(rows_in_cut, a.heads);   // at most a third of `from`
+    // whole sequences, cut ones and their stretches in one number, 20 bits each
     int64_t total = 0;
     for (int base = 0; base < a.batch.sequences; base += 256) {
         RowSpan span{0, 0};
         if (base + t < a.batch.sequences)
             span = rows_of(a.batch, base + t);
         const int rows = span.last - span.first;
-        const int most = rows >= 2 * stretch ? rows / stretch : 1;
+        const bool cut = rows >= from;
+        const int most = cut ? rows / stretch : 1;
         const int each = ((rows + most - 1) / most + C - 1) / C * C;
-        const int parts = rows <= over ? 0 : most > 1 ? (rows + each - 1) / each : 1;   // (none of them empty)
-        const int64_t own = parts | (parts > 1 ? (1ll << 20 | static_cast<int64_t>(parts) << 40) : 0);
+        const int parts = rows <= over ? 0 : cut ? (rows + each - 1) / each : 1;   // (none of them empty)
+        const int64_t own = cut ? 1ll << 20 | static_cast<int64_t>(parts) << 40 : parts;
         s_count[t] = own;
         __syncthreads();
         for (int step = 1; step < min(256, a.batch.sequences - base); step *= 2) {
@@ -864,56 +891,60 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int stretch, int room,
             __syncthreads();
         }
         const int64_t before = total + s_count[t] - own;
-        const int at = before & 0xfffff, cut = before >> 20 & 0xfffff, record = static_cast<int>(before >> 40);
+        const int record = static_cast<int>(before >> 40), at = cut ? whole + record : static_cast<int>(before & 0xfffff);
         for (int k = 0; k < parts; k++) {
             const Stretch part{base + t, span.first + k * each, k + 1 < parts ? span.first + (k + 1) * each : span.last,
-                               parts > 1 ? record : -1, k, parts};
+                               cut ? record : -1, k, parts};
             plan->list[at + k] = part;
-            if (parts > 1 && k == 0)
-                plan->list[room + cut] = part;
+            if (cut && k == 0)
+                plan->list[room + (before >> 20 & 0xfffff)] = part;
         }
         total += s_count[min(255, a.batch.sequences - base - 1)];
         __syncthreads();
     }
     if (t == 0) {
-        plan->stretches = total & 0xfffff;
+        plan->stretches = static_cast<int>((total & 0xfffff) + (total >> 40));
         plan->cut = total >> 20 & 0xfffff;
     }
 }
 
 }  // namespace
 
-// Stretches: at most one for every `over` + 1 rows that is a sequence's only one, and HEAD_STRETCHES / heads of cut ones.
 constexpr int FEW_ROWS = 12;             // sequences of up to this many rows go row by row: 12 rows of 8 x 32 heads 10.4 us (by
                                          // blocks 10.9), of 64 x 32 36 (47); 16 rows 12.9 (11.4) and 43 (50)
-constexpr int WHOLE_ROOM = ROW_SEQUENCES_MAX;
 
-constexpr int64_t PLAN_BYTES = (sizeof(Plan) + (WHOLE_ROOM + 2 * HEAD_STRETCHES) * sizeof(Stretch) + 255) / 256 * 256;
+// The list: every sequence that goes by blocks, at most, the stretches, and the cut sequences again (three stretches each, at least).
+constexpr int64_t PLAN_BYTES = (sizeof(Plan) + (ROW_SEQUENCES_MAX + HEAD_STRETCHES * 4 / 3) * sizeof(Stretch) + 255) / 256 * 256;
 
 int64_t wkv_rows_workspace_bytes(int) { return PLAN_BYTES + static_cast<int64_t>(HEAD_STRETCHES) * RECORD * 4; }
 
 hipError_t launch_wkv_rows(const WkvRowsArgs& a, hipStream_t s)
 {
-    const unsigned grid = static_cast<unsigned>(a.batch.sequences) * a.heads;
-    Plan* const plan = reinterpret_cast<Plan*>(a.workspace);
-    float* const records = a.workspace + PLAN_BYTES / 4;
+    const unsigned heads = static_cast<unsigned>(a.heads), grid = static_cast<unsigned>(a.batch.sequences) * heads;
+    auto few = [&](int most, unsigned more, int from, int room, Plan* plan) {
+        hipLaunchKernelGGL(wkv_few_kernel, dim3(grid + more), dim3(256), 0, s, a, most, from, room, plan);
+    };
     if (a.batch.max_rows <= FEW_ROWS) {
-        hipLaunchKernelGGL(wkv_few_kernel, dim3(grid), dim3(256), 0, s, a, INT32_MAX, 0, 0, nullptr);
+        few(INT32_MAX, 0, 0, 0, nullptr);
         return hipGetLastError();
     }
-    const int stretch = stretch_rows(a);
-    if (stretch == 0) {
-        hipLaunchKernelGGL(wkv_few_kernel, dim3(grid), dim3(256), 0, s, a, FEW_ROWS, 0, 0, nullptr);
+    const int from = cut_from(a);
+    if (from == 0) {
+        few(FEW_ROWS, 0, 0, 0, nullptr);
         hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_SEQUENCES>, dim3(grid), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, nullptr, nullptr);
         return hipGetLastError();
     }
-    // what the host knows of the list's length
-    const int whole = a.batch.rows / (FEW_ROWS + 1) < a.batch.sequences ? a.batch.rows / (FEW_ROWS + 1) : a.batch.sequences;
-    const int cut_parts = a.batch.rows / stretch, room = whole + cut_parts;
-    const unsigned heads = static_cast<unsigned>(a.heads);
-    hipLaunchKernelGGL(wkv_few_kernel, dim3(grid + 1), dim3(256), 0, s, a, FEW_ROWS, stretch, room, plan);
+    Plan* const plan = reinterpret_cast<Plan*>(a.workspace);
+    float* const records = a.workspace + PLAN_BYTES / 4;
+    // What the host knows of the list's length.  Stretches have at least LEAST_STRETCH rows, and
+    // as many as share all cut rows and heads out to HEAD_STRETCHES workgroups.
+    auto least = [](int x, int y) { return x < y ? x : y; };
+    const int whole = least(a.batch.rows / (FEW_ROWS + 1), a.batch.sequences);
+    const int parts = least(a.batch.rows / LEAST_STRETCH, HEAD_STRETCHES / a.heads), room = whole + parts;
+    const int cut = least(a.batch.rows / from, parts / 3);
+    few(FEW_ROWS, 1, from, room, plan);
     hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_TRANSFERS>, dim3(room * heads), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, plan, records);
-    hipLaunchKernelGGL(wkv_join_kernel, dim3((cut_parts / 2) * heads * 4), dim3(256), 0, s, a, plan, room, records);
+    hipLaunchKernelGGL(wkv_join_kernel, dim3(cut * heads * 4), dim3(256), 0, s, a, plan, room, records);
     hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_STRETCHES>, dim3(room * heads), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, plan, records);
     return hipGetLastError();
 }

@@ -235,7 +235,8 @@ def test_wkv_rows(hip, counts, heads, first, fmt):
     _check_wkv(hip, _wkv_inputs(rng, rows, heads, first, slots), heads, first, starts, source, to, fmt)
 
 
-@pytest.mark.parametrize("heads,counts", [(1, [1500]), (2, [700, 90, 1, 260])])
+@pytest.mark.parametrize("heads,counts", [(1, [1500]), (2, [700, 90, 1, 260]), (64, [700, 1500, 13, 0, 40, 900, 1]),
+                                          (4, [20] * 150 + [640, 0, 1] + [13] * 149 + [900])])
 def test_wkv_rows_long(hip, heads, counts):
     """Long sequences, which may be shared out over their length."""
     rng = np.random.default_rng(len(counts))
