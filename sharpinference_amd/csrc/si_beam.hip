@@ -17,8 +17,8 @@ constexpr float LOG2E = 1.44269504088896f;
 constexpr int TILE = 2048, PER = TILE / 64;   // values of a wave's tile, and of a lane's
 constexpr int KEPT = 256;                     // values that are ranked together
 constexpr int ROOM = KEPT + CANDIDATES_MAX + 8;
-constexpr int SHOWN = 24;                     // lanes of a tile whose values are looked at one by one
-constexpr int SCAN_WAVES = 4, MERGE_WAVES = 8;
+constexpr int LARGEST = 24;                   // a lane's 16-byte words of a group of tiles, whose largest values are held
+constexpr int SCAN_WAVES = 4, MERGE_WAVES = 16;
 constexpr float INF = __builtin_inff();
 
 typedef uint32_t Sixteen __attribute__((ext_vector_type(4), aligned(1)));   // bytes at any address, in one load or store
@@ -140,7 +140,8 @@ __device__ __forceinline__ double wave_sum(double v)
 }
 
 // How a row is cut: tiles a part, parts a row.  A wave takes a part; where there are
-// more tiles than the card holds waves of this kernel, it takes several one after another.
+// more tiles than the card holds waves of this kernel, it takes several one after another (192 rows of 98 tiles, with the merge:
+// five a wave 26 us, ten 27, three 25 to 27, one 35).
 struct Cut {
     int tiles, parts;
 };
@@ -168,15 +169,17 @@ __device__ __forceinline__ float value_at(const void* p, int64_t i)
         return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i]) << 16);
 }
 
-// One wave a part of a row.  Bound by vector instructions (about
-// ten a value, the exponential among them) where the logits are 16 bits, in small calls by the launch and one tile's latency.
+// One wave a part of a row.  Over a group of tiles it takes the sum and each 16-byte word's largest value; then it reads the
+// words again that may hold one of the best (some dozens, by the groups' bound), and ranks those values together: ranked tile by tile
+// out of registers, that part took as long as the rest.  Bound by HBM, then by the tail of ranking and launch: 24 sequences of 8 beams over
+// 200064 16-bit logits, 65 MB of them read, 20 us, 3.2 TB/s (17 without ranking; tile by tile 28).  One sequence of 4 beams over
+// 65536 FP32 logits: 5.2 us, the launch and one chain of round trips.
 template <int FMT>
 __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs a, int rows, int tiles, int parts, Part* part, Key* keys)
 {
     __shared__ Key s_kept[SCAN_WAVES][ROOM], s_list[SCAN_WAVES][CANDIDATES_MAX];
-    __shared__ float4 s_shown[SCAN_WAVES][SHOWN][PER / 4];
-    __shared__ int s_lane[SCAN_WAVES][SHOWN];
-    constexpr int SIZE = FMT == ROWS_OUT_F32 ? 4 : 2, VEC = 16 / SIZE, LOADS = PER / VEC;
+    __shared__ float4 s_largest[SCAN_WAVES][LARGEST / 4][64];
+    constexpr int SIZE = FMT == ROWS_OUT_F32 ? 4 : 2, VEC = 16 / SIZE, LOADS = PER / VEC, GROUP = LARGEST / LOADS;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t unit = static_cast<int64_t>(blockIdx.x) * SCAN_WAVES + wave;
     if (unit >= static_cast<int64_t>(rows) * parts)
@@ -184,14 +187,27 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
     const int row = static_cast<int>(unit / parts), p = static_cast<int>(unit - static_cast<int64_t>(row) * parts);
     const int first = p * tiles * TILE, last = min(first + tiles * TILE, a.vocab);
     const char* const x = static_cast<const char*>(a.logits) + row * a.stride * SIZE;
+    // Word `at` of the row (tokens at and the following), or, behind the row's last whole word, that one: what lies before `at` in it
+    // does not count.  A row of less than a word is put together value by value.
+    const int last_word = a.vocab - VEC;
+    auto word = [&](int at) {
+        if (last_word >= 0)
+            return *reinterpret_cast<const Sixteen*>(x + static_cast<int64_t>(min(at, last_word)) * SIZE);
+        Sixteen got = {0, 0, 0, 0};
+        for (int j = 0; j < a.vocab; j++) {
+            const uint32_t bits = SIZE == 4 ? reinterpret_cast<const uint32_t*>(x)[j] : reinterpret_cast<const uint16_t*>(x)[j];
+            const int to = VEC - a.vocab + j;   // the row ends where the word does
+            got[to * SIZE / 4] |= bits << (SIZE == 4 ? 0 : to % 2 * 16);
+        }
+        return got;
+    };
     Sixteen raw[LOADS];
-    auto request = [&](int base) {   // a whole tile
+    auto request = [&](int base) {
 #pragma unroll
         for (int j = 0; j < LOADS; j++)
-            raw[j] = *reinterpret_cast<const Sixteen*>(x + (static_cast<int64_t>(base) + VEC * (lane + 64 * j)) * SIZE);
+            raw[j] = word(base + VEC * (lane + 64 * j));
     };
-    if (first + TILE <= last)
-        request(first);
+    request(first);
     if (a.done && a.done[row] != 0)
         return;   // its logits do not count
     const int k = a.candidates;
@@ -200,96 +216,115 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
         list[lane] = 0;
     wave_sync();
     Key* const kept = s_kept[wave];
-    float most = -INF, sum = 0.0f, over = -INF;
-    int pending = 0;   // kept ones that are not in the list yet
-    for (int base = first; base < last; base += TILE) {
-        float v[PER];
-        const bool full = base + TILE <= last;
-        // token of value j: neighbours in a 16-byte load, or (a row's last tile) every 64th
-        auto token = [&](int lane, int j) {
-            return static_cast<uint32_t>(base + (full ? VEC * (lane + 64 * (j / VEC)) + j % VEC : lane + 64 * j));
-        };
-        auto key_of = [&](float x, int lane, int j) { return static_cast<Key>(order_of(x)) << 32 | (0xffffffffu - token(lane, j)); };
-        if (full) {
-            if (base > first)
-                request(base);
+    float4(*const largest)[64] = s_largest[wave];
+    uint16_t* const found = reinterpret_cast<uint16_t*>(largest);   // (after `largest` is used)
+    float most = -INF, sum = 0.0f;
+    Key least = 0;   // the list's last
+    for (int group = first; group < last; group += GROUP * TILE) {
+        const int end = min(group + GROUP * TILE, last);
+        float lane_best = -INF;
+        int count = 0;   // of tiles
+        for (int base = group; base < end; base += TILE, count++) {
+            float v[PER];
 #pragma unroll
             for (int j = 0; j < PER; j++)
                 v[j] = value_at<FMT>(&raw[j / VEC], j % VEC);
-        } else {
+            if (base + TILE < last)
+                request(base + TILE);
+            if (base + TILE > a.vocab) {
 #pragma unroll
-            for (int j = 0; j < PER; j++)
-                v[j] = value_at<FMT>(x, min(base + lane + 64 * j, last - 1));
+                for (int j = 0; j < PER; j++) {
+                    const int at = base + VEC * (lane + 64 * (j / VEC));
+                    v[j] = min(at, last_word) + j % VEC >= at ? v[j] : -INF;
+                }
+            }
+            float best[LOADS];
 #pragma unroll
-            for (int j = 0; j < PER; j++)
-                v[j] = base + lane + 64 * j < last ? v[j] : -INF;
+            for (int j = 0; j < LOADS; j++) {
+                best[j] = v[j * VEC];
+#pragma unroll
+                for (int i = 1; i < VEC; i++)
+                    best[j] = fmaxf(best[j], v[j * VEC + i]);
+                best[j] = fmaxf(best[j], -INF);   // (a word of NaN)
+            }
+            float tile_best = best[0];
+#pragma unroll
+            for (int j = 0; j < LOADS; j += 4)
+                largest[count * (LOADS / 4) + j / 4][lane] = make_float4(best[j], best[j + 1], best[j + 2], best[j + 3]);
+#pragma unroll
+            for (int j = 1; j < LOADS; j++)
+                tile_best = fmaxf(tile_best, best[j]);
+            lane_best = fmaxf(lane_best, tile_best);
+            const float top = fmaxf(rows_max(row_max<16>(tile_best)), most);
+            const float shift = top == -INF ? 0.0f : top;
+            float add = 0.0f, more = 0.0f;
+#pragma unroll
+            for (int j = 0; j < PER; j += 2) {
+                add += __builtin_amdgcn_exp2f((v[j] - shift) * LOG2E);
+                more += __builtin_amdgcn_exp2f((v[j + 1] - shift) * LOG2E);
+            }
+            sum = sum * (most == -INF ? 0.0f : __builtin_amdgcn_exp2f((most - top) * LOG2E)) + (add + more);
+            most = top;
         }
-        float best = -INF;
-#pragma unroll
-        for (int j = 0; j < PER; j += 4)
-            best = fmaxf(best, fmaxf(fmaxf(v[j], v[j + 1]), fmaxf(v[j + 2], v[j + 3])));
-        const float top = fmaxf(rows_max(row_max<16>(best)), most);
-        const float shift = top == -INF ? 0.0f : top;
-        float add = 0.0f, more = 0.0f;
-#pragma unroll
-        for (int j = 0; j < PER; j += 2) {
-            add += __builtin_amdgcn_exp2f((v[j] - shift) * LOG2E);
-            more += __builtin_amdgcn_exp2f((v[j + 1] - shift) * LOG2E);
-        }
-        sum = sum * (most == -INF ? 0.0f : __builtin_amdgcn_exp2f((most - top) * LOG2E)) + (add + more);
-        most = top;
-        // Only values over the list's last so far (one equal to it has a higher token: tiles come in order), and over the groups'
-        // bound, can be among the best k: some dozens of 2048 spread ones, in as many lanes or fewer.  Those
-        // lanes show all their values, and the wave looks at them together.
-        if (__ballot(best > over) == 0)
+        // The words that hold a value over the list's last so far (one equal to it has a higher token: groups come in order)
+        // and over the groups' bound.
+        const float over = least_of(list, k);
+        if (__ballot(lane_best > over) == 0)
             continue;
-        const float bound = group_bound(best, k);
-        const bool shows = best > over && best >= bound;
-        const uint64_t lanes = __ballot(shows);
-        const int shown = __popcll(lanes);
-        if (shown <= SHOWN) {
-            if (shows) {
-                const int at = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32),
-                                                         __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0));
-                s_lane[wave][at] = lane;
+        const float bound = fmaxf(group_bound(lane_best, k), over);
+        uint32_t mine = 0;
+        for (int i = 0; i < count * (LOADS / 4); i++) {
+            const float4 m = largest[i][lane];
+            mine |= ((m.x >= bound ? 1u : 0u) | (m.y >= bound ? 2u : 0u) | (m.z >= bound ? 4u : 0u) | (m.w >= bound ? 8u : 0u)) << 4 * i;
+        }
+        wave_sync();
+        int at = 0, words = 0;   // found in lanes before, and in all
+        const int own = __popc(mine);
 #pragma unroll
-                for (int j = 0; j < PER; j += 4)
-                    s_shown[wave][at][j / 4] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        for (int bit = 0; bit < 5; bit++) {   // (at most LARGEST)
+            const uint64_t lanes = __ballot(own >> bit & 1);
+            at += __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32),
+                                            __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0)) << bit;
+            words += __popcll(lanes) << bit;
+        }
+        while (mine != 0) {
+            found[at++] = static_cast<uint16_t>(__builtin_ctz(mine) << 6 | lane);
+            mine &= mine - 1;
+        }
+        wave_sync();
+        int held = 0;
+        auto key_of = [&](float v, int token) { return static_cast<Key>(order_of(v)) << 32 | (0xffffffffu - static_cast<uint32_t>(token)); };
+        for (int base = 0; base < words; base += 64) {
+            const int which = found[min(base + lane, words - 1)], i = which >> 6;
+            const int from = group + i / LOADS * TILE + VEC * ((which & 63) + 64 * (i % LOADS)), start = min(from, last_word);
+            const Sixteen got = word(from);
+            const bool in = base + lane < words;
+            int more = held;
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const float v = value_at<FMT>(&got, j);
+                more = append(in && v >= bound && v > -INF && start + j >= from, [&] { return key_of(v, start + j); }, more, kept);
             }
-            wave_sync();
-            int count = pending;
-            constexpr int TURN = 4;   // values a lane at a time
-            for (int i = 0; i < shown * PER; i += 64 * TURN) {
-                float x[TURN];
-#pragma unroll
-                for (int m = 0; m < TURN; m++)   // (rows behind the shown ones: whatever they hold is passed over)
-                    x[m] = reinterpret_cast<const float*>(s_shown[wave])[min(i + 64 * m, (SHOWN - 2) * PER) + lane];
-#pragma unroll
-                for (int m = 0; m < TURN; m++) {
-                    const int at = (i + 64 * m + lane) / PER, j = (i + 64 * m + lane) % PER;
-                    count = append(at < shown && x[m] > over && x[m] >= bound, [&] { return key_of(x[m], s_lane[wave][at], j); },
-                                   count, kept);
-                }
-            }
-            if (count <= KEPT) {
-                pending = count;
-                if (over == -INF || pending > 64) {
-                    rank_kept(pending, k, kept, list);
-                    over = least_of(list, k);
-                    pending = 0;
-                }
+            if (more <= KEPT) {
+                held = more;
                 continue;
             }
-            // (more than there is room for: the kept ones of earlier tiles are in place, this tile's go a few at a time)
+            // more than there is room for: what was kept before these words is in place, these go a value a lane at a time
+            for (int j = 0; j < VEC; j++) {
+                if (held > KEPT - 64) {
+                    rank_kept(held, k, kept, list);
+                    held = 0;
+                    least = list[k - 1];
+                }
+                const float v = value_at<FMT>(x, max(start + j, 0));
+                const Key key = key_of(v, start + j);
+                held = append(in && v >= bound && v > -INF && start + j >= from && key > least, [&] { return key; }, held, kept);
+            }
         }
-        if (pending > 0)
-            rank_kept(pending, k, kept, list);
-        pending = 0;
-        merge_tile<PER>(v, bound, [&](int j) { return key_of(v[j], lane, j); }, k, kept, list);
-        over = least_of(list, k);
+        if (held > 0)
+            rank_kept(held, k, kept, list);
+        least = list[k - 1];
     }
-    if (pending > 0)
-        rank_kept(pending, k, kept, list);
     sum = rows_sum(row_sum<16>(sum));
     if (lane == 0)
         part[unit] = {most, sum};
@@ -297,25 +332,56 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
         keys[unit * k + lane] = list[lane];
 }
 
-// One workgroup a sequence: each wave joins rows' parts, then all candidates of the rows are
-// ranked by score.  A chain of round trips: what does not hang on another load is requested first.
+// One workgroup a sequence.  Half of the waves merge their rows' parts' lists, the other half sum their rows; then all candidates
+// of the rows are ranked by score, each wave counting the larger ones among its share of them.  A chain of round trips, bound by
+// their latency: what does not hang on another load is requested first (24 sequences of 8 beams 6.2 us, one of 4 beams 4.6;
+// with sums and lists one after the other and each candidate's rank in one thread 8.1 and 5.2).
 __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a, int parts, const Part* part, const Key* keys)
 {
-    constexpr int LANE_KEYS = 8;
-    __shared__ Key s_kept[MERGE_WAVES][ROOM];
+    constexpr int LANE_KEYS = 8, HALF = MERGE_WAVES / 2;
+    __shared__ Key s_kept[HALF][ROOM];
     __shared__ Key s_list[BEAMS_MAX][CANDIDATES_MAX];
-    __shared__ double s_score[BEAMS_MAX * CANDIDATES_MAX];
-    __shared__ int s_parent[CANDIDATES_MAX], s_slot[BEAMS_MAX], s_count;
+    __shared__ double s_log[BEAMS_MAX], s_score[BEAMS_MAX * CANDIDATES_MAX];
+    __shared__ float s_most[BEAMS_MAX];
+    __shared__ int s_rank[BEAMS_MAX * CANDIDATES_MAX], s_parent[CANDIDATES_MAX];
+    __shared__ int s_slot[BEAMS_MAX], s_child[BEAMS_MAX], s_free[BEAMS_MAX], s_count;
     const int s = blockIdx.x, t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int k = a.candidates, beams = a.beams;
-    if (t == 0)
-        s_count = 0;
-    if (t < beams)
-        s_slot[t] = a.slots ? a.slots[static_cast<int64_t>(s) * beams + t] : 0;
-    for (int b = wave; b < beams; b += MERGE_WAVES) {
-        const int64_t row = static_cast<int64_t>(s) * beams + b;
-        const Part* const mine = part + row * parts;
+    const int k = a.candidates, beams = a.beams, all = beams * k;
+    const int64_t first_row = static_cast<int64_t>(s) * beams;
+    // thread t's candidate: t - b k of beam b
+    const int beam = t < all ? t / k : 0;
+    const double given = a.scores[first_row + beam];
+    const bool ended = a.done && a.done[first_row + beam] != 0;
+    const int slot = a.slots && t < beams ? a.slots[first_row + t] : 0;
+    for (int b = wave % HALF; b < beams; b += HALF) {
+        const int64_t row = first_row + b;
+        const bool row_ended = a.done && a.done[row] != 0;
+        if (wave >= HALF) {
+            const Part* const mine = part + row * parts;
+            Part held = mine[min(lane, parts - 1)];
+            if (row_ended)
+                continue;
+            if (lane >= parts)
+                held = {-INF, 0.0f};
+            float most = held.most;
+            for (int i = lane + 64; i < parts; i += 64)
+                most = fmaxf(most, mine[i].most);
+            most = rows_max(row_max<16>(most));
+            // (a part without a finite logit has the sum 0, or NaN)
+            auto scaled = [&](Part q) {
+                return static_cast<double>(q.sum) * (q.most == -INF ? 1.0f : __builtin_amdgcn_exp2f((q.most - most) * LOG2E));
+            };
+            double sum = scaled(held);
+            for (int i = lane + 64; i < parts; i += 64)
+                sum += scaled(mine[i]);
+            const double log_sum = log(wave_sum(sum));
+            if (lane == 0) {
+                s_most[b] = most;
+                s_log[b] = log_sum;
+            }
+            continue;
+        }
         const Key* const from = keys + row * parts * k;
         const int total = parts * k;
         Key key[LANE_KEYS];
@@ -324,36 +390,12 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
             for (int j = 0; j < LANE_KEYS; j++)
                 key[j] = from[min(base + 64 * j + lane, total - 1)];
         };
-        const double given = a.scores[row];
-        const bool ended = a.done && a.done[row] != 0;
-        Part held = mine[min(lane, parts - 1)];
         request(0);
         Key* const list = s_list[b];
         if (lane < CANDIDATES_MAX)
-            list[lane] = 0;
+            list[lane] = row_ended && lane == 0 ? 0xffffffffu - static_cast<uint32_t>(a.end_token) : 0;
         wave_sync();
-        if (ended) {
-            if (lane < k)
-                s_score[b * k + lane] = lane == 0 ? given : -__builtin_inf();
-            if (lane == 0)
-                list[0] = 0xffffffffu - static_cast<uint32_t>(a.end_token);
-            continue;
-        }
-        if (lane >= parts)
-            held = {-INF, 0.0f};
-        float most = held.most;
-        for (int i = lane + 64; i < parts; i += 64)
-            most = fmaxf(most, mine[i].most);
-        most = rows_max(row_max<16>(most));
-        // (a part without a finite logit has the sum 0, or NaN)
-        auto scaled = [&](Part q) {
-            return static_cast<double>(q.sum) * (q.most == -INF ? 1.0f : __builtin_amdgcn_exp2f((q.most - most) * LOG2E));
-        };
-        double sum = scaled(held);
-        for (int i = lane + 64; i < parts; i += 64)
-            sum += scaled(mine[i]);
-        const double log_sum = log(wave_sum(sum));
-        for (int base = 0; base < total; base += 64 * LANE_KEYS) {
+        for (int base = 0; base < total && !row_ended; base += 64 * LANE_KEYS) {
             if (base > 0)
                 request(base);
             float v[LANE_KEYS], best = -INF;
@@ -363,43 +405,64 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
                 v[j] = order == 0 ? -INF : logit_of(order);
                 best = fmaxf(best, v[j]);
             }
-            merge_tile<LANE_KEYS>(v, group_bound(best, k), [&](int j) { return key[j]; }, k, s_kept[wave], list);
+            const float bound = fmaxf(group_bound(best, k), least_of(list, k));
+            int count = 0;
+#pragma unroll
+            for (int j = 0; j < LANE_KEYS; j++)
+                count = append(v[j] >= bound && v[j] > -INF, [&] { return key[j]; }, count, s_kept[wave]);
+            if (count <= KEPT)
+                rank_kept(count, k, s_kept[wave], list);
+            else
+                merge_tile<LANE_KEYS>(v, bound, [&](int j) { return key[j]; }, k, s_kept[wave], list);
         }
-        if (lane < k) {
-            const Key got = list[lane];
-            const double x = static_cast<double>(logit_of(static_cast<uint32_t>(got >> 32)));
-            const double score = given + ((x - static_cast<double>(most)) - log_sum);
-            s_score[b * k + lane] = got != 0 && fabs(score) < __builtin_inf() ? score : -__builtin_inf();
+    }
+    if (t < beams) {
+        s_slot[t] = slot;
+        s_child[t] = BEAMS_MAX;
+    }
+    if (t == 0)
+        s_count = 0;
+    __syncthreads();
+    const Key got = t < all ? s_list[beam][t - beam * k] : 0;
+    const double x = static_cast<double>(logit_of(static_cast<uint32_t>(got >> 32)));
+    double score = given + ((x - static_cast<double>(s_most[beam])) - s_log[beam]);
+    if (ended)
+        score = t == beam * k ? given : -__builtin_inf();
+    const bool counts = got != 0 && fabs(score) < __builtin_inf();
+    if (t < all) {
+        s_score[t] = counts ? score : -__builtin_inf();
+        s_rank[t] = 0;
+    }
+    const uint64_t counted = __ballot(counts);
+    if (lane == 0 && counted != 0)
+        atomicAdd(&s_count, __popcll(counted));
+    __syncthreads();
+    const int share = (all + MERGE_WAVES - 1) / MERGE_WAVES, last = min((wave + 1) * share, all);
+    for (int i = lane; i < all; i += 64) {
+        const double mine = s_score[i];
+        int larger = 0;
+#pragma unroll 4
+        for (int j = wave * share; j < last; j++) {
+            const double other = s_score[j];
+            larger += other > mine || (other == mine && j < i);
         }
+        if (larger != 0)
+            atomicAdd(&s_rank[i], larger);
     }
     __syncthreads();
     const int64_t out = static_cast<int64_t>(s) * k;
-    const int i = t;   // at most 16 * 32 candidates
-    if (i < beams * k) {
-        const double mine = s_score[i];
-        if (fabs(mine) < __builtin_inf()) {
-            int rank = 0;
-#pragma unroll 8
-            for (int j = 0; j < beams * k; j++) {
-                const double other = s_score[j];
-                rank += other > mine || (other == mine && j < i);
-            }
-            atomicAdd(&s_count, 1);
-            if (rank < k) {
-                const int b = i / k;
-                const int token = static_cast<int>(0xffffffffu - static_cast<uint32_t>(s_list[b][i - b * k]));
-                a.parents[out + rank] = b;
-                a.tokens[out + rank] = token;
-                a.new_scores[out + rank] = static_cast<float>(mine);
-                if (a.new_done)
-                    a.new_done[out + rank] = token == a.end_token;
-                s_parent[rank] = b;
-            }
-        }
+    if (counts && s_rank[t] < k) {
+        const int rank = s_rank[t], token = static_cast<int>(0xffffffffu - static_cast<uint32_t>(got));
+        a.parents[out + rank] = beam;
+        a.tokens[out + rank] = token;
+        a.new_scores[out + rank] = static_cast<float>(score);
+        if (a.new_done)
+            a.new_done[out + rank] = token == a.end_token;
+        s_parent[rank] = beam;
+        if (a.slots)
+            atomicMin(&s_child[beam], rank);
     }
-    __syncthreads();
-    const int count = min(s_count, k);
-    if (t >= count && t < k) {
+    if (t >= s_count && t < k) {
         a.parents[out + t] = -1;
         a.tokens[out + t] = -1;
         a.new_scores[out + t] = -INF;
@@ -412,33 +475,18 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
     __syncthreads();
     if (t >= 64)
         return;
-    // candidates = beams, one a lane
-    const int parent = t < beams ? s_parent[t] : -1, own = t < beams ? s_slot[t] : 0;
-    uint32_t childless = 0;
-    bool keeps = false;
-    for (int b = 0; b < beams; b++) {
-        const uint64_t children = __ballot(parent == b);
-        if (children == 0)
-            childless |= 1u << b;
-        else
-            keeps = keeps || t == __builtin_ctzll(children);
-    }
-    const uint64_t take_over = __ballot(t < beams && !keeps);
-    const int turn = __popcll(take_over & ((1ull << t) - 1));   // of the candidates that take over a slot
-    int slot = 0, source = -1, free = 0;
-    for (int b = 0; b < beams; b++) {
-        const int of_b = __builtin_amdgcn_readlane(own, b);
-        if (parent == b)
-            source = of_b;
-        if (childless >> b & 1) {
-            if (free == turn)
-                slot = of_b;
-            free++;
-        }
-    }
+    // candidates = beams, one a lane: a parent's first child keeps its slot, the others take those of beams without children in turn
+    const int parent = t < beams ? s_parent[t] : -1;
+    const bool keeps = parent >= 0 && s_child[parent] == t;
+    const uint64_t before = (1ull << t) - 1;
+    const uint64_t take_over = __ballot(t < beams && !keeps), childless = __ballot(t < beams && s_child[t] == BEAMS_MAX);
+    if (childless >> t & 1)
+        s_free[__popcll(childless & before)] = slot;
+    wave_sync();
     if (t < beams) {
+        const int source = parent >= 0 ? s_slot[parent] : -1;
         a.from[out + t] = source;
-        a.to[out + t] = keeps ? source : slot;
+        a.to[out + t] = keeps ? source : s_free[__popcll(take_over & before)];
     }
 }
 

@@ -393,6 +393,15 @@ def test_beam_select_many_rows(hip):
         _check_beams(hip, logits, -2 * rng.random(320), None, rng.permutation(320) if k == 8 else None, 8, k, native.F32)
 
 
+def test_beam_select_parts_of_many_tiles(hip):
+    """A wave's part in more tiles than it looks at together; rows among them that rise, and rows of few different values."""
+    rng = np.random.default_rng(5)
+    logits = rng.standard_normal((3104, 9000), dtype=np.float32)
+    logits[::7].sort(axis=1)
+    logits[3::7] = np.round(logits[3::7])
+    _check_beams(hip, logits, -2 * rng.random(3104), None, rng.permutation(3104), 16, 16, native.F32)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_beam_select_ties(hip, fmt):
     """Equal logits, equal beams, zeros of both signs: the lowest first; more equal values than are ranked together."""
