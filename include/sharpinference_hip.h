@@ -678,11 +678,14 @@ typedef struct si_hip_rwkv7_wkv_rows_args {
     int32_t output_format;     /* SI_HIP_F32, SI_HIP_F16 or SI_HIP_BF16 */
 } si_hip_rwkv7_wkv_rows_args;
 
+/* Whatever the batch: about 32 MiB. */
 int si_hip_rwkv7_wkv_rows_workspace_bytes(int heads, uint64_t* bytes);
 
 /* si_hip_rwkv7_wkv (its formulas, in FP32) for every row of the batch, row after row of
  * each sequence through the sequence's state; output rounded once.  [rows] arrays, state and
  * workspace 16-byte aligned.  A value that is not finite changes nothing of rows before its own.
+ * Rows are taken in blocks and long sequences in stretches at once, which the whole batch decides: the same batch
+ * gives the same bits, but beside other sequences a row or a state may differ in its last ones.
  * Replaces: the WKV node chain (PortableRwkv7GraphProvider.cs:224-276), run token after
  * token there. */
 int si_hip_rwkv7_wkv_rows(si_hip_context* ctx, const si_hip_rwkv7_wkv_rows_args* args);

@@ -715,9 +715,12 @@ __device__ __forceinline__ StateEnds state_ends(const WkvRowsArgs& a, int s, int
 }
 
 // One head of one sequence or stretch, block after block.  While the state's waves take block i
-// (64 matrix instructions each), the others prepare block i + 1 (32 each, and the
-// exponentials), in three phases between barriers.  FP32 matrix instructions take the vector units' place (32 and 5 cycles side by
-// side on a SIMD take 50 in all): a block costs 3072 cycles of them and about 800 vector instructions a SIMD.
+// (72 matrix instructions each), the others prepare block i + 1 (20 each, and the
+// exponentials), in three phases between barriers.  Bound by the SIMDs: FP32 matrix instructions take 32 cycles each in the vector
+// units' place, so that a block costs a SIMD 92 * 32 = 2944 cycles of them and about 800 vector instructions, 5100 to 5500 cycles
+// in all; two workgroups a compute unit fill one another's barriers (three groups of waves in one, or two that prepare, were
+// faster alone, 7000 and 7700 cycles a block for 8900, and slower together, 1560 and 1580 us for 1024 heads of equal length, 1370).
+// Eight sequences of 1000 rows, 32 heads, one workgroup a compute unit: 234 us.
 enum ChunkPass { CHUNK_SEQUENCES, CHUNK_STRETCHES, CHUNK_TRANSFERS };
 
 template <int PASS>
@@ -759,7 +762,7 @@ __global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs
     const Blocks blocks{span.first, span.last, span.first};
     if (threadIdx.x >= CHUNK_THREADS / 2)
         chunk_prepare<PASS == CHUNK_TRANSFERS>(a, lds, h, blocks);
-    else if (PASS == CHUNK_TRANSFERS)
+    else if constexpr (PASS == CHUNK_TRANSFERS)
         chunk_transfer(lds, record, blocks);
     else
         chunk_advance(a, lds, h, ends, blocks);
@@ -767,7 +770,8 @@ __global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs
 
 // The states between a cut sequence's stretches.  A workgroup takes 16 values of one head, each of its waves 16 keys:
 // a stretch costs it 16 matrix instructions a wave, an exchange of the state's tiles through LDS, and 4 KiB of M a wave,
-// requested AHEAD stretches before (their round trip takes longer than the products: 0.5 us a stretch, one ahead 1.2).
+// requested AHEAD stretches before (their round trip takes longer than the products: one ahead 1.2 us a stretch).  Bound by the chain of
+// stretches: 0.46 us each, of which the matrix instructions are 0.25 (16 stretches of 32 heads 13 us, 42 of 12 heads 25).
 __global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, const Plan* plan, int room, float* records)
 {
     constexpr int AHEAD = 4;
@@ -794,26 +798,32 @@ __global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, const Plan
     for (int k = 0; k < AHEAD; k++)
         load(k, m[k], add[k]);
     *tile_of(steps) = w == 0 ? S[0] : w == 1 ? S[1] : w == 2 ? S[2] : S[3];
-    for (int base = 0; base < steps; base += AHEAD) {
+    auto step = [&](int at, int k, bool more) {
+        f4 other = {0.0f, 0.0f, 0.0f, 0.0f}, sum = add[k];
+        sum = mfma4(m[k][0], S[0], sum);
+        other = mfma4(m[k][1], S[1], other);
+        sum = mfma4(m[k][2], S[2], sum);
+        other = mfma4(m[k][3], S[3], other);
+        sum += other;
+        if (more)
+            load(at + AHEAD, m[k], add[k]);
+        *tile_of(at) = sum;   // the next stretch's start, in N's place
+        s_tile[k & 1][w][lane] = sum;
+        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < AHEAD; k++) {
-            if (base + k >= steps)
-                break;
-            f4 other = {0.0f, 0.0f, 0.0f, 0.0f}, sum = add[k];
-            sum = mfma4(m[k][0], S[0], sum);
-            other = mfma4(m[k][1], S[1], other);
-            sum = mfma4(m[k][2], S[2], sum);
-            other = mfma4(m[k][3], S[3], other);
-            sum += other;
-            load(base + k + AHEAD, m[k], add[k]);
-            *tile_of(base + k) = sum;   // the next stretch's start, in N's place
-            s_tile[k & 1][w][lane] = sum;
-            __syncthreads();
+        for (int j = 0; j < 4; j++)
+            S[j] = s_tile[k & 1][j][lane];
+    };
+    // (no way out of the loop's middle: it would lead past its head, which then waits for every load)
+    int base = 0;
+    for (; base + AHEAD <= steps; base += AHEAD)
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                S[j] = s_tile[k & 1][j][lane];
-        }
-    }
+        for (int k = 0; k < AHEAD; k++)
+            step(base + k, k, true);
+#pragma unroll
+    for (int k = 0; k < AHEAD - 1; k++)
+        if (base + k < steps)
+            step(base + k, k, false);
 }
 
 // Rows of a stretch where so many rows are cut: the card's workgroups share them with their heads; where that gives each more
