@@ -528,6 +528,7 @@ struct StateEnds {
     const float* from; // [64][64], or null: all `fill`
     float fill;
     float* to;         // [64][64], or null
+    f4* end;           // tiles as in start, or null
 };
 
 __device__ __forceinline__ void load_state(const StateEnds& ends, int w, f4 (&S)[4])
@@ -617,6 +618,11 @@ __device__ void chunk_advance(const WkvRowsArgs& a, ChunkLds& lds, int h, const 
         for (int j = 0; j < 4; j++)
             *reinterpret_cast<f4*>(ends.to + (16 * w + t) * N + 16 * j + 4 * g) = S[j];
     }
+    if (ends.end) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            ends.end[(4 * w + j) * 64 + lane] = S[j];
+    }
 }
 
 // A stretch's transfer: the state behind it is S M + (S's start at zero), and M's rows are 64 more states that start as
@@ -685,13 +691,14 @@ __device__ void chunk_transfer(ChunkLds& lds, float* record, Blocks blocks)
 
 // ---- long sequences in stretches ---------------------------------------------------------------
 //
-// Where the heads of all sequences are too few for the card, long sequences are cut: (1) each stretch's transfer
-// (M, N), all stretches at once; (2) the states between them, S_(i+1) = S_i M_i + N_i; (3) every stretch as a
-// sequence of its own.  (1) costs about 0.8 of (3).
+// Where the heads of all sequences are too few for the card, long sequences are cut: (1) each first stretch as a
+// sequence of its own, beside the transfers (M, N) of the others but the last; (2) the states between them,
+// S_(i+1) = S_i M_i + N_i; (3) every other stretch, from its state on, beside the sequences that are whole.  A transfer costs
+// 0.95 of its stretch.
 
-constexpr int RECORD = 2 * N * N;        // floats of a stretch and head: M^T; N, later the next stretch's start
+constexpr int RECORD = 2 * N * N;        // floats of a stretch and head: M^T; N (the first's: its state), then the next stretch's start
 constexpr int CARD = 512;                // workgroups of wkv_chunk_kernel that the card holds: two a compute unit
-constexpr int HEAD_STRETCHES = 2 * CARD; // stretches times heads, at most
+constexpr int HEAD_STRETCHES = 2 * CARD; // stretches (but each sequence's last) times heads, at most
 constexpr int LONG_STRETCH = 256;
 constexpr int LEAST_STRETCH = 64;        // rows
 
@@ -711,7 +718,7 @@ __device__ __forceinline__ StateEnds state_ends(const WkvRowsArgs& a, int s, int
     const int from = a.batch.from[s], to = a.batch.to[s];
     auto at = [&](int slot) { return a.state + (static_cast<int64_t>(slot) * a.heads + h) * N * N; };
     return {nullptr, from >= 0 && from < a.batch.slots ? at(from) : nullptr, from == -1 ? 0.0f : __builtin_nanf(""),
-            to >= 0 && to < a.batch.slots ? at(to) : nullptr};
+            to >= 0 && to < a.batch.slots ? at(to) : nullptr, nullptr};
 }
 
 // One head of one sequence or stretch, block after block.  While the state's waves take block i
@@ -731,6 +738,7 @@ __global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs
     RowSpan span;
     StateEnds ends;
     float* record = nullptr;
+    bool transfer = false;
     if constexpr (PASS == CHUNK_SEQUENCES) {
         span = rows_of(a.batch, s);
         if (span.last - span.first <= over)
@@ -742,17 +750,21 @@ __global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs
         const Stretch part = plan->list[s];
         span = {part.first, part.last};
         auto record_of = [&](int i) { return records + (static_cast<int64_t>(part.record + i) * a.heads + h) * RECORD; };
-        if (PASS == CHUNK_TRANSFERS) {
+        if constexpr (PASS == CHUNK_TRANSFERS) {
             if (part.record < 0 || part.index == part.count - 1)
                 return;
             record = record_of(part.index);
-        } else {
-            ends = state_ends(a, part.sequence, h);
-            if (part.record >= 0) {   // (the first stretch's start lies in the last one's record)
-                ends.start = reinterpret_cast<const f4*>(record_of(part.index ? part.index - 1 : part.count - 1) + N * N);
-                ends.to = part.index == part.count - 1 ? ends.to : nullptr;
-            }
+            transfer = part.index > 0;
+        } else if (part.record >= 0 && part.index == 0) {
+            return;
         }
+        ends = state_ends(a, part.sequence, h);
+        if (part.record >= 0 && part.index > 0)
+            ends.start = reinterpret_cast<const f4*>(record_of(part.index - 1) + N * N);
+        if (part.index < part.count - 1)
+            ends.to = nullptr;
+        if (PASS == CHUNK_TRANSFERS)
+            ends.end = reinterpret_cast<f4*>(record + N * N);
     }
     span.first = __builtin_amdgcn_readfirstlane(span.first);
     span.last = __builtin_amdgcn_readfirstlane(span.last);
@@ -760,10 +772,18 @@ __global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs
         lds.block[threadIdx.x].odd = 0;
     __syncthreads();
     const Blocks blocks{span.first, span.last, span.first};
-    if (threadIdx.x >= CHUNK_THREADS / 2)
-        chunk_prepare<PASS == CHUNK_TRANSFERS>(a, lds, h, blocks);
-    else if constexpr (PASS == CHUNK_TRANSFERS)
-        chunk_transfer(lds, record, blocks);
+    const bool prepares = threadIdx.x >= CHUNK_THREADS / 2;
+    if constexpr (PASS == CHUNK_TRANSFERS) {
+        if (transfer) {
+            if (prepares)
+                chunk_prepare<true>(a, lds, h, blocks);
+            else
+                chunk_transfer(lds, record, blocks);
+            return;
+        }
+    }
+    if (prepares)
+        chunk_prepare<false>(a, lds, h, blocks);
     else
         chunk_advance(a, lds, h, ends, blocks);
 }
@@ -785,19 +805,18 @@ __global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, const Plan
     auto record_of = [&](int k) { return records + (static_cast<int64_t>(part.record + k) * a.heads + h) * RECORD; };
     auto tile_of = [&](int k) { return reinterpret_cast<f4*>(record_of(k) + N * N) + (4 * i + w) * 64 + lane; };
     f4 S[4], m[AHEAD][4], add[AHEAD];
-    const int steps = part.count - 1;
+    const int last = part.count - 2;   // the last one with a record
     auto load = [&](int k, f4(&rows)[4], f4& n) {
-        const int at = min(k, steps - 1);   // (behind the last step: read again, not used)
+        const int at = min(k, last);   // (behind it: read again, not used)
 #pragma unroll
         for (int j = 0; j < 4; j++)
             rows[j] = *reinterpret_cast<const f4*>(record_of(at) + (16 * w + t) * N + 16 * j + 4 * g);
         n = *tile_of(at);
     };
-    load_state(state_ends(a, part.sequence, h), i, S);
+    load_state({reinterpret_cast<const f4*>(record_of(0) + N * N)}, i, S);
 #pragma unroll
     for (int k = 0; k < AHEAD; k++)
-        load(k, m[k], add[k]);
-    *tile_of(steps) = w == 0 ? S[0] : w == 1 ? S[1] : w == 2 ? S[2] : S[3];
+        load(1 + k, m[k], add[k]);
     auto step = [&](int at, int k, bool more) {
         f4 other = {0.0f, 0.0f, 0.0f, 0.0f}, sum = add[k];
         sum = mfma4(m[k][0], S[0], sum);
@@ -815,35 +834,37 @@ __global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, const Plan
             S[j] = s_tile[k & 1][j][lane];
     };
     // (no way out of the loop's middle: it would lead past its head, which then waits for every load)
-    int base = 0;
-    for (; base + AHEAD <= steps; base += AHEAD)
+    int base = 1;
+    for (; base + AHEAD <= last + 1; base += AHEAD)
 #pragma unroll
         for (int k = 0; k < AHEAD; k++)
             step(base + k, k, true);
 #pragma unroll
     for (int k = 0; k < AHEAD - 1; k++)
-        if (base + k < steps)
+        if (base + k <= last)
             step(base + k, k, false);
 }
 
-// Rows of a stretch where so many rows are cut: the card's workgroups share them with their heads; where that gives each more
-// than LONG_STRETCH, twice as many workgroups do, which even out better beside whole sequences (eight prompts of 500 to 3000
-// rows of 32 heads 560 us, by CARD 648; one of 4001 225, by twice CARD 246).
-__host__ __device__ inline int stretch_rows(int64_t rows, int heads)
+// Rows of a stretch where so many rows of so many sequences are cut: the card's workgroups share them with their heads; where that
+// gives each more than LONG_STRETCH, twice as many workgroups do, which even out better beside whole sequences (32 heads; eight
+// prompts of 500 to 3000 rows 526 us, by CARD 603, three of 1000 to 6000 rows 539 and 704; one of 4001 rows, by CARD, 217, by
+// twice as many 245).
+__host__ __device__ inline int stretch_rows(int64_t rows, int heads, int cut)
 {
-    const int64_t each = (rows * heads + CARD - 1) / CARD, half = (each + 1) / 2;
+    const int64_t work = rows * heads, more = static_cast<int64_t>(cut) * heads;   // (of each sequence one stretch is idle in every pass)
+    const int64_t each = (work + CARD + more - 1) / (CARD + more), half = (work + HEAD_STRETCHES + more - 1) / (HEAD_STRETCHES + more);
     const int64_t least = each < LONG_STRETCH ? each : half > LONG_STRETCH ? half : LONG_STRETCH;
     return static_cast<int>((least > LEAST_STRETCH ? least + C - 1 : LEAST_STRETCH) / C * C);
 }
 
 // From how many rows on a launch cuts its sequences, or 0: none.  Cutting costs the transfers and the join, and pays where the
-// longest sequence has 2.5 times the rows that all, shared out evenly, give a workgroup (eight of 1000 rows of 32 heads, at 2:
-// 230 us whole, 342 cut; sixteen of 100 to 3000, at 3.2: 862 and 624), and for the sequences that become three stretches or
-// more (thirty of 16 to 4000: 880 us, from two on 905).
+// longest sequence has 2.5 times the rows that all, shared out evenly, give a workgroup (32 heads; eight of 1000 rows, at 2:
+// 234 us whole, 286 cut; sixteen of 100 to 3000, at 3.2: 860 and 600), and for the sequences that become three stretches or
+// more: two would follow one another.
 int cut_from(const WkvRowsArgs& a)
 {
     const int64_t each = (static_cast<int64_t>(a.batch.rows) * a.heads + CARD - 1) / CARD;
-    const int from = 3 * stretch_rows(a.batch.rows, a.heads);
+    const int from = 3 * stretch_rows(a.batch.rows, a.heads, 0);
     return a.batch.max_rows >= from && 2ll * a.batch.max_rows >= 5 * each ? from : 0;
 }
 
@@ -853,18 +874,19 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Pl
 {
     __shared__ int64_t s_count[256];
     const int t = threadIdx.x;
-    // Rows in all, rows in sequences that are cut, sequences that are not.  Where starts fall, sequences may share rows, and the
+    // Rows in all, rows in sequences that are cut, sequences that are not and that are.  Where starts fall, sequences may share rows, and the
     // list's room is for rows that are one sequence's.
-    float sums[3] = {};   // (exact to 2^24; whether the first passes 2^20: a sum that does cannot round below it)
+    float sums[4] = {};   // (exact to 2^24; whether the first passes 2^20: a sum that does cannot round below it)
     for (int i = t; i < a.batch.sequences; i += 256) {
         const RowSpan span = rows_of(a.batch, i);
         const int rows = span.last - span.first;
         sums[0] += static_cast<float>(rows);
         sums[1] += rows >= from ? static_cast<float>(rows) : 0.0f;
         sums[2] += rows > over && rows < from ? 1.0f : 0.0f;
+        sums[3] += rows >= from ? 1.0f : 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < 3; i++) {
+    for (int i = 0; i < 4; i++) {
         sums[i] = wave_sum(sums[i]);
         if ((t & 63) == 0)
             s_count[4 * i + (t >> 6)] = static_cast<int64_t>(sums[i]);
@@ -872,14 +894,14 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Pl
     __syncthreads();
     auto sum_of = [&](int i) { return s_count[4 * i] + s_count[4 * i + 1] + s_count[4 * i + 2] + s_count[4 * i + 3]; };
     const int64_t rows_in_all = sum_of(0), rows_in_cut = sum_of(1);
-    const int whole = static_cast<int>(sum_of(2));
+    const int whole = static_cast<int>(sum_of(2)), cuts = static_cast<int>(sum_of(3));
     __syncthreads();
     if (rows_in_all > a.batch.rows) {
         if (t == 0)
             plan->stretches = plan->cut = 0;
         return;
     }
-    const int stretch = stretch_rows(rows_in_cut, a.heads);   // at most a third of `from`
+    const int stretch = stretch_rows(rows_in_cut, a.heads, cuts);   // at most a third of `from`
     // whole sequences, cut ones and their stretches in one number, 20 bits each
     int64_t total = 0;
     for (int base = 0; base < a.batch.sequences; base += 256) {
@@ -901,13 +923,14 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Pl
             __syncthreads();
         }
         const int64_t before = total + s_count[t] - own;
-        const int record = static_cast<int>(before >> 40), at = cut ? whole + record : static_cast<int>(before & 0xfffff);
+        const int cut_before = before >> 20 & 0xfffff, parts_before = static_cast<int>(before >> 40);
+        const int record = parts_before - cut_before, at = cut ? whole + parts_before : static_cast<int>(before & 0xfffff);
         for (int k = 0; k < parts; k++) {
             const Stretch part{base + t, span.first + k * each, k + 1 < parts ? span.first + (k + 1) * each : span.last,
                                cut ? record : -1, k, parts};
             plan->list[at + k] = part;
             if (cut && k == 0)
-                plan->list[room + (before >> 20 & 0xfffff)] = part;
+                plan->list[room + cut_before] = part;
         }
         total += s_count[min(255, a.batch.sequences - base - 1)];
         __syncthreads();
@@ -923,8 +946,9 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Pl
 constexpr int FEW_ROWS = 12;             // sequences of up to this many rows go row by row: 12 rows of 8 x 32 heads 10.4 us (by
                                          // blocks 10.9), of 64 x 32 36 (47); 16 rows 12.9 (11.4) and 43 (50)
 
-// The list: every sequence that goes by blocks, at most, the stretches, and the cut sequences again (three stretches each, at least).
-constexpr int64_t PLAN_BYTES = (sizeof(Plan) + (ROW_SEQUENCES_MAX + HEAD_STRETCHES * 4 / 3) * sizeof(Stretch) + 255) / 256 * 256;
+// The list: every sequence that goes by blocks, at most, the stretches, and the cut sequences again (at most half as many as
+// stretches with a record: each has three stretches or more).
+constexpr int64_t PLAN_BYTES = (sizeof(Plan) + (ROW_SEQUENCES_MAX + HEAD_STRETCHES * 2) * sizeof(Stretch) + 255) / 256 * 256;
 
 int64_t wkv_rows_workspace_bytes(int) { return PLAN_BYTES + static_cast<int64_t>(HEAD_STRETCHES) * RECORD * 4; }
 
@@ -947,11 +971,11 @@ hipError_t launch_wkv_rows(const WkvRowsArgs& a, hipStream_t s)
     Plan* const plan = reinterpret_cast<Plan*>(a.workspace);
     float* const records = a.workspace + PLAN_BYTES / 4;
     // What the host knows of the list's length.  Stretches have at least LEAST_STRETCH rows, and
-    // as many as share all cut rows and heads out to HEAD_STRETCHES workgroups.
+    // as many as share all cut rows and heads out to HEAD_STRETCHES workgroups and one more for each sequence and head.
     auto least = [](int x, int y) { return x < y ? x : y; };
     const int whole = least(a.batch.rows / (FEW_ROWS + 1), a.batch.sequences);
-    const int parts = least(a.batch.rows / LEAST_STRETCH, HEAD_STRETCHES / a.heads), room = whole + parts;
-    const int cut = least(a.batch.rows / from, parts / 3);
+    const int records_most = HEAD_STRETCHES / a.heads, cut = least(a.batch.rows / from, records_most / 2);
+    const int room = whole + least(a.batch.rows / LEAST_STRETCH, records_most + cut);
     few(FEW_ROWS, 1, from, room, plan);
     hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_TRANSFERS>, dim3(room * heads), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, plan, records);
     hipLaunchKernelGGL(wkv_join_kernel, dim3(cut * heads * 4), dim3(256), 0, s, a, plan, room, records);
