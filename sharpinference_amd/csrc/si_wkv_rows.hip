@@ -791,7 +791,7 @@ __global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs
 // The states between a cut sequence's stretches.  A workgroup takes 16 values of one head, each of its waves 16 keys:
 // a stretch costs it 16 matrix instructions a wave, an exchange of the state's tiles through LDS, and 4 KiB of M a wave,
 // requested AHEAD stretches before (their round trip takes longer than the products: one ahead 1.2 us a stretch).  Bound by the chain of
-// stretches: 0.46 us each, of which the matrix instructions are 0.25 (16 stretches of 32 heads 13 us, 42 of 12 heads 25).
+// stretches: 0.46 us each, of which the matrix instructions are 0.25 (17 stretches of 32 heads 11 us, 43 of 12 heads 22).
 __global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, const Plan* plan, int room, float* records)
 {
     constexpr int AHEAD = 4;
