@@ -176,6 +176,7 @@ class Rwkv7RowsSession:
     def beam_search(self, prompts: Sequence[Sequence[int]], beams: int, steps: int,
                     end_token: Optional[int] = None) -> List[List[Hypothesis]]:
         """The `beams` best continuations of each prompt by `steps` tokens (fewer behind an end token), best first.
+        The states take slots 0 to len(prompts) * beams - 1.
 
         A token is one replayed plan: the candidates of all beams, the moves of their states, and the step of the tokens they
         chose; only the choices come back."""

@@ -552,7 +552,7 @@ def test_recorded_calls_read_their_arrays_at_each_replay(hip):
 
 
 def test_rows_and_slots_far_into_their_arrays(hip):
-    """Rows, slots and logits more than 4 GiB into their buffers."""
+    """Rows and slots more than 4 GiB into their buffers, logits more than 2."""
     rng = np.random.default_rng(13)
     # 540000 rows of 32 heads: 4.4 GB an array; only the last 43 are sequences' rows, and slot 8600 is 4.5 GB into the states
     heads, rows, slots, tail = 32, 540000, 8601, 43
