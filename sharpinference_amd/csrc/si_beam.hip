@@ -17,13 +17,15 @@ constexpr float LOG2E = 1.44269504088896f;
 constexpr int TILE = 2048, PER = TILE / 64;   // values of a wave's tile, and of a lane's
 constexpr int KEPT = 256;                     // values that are ranked together
 constexpr int ROOM = KEPT + CANDIDATES_MAX + 8;
+constexpr int HALVES = 5;                     // of the way from a bound to the largest value
 constexpr int LARGEST = 24;                   // a lane's 16-byte words of a group of tiles, whose largest values are held
-constexpr int SCAN_WAVES = 4, MERGE_WAVES = 16;
+constexpr int SCAN_WAVES = 4, MERGE_WAVES = BEAMS_MAX;
 constexpr float INF = __builtin_inff();
 
 typedef uint32_t Sixteen __attribute__((ext_vector_type(4), aligned(1)));   // bytes at any address, in one load or store
 
 typedef unsigned long long Key;   // order of a logit (high word: 0 for none) and of its token, lowest last
+typedef Key KeyPair __attribute__((ext_vector_type(2)));
 
 // Order of a logit: larger for larger values, 0 for -infinity and NaN; -0 as 0.
 __device__ __forceinline__ uint32_t order_of(float v)
@@ -46,6 +48,24 @@ __device__ __forceinline__ float group_bound(float best, int k)
     return -rows_max(row_max<16>(-best));
 }
 
+// A value that k lanes' largest ones or more reach, near the k-th of them: the groups' bound, raised by halves of what lies
+// between it and the largest.  The groups' alone lets k H_k values through (54 of 2048 spread ones for k = 16), this one few more
+// than k: 8 sequences of 16 beams over 151936 values 27 us where that one takes 49, 2 of 9 beams and 18 candidates 15 and 36.
+__device__ __forceinline__ float near_kth(float best, int k)
+{
+    float low = group_bound(best, k), high = rows_max(row_max<16>(best));
+    if (low == -INF && __popcll(__ballot(best > -INF)) >= k)   // (a group without a value, but lanes enough)
+        low = -rows_max(row_max<16>(best > -INF ? -best : -INF));
+#pragma unroll
+    for (int i = 0; i < HALVES; i++) {
+        const float middle = 0.5f * low + 0.5f * high;
+        const bool reached = __popcll(__ballot(best >= middle)) >= k;
+        low = reached ? middle : low;
+        high = reached ? high : middle;
+    }
+    return low;
+}
+
 // Puts `count` kept keys and the list's own (k of them, sorted, 0 for none) in order: a key's place is the number of larger ones.
 __device__ __forceinline__ void rank_kept(int count, int k, Key* kept, Key* list)
 {
@@ -61,13 +81,13 @@ __device__ __forceinline__ void rank_kept(int count, int k, Key* kept, Key* list
         const Key mine = kept[i];
         int rank = 0;
         for (int j = 0; j < count; j += 8) {   // eight at a time: a chain of LDS reads else
-            Key other[8];
+            KeyPair other[4];
 #pragma unroll
-            for (int m = 0; m < 8; m++)
-                other[m] = kept[j + m];
+            for (int m = 0; m < 4; m++)
+                other[m] = *reinterpret_cast<const KeyPair*>(kept + j + 2 * m);
 #pragma unroll
-            for (int m = 0; m < 8; m++)
-                rank += other[m] > mine;
+            for (int m = 0; m < 4; m++)
+                rank += (other[m][0] > mine) + (other[m][1] > mine);
         }
         if (rank < k)
             list[rank] = mine;
@@ -141,7 +161,8 @@ __device__ __forceinline__ double wave_sum(double v)
 
 // How a row is cut: tiles a part, parts a row.  A wave takes a part; where there are
 // more tiles than the card holds waves of this kernel, it takes several one after another (192 rows of 98 tiles, with the merge:
-// five a wave 26 us, ten 27, three 25 to 27, one 35).
+// five a wave 26 us, ten 27, three 25 to 27, one 35).  Larger parts for fewer keys to merge do not pay (a sequence of 16 beams and 32
+// candidates: 98 parts 29 us, 25 or 49 42 to 43).
 struct Cut {
     int tiles, parts;
 };
@@ -170,14 +191,15 @@ __device__ __forceinline__ float value_at(const void* p, int64_t i)
 }
 
 // One wave a part of a row.  Over a group of tiles it takes the sum and each 16-byte word's largest value; then it reads the
-// words again that may hold one of the best (some dozens, by the groups' bound), and ranks those values together: ranked tile by tile
+// words again that may hold one of the best (few more than those), and ranks those values together: ranked tile by tile
 // out of registers, that part took as long as the rest.  Bound by HBM, then by the tail of ranking and launch: 24 sequences of 8 beams over
-// 200064 16-bit logits, 65 MB of them read, 20 us, 3.2 TB/s (17 without ranking; tile by tile 28).  One sequence of 4 beams over
-// 65536 FP32 logits: 5.2 us, the launch and one chain of round trips.
+// 200064 16-bit logits, 65 MB of them read, 18.5 us, 3.5 TB/s (17 without ranking; tile by tile 28).  One sequence of 4 beams over
+// 65536 FP32 logits: 5.1 us, the launch and one chain of round trips.
 template <int FMT>
 __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs a, int rows, int tiles, int parts, Part* part, Key* keys)
 {
-    __shared__ Key s_kept[SCAN_WAVES][ROOM], s_list[SCAN_WAVES][CANDIDATES_MAX];
+    alignas(16) __shared__ Key s_kept[SCAN_WAVES][ROOM];
+    __shared__ Key s_list[SCAN_WAVES][CANDIDATES_MAX];
     __shared__ float4 s_largest[SCAN_WAVES][LARGEST / 4][64];
     constexpr int SIZE = FMT == ROWS_OUT_F32 ? 4 : 2, VEC = 16 / SIZE, LOADS = PER / VEC, GROUP = LARGEST / LOADS;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -271,7 +293,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
         const float over = least_of(list, k);
         if (__ballot(lane_best > over) == 0)
             continue;
-        const float bound = fmaxf(group_bound(lane_best, k), over);
+        const float bound = fmaxf(near_kth(lane_best, k), over);
         uint32_t mine = 0;
         for (int i = 0; i < count * (LOADS / 4); i++) {
             const float4 m = largest[i][lane];
@@ -332,19 +354,19 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
         keys[unit * k + lane] = list[lane];
 }
 
-// One workgroup a sequence.  Half of the waves merge their rows' parts' lists, the other half sum their rows; then all candidates
-// of the rows are ranked by score, each wave counting the larger ones among its share of them.  A chain of round trips, bound by
-// their latency: what does not hang on another load is requested first (24 sequences of 8 beams 6.2 us, one of 4 beams 4.6;
-// with sums and lists one after the other and each candidate's rank in one thread 8.1 and 5.2).
+// One workgroup a sequence.  Wave b merges the lists of row b's parts, wave 15 - b sums the row; then all candidates
+// of the rows are ranked by score.  A chain of round trips, bound by their latency, with many beams by the 16 waves' instructions
+// on one compute unit: what does not hang on another load is requested first, and only keys and candidates that near_kth lets through
+// are ranked (24 sequences of 8 beams 6.1 us, one of 4 beams 4.7, 3 of 16 beams over one part a row 7.0, of one part's list and
+// every candidate against every other 11.5; 98 parts of 32 candidates 21.5, each 512 keys ranked by themselves 55).
 __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a, int parts, const Part* part, const Key* keys)
 {
-    constexpr int LANE_KEYS = 8, HALF = MERGE_WAVES / 2;
-    __shared__ Key s_kept[HALF][ROOM];
+    constexpr int LANE_KEYS = 8;
+    alignas(16) __shared__ Key s_kept[MERGE_WAVES][ROOM];
     __shared__ Key s_list[BEAMS_MAX][CANDIDATES_MAX];
-    __shared__ double s_log[BEAMS_MAX], s_score[BEAMS_MAX * CANDIDATES_MAX];
+    __shared__ double s_log[BEAMS_MAX], s_score[BEAMS_MAX * CANDIDATES_MAX], s_top_score[BEAMS_MAX * CANDIDATES_MAX];
     __shared__ float s_most[BEAMS_MAX];
-    __shared__ int s_rank[BEAMS_MAX * CANDIDATES_MAX], s_parent[CANDIDATES_MAX];
-    __shared__ int s_slot[BEAMS_MAX], s_child[BEAMS_MAX], s_free[BEAMS_MAX], s_count;
+    __shared__ int s_top[BEAMS_MAX * CANDIDATES_MAX], s_parent[CANDIDATES_MAX], s_slot[BEAMS_MAX], s_free[BEAMS_MAX];
     const int s = blockIdx.x, t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int k = a.candidates, beams = a.beams, all = beams * k;
@@ -354,48 +376,60 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
     const double given = a.scores[first_row + beam];
     const bool ended = a.done && a.done[first_row + beam] != 0;
     const int slot = a.slots && t < beams ? a.slots[first_row + t] : 0;
-    for (int b = wave % HALF; b < beams; b += HALF) {
-        const int64_t row = first_row + b;
-        const bool row_ended = a.done && a.done[row] != 0;
-        if (wave >= HALF) {
-            const Part* const mine = part + row * parts;
-            Part held = mine[min(lane, parts - 1)];
-            if (row_ended)
-                continue;
-            if (lane >= parts)
-                held = {-INF, 0.0f};
-            float most = held.most;
-            for (int i = lane + 64; i < parts; i += 64)
-                most = fmaxf(most, mine[i].most);
-            most = rows_max(row_max<16>(most));
-            // (a part without a finite logit has the sum 0, or NaN)
-            auto scaled = [&](Part q) {
-                return static_cast<double>(q.sum) * (q.most == -INF ? 1.0f : __builtin_amdgcn_exp2f((q.most - most) * LOG2E));
-            };
-            double sum = scaled(held);
-            for (int i = lane + 64; i < parts; i += 64)
-                sum += scaled(mine[i]);
-            const double log_sum = log(wave_sum(sum));
-            if (lane == 0) {
-                s_most[b] = most;
-                s_log[b] = log_sum;
-            }
-            continue;
-        }
-        const Key* const from = keys + row * parts * k;
-        const int total = parts * k;
-        Key key[LANE_KEYS];
-        auto request = [&](int base) {
+    // a beam's keys, requested; the sum of another's row; the keys' list
+    auto ended_at = [&](int b) { return a.done && a.done[first_row + b] != 0; };
+    const int own = wave < beams ? wave : 0, total = parts * k;
+    const Key* const from = keys + (first_row + own) * total;
+    const bool own_ended = ended_at(own);
+    Key key[LANE_KEYS];
+    auto request = [&](int base) {
 #pragma unroll
-            for (int j = 0; j < LANE_KEYS; j++)
-                key[j] = from[min(base + 64 * j + lane, total - 1)];
-        };
+        for (int j = 0; j < LANE_KEYS; j++)
+            key[j] = from[min(base + 64 * j + lane, total - 1)];
+    };
+    if (wave < beams)
         request(0);
-        Key* const list = s_list[b];
+    const int summed = MERGE_WAVES - 1 - wave;
+    if (summed < beams && !ended_at(summed)) {
+        const Part* const mine = part + (first_row + summed) * parts;
+        Part held = mine[min(lane, parts - 1)];
+        if (lane >= parts)
+            held = {-INF, 0.0f};
+        float most = held.most;
+        for (int i = lane + 64; i < parts; i += 64)
+            most = fmaxf(most, mine[i].most);
+        most = rows_max(row_max<16>(most));
+        // (a part without a finite logit has the sum 0, or NaN)
+        auto scaled = [&](Part q) {
+            return static_cast<double>(q.sum) * (q.most == -INF ? 1.0f : __builtin_amdgcn_exp2f((q.most - most) * LOG2E));
+        };
+        double sum = scaled(held);
+        for (int i = lane + 64; i < parts; i += 64)
+            sum += scaled(mine[i]);
+        const double log_sum = log(wave_sum(sum));
+        if (lane == 0) {
+            s_most[summed] = most;
+            s_log[summed] = log_sum;
+        }
+    }
+    if (wave < beams) {
+        Key* const list = s_list[wave];
         if (lane < CANDIDATES_MAX)
-            list[lane] = row_ended && lane == 0 ? 0xffffffffu - static_cast<uint32_t>(a.end_token) : 0;
+            list[lane] = own_ended && lane == 0 ? 0xffffffffu - static_cast<uint32_t>(a.end_token) : 0;
         wave_sync();
-        for (int base = 0; base < total && !row_ended; base += 64 * LANE_KEYS) {
+        // In several turns: a value that k parts' largest ones reach, with which few keys are left.
+        float reached = -INF, over = -INF;
+        if (total > 64 * LANE_KEYS && !own_ended) {
+            float top = -INF;
+            for (int i = lane; i < parts; i += 64)
+                top = fmaxf(top, part[(first_row + own) * parts + i].most);
+            reached = near_kth(top, k);
+        }
+        int held = 0;   // kept ones that are not in the list yet
+        const bool joined = own_ended || parts == 1;   // (one part's list is the row's)
+        if (!own_ended && parts == 1 && lane < k)
+            list[lane] = key[0];
+        for (int base = 0; base < total && !joined; base += 64 * LANE_KEYS) {
             if (base > 0)
                 request(base);
             float v[LANE_KEYS], best = -INF;
@@ -405,64 +439,83 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
                 v[j] = order == 0 ? -INF : logit_of(order);
                 best = fmaxf(best, v[j]);
             }
-            const float bound = fmaxf(group_bound(best, k), least_of(list, k));
-            int count = 0;
+            const float bound = fmaxf(reached == -INF ? near_kth(best, k) : reached, over);
+            int count = held;
 #pragma unroll
             for (int j = 0; j < LANE_KEYS; j++)
-                count = append(v[j] >= bound && v[j] > -INF, [&] { return key[j]; }, count, s_kept[wave]);
-            if (count <= KEPT)
-                rank_kept(count, k, s_kept[wave], list);
-            else
-                merge_tile<LANE_KEYS>(v, bound, [&](int j) { return key[j]; }, k, s_kept[wave], list);
+                if (base + 64 * j < total)
+                    count = append(v[j] >= bound && v[j] > -INF, [&] { return key[j]; }, count, s_kept[wave]);
+            if (count <= KEPT) {
+                held = count;
+                continue;
+            }
+            rank_kept(held, k, s_kept[wave], list);
+            merge_tile<LANE_KEYS>(v, bound, [&](int j) { return key[j]; }, k, s_kept[wave], list);
+            over = least_of(list, k);
+            held = 0;
         }
+        if (held > 0)
+            rank_kept(held, k, s_kept[wave], list);
     }
-    if (t < beams) {
-        s_slot[t] = slot;
-        s_child[t] = BEAMS_MAX;
-    }
-    if (t == 0)
-        s_count = 0;
     __syncthreads();
     const Key got = t < all ? s_list[beam][t - beam * k] : 0;
     const double x = static_cast<double>(logit_of(static_cast<uint32_t>(got >> 32)));
     double score = given + ((x - static_cast<double>(s_most[beam])) - s_log[beam]);
     if (ended)
         score = t == beam * k ? given : -__builtin_inf();
-    const bool counts = got != 0 && fabs(score) < __builtin_inf();
-    if (t < all) {
-        s_score[t] = counts ? score : -__builtin_inf();
-        s_rank[t] = 0;
-    }
-    const uint64_t counted = __ballot(counts);
-    if (lane == 0 && counted != 0)
-        atomicAdd(&s_count, __popcll(counted));
+    if (t < all)
+        s_score[t] = got != 0 && fabs(score) < __builtin_inf() ? score : -__builtin_inf();
     __syncthreads();
-    const int share = (all + MERGE_WAVES - 1) / MERGE_WAVES, last = min((wave + 1) * share, all);
-    for (int i = lane; i < all; i += 64) {
-        const double mine = s_score[i];
-        int larger = 0;
-#pragma unroll 4
-        for (int j = wave * share; j < last; j++) {
-            const double other = s_score[j];
-            larger += other > mine || (other == mine && j < i);
+    if (wave > 0)
+        return;
+    // The candidates among which the best k are (their scores rounded to FP32: the order stays), put in order by the number of
+    // larger ones (of equal ones the first).
+    constexpr int PERL = BEAMS_MAX * CANDIDATES_MAX / 64;
+    float v[PERL], best = -INF;
+#pragma unroll
+    for (int j = 0; j < PERL; j++) {
+        v[j] = 64 * j < all && lane + 64 * j < all ? static_cast<float>(s_score[lane + 64 * j]) : -INF;
+        best = fmaxf(best, v[j]);
+    }
+    const float bound = all <= 32 ? -INF : near_kth(best, k);   // (so few are ranked as soon as a bound is found)
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < PERL; j++) {
+        if (64 * j >= all)
+            break;
+        const bool in = v[j] >= bound && v[j] > -INF;
+        const uint64_t lanes = __ballot(in);
+        if (in) {
+            const int at = count + __popcll(lanes & ((1ull << lane) - 1));
+            s_top[at] = lane + 64 * j;
+            s_top_score[at] = s_score[lane + 64 * j];
         }
-        if (larger != 0)
-            atomicAdd(&s_rank[i], larger);
+        count += __popcll(lanes);
     }
-    __syncthreads();
+    wave_sync();
     const int64_t out = static_cast<int64_t>(s) * k;
-    if (counts && s_rank[t] < k) {
-        const int rank = s_rank[t], token = static_cast<int>(0xffffffffu - static_cast<uint32_t>(got));
-        a.parents[out + rank] = beam;
-        a.tokens[out + rank] = token;
-        a.new_scores[out + rank] = static_cast<float>(score);
-        if (a.new_done)
-            a.new_done[out + rank] = token == a.end_token;
-        s_parent[rank] = beam;
-        if (a.slots)
-            atomicMin(&s_child[beam], rank);
+    const float per_beam = 1.0f / static_cast<float>(k);
+    for (int i = lane; i < count; i += 64) {
+        const int c = s_top[i];
+        const double mine = s_top_score[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < count; j++) {   // (of equal ones the lower candidate first: they lie in their order)
+            const double other = s_top_score[j];
+            rank += other > mine || (other == mine && j < i);
+        }
+        if (rank < k) {
+            const int parent = static_cast<int>((static_cast<float>(c) + 0.5f) * per_beam);   // c / k: exact for so few
+            const int token = static_cast<int>(0xffffffffu - static_cast<uint32_t>(s_list[parent][c - parent * k]));
+            a.parents[out + rank] = parent;
+            a.tokens[out + rank] = token;
+            a.new_scores[out + rank] = static_cast<float>(mine);
+            if (a.new_done)
+                a.new_done[out + rank] = token == a.end_token;
+            s_parent[rank] = parent;
+        }
     }
-    if (t >= s_count && t < k) {
+    if (t >= count && t < k) {
         a.parents[out + t] = -1;
         a.tokens[out + t] = -1;
         a.new_scores[out + t] = -INF;
@@ -472,21 +525,26 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
     }
     if (!a.slots)
         return;
-    __syncthreads();
-    if (t >= 64)
-        return;
     // candidates = beams, one a lane: a parent's first child keeps its slot, the others take those of beams without children in turn
+    wave_sync();
     const int parent = t < beams ? s_parent[t] : -1;
-    const bool keeps = parent >= 0 && s_child[parent] == t;
+    uint64_t keepers = 0, childless = 0;
+    for (int b = 0; b < beams; b++) {
+        const uint64_t children = __ballot(parent == b);
+        keepers |= children & -children;
+        childless |= children == 0 ? 1ull << b : 0;
+    }
+    if (t < beams)
+        s_slot[t] = slot;
     const uint64_t before = (1ull << t) - 1;
-    const uint64_t take_over = __ballot(t < beams && !keeps), childless = __ballot(t < beams && s_child[t] == BEAMS_MAX);
     if (childless >> t & 1)
         s_free[__popcll(childless & before)] = slot;
     wave_sync();
     if (t < beams) {
         const int source = parent >= 0 ? s_slot[parent] : -1;
+        const bool keeps = keepers >> t & 1;
         a.from[out + t] = source;
-        a.to[out + t] = keeps ? source : s_free[__popcll(take_over & before)];
+        a.to[out + t] = keeps ? source : s_free[__popcll(~keepers & before)];
     }
 }
 

@@ -417,6 +417,17 @@ def test_beam_select_ties(hip, fmt):
         _check_beams(hip, np.sort(logits, 1), scores, None, None, 4, 7, fmt)
 
 
+def test_beam_select_equal_over_many_parts(hip):
+    """More equal logits over a row's parts than are ranked together; parts of them masked; one beam's tokens before the next's."""
+    logits = np.zeros((4, 70000), np.float32)
+    logits[1, :65000] = -np.inf
+    logits[2, ::3] = 1.0
+    logits[3] = np.arange(70000) // 7000
+    _check_beams(hip, logits, np.array([-1, -1, -2, -2]), None, None, 2, 32, native.F32)
+    _check_beams(hip, logits, np.array([-1, -1, -1, -1]), None, np.arange(4), 4, 4, native.F16)
+    _check_beams(hip, logits[:, ::-1], np.zeros(4), None, None, 4, 29, native.BF16)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_beam_select_masks(hip, fmt):
     """Masked logits (-infinity, and the type's lowest), rows with nothing left, beams that are none, NaN and infinity."""
