@@ -30,43 +30,42 @@ struct Plan;
 __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Plan* plan);
 
 // Sequences of few rows: a workgroup takes one head of one sequence, the state
-// in registers (a thread holds 8 columns of two state rows: 8 lanes a state
+// in registers (a thread holds 8 columns of one or two state rows: 8 lanes a state
 // row, whose sums take three DPP steps, and half the LDS reads of 16 columns
-// of one row).  Four rows at a time: wave w prepares row w (one element a
-// lane), all waves take the four rows through the state, wave w normalises row w.
+// of one row).  As many rows at a time as there are waves: wave w prepares row w (one element a
+// lane), all waves take the rows through the state, wave w normalises row w.
 // Bound by reading and writing the state (32 KiB a head) where a sequence
-// brings one row; by vector instructions (92 a row and wave) and LDS reads
+// brings one row; by vector instructions (92 a row and wave of four) and LDS reads
 // (10 b128 a lane and row) where it brings many.
-// With a plan to make, the last workgroup makes it.
-__global__ __launch_bounds__(256) void wkv_few_kernel(WkvRowsArgs a, int most, int cut, int room, Plan* plan)
+template <int WAVES>
+struct FewLds {
+    float4 vec[WAVES][5][N / 4];   // decay, key, kn, kn * a, r of the rows
+    float value[WAVES][N], y[WAVES][N];
+};
+
+template <int WAVES>
+__device__ __forceinline__ void few_rows(const WkvRowsArgs& a, FewLds<WAVES>& lds, int s, int h, RowSpan span)
 {
-    __shared__ float4 s_vec[4][5][N / 4];   // decay, key, kn, kn * a, r of the four rows
-    __shared__ float s_value[4][N], s_y[4][N];
-    const int s = blockIdx.x / a.heads, h = blockIdx.x - s * a.heads;
-    if (s == a.batch.sequences)
-        return make_plan(a, most, cut, room, plan);
-    const RowSpan span = rows_of(a.batch, s);
+    constexpr int OWN = 8 / WAVES, APART = 8 * WAVES;   // state rows of a thread, and how far apart they lie
     const int from = a.batch.from[s], to = a.batch.to[s];
-    if (span.last - span.first < 1 || span.last - span.first > most)
-        return;
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int64_t width = static_cast<int64_t>(a.heads) * N;
     const int e = h * N + lane;
 
     const int c = t & 7, i0 = t >> 3;
-    float4 sv[2][2];
+    float4 sv[OWN][2];
     if (from >= 0 && from < a.batch.slots) {
         const float* S = a.state + (static_cast<int64_t>(from) * a.heads + h) * N * N;
 #pragma unroll
-        for (int p = 0; p < 2; p++)
+        for (int p = 0; p < OWN; p++)
 #pragma unroll
             for (int q = 0; q < 2; q++)
-                sv[p][q] = *reinterpret_cast<const float4*>(S + (i0 + 32 * p) * N + 32 * q + 4 * c);
+                sv[p][q] = *reinterpret_cast<const float4*>(S + (i0 + APART * p) * N + 32 * q + 4 * c);
     } else {
         const float z = from == -1 ? 0.0f : __builtin_nanf("");
 #pragma unroll
-        for (int p = 0; p < 2; p++)
+        for (int p = 0; p < OWN; p++)
             sv[p][0] = sv[p][1] = make_float4(z, z, z, z);
     }
     const bool first = a.first_layer != 0;
@@ -88,7 +87,7 @@ __global__ __launch_bounds__(256) void wkv_few_kernel(WkvRowsArgs a, int most, i
         return x;
     };
     RowIn next = load(span.first + wave);
-    for (int base = span.first; base < span.last; base += 4) {
+    for (int base = span.first; base < span.last; base += WAVES) {
         const RowIn x = next;
         const int row = base + wave;
         float value = 0.0f, bonus = 0.0f;
@@ -104,56 +103,63 @@ __global__ __launch_bounds__(256) void wkv_few_kernel(WkvRowsArgs a, int most, i
             if (first)
                 a.v_first[row * width + e] = x.v;
             bonus = wave_sum(key * x.r * rk);
-            float* vec = reinterpret_cast<float*>(s_vec[wave]);
+            float* vec = reinterpret_cast<float*>(lds.vec[wave]);
             vec[lane] = decay;
             vec[N + lane] = key;
             vec[2 * N + lane] = kn;
             vec[3 * N + lane] = kn * ad;
             vec[4 * N + lane] = x.r;
-            s_value[wave][lane] = value;
+            lds.value[wave][lane] = value;
         }
-        next = load(row + 4);
+        next = load(row + WAVES);
         __syncthreads();
-        const int live = min(4, span.last - base);
+        const int live = min(WAVES, span.last - base);
         for (int j = 0; j < live; j++) {
-            float p0 = 0.0f, p1 = 0.0f, y0 = 0.0f, y1 = 0.0f;
-            const float v0i = s_value[j][i0], v1i = s_value[j][i0 + 32];
+            float kept[OWN], y[OWN], value_of[OWN];   // -S kn, S r, the row's value
             auto dot = [](float4 x, float4 y, float acc) {
                 return fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, fmaf(x.x, y.x, acc))));
             };
 #pragma unroll
-            for (int q = 0; q < 2; q++) {
-                const float4 kn = s_vec[j][2][8 * q + c];
-                p0 = dot(sv[0][q], kn, p0);
-                p1 = dot(sv[1][q], kn, p1);
+            for (int p = 0; p < OWN; p++) {
+                kept[p] = y[p] = 0.0f;
+                value_of[p] = lds.value[j][i0 + APART * p];
             }
-            p0 = -row_sum<8>(p0);
-            p1 = -row_sum<8>(p1);
 #pragma unroll
             for (int q = 0; q < 2; q++) {
-                const float4 d = s_vec[j][0][8 * q + c], k = s_vec[j][1][8 * q + c], ak = s_vec[j][3][8 * q + c],
-                             r = s_vec[j][4][8 * q + c];
+                const float4 kn = lds.vec[j][2][8 * q + c];
+#pragma unroll
+                for (int p = 0; p < OWN; p++)
+                    kept[p] = dot(sv[p][q], kn, kept[p]);
+            }
+#pragma unroll
+            for (int p = 0; p < OWN; p++)
+                kept[p] = -row_sum<8>(kept[p]);
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const float4 d = lds.vec[j][0][8 * q + c], k = lds.vec[j][1][8 * q + c], ak = lds.vec[j][3][8 * q + c],
+                             r = lds.vec[j][4][8 * q + c];
                 auto step = [&](float4& S, float p, float v) {
                     S.x = fmaf(p, ak.x, fmaf(v, k.x, S.x * d.x));
                     S.y = fmaf(p, ak.y, fmaf(v, k.y, S.y * d.y));
                     S.z = fmaf(p, ak.z, fmaf(v, k.z, S.z * d.z));
                     S.w = fmaf(p, ak.w, fmaf(v, k.w, S.w * d.w));
                 };
-                step(sv[0][q], p0, v0i);
-                step(sv[1][q], p1, v1i);
-                y0 = dot(sv[0][q], r, y0);
-                y1 = dot(sv[1][q], r, y1);
+#pragma unroll
+                for (int p = 0; p < OWN; p++) {
+                    step(sv[p][q], kept[p], value_of[p]);
+                    y[p] = dot(sv[p][q], r, y[p]);
+                }
             }
-            y0 = row_sum<8>(y0);
-            y1 = row_sum<8>(y1);
-            if (c == 0) {
-                s_y[j][i0] = y0;
-                s_y[j][i0 + 32] = y1;
+#pragma unroll
+            for (int p = 0; p < OWN; p++) {
+                y[p] = row_sum<8>(y[p]);
+                if (c == 0)
+                    lds.y[j][i0 + APART * p] = y[p];
             }
         }
         __syncthreads();
         if (row < span.last) {
-            const float y = s_y[wave][lane];
+            const float y = lds.y[wave][lane];
             const float d = y - wave_sum(y) * (1.0f / N);
             const float var = wave_sum(d * d) * (1.0f / N);
             const float ln = d * (1.0f / sqrtf(var + GROUP_EPS)) * lw + lb;
@@ -163,11 +169,23 @@ __global__ __launch_bounds__(256) void wkv_few_kernel(WkvRowsArgs a, int most, i
     if (to >= 0 && to < a.batch.slots) {
         float* S = a.state + (static_cast<int64_t>(to) * a.heads + h) * N * N;
 #pragma unroll
-        for (int p = 0; p < 2; p++)
+        for (int p = 0; p < OWN; p++)
 #pragma unroll
             for (int q = 0; q < 2; q++)
-                *reinterpret_cast<float4*>(S + (i0 + 32 * p) * N + 32 * q + 4 * c) = sv[p][q];
+                *reinterpret_cast<float4*>(S + (i0 + APART * p) * N + 32 * q + 4 * c) = sv[p][q];
     }
+}
+
+// With a plan to make, the last workgroup makes it.
+__global__ __launch_bounds__(256) void wkv_few_kernel(WkvRowsArgs a, int most, int cut, int room, Plan* plan)
+{
+    __shared__ FewLds<4> lds;
+    const int s = blockIdx.x / a.heads, h = blockIdx.x - s * a.heads;
+    if (s == a.batch.sequences)
+        return make_plan(a, most, cut, room, plan);
+    const RowSpan span = rows_of(a.batch, s);
+    if (span.last - span.first >= 1 && span.last - span.first <= most)
+        few_rows<4>(a, lds, s, h, span);
 }
 
 // ---- blocks of 16 rows on the matrix cores ----------------------------------------------------
@@ -733,7 +751,11 @@ enum ChunkPass { CHUNK_SEQUENCES, CHUNK_STRETCHES, CHUNK_TRANSFERS };
 template <int PASS>
 __global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs a, int over, const Plan* plan, float* records)
 {
-    __shared__ ChunkLds lds;
+    __shared__ union {
+        ChunkLds blocks;
+        FewLds<CHUNK_THREADS / 64> few;
+    } shared;
+    ChunkLds& lds = shared.blocks;
     const int s = blockIdx.x / a.heads, h = blockIdx.x - s * a.heads;
     RowSpan span;
     StateEnds ends;
@@ -741,8 +763,11 @@ __global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs
     bool transfer = false;
     if constexpr (PASS == CHUNK_SEQUENCES) {
         span = rows_of(a.batch, s);
-        if (span.last - span.first <= over)
+        if (span.last - span.first <= over) {
+            if (span.last > span.first)
+                few_rows<CHUNK_THREADS / 64>(a, shared.few, s, h, span);
             return;
+        }
         ends = state_ends(a, s, h);
     } else {
         if (s >= plan->stretches)
@@ -964,7 +989,6 @@ hipError_t launch_wkv_rows(const WkvRowsArgs& a, hipStream_t s)
     }
     const int from = cut_from(a);
     if (from == 0) {
-        few(FEW_ROWS, 0, 0, 0, nullptr);
         hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_SEQUENCES>, dim3(grid), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, nullptr, nullptr);
         return hipGetLastError();
     }
