@@ -27,7 +27,7 @@ struct RowIn {
 };
 
 struct Plan;
-__device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Plan* plan);
+__device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Plan* plan);   // by 256 threads
 
 // Sequences of few rows: a workgroup takes one head of one sequence, the state
 // in registers (a thread holds 8 columns of one or two state rows: 8 lanes a state
@@ -35,8 +35,8 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Pl
 // of one row).  As many rows at a time as there are waves: wave w prepares row w (one element a
 // lane), all waves take the rows through the state, wave w normalises row w.
 // Bound by reading and writing the state (32 KiB a head) where a sequence
-// brings one row; by vector instructions (92 a row and wave of four) and LDS reads
-// (10 b128 a lane and row) where it brings many.
+// brings one row (64 of them, 32 heads, 13.4 us, 5.4 TB/s); by vector instructions (92 a row and wave of four) and LDS reads
+// (10 b128 a lane and row) where it brings many (64 of 8 rows 28 us).
 template <int WAVES>
 struct FewLds {
     float4 vec[WAVES][5][N / 4];   // decay, key, kn, kn * a, r of the rows
@@ -177,15 +177,16 @@ __device__ __forceinline__ void few_rows(const WkvRowsArgs& a, FewLds<WAVES>& ld
 }
 
 // With a plan to make, the last workgroup makes it.
-__global__ __launch_bounds__(256) void wkv_few_kernel(WkvRowsArgs a, int most, int cut, int room, Plan* plan)
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void wkv_few_kernel(WkvRowsArgs a, int most, int cut, int room, Plan* plan)
 {
-    __shared__ FewLds<4> lds;
+    __shared__ FewLds<WAVES> lds;
     const int s = blockIdx.x / a.heads, h = blockIdx.x - s * a.heads;
-    if (s == a.batch.sequences)
+    if (WAVES == 4 && s == a.batch.sequences)
         return make_plan(a, most, cut, room, plan);
     const RowSpan span = rows_of(a.batch, s);
     if (span.last - span.first >= 1 && span.last - span.first <= most)
-        few_rows<4>(a, lds, s, h, span);
+        few_rows<WAVES>(a, lds, s, h, span);
 }
 
 // ---- blocks of 16 rows on the matrix cores ----------------------------------------------------
@@ -968,8 +969,10 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Pl
 
 }  // namespace
 
-constexpr int FEW_ROWS = 12;             // sequences of up to this many rows go row by row: 12 rows of 8 x 32 heads 10.4 us (by
-                                         // blocks 10.9), of 64 x 32 36 (47); 16 rows 12.9 (11.4) and 43 (50)
+// Sequences of up to this many rows go row by row (32 heads; one sequence of 12 rows 7.4 us, of 14 rows 8.1, by blocks 7.4 both; eight of
+// 9 rows 7.7, by blocks 8.6, of 14 9.9 and 9.1), and of up to this many where workgroups wait for one another (64 of 17 rows 47,
+// by blocks 63, of 24 59 and 66; beside twice the card's workgroups, 32 of 1 to 24 rows, it is 25 and 22).
+constexpr int FEW_ROWS = 12, MANY_FEW_ROWS = 24;
 
 // The list: every sequence that goes by blocks, at most, the stretches, and the cut sequences again (at most half as many as
 // stretches with a record: each has three stretches or more).
@@ -980,16 +983,19 @@ int64_t wkv_rows_workspace_bytes(int) { return PLAN_BYTES + static_cast<int64_t>
 hipError_t launch_wkv_rows(const WkvRowsArgs& a, hipStream_t s)
 {
     const unsigned heads = static_cast<unsigned>(a.heads), grid = static_cast<unsigned>(a.batch.sequences) * heads;
-    auto few = [&](int most, unsigned more, int from, int room, Plan* plan) {
-        hipLaunchKernelGGL(wkv_few_kernel, dim3(grid + more), dim3(256), 0, s, a, most, from, room, plan);
-    };
-    if (a.batch.max_rows <= FEW_ROWS) {
-        few(INT32_MAX, 0, 0, 0, nullptr);
+    const int over = grid <= 2 * CARD ? FEW_ROWS : MANY_FEW_ROWS;
+    if (a.batch.max_rows <= over) {
+        // Eight waves a head where that leaves no workgroup waiting for another (seven sequences of 3 to 6 rows, 32 heads, 5.6 us, of four
+        // 6.9; 64 of one row 14.3 and 13.5).
+        if (grid <= CARD)
+            hipLaunchKernelGGL(wkv_few_kernel<8>, dim3(grid), dim3(512), 0, s, a, INT32_MAX, 0, 0, nullptr);
+        else
+            hipLaunchKernelGGL(wkv_few_kernel<4>, dim3(grid), dim3(256), 0, s, a, INT32_MAX, 0, 0, nullptr);
         return hipGetLastError();
     }
     const int from = cut_from(a);
     if (from == 0) {
-        hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_SEQUENCES>, dim3(grid), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, nullptr, nullptr);
+        hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_SEQUENCES>, dim3(grid), dim3(CHUNK_THREADS), 0, s, a, over, nullptr, nullptr);
         return hipGetLastError();
     }
     Plan* const plan = reinterpret_cast<Plan*>(a.workspace);
@@ -1000,7 +1006,7 @@ hipError_t launch_wkv_rows(const WkvRowsArgs& a, hipStream_t s)
     const int whole = least(a.batch.rows / (FEW_ROWS + 1), a.batch.sequences);
     const int records_most = HEAD_STRETCHES / a.heads, cut = least(a.batch.rows / from, records_most / 2);
     const int room = whole + least(a.batch.rows / LEAST_STRETCH, records_most + cut);
-    few(FEW_ROWS, 1, from, room, plan);
+    hipLaunchKernelGGL(wkv_few_kernel<4>, dim3(grid + 1), dim3(256), 0, s, a, FEW_ROWS, from, room, plan);
     hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_TRANSFERS>, dim3(room * heads), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, plan, records);
     hipLaunchKernelGGL(wkv_join_kernel, dim3(cut * heads * 4), dim3(256), 0, s, a, plan, room, records);
     hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_STRETCHES>, dim3(room * heads), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, plan, records);
