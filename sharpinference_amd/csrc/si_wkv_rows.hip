@@ -719,7 +719,8 @@ constexpr int RECORD = 2 * N * N;        // floats of a stretch and head: M^T; N
 constexpr int CARD = 512;                // workgroups of wkv_chunk_kernel that the card holds: two a compute unit
 constexpr int HEAD_STRETCHES = 2 * CARD; // stretches (but each sequence's last) times heads, at most
 constexpr int LONG_STRETCH = 256;
-constexpr int LEAST_STRETCH = 64;        // rows
+constexpr int LEAST_STRETCH = 48, LEAST_CUT = 176;   // rows of a stretch, and of a sequence that is cut, at least (one of 250 rows, 32 heads,
+                                                     // 44 us, in stretches of 64 55; of 150, cut 42, whole 38)
 
 struct Stretch {
     int sequence, first, last;   // rows
@@ -885,13 +886,15 @@ __host__ __device__ inline int stretch_rows(int64_t rows, int heads, int cut)
 
 // From how many rows on a launch cuts its sequences, or 0: none.  Cutting costs the transfers and the join, and pays where the
 // longest sequence has 2.5 times the rows that all, shared out evenly, give a workgroup (32 heads; eight of 1000 rows, at 2:
-// 234 us whole, 286 cut; sixteen of 100 to 3000, at 3.2: 860 and 600), and for the sequences that become three stretches or
-// more: two would follow one another.
+// 234 us whole, 286 cut; sixteen of 100 to 3000, at 3.2: 860 and 610) and becomes three stretches or more.  Where stretches are not
+// long, shorter ones that become two, without transfers, then need not wait whole for the last pass (five of 300 to 1500 207 us,
+// from three on 250; the sixteen, whose stretches are long, 659 and 615).
 int cut_from(const WkvRowsArgs& a)
 {
     const int64_t each = (static_cast<int64_t>(a.batch.rows) * a.heads + CARD - 1) / CARD;
-    const int from = 3 * stretch_rows(a.batch.rows, a.heads, 0);
-    return a.batch.max_rows >= from && 2ll * a.batch.max_rows >= 5 * each ? from : 0;
+    const int stretch = stretch_rows(a.batch.rows, a.heads, 0);
+    const int longest = a.batch.max_rows;
+    return longest >= LEAST_CUT && longest >= 3 * stretch && 2ll * longest >= 5 * each ? (stretch > LONG_STRETCH ? 3 : 2) * stretch : 0;
 }
 
 // The list of stretches of all sequences over `over` rows, by one workgroup: 4096 sequences in turns of 256.
@@ -927,7 +930,7 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Pl
             plan->stretches = plan->cut = 0;
         return;
     }
-    const int stretch = stretch_rows(rows_in_cut, a.heads, cuts);   // at most a third of `from`
+    const int stretch = stretch_rows(rows_in_cut, a.heads, cuts);   // at most half of `from`
     // whole sequences, cut ones and their stretches in one number, 20 bits each
     int64_t total = 0;
     for (int base = 0; base < a.batch.sequences; base += 256) {
@@ -974,9 +977,9 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Pl
 // by blocks 63, of 24 59 and 66; beside twice the card's workgroups, 32 of 1 to 24 rows, it is 25 and 22).
 constexpr int FEW_ROWS = 12, MANY_FEW_ROWS = 24;
 
-// The list: every sequence that goes by blocks, at most, the stretches, and the cut sequences again (at most half as many as
-// stretches with a record: each has three stretches or more).
-constexpr int64_t PLAN_BYTES = (sizeof(Plan) + (ROW_SEQUENCES_MAX + HEAD_STRETCHES * 2) * sizeof(Stretch) + 255) / 256 * 256;
+// The list: every sequence that goes by blocks, at most, the stretches, and the cut sequences again (at most as many as
+// stretches with a record: each has two stretches or more).
+constexpr int64_t PLAN_BYTES = (sizeof(Plan) + (ROW_SEQUENCES_MAX + HEAD_STRETCHES * 3) * sizeof(Stretch) + 255) / 256 * 256;
 
 int64_t wkv_rows_workspace_bytes(int) { return PLAN_BYTES + static_cast<int64_t>(HEAD_STRETCHES) * RECORD * 4; }
 
@@ -1004,7 +1007,7 @@ hipError_t launch_wkv_rows(const WkvRowsArgs& a, hipStream_t s)
     // as many as share all cut rows and heads out to HEAD_STRETCHES workgroups and one more for each sequence and head.
     auto least = [](int x, int y) { return x < y ? x : y; };
     const int whole = least(a.batch.rows / (FEW_ROWS + 1), a.batch.sequences);
-    const int records_most = HEAD_STRETCHES / a.heads, cut = least(a.batch.rows / from, records_most / 2);
+    const int records_most = HEAD_STRETCHES / a.heads, cut = least(a.batch.rows / from, records_most);
     const int room = whole + least(a.batch.rows / LEAST_STRETCH, records_most + cut);
     hipLaunchKernelGGL(wkv_few_kernel<4>, dim3(grid + 1), dim3(256), 0, s, a, FEW_ROWS, from, room, plan);
     hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_TRANSFERS>, dim3(room * heads), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, plan, records);
