@@ -20,7 +20,7 @@ constexpr int ROOM = KEPT + CANDIDATES_MAX + 8;
 constexpr int HALVES = 5;                     // of the way from a bound to the largest value
 constexpr int LARGEST = 24;                   // a lane's 16-byte words of a group of tiles, whose largest values are held
 constexpr int SCAN_WAVES = 4, MERGE_WAVES = BEAMS_MAX;
-constexpr float INF = __builtin_inff();
+constexpr float INF = __builtin_inff(), LOWEST = -3.402823466e38f;   // of the finite values
 
 typedef uint32_t Sixteen __attribute__((ext_vector_type(4), aligned(1)));   // bytes at any address, in one load or store
 
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
         const float over = least_of(list, k);
         if (__ballot(lane_best > over) == 0)
             continue;
-        const float bound = fmaxf(near_kth(lane_best, k), over);
+        const float bound = fmaxf(fmaxf(near_kth(lane_best, k), over), LOWEST);
         uint32_t mine = 0;
         for (int i = 0; i < count * (LOADS / 4); i++) {
             const float4 m = largest[i][lane];
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
                 const float v = value_at<FMT>(&got, j);
-                more = append(in && v >= bound && v > -INF && start + j >= from, [&] { return key_of(v, start + j); }, more, kept);
+                more = append(in && v >= bound && start + j >= from, [&] { return key_of(v, start + j); }, more, kept);
             }
             if (more <= KEPT) {
                 held = more;
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
                 }
                 const float v = value_at<FMT>(x, max(start + j, 0));
                 const Key key = key_of(v, start + j);
-                held = append(in && v >= bound && v > -INF && start + j >= from && key > least, [&] { return key; }, held, kept);
+                held = append(in && v >= bound && start + j >= from && key > least, [&] { return key; }, held, kept);
             }
         }
         if (held > 0)
