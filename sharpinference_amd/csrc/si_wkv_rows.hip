@@ -741,6 +741,45 @@ __device__ __forceinline__ StateEnds state_ends(const WkvRowsArgs& a, int s, int
             to >= 0 && to < a.batch.slots ? at(to) : nullptr, nullptr};
 }
 
+// Rows of a stretch where so many rows of so many sequences are cut: the card's workgroups share them with their heads; where that
+// gives each more than LONG_STRETCH, twice as many workgroups do, which even out better beside whole sequences (32 heads; eight
+// prompts of 500 to 3000 rows 526 us, by CARD 603, three of 1000 to 6000 rows 539 and 704; one of 4001 rows, by CARD, 217, by
+// twice as many 245).
+__host__ __device__ inline int stretch_rows(int64_t rows, int heads, int cut)
+{
+    const int64_t work = rows * heads, more = static_cast<int64_t>(cut) * heads;   // (of each sequence one stretch is idle in every pass)
+    const int64_t each = (work + CARD + more - 1) / (CARD + more), half = (work + HEAD_STRETCHES + more - 1) / (HEAD_STRETCHES + more);
+    const int64_t least = each < LONG_STRETCH ? each : half > LONG_STRETCH ? half : LONG_STRETCH;
+    return static_cast<int>((least > LEAST_STRETCH ? least + C - 1 : LEAST_STRETCH) / C * C);
+}
+
+// How a sequence of so many rows lies in its stretches: rows of each but the last, and their number (none of them empty).
+struct Parts {
+    int each, count;
+};
+__device__ __forceinline__ Parts parts_of(int rows, bool cut, int stretch)
+{
+    const int most = cut ? rows / stretch : 1;
+    const int each = ((rows + most - 1) / most + C - 1) / C * C;
+    return {each, cut ? (rows + each - 1) / each : 1};
+}
+__device__ __forceinline__ Stretch stretch_of(int sequence, RowSpan span, Parts parts, int record, int index)
+{
+    return {sequence, span.first + index * parts.each,
+            index + 1 < parts.count ? span.first + (index + 1) * parts.each : span.last, record, index, parts.count};
+}
+
+// Stretch `index` of a batch's only sequence; false where it has none.  (One sequence needs no plan, and its launch: 4 us.)
+__device__ __forceinline__ bool sole_stretch(const WkvRowsArgs& a, int from, int index, Stretch* part)
+{
+    const RowSpan span = rows_of(a.batch, 0);
+    const int rows = span.last - span.first;
+    const bool cut = rows >= from;
+    const Parts parts = parts_of(rows, cut, cut ? stretch_rows(rows, a.heads, 1) : 1);
+    *part = stretch_of(0, span, parts, cut ? 0 : -1, index);
+    return index < parts.count;
+}
+
 // One head of one sequence or stretch, block after block.  While the state's waves take block i
 // (72 matrix instructions each), the others prepare block i + 1 (20 each, and the
 // exponentials), in three phases between barriers.  Bound by the SIMDs: FP32 matrix instructions take 32 cycles each in the vector
@@ -751,7 +790,7 @@ __device__ __forceinline__ StateEnds state_ends(const WkvRowsArgs& a, int s, int
 enum ChunkPass { CHUNK_SEQUENCES, CHUNK_STRETCHES, CHUNK_TRANSFERS };
 
 template <int PASS>
-__global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs a, int over, const Plan* plan, float* records)
+__global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs a, int over, int from, const Plan* plan, float* records)
 {
     __shared__ union {
         ChunkLds blocks;
@@ -772,9 +811,20 @@ __global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs
         }
         ends = state_ends(a, s, h);
     } else {
-        if (s >= plan->stretches)
-            return;
-        const Stretch part = plan->list[s];
+        Stretch part;
+        if (plan == nullptr) {
+            if (!sole_stretch(a, from, s, &part))
+                return;
+            if (part.count == 1 && part.last - part.first <= over) {
+                if (PASS == CHUNK_TRANSFERS && part.last > part.first)
+                    few_rows<CHUNK_THREADS / 64>(a, shared.few, 0, h, {part.first, part.last});
+                return;
+            }
+        } else {
+            if (s >= plan->stretches)
+                return;
+            part = plan->list[s];
+        }
         span = {part.first, part.last};
         auto record_of = [&](int i) { return records + (static_cast<int64_t>(part.record + i) * a.heads + h) * RECORD; };
         if constexpr (PASS == CHUNK_TRANSFERS) {
@@ -819,14 +869,20 @@ __global__ __launch_bounds__(CHUNK_THREADS, 4) void wkv_chunk_kernel(WkvRowsArgs
 // a stretch costs it 16 matrix instructions a wave, an exchange of the state's tiles through LDS, and 4 KiB of M a wave,
 // requested AHEAD stretches before (their round trip takes longer than the products: one ahead 1.2 us a stretch).  Bound by the chain of
 // stretches: 0.46 us each, of which the matrix instructions are 0.25 (17 stretches of 32 heads 11 us, 43 of 12 heads 22).
-__global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, const Plan* plan, int room, float* records)
+__global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, int from, const Plan* plan, int room, float* records)
 {
     constexpr int AHEAD = 4;
     __shared__ f4 s_tile[2][4][64];
     const int c = blockIdx.x / (4 * a.heads), rest = blockIdx.x - c * 4 * a.heads, h = rest >> 2, i = rest & 3;
-    if (c >= plan->cut)
-        return;
-    const Stretch part = plan->list[room + c];
+    Stretch part;
+    if (plan == nullptr) {
+        if (c > 0 || !sole_stretch(a, from, 0, &part) || part.record < 0)
+            return;
+    } else {
+        if (c >= plan->cut)
+            return;
+        part = plan->list[room + c];
+    }
     const int lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     auto record_of = [&](int k) { return records + (static_cast<int64_t>(part.record + k) * a.heads + h) * RECORD; };
@@ -870,18 +926,6 @@ __global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, const Plan
     for (int k = 0; k < AHEAD - 1; k++)
         if (base + k <= last)
             step(base + k, k, false);
-}
-
-// Rows of a stretch where so many rows of so many sequences are cut: the card's workgroups share them with their heads; where that
-// gives each more than LONG_STRETCH, twice as many workgroups do, which even out better beside whole sequences (32 heads; eight
-// prompts of 500 to 3000 rows 526 us, by CARD 603, three of 1000 to 6000 rows 539 and 704; one of 4001 rows, by CARD, 217, by
-// twice as many 245).
-__host__ __device__ inline int stretch_rows(int64_t rows, int heads, int cut)
-{
-    const int64_t work = rows * heads, more = static_cast<int64_t>(cut) * heads;   // (of each sequence one stretch is idle in every pass)
-    const int64_t each = (work + CARD + more - 1) / (CARD + more), half = (work + HEAD_STRETCHES + more - 1) / (HEAD_STRETCHES + more);
-    const int64_t least = each < LONG_STRETCH ? each : half > LONG_STRETCH ? half : LONG_STRETCH;
-    return static_cast<int>((least > LEAST_STRETCH ? least + C - 1 : LEAST_STRETCH) / C * C);
 }
 
 // From how many rows on a launch cuts its sequences, or 0: none.  Cutting costs the transfers and the join, and pays where the
@@ -939,9 +983,8 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Pl
             span = rows_of(a.batch, base + t);
         const int rows = span.last - span.first;
         const bool cut = rows >= from;
-        const int most = cut ? rows / stretch : 1;
-        const int each = ((rows + most - 1) / most + C - 1) / C * C;
-        const int parts = rows <= over ? 0 : cut ? (rows + each - 1) / each : 1;   // (none of them empty)
+        const Parts lie = parts_of(rows, cut, stretch);
+        const int parts = rows <= over ? 0 : lie.count;
         const int64_t own = cut ? 1ll << 20 | static_cast<int64_t>(parts) << 40 : parts;
         s_count[t] = own;
         __syncthreads();
@@ -955,8 +998,7 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Pl
         const int cut_before = before >> 20 & 0xfffff, parts_before = static_cast<int>(before >> 40);
         const int record = parts_before - cut_before, at = cut ? whole + parts_before : static_cast<int>(before & 0xfffff);
         for (int k = 0; k < parts; k++) {
-            const Stretch part{base + t, span.first + k * each, k + 1 < parts ? span.first + (k + 1) * each : span.last,
-                               cut ? record : -1, k, parts};
+            const Stretch part = stretch_of(base + t, span, lie, cut ? record : -1, k);
             plan->list[at + k] = part;
             if (cut && k == 0)
                 plan->list[room + cut_before] = part;
@@ -998,10 +1040,10 @@ hipError_t launch_wkv_rows(const WkvRowsArgs& a, hipStream_t s)
     }
     const int from = cut_from(a);
     if (from == 0) {
-        hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_SEQUENCES>, dim3(grid), dim3(CHUNK_THREADS), 0, s, a, over, nullptr, nullptr);
+        hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_SEQUENCES>, dim3(grid), dim3(CHUNK_THREADS), 0, s, a, over, 0, nullptr, nullptr);
         return hipGetLastError();
     }
-    Plan* const plan = reinterpret_cast<Plan*>(a.workspace);
+    Plan* const plan = a.batch.sequences > 1 ? reinterpret_cast<Plan*>(a.workspace) : nullptr;
     float* const records = a.workspace + PLAN_BYTES / 4;
     // What the host knows of the list's length.  Stretches have at least LEAST_STRETCH rows, and
     // as many as share all cut rows and heads out to HEAD_STRETCHES workgroups and one more for each sequence and head.
@@ -1009,10 +1051,11 @@ hipError_t launch_wkv_rows(const WkvRowsArgs& a, hipStream_t s)
     const int whole = least(a.batch.rows / (FEW_ROWS + 1), a.batch.sequences);
     const int records_most = HEAD_STRETCHES / a.heads, cut = least(a.batch.rows / from, records_most);
     const int room = whole + least(a.batch.rows / LEAST_STRETCH, records_most + cut);
-    hipLaunchKernelGGL(wkv_few_kernel<4>, dim3(grid + 1), dim3(256), 0, s, a, FEW_ROWS, from, room, plan);
-    hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_TRANSFERS>, dim3(room * heads), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, plan, records);
-    hipLaunchKernelGGL(wkv_join_kernel, dim3(cut * heads * 4), dim3(256), 0, s, a, plan, room, records);
-    hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_STRETCHES>, dim3(room * heads), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, plan, records);
+    if (plan)
+        hipLaunchKernelGGL(wkv_few_kernel<4>, dim3(grid + 1), dim3(256), 0, s, a, FEW_ROWS, from, room, plan);
+    hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_TRANSFERS>, dim3(room * heads), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, from, plan, records);
+    hipLaunchKernelGGL(wkv_join_kernel, dim3(cut * heads * 4), dim3(256), 0, s, a, from, plan, room, records);
+    hipLaunchKernelGGL(wkv_chunk_kernel<CHUNK_STRETCHES>, dim3(room * heads), dim3(CHUNK_THREADS), 0, s, a, FEW_ROWS, from, plan, records);
     return hipGetLastError();
 }
 

@@ -244,6 +244,25 @@ def test_wkv_rows_long(hip, heads, counts):
     _check_wkv(hip, _wkv_inputs(rng, rows, heads, False, slots), heads, False, starts, source, to, native.F32)
 
 
+@pytest.mark.parametrize("starts", [[0, 0], [3, 8], [5, 120], [100, 300], [0, 640], [0, 0, 5, 25], [2, 4, 400, 400], [0, 100, 600]])
+def test_wkv_rows_fewer_than_stated(hip, starts):
+    """Sequences, one among them, that bring fewer rows than the launch goes by."""
+    rng = np.random.default_rng(sum(starts))
+    n = len(starts) - 1
+    _check_wkv(hip, _wkv_inputs(rng, 640, 3, False, 2 * n), 3, False, starts, range(n), range(n, 2 * n), native.F32, max_rows=640)
+
+
+@pytest.mark.parametrize("starts", [[0, 600, 300, 640], [0, 200, 150, 500], [0, 700, 500], [-4, 300, 500], [500, 20]])
+def test_wkv_rows_starts_that_fall(hip, starts):
+    """Starts that fall or leave the rows: anything in those rows and slots, nothing outside of them."""
+    rng = np.random.default_rng(12)
+    n = len(starts) - 1
+    inp = _wkv_inputs(rng, 640, 2, False, 2 * n)
+    raw, state, _ = _run_wkv(hip, inp, 2, False, starts, range(n), range(n, 2 * n), native.F32, 640)
+    assert np.array_equal(state[:n], inp["state"][:n])
+    assert np.all(raw[max(min(max(starts), 640), 0):] == FILL)
+
+
 @pytest.mark.parametrize("count", [3, 20, 200])
 def test_wkv_rows_slots(hip, count):
     """From and to the same slot, one slot for several, none, no slots; a bound on the rows that is too low."""
