@@ -10,16 +10,25 @@ namespace {
 
 constexpr int PER = 8;   // values of a row a thread
 
-// A workgroup of THREADS takes `run` rows one after another, eight values of a row a thread (neighbours where
-// EIGHTS, else every THREADS-th).  Weights and mixes stay in registers, and so does the row before: only a run's
+// How a thread's eight values of a row lie: ALIGNED: neighbours at multiples of 16 bytes.  NEIGHBOURS: at any address; where
+// eight does not divide the width, the last thread takes the last eight, of which the thread before has some too: it leaves them out of the
+// sums and writes them again (the state's are read two barriers before).  SINGLE: every THREADS-th (widths under eight; 3900 rows of
+// 2047 in six mixes so 64 us, as neighbours 46).
+enum Lie { ALIGNED, NEIGHBOURS, SINGLE };
+typedef float AlignedFour __attribute__((ext_vector_type(4)));
+typedef float AnyFour __attribute__((ext_vector_type(4), aligned(4)));
+
+// A workgroup of THREADS, as many as a row has eights, takes `run` rows one after another (4000 rows of 768 in six mixes 20 us,
+// with 256 threads 33).  Weights and mixes stay in registers, and so does the row before: only a run's
 // first row is normalised twice.  The next row is requested while this one is normalised.  The sequence's
 // state is read by the workgroup of its first row, which also normalises the last row for the state's slot:
 // the slot has one reader and writer, whatever the other workgroups have done by then.
-// Bound by HBM: 4 bytes in (8 with a residual, 4 more out) and 2 or 4 out a mix; a single row by its
-// round trips.
-// HELD: mixes that registers hold (0: they are loaded with every row: 1024 threads leave no room for more than one).
+// Bound by HBM: 4 bytes in (8 with a residual, 4 more out) and 2 or 4 out a mix (3900 rows of 2048 in six mixes 37 us, 5.5 TB/s);
+// a single row by its round trips (16 rows 4.7 us).
+// HELD: mixes that registers hold (0: they are loaded with every row: 1024 threads leave no room for more than one; 976 rows of 8192 in
+// six mixes 44 us, 1953 of 4096 40).
 // PAST: outputs go past the L2s.
-template <int THREADS, bool EIGHTS, int HELD, bool PAST, typename OUT>
+template <int THREADS, Lie LIE, int HELD, bool PAST, typename OUT>
 __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int run)
 {
     constexpr int WAVES = THREADS / 64;
@@ -27,17 +36,20 @@ __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int ru
     __shared__ int s_at[WAVES];
     const int t = threadIdx.x, wave = t >> 6, n = a.n;
     const RowBatch& b = a.batch;
-    auto place = [&](int j) { return EIGHTS ? PER * t + j : t + THREADS * j; };
+    const int base = LIE == NEIGHBOURS ? min(PER * t, n - PER) : PER * t;
+    auto place = [&](int j) { return LIE != SINGLE ? base + j : t + THREADS * j; };
+    auto counts = [&](int j) { return place(j) < n && (LIE != NEIGHBOURS || place(j) >= PER * t); };
     auto load = [&](const float* p, float* v) {
-        if constexpr (EIGHTS) {
-            float4 f[2] = {};
+        if constexpr (LIE != SINGLE) {
+            using Four = std::conditional_t<LIE == ALIGNED, AlignedFour, AnyFour>;
+            Four f[2] = {};
             if (PER * t < n) {
-                f[0] = *reinterpret_cast<const float4*>(p + PER * t);
-                f[1] = *reinterpret_cast<const float4*>(p + PER * t + 4);
+                f[0] = *reinterpret_cast<const Four*>(p + base);
+                f[1] = *reinterpret_cast<const Four*>(p + base + 4);
             }
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                v[4 * j] = f[j].x, v[4 * j + 1] = f[j].y, v[4 * j + 2] = f[j].z, v[4 * j + 3] = f[j].w;
+            for (int j = 0; j < PER; j++)
+                v[j] = f[j / 4][j % 4];
         } else {
 #pragma unroll
             for (int j = 0; j < PER; j++)
@@ -46,15 +58,15 @@ __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int ru
     };
     auto store = [&](auto* p, const float* v) {
         using T = std::remove_reference_t<decltype(*p)>;
-        if constexpr (EIGHTS) {
-            typedef T Eight __attribute__((ext_vector_type(PER)));
+        if constexpr (LIE != SINGLE) {
+            typedef T Eight __attribute__((ext_vector_type(PER), aligned(LIE == ALIGNED ? 16 : sizeof(T))));
             const Eight e = {static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3]),
                              static_cast<T>(v[4]), static_cast<T>(v[5]), static_cast<T>(v[6]), static_cast<T>(v[7])};
             if (PER * t < n) {
                 if constexpr (PAST)   // (a choice at run time is merged into one ordinary store)
-                    __builtin_nontemporal_store(e, reinterpret_cast<Eight*>(p + PER * t));
+                    __builtin_nontemporal_store(e, reinterpret_cast<Eight*>(p + base));
                 else
-                    *reinterpret_cast<Eight*>(p + PER * t) = e;
+                    *reinterpret_cast<Eight*>(p + base) = e;
             }
         } else {
 #pragma unroll
@@ -112,7 +124,7 @@ __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int ru
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             v[j] = a.residual ? x[j] + add[j] : x[j];
-            sum += v[j];
+            sum += LIE != NEIGHBOURS || counts(j) ? v[j] : 0.0f;
         }
         return sum;
     };
@@ -121,8 +133,8 @@ __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int ru
         float squares = 0.0f;
 #pragma unroll
         for (int j = 0; j < PER; j++) {
-            v[j] = place(j) < n ? v[j] - mean : 0.0f;
-            squares = fmaf(v[j], v[j], squares);
+            v[j] -= mean;
+            squares = counts(j) ? fmaf(v[j], v[j], squares) : squares;
         }
         const float inv = 1.0f / sqrtf(block_sum(squares, s_squares) / static_cast<float>(n) + a.eps);
 #pragma unroll
@@ -213,27 +225,29 @@ __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int ru
     }
 }
 
-template <int THREADS, bool EIGHTS, int HELD, bool PAST>
+template <int THREADS, Lie LIE, int HELD, bool PAST>
 void launch(const MixRowsArgs& a, int run, hipStream_t s)
 {
     const dim3 grid((a.batch.rows + run - 1) / run);
     if (a.out_format == ROWS_OUT_F32)
-        hipLaunchKernelGGL((mix_rows_kernel<THREADS, EIGHTS, HELD, PAST, float>), grid, dim3(THREADS), 0, s, a, run);
+        hipLaunchKernelGGL((mix_rows_kernel<THREADS, LIE, HELD, PAST, float>), grid, dim3(THREADS), 0, s, a, run);
     else if (a.out_format == ROWS_OUT_F16)
-        hipLaunchKernelGGL((mix_rows_kernel<THREADS, EIGHTS, HELD, PAST, _Float16>), grid, dim3(THREADS), 0, s, a, run);
+        hipLaunchKernelGGL((mix_rows_kernel<THREADS, LIE, HELD, PAST, _Float16>), grid, dim3(THREADS), 0, s, a, run);
     else
-        hipLaunchKernelGGL((mix_rows_kernel<THREADS, EIGHTS, HELD, PAST, __bf16>), grid, dim3(THREADS), 0, s, a, run);
+        hipLaunchKernelGGL((mix_rows_kernel<THREADS, LIE, HELD, PAST, __bf16>), grid, dim3(THREADS), 0, s, a, run);
 }
 
 template <int THREADS, int HELD>
-void launch(const MixRowsArgs& a, bool eights, bool past, int run, hipStream_t s)
+void launch(const MixRowsArgs& a, bool aligned, bool past, int run, hipStream_t s)
 {
-    if (eights && past)
-        launch<THREADS, true, HELD, true>(a, run, s);
-    else if (eights)
-        launch<THREADS, true, HELD, false>(a, run, s);
+    if (aligned && past)
+        launch<THREADS, ALIGNED, HELD, true>(a, run, s);
+    else if (aligned)
+        launch<THREADS, ALIGNED, HELD, false>(a, run, s);
+    else if (past)
+        launch<THREADS, NEIGHBOURS, HELD, true>(a, run, s);
     else
-        launch<THREADS, false, HELD, false>(a, run, s);
+        launch<THREADS, NEIGHBOURS, HELD, false>(a, run, s);
 }
 
 template <int THREADS>
@@ -241,31 +255,41 @@ void launch(const MixRowsArgs& a, hipStream_t s)
 {
     constexpr int MANY = THREADS == 1024 ? 0 : MIX_MAX;
     auto aligned16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
-    const bool eights = a.n % 8 == 0 && aligned16(a.x) && aligned16(a.residual) && aligned16(a.weight) && aligned16(a.bias) &&
+    const bool aligned = a.n % 8 == 0 && aligned16(a.x) && aligned16(a.residual) && aligned16(a.weight) && aligned16(a.bias) &&
                         aligned16(a.mix) && aligned16(a.state) && aligned16(a.updated) && aligned16(a.out);
     // Outputs that the L2s (32 MiB) cannot keep for the next kernel go past them: 4000 rows of 2048 values in six mixes
     // take 43 us instead of 66.  Smaller ones stay there for the products that read them.
     const int64_t out = static_cast<int64_t>(a.batch.rows) * a.n *
                         ((a.out_format == ROWS_OUT_F32 ? 4 : 2) * (a.mixes > 0 ? a.mixes : 1) + (a.residual ? 4 : 0));
     const bool past = out > (16 << 20);
-    // Runs such that so many waves a compute unit have one each; few rows one a workgroup.  Odd ones: at 4 or 8 rows a
+    // Runs such that so many waves a compute unit have one each, of wide rows as many whole workgroups (976 rows of 8192 in six mixes 44
+    // us, at 0.9 workgroups a compute unit 65); few rows one a workgroup.  Odd ones: at 4 or 8 rows a
     // run the workgroups' rows lie a power of two apart, and 4000 rows take 48 and 55 us, at 3, 5 and 9 rows 43, 41 and 36.
-    const int waves = a.mixes <= 1 ? 20 : 7, resident = 256 * waves * 64 / THREADS, rows = a.batch.rows;
-    const int run = rows <= 2 * resident ? 1 : rows < 15 * resident ? ((rows + resident - 1) / resident) | 1 : 15;
+    const int waves = a.mixes <= 1 ? 20 : 7, most = waves * 64 / THREADS, rows = a.batch.rows;
+    const int resident = THREADS < 512 ? 256 * waves * 64 / THREADS : 256 * (most > 1 ? most : 1);
+    const int run = rows <= resident ? 1 : rows < 15 * resident ? ((rows + resident - 1) / resident) | 1 : 15;
     if (a.mixes <= 1)
-        launch<THREADS, 1>(a, eights, past, run, s);
+        launch<THREADS, 1>(a, aligned, past, run, s);
     else
-        launch<THREADS, MANY>(a, eights, past, run, s);
+        launch<THREADS, MANY>(a, aligned, past, run, s);
 }
 
 }  // namespace
 
 hipError_t launch_layernorm_mix_rows(const MixRowsArgs& a, hipStream_t s)
 {
-    if (a.n <= 256 * PER)
+    if (a.n < PER)
+        launch<64, SINGLE, MIX_MAX, false>(a, 1, s);
+    else if (a.n <= 64 * PER)
+        launch<64>(a, s);
+    else if (a.n <= 128 * PER)
+        launch<128>(a, s);
+    else if (a.n <= 256 * PER)
         launch<256>(a, s);
     else if (a.n <= 512 * PER)
         launch<512>(a, s);
+    else if (a.n <= 768 * PER)
+        launch<768>(a, s);
     else
         launch<1024>(a, s);
     return hipGetLastError();

@@ -118,6 +118,17 @@ def test_mix_rows(hip, n, mixes, fmt, counts):
     _check_mix(hip, inp, starts, source, to, slots, fmt)
 
 
+@pytest.mark.parametrize("n,mixes", [(7, 2), (8, 1), (9, 2), (15, 6), (511, 1), (515, 6), (1000, 6), (1027, 3), (2051, 1), (4099, 6),
+                                     (5003, 6), (6144, 2), (6145, 1)])
+def test_mix_rows_widths(hip, n, mixes):
+    """Widths over which threads and values do not come out even, sequences that stay in their slots."""
+    rng = np.random.default_rng(n)
+    starts, source, to, slots, rows = _lay(rng, [1, 1, 6, 1, 2, 1])
+    inp = _mix_inputs(rng, rows, n, mixes, n % 2 == 0, slots)
+    for fmt in (native.BF16, native.F32):
+        _check_mix(hip, inp, starts, to, to, slots, fmt)
+
+
 @pytest.mark.parametrize("rows,sequences,n", [(1500, 1, 300), (4100, 3, 64), (5000, 4096, 36), (1030, 1030, 256)])
 def test_mix_rows_many(hip, rows, sequences, n):
     """More rows than a workgroup takes in one run; as many sequences as a call takes."""
