@@ -558,20 +558,21 @@ constexpr int COPY_THREADS = 256, COPY_BYTES = COPY_THREADS * 16 * 2;   // of a 
 // through them 47; 4 or 16 KiB a workgroup 56 and 45; a plain copy of the bytes 65).  Bound by HBM, small moves
 // by the launch.
 __global__ __launch_bounds__(COPY_THREADS) void copy_slots_kernel(SlotArrays arrays, int64_t slots, const int32_t* from, const int32_t* to,
-                                                                  int moves)
+                                                                  int moves, int lanes)
 {
+    const int t = threadIdx.x & (lanes - 1), turn = blockIdx.y * (COPY_THREADS / lanes) + threadIdx.x / lanes;
     const si_hip_slot_array a = arrays.at[blockIdx.z];
     const uint64_t first = static_cast<uint64_t>(blockIdx.x) * COPY_BYTES;
     if (first >= a.slot_bytes)
         return;
     const uint64_t last = min(first + COPY_BYTES, a.slot_bytes);
-    for (int i = blockIdx.y; i < moves; i += gridDim.y) {
+    for (int i = turn; i < moves; i += gridDim.y * (COPY_THREADS / lanes)) {
         const int64_t source = from[i], target = to[i];
         if (source < 0 || target < 0 || source >= slots || target >= slots || source == target)
             continue;
         const char* const src = static_cast<char*>(a.base) + source * a.slot_bytes;
         char* const dst = static_cast<char*>(a.base) + target * a.slot_bytes;
-        if (last - first == COPY_BYTES) {
+        if (last - first == COPY_BYTES) {   // (of such slots a workgroup takes one)
             Sixteen v[2];
 #pragma unroll
             for (int j = 0; j < 2; j++)
@@ -581,10 +582,10 @@ __global__ __launch_bounds__(COPY_THREADS) void copy_slots_kernel(SlotArrays arr
                 __builtin_nontemporal_store(v[j], reinterpret_cast<Sixteen*>(dst + first + (threadIdx.x + COPY_THREADS * j) * 16));
         } else {
             const uint64_t whole = first + (last - first) / 16 * 16;
-            for (uint64_t at = first + threadIdx.x * 16; at < whole; at += COPY_THREADS * 16)
+            for (uint64_t at = first + t * 16; at < whole; at += lanes * 16)
                 *reinterpret_cast<Sixteen*>(dst + at) = *reinterpret_cast<const Sixteen*>(src + at);
-            if (whole + threadIdx.x < last)
-                dst[whole + threadIdx.x] = src[whole + threadIdx.x];
+            if (whole + t < last)
+                dst[whole + t] = src[whole + t];
         }
     }
 }
@@ -629,8 +630,10 @@ hipError_t launch_copy_slots(const si_hip_slot_array* arrays, int count, int64_t
             some.at[i] = arrays[first + i];
             most = most > some.at[i].slot_bytes ? most : some.at[i].slot_bytes;
         }
-        const dim3 grid(static_cast<unsigned>((most + COPY_BYTES - 1) / COPY_BYTES), moves < 65535 ? moves : 65535, n);
-        hipLaunchKernelGGL(copy_slots_kernel, grid, dim3(COPY_THREADS), 0, s, some, slots, from, to, moves);
+        // Small slots several a workgroup (500 moves in 64 arrays of 364 bytes 6.3 us, one a workgroup 22).
+        const int lanes = most <= 1024 ? 16 : most <= 4096 ? 64 : COPY_THREADS, turns = (moves + COPY_THREADS / lanes - 1) / (COPY_THREADS / lanes);
+        const dim3 grid(static_cast<unsigned>((most + COPY_BYTES - 1) / COPY_BYTES), turns < 65535 ? turns : 65535, n);
+        hipLaunchKernelGGL(copy_slots_kernel, grid, dim3(COPY_THREADS), 0, s, some, slots, from, to, moves, lanes);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess)
             return e;

@@ -497,7 +497,7 @@ def test_beam_select_ended_beams(hip):
 
 # ---- slot moves ----------------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("sizes", [[1], [3, 17, 16384], [16, 16400, 40000, 16384 * 3 + 5], [4097] * 70])
+@pytest.mark.parametrize("sizes", [[1], [1000, 24, 1024], [2500, 16, 4096], [3, 17, 16384], [16, 16400, 40000, 16384 * 3 + 5], [4097] * 70])
 @pytest.mark.parametrize("shift", [0, 1, 4])
 def test_copy_slots(hip, sizes, shift):
     rng = np.random.default_rng(len(sizes))
