@@ -366,7 +366,7 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
     __shared__ Key s_list[BEAMS_MAX][CANDIDATES_MAX];
     __shared__ double s_log[BEAMS_MAX], s_score[BEAMS_MAX * CANDIDATES_MAX], s_top_score[BEAMS_MAX * CANDIDATES_MAX];
     __shared__ float s_most[BEAMS_MAX];
-    __shared__ int s_top[BEAMS_MAX * CANDIDATES_MAX], s_parent[CANDIDATES_MAX], s_slot[BEAMS_MAX], s_free[BEAMS_MAX];
+    __shared__ int s_top[BEAMS_MAX * CANDIDATES_MAX], s_parent[CANDIDATES_MAX], s_slot[BEAMS_MAX], s_child[BEAMS_MAX], s_free[BEAMS_MAX];
     const int s = blockIdx.x, t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int k = a.candidates, beams = a.beams, all = beams * k;
@@ -468,6 +468,10 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
     __syncthreads();
     if (wave > 0)
         return;
+    if (t < beams) {
+        s_slot[t] = slot;
+        s_child[t] = BEAMS_MAX;   // a beam's first candidate
+    }
     // The candidates among which the best k are (their scores rounded to FP32: the order stays), put in order by the number of
     // larger ones (of equal ones the first).
     constexpr int PERL = BEAMS_MAX * CANDIDATES_MAX / 64;
@@ -528,14 +532,11 @@ __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a
     // candidates = beams, one a lane: a parent's first child keeps its slot, the others take those of beams without children in turn
     wave_sync();
     const int parent = t < beams ? s_parent[t] : -1;
-    uint64_t keepers = 0, childless = 0;
-    for (int b = 0; b < beams; b++) {
-        const uint64_t children = __ballot(parent == b);
-        keepers |= children & -children;
-        childless |= children == 0 ? 1ull << b : 0;
-    }
-    if (t < beams)
-        s_slot[t] = slot;
+    if (parent >= 0)
+        atomicMin(&s_child[parent], t);
+    wave_sync();
+    const uint64_t keepers = __ballot(parent >= 0 && s_child[max(parent, 0)] == t);
+    const uint64_t childless = __ballot(t < beams && s_child[min(t, BEAMS_MAX - 1)] == BEAMS_MAX);
     const uint64_t before = (1ull << t) - 1;
     if (childless >> t & 1)
         s_free[__popcll(childless & before)] = slot;
