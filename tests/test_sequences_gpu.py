@@ -255,6 +255,14 @@ def test_wkv_rows_long(hip, heads, counts):
     _check_wkv(hip, _wkv_inputs(rng, rows, heads, False, slots), heads, False, starts, source, to, native.F32)
 
 
+@pytest.mark.parametrize("most", [3, 20, 45])
+def test_wkv_rows_of_many_heads(hip, most):
+    """More heads than the card takes at once, of sequences of few rows and of some more."""
+    rng = np.random.default_rng(most)
+    starts, source, to, slots, rows = _lay(rng, list(rng.integers(0, most, 50)) + [most], tail=1)
+    _check_wkv(hip, _wkv_inputs(rng, rows, 24, most == 20, slots), 24, most == 20, starts, source, to, native.BF16)
+
+
 @pytest.mark.parametrize("starts", [[0, 0], [3, 8], [5, 120], [100, 300], [0, 640], [0, 0, 5, 25], [2, 4, 400, 400], [0, 100, 600]])
 def test_wkv_rows_fewer_than_stated(hip, starts):
     """Sequences, one among them, that bring fewer rows than the launch goes by."""
