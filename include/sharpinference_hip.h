@@ -694,7 +694,7 @@ typedef struct si_hip_beam_select_args {
     const void* logits;        /* [sequences * beams] rows of vocab values of logits_format, `stride` values apart */
     const float* scores;       /* [sequences * beams]: each beam's log-probability so far; not finite: no beam */
     const int32_t* done;       /* optional [sequences * beams]: not 0: the beam has ended */
-    const int32_t* slots;      /* optional [sequences * beams]: the slot of each beam's state */
+    const int32_t* slots;      /* optional [sequences * beams]: the slot of each beam's state, each another */
     int32_t* parents;          /* [sequences][candidates]: the beam, 0..beams - 1, that the candidate continues */
     int32_t* tokens;           /* [sequences][candidates] */
     float* new_scores;         /* [sequences][candidates]; may be `scores` when candidates = beams */
