@@ -56,6 +56,7 @@ class Rwkv7RowsSession:
         self.embedded, self.hidden, self.norm, self.mixed = rows(D), [rows(D), rows(D)], rows(D), rows(6 * D)
         self.r, self.k, self.v, self.att, self.add, self.v_first = (rows(D) for _ in range(6))
         self.lora = {n: rows(rank) for n, rank in (("w", cfg.rank_w), ("a", cfg.rank_a), ("g", cfg.rank_g), ("v", cfg.rank_v))}
+        self.activated = rows(max(cfg.rank_w, cfg.rank_g))   # of one LoRA vector at a time
         self.lora_out = {n: rows(D) for n in "wagv"}
         self.ffn, self.ffn_relu = rows(F), rows(F)
         self.logits = rows(V)
@@ -110,9 +111,9 @@ class Rwkv7RowsSession:
             for name, (m, rank, function) in ranks.items():
                 hidden = self.lora[name].ptr
                 product(p[name + "1"], mixed[m], hidden, rank, D)
-                if function:   # (on the product's place in the mixed rows, which no product reads any more)
-                    hip.t0_elementwise(function, hidden, 0, mixed[m], ROWS * rank)
-                    hidden = mixed[m]
+                if function:
+                    hip.t0_elementwise(function, hidden, 0, self.activated.ptr, ROWS * rank)
+                    hidden = self.activated.ptr
                 product(p[name + "2"], hidden, self.lora_out[name].ptr, D, rank)
             out = {n: b.ptr for n, b in self.lora_out.items()}
             hip.rwkv7_wkv_rows(native.Rwkv7WkvRowsArgs(
