@@ -684,6 +684,7 @@ int si_hip_rwkv7_wkv_rows_workspace_bytes(int heads, uint64_t* bytes);
 /* si_hip_rwkv7_wkv (its formulas, in FP32) for every row of the batch, row after row of
  * each sequence through the sequence's state; output rounded once.  [rows] arrays, state and
  * workspace 16-byte aligned.  A value that is not finite changes nothing of rows before its own.
+ * (A row whose own r and k k_k have a product, summed over the head, beyond FP32 may be not finite itself.)
  * Rows are taken in blocks and long sequences in stretches at once, which the whole batch decides: the same batch
  * gives the same bits, but beside other sequences a row or a state may differ in its last ones.
  * Replaces: the WKV node chain (PortableRwkv7GraphProvider.cs:224-276), run token after

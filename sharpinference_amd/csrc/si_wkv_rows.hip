@@ -451,7 +451,9 @@ __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks
             rh[v] = x.r[v] * decay;
             squares[v] = sk * sk;
             bonus[v] = key * x.r[v] * rk;
-            top = largest(largest(top, al[v], kh[v]), rh[v], va[v]);   // (beta is at most alpha / decay)
+            // sk in alpha's and beta's place: alpha is at most that, beta 2^14 times that (one over the block's decays), so that
+            // under 2^50 a product of two rows is at most 64 * 2^(50 + 64).  (beta / alpha is up to 2^27, and khat may be 0.)
+            top = largest(largest(top, sk, kh[v]), rh[v], va[v]);
         }
         put_column4(b.alpha, 4 * g, ch, al);
         if (!TRANSFER)
