@@ -40,3 +40,13 @@ def test_large_key_before_a_large_readout(hip, count, at):
     inp["r"][at + 1] = np.sign(inp["k"][at]) * np.float32(2.0 ** 63.4) * (1 + 0.4 * rng.random(128).astype(np.float32))
     inp["state"] *= np.float32(1e-6)
     _check(hip, inp, 2, count, UNDERFLOW)
+
+
+@pytest.mark.parametrize("count", [1, 5, 13, 20, 33, 400])
+def test_decays_at_both_ends(hip, count):
+    """w0 of plus and minus infinity: the fastest decay and none, in every row (and in no row that a block does not have)."""
+    rng = np.random.default_rng(count)
+    inp = _wkv_inputs(rng, count, 2, False, 3)
+    inp["w0"][3::7] = np.inf
+    inp["w0"][5::7] = -np.inf
+    _check(hip, inp, 2, count)
