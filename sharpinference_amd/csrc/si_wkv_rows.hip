@@ -414,15 +414,14 @@ __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks
         BlockLds& b = lds.block[stage & 1];
         const int at = blocks.at, rows = blocks.last() - at;
         // 1: the rows' factors
-        f4 al, rh, be, kh, va, cum, squares, bonus;
-#pragma unroll
-        for (int v = 0; v < 4; v++)
-            cum[v] = -0.606531f * LOG2E * sigmoid_shifted(x.wl[v], w0);
-        if (rows < C) {   // a decay of 1 (whatever w0 is), the rest 0
+        constexpr float FASTEST = -0.606531f * LOG2E;   // a row's decay at most, as an exponent
+        f4 fastest = {FASTEST, FASTEST, FASTEST, FASTEST};
+        if (rows < C) {   // a decay of 1 (whatever w0 is: by the factor, since no w_lora gives it where w0 is infinite), the rest 0
 #pragma unroll
             for (int v = 0; v < 4; v++) {
                 const bool in = 4 * g + v < rows;
-                cum[v] = in ? cum[v] : 0.0f;
+                x.wl[v] = in ? x.wl[v] : 0.0f;
+                fastest[v] = in ? FASTEST : 0.0f;
                 x.al[v] = in ? x.al[v] : 0.0f;
                 x.vl[v] = in ? x.vl[v] : 0.0f;
                 x.vf[v] = in ? x.vf[v] : 0.0f;
@@ -431,6 +430,10 @@ __device__ void chunk_prepare(const WkvRowsArgs& a, ChunkLds& lds, int h, Blocks
                 x.r[v] = in ? x.r[v] : 0.0f;
             }
         }
+        f4 al, rh, be, kh, va, cum, squares, bonus;
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+            cum[v] = fastest[v] * sigmoid_shifted(x.wl[v], w0);
         cum[1] += cum[0];
         cum[2] += cum[1];
         cum[3] += cum[2];
