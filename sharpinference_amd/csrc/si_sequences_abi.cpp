@@ -333,6 +333,9 @@ int si_hip_copy_slots(si_hip_context* ctx, const si_hip_slot_array* arrays, int 
         if (!arrays[i].base || arrays[i].slot_bytes < 1 || arrays[i].slot_bytes > MAX_SLOT_BYTES)
             return fail(ctx, SI_HIP_ERR_ARGUMENT, "%s: array %d is null or its slots of %llu bytes lie outside 1..2^36", op, i,
                         static_cast<unsigned long long>(arrays[i].slot_bytes));
+        if (static_cast<uint64_t>(slots) > (UINT64_MAX - reinterpret_cast<uintptr_t>(arrays[i].base)) / arrays[i].slot_bytes)
+            return fail(ctx, SI_HIP_ERR_ARGUMENT, "%s: array %d, %lld slots of %llu bytes, passes the address space", op, i,
+                        static_cast<long long>(slots), static_cast<unsigned long long>(arrays[i].slot_bytes));
         const uint64_t size = arrays[i].slot_bytes * static_cast<uint64_t>(slots);
         if (overlaps(arrays[i].base, size, from, bytes) || overlaps(arrays[i].base, size, to, bytes))
             return fail(ctx, SI_HIP_ERR_ARGUMENT, "%s: array %d overlaps from or to", op, i);
