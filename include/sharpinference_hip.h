@@ -729,7 +729,7 @@ int si_hip_beam_select_workspace_bytes(int sequences, int beams, int candidates,
 int si_hip_beam_select(si_hip_context* ctx, const si_hip_beam_select_args* args);
 
 typedef struct si_hip_slot_array {
-    void* base;                /* [slots] of slot_bytes */
+    void* base;                /* [slots] of slot_bytes, inside the address space */
     uint64_t slot_bytes;       /* at least 1 */
 } si_hip_slot_array;
 

@@ -50,7 +50,7 @@ __device__ __forceinline__ float group_bound(float best, int k)
 
 // A value that k lanes' largest ones or more reach, near the k-th of them: the groups' bound, raised by halves of what lies
 // between it and the largest.  The groups' alone lets k H_k values through (54 of 2048 spread ones for k = 16), this one few more
-// than k: 8 sequences of 16 beams over 151936 values 27 us where that one takes 49, 2 of 9 beams and 18 candidates 15 and 36.
+// than k: 8 sequences of 16 beams over 151936 values 29 us where that one takes 62, 2 of 9 beams and 18 candidates 14 and 40.
 __device__ __forceinline__ float near_kth(float best, int k)
 {
     float low = group_bound(best, k), high = rows_max(row_max<16>(best));
@@ -161,8 +161,8 @@ __device__ __forceinline__ double wave_sum(double v)
 
 // How a row is cut: tiles a part, parts a row.  A wave takes a part; where there are
 // more tiles than the card holds waves of this kernel, it takes several one after another (192 rows of 98 tiles, with the merge:
-// five a wave 26 us, ten 27, three 25 to 27, one 35).  Larger parts for fewer keys to merge do not pay (a sequence of 16 beams and 32
-// candidates: 98 parts 29 us, 25 or 49 42 to 43).
+// five a wave 23.1 us, ten 23.3, three 24.0, one 30).  Larger parts for fewer keys to merge pay a little in some shapes and cost more in others
+// (a sequence of 16 beams and 32 candidates: 98 parts 28 to 31 us, 49 26, 25 43).
 struct Cut {
     int tiles, parts;
 };
@@ -193,7 +193,7 @@ __device__ __forceinline__ float value_at(const void* p, int64_t i)
 // One wave a part of a row.  Over a group of tiles it takes the sum and each 16-byte word's largest value; then it reads the
 // words again that may hold one of the best (few more than those), and ranks those values together: ranked tile by tile
 // out of registers, that part took as long as the rest.  Bound by HBM, then by the tail of ranking and launch: 24 sequences of 8 beams over
-// 200064 16-bit logits, 65 MB of them read, 18.5 us, 3.5 TB/s (17 without ranking; tile by tile 28).  One sequence of 4 beams over
+// 200064 16-bit logits, 65 MB of them read, 18.2 us, 3.6 TB/s (tile by tile 28).  One sequence of 4 beams over
 // 65536 FP32 logits: 5.1 us, the launch and one chain of round trips.
 template <int FMT>
 __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs a, int rows, int tiles, int parts, Part* part, Key* keys)
@@ -357,8 +357,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 4) void beam_scan_kernel(BeamArgs 
 // One workgroup a sequence.  Wave b merges the lists of row b's parts, wave 15 - b sums the row; then all candidates
 // of the rows are ranked by score.  A chain of round trips, bound by their latency, with many beams by the 16 waves' instructions
 // on one compute unit: what does not hang on another load is requested first, and only keys and candidates that near_kth lets through
-// are ranked (24 sequences of 8 beams 6.1 us, one of 4 beams 4.7, 3 of 16 beams over one part a row 7.0, of one part's list and
-// every candidate against every other 11.5; 98 parts of 32 candidates 21.5, each 512 keys ranked by themselves 55).
+// are ranked (24 sequences of 8 beams 6.0 us, one of 4 beams 4.5, 3 of 16 beams over one part a row 6.5; 16 beams' 98 parts of 32
+// candidates 22).
 __global__ __launch_bounds__(64 * MERGE_WAVES) void beam_merge_kernel(BeamArgs a, int parts, const Part* part, const Key* keys)
 {
     constexpr int LANE_KEYS = 8;

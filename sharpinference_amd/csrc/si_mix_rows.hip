@@ -13,20 +13,20 @@ constexpr int PER = 8;   // values of a row a thread
 // How a thread's eight values of a row lie: ALIGNED: neighbours at multiples of 16 bytes.  NEIGHBOURS: at any address; where
 // eight does not divide the width, the last thread takes the last eight, of which the thread before has some too: it leaves them out of the
 // sums and writes them again (the state's are read two barriers before).  SINGLE: every THREADS-th (widths under eight; 3900 rows of
-// 2047 in six mixes so 64 us, as neighbours 46).
+// 2047 in six mixes so 56 us, as neighbours 41).
 enum Lie { ALIGNED, NEIGHBOURS, SINGLE };
 typedef float AlignedFour __attribute__((ext_vector_type(4)));
 typedef float AnyFour __attribute__((ext_vector_type(4), aligned(4)));
 
-// A workgroup of THREADS, as many as a row has eights, takes `run` rows one after another (4000 rows of 768 in six mixes 20 us,
-// with 256 threads 33).  Weights and mixes stay in registers, and so does the row before: only a run's
+// A workgroup of THREADS, as many as a row has eights, takes `run` rows one after another (4000 rows of 768 in six mixes 15 us,
+// with 256 threads 21).  Weights and mixes stay in registers, and so does the row before: only a run's
 // first row is normalised twice.  The next row is requested while this one is normalised.  The sequence's
 // state is read by the workgroup of its first row, which also normalises the last row for the state's slot:
 // the slot has one reader and writer, whatever the other workgroups have done by then.
-// Bound by HBM: 4 bytes in (8 with a residual, 4 more out) and 2 or 4 out a mix (3900 rows of 2048 in six mixes 37 us, 5.5 TB/s);
-// a single row by its round trips (16 rows 4.7 us).
+// Bound by HBM: 4 bytes in (8 with a residual, 4 more out) and 2 or 4 out a mix (4163 rows of 2048 with the residual in six mixes 37.5 us, 5.5
+// TB/s); a single row by its round trips (16 rows 4.5 us).
 // HELD: mixes that registers hold (0: they are loaded with every row: 1024 threads leave no room for more than one; 976 rows of 8192 in
-// six mixes 44 us, 1953 of 4096 40).
+// six mixes 39 us, 1953 of 4096 34).
 // PAST: outputs go past the L2s.
 template <int THREADS, Lie LIE, int HELD, bool PAST, typename OUT>
 __global__ __launch_bounds__(THREADS) void mix_rows_kernel(MixRowsArgs a, int run)
@@ -258,13 +258,13 @@ void launch(const MixRowsArgs& a, hipStream_t s)
     const bool aligned = a.n % 8 == 0 && aligned16(a.x) && aligned16(a.residual) && aligned16(a.weight) && aligned16(a.bias) &&
                         aligned16(a.mix) && aligned16(a.state) && aligned16(a.updated) && aligned16(a.out);
     // Outputs that the L2s (32 MiB) cannot keep for the next kernel go past them: 4000 rows of 2048 values in six mixes
-    // take 43 us instead of 66.  Smaller ones stay there for the products that read them.
+    // take 35 us instead of 47.  Smaller ones stay there for the products that read them.
     const int64_t out = static_cast<int64_t>(a.batch.rows) * a.n *
                         ((a.out_format == ROWS_OUT_F32 ? 4 : 2) * (a.mixes > 0 ? a.mixes : 1) + (a.residual ? 4 : 0));
     const bool past = out > (16 << 20);
-    // Runs such that so many waves a compute unit have one each, of wide rows as many whole workgroups (976 rows of 8192 in six mixes 44
-    // us, at 0.9 workgroups a compute unit 65); few rows one a workgroup.  Odd ones: at 4 or 8 rows a
-    // run the workgroups' rows lie a power of two apart, and 4000 rows take 48 and 55 us, at 3, 5 and 9 rows 43, 41 and 36.
+    // Runs such that so many waves a compute unit have one each, of wide rows as many whole workgroups (976 rows of 8192 in six mixes 39
+    // us, at 0.9 workgroups a compute unit 52); few rows one a workgroup.  4000 rows of 2048 take so, 9 rows a run, 35 us; with runs of 3,
+    // 4, 5 and 8 rows 38, 41, 45 and 36 (odd ones keep the workgroups' rows from lying a power of two apart).
     const int waves = a.mixes <= 1 ? 20 : 7, most = waves * 64 / THREADS, rows = a.batch.rows;
     const int resident = THREADS < 512 ? 256 * waves * 64 / THREADS : 256 * (most > 1 ? most : 1);
     const int run = rows <= resident ? 1 : rows < 15 * resident ? ((rows + resident - 1) / resident) | 1 : 15;

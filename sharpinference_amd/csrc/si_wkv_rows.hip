@@ -35,8 +35,8 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Pl
 // of one row).  As many rows at a time as there are waves: wave w prepares row w (one element a
 // lane), all waves take the rows through the state, wave w normalises row w.
 // Bound by reading and writing the state (32 KiB a head) where a sequence
-// brings one row (64 of them, 32 heads, 13.4 us, 5.4 TB/s); by vector instructions (92 a row and wave of four) and LDS reads
-// (10 b128 a lane and row) where it brings many (64 of 8 rows 28 us).
+// brings one row (64 of them, 32 heads, 13.1 us, 5.5 TB/s); by vector instructions (92 a row and wave of four) and LDS reads
+// (10 b128 a lane and row) where it brings many (64 of 8 rows 25 us).
 template <int WAVES>
 struct FewLds {
     float4 vec[WAVES][5][N / 4];   // decay, key, kn, kn * a, r of the rows
@@ -725,7 +725,7 @@ constexpr int CARD = 512;                // workgroups of wkv_chunk_kernel that 
 constexpr int HEAD_STRETCHES = 2 * CARD; // stretches (but each sequence's last) times heads, at most
 constexpr int LONG_STRETCH = 256;
 constexpr int LEAST_STRETCH = 48, LEAST_CUT = 176;   // rows of a stretch, and of a sequence that is cut, at least (one of 250 rows, 32 heads,
-                                                     // 44 us, in stretches of 64 55; of 150, cut 42, whole 38)
+                                                     // 41 us, in stretches of 64 53, whole 59; of 150, cut 40, whole 38)
 
 struct Stretch {
     int sequence, first, last;   // rows
@@ -748,8 +748,8 @@ __device__ __forceinline__ StateEnds state_ends(const WkvRowsArgs& a, int s, int
 
 // Rows of a stretch where so many rows of so many sequences are cut: the card's workgroups share them with their heads; where that
 // gives each more than LONG_STRETCH, twice as many workgroups do, which even out better beside whole sequences (32 heads; eight
-// prompts of 500 to 3000 rows 526 us, by CARD 603, three of 1000 to 6000 rows 539 and 704; one of 4001 rows, by CARD, 217, by
-// twice as many 245).
+// prompts of 500 to 3000 rows 518 us, by CARD 590, three of 1000 to 6000 rows 530 and 702; one of 4001 rows, by CARD, 195, by
+// twice as many 225).
 __host__ __device__ inline int stretch_rows(int64_t rows, int heads, int cut)
 {
     const int64_t work = rows * heads, more = static_cast<int64_t>(cut) * heads;   // (of each sequence one stretch is idle in every pass)
@@ -791,7 +791,7 @@ __device__ __forceinline__ bool sole_stretch(const WkvRowsArgs& a, int from, int
 // units' place, so that a block costs a SIMD 92 * 32 = 2944 cycles of them and about 800 vector instructions, 5100 to 5500 cycles
 // in all; two workgroups a compute unit fill one another's barriers (three groups of waves in one, or two that prepare, were
 // faster alone, 7000 and 7700 cycles a block for 8900, and slower together, 1560 and 1580 us for 1024 heads of equal length, 1370).
-// Eight sequences of 1000 rows, 32 heads, one workgroup a compute unit: 234 us.
+// Eight sequences of 1000 rows, 32 heads, one workgroup a compute unit: 220 us.
 enum ChunkPass { CHUNK_SEQUENCES, CHUNK_STRETCHES, CHUNK_TRANSFERS };
 
 template <int PASS>
@@ -935,9 +935,9 @@ __global__ __launch_bounds__(256) void wkv_join_kernel(WkvRowsArgs a, int from, 
 
 // From how many rows on a launch cuts its sequences, or 0: none.  Cutting costs the transfers and the join, and pays where the
 // longest sequence has 2.5 times the rows that all, shared out evenly, give a workgroup (32 heads; eight of 1000 rows, at 2:
-// 234 us whole, 286 cut; sixteen of 100 to 3000, at 3.2: 860 and 610) and becomes three stretches or more.  Where stretches are not
-// long, shorter ones that become two, without transfers, then need not wait whole for the last pass (five of 300 to 1500 207 us,
-// from three on 250; the sixteen, whose stretches are long, 659 and 615).
+// 220 us whole, 259 cut; sixteen of 100 to 3000, at 3.2: 856 and 595) and becomes three stretches or more.  Where stretches are not
+// long, shorter ones that become two, without transfers, then need not wait whole for the last pass (five of 300 to 1500 212 us,
+// from three on 249; the sixteen, whose stretches are long, 644 and 595).
 int cut_from(const WkvRowsArgs& a)
 {
     const int64_t each = (static_cast<int64_t>(a.batch.rows) * a.heads + CARD - 1) / CARD;
@@ -1019,9 +1019,9 @@ __device__ void make_plan(const WkvRowsArgs& a, int over, int from, int room, Pl
 
 }  // namespace
 
-// Sequences of up to this many rows go row by row (32 heads; one sequence of 12 rows 7.4 us, of 14 rows 8.1, by blocks 7.4 both; eight of
-// 9 rows 7.7, by blocks 8.6, of 14 9.9 and 9.1), and of up to this many where workgroups wait for one another (64 of 17 rows 47,
-// by blocks 63, of 24 59 and 66; beside twice the card's workgroups, 32 of 1 to 24 rows, it is 25 and 22).
+// Sequences of up to this many rows go row by row (32 heads; one sequence of 12 rows 7.2 us, of 14 rows 7.9, by blocks 7.2 both; eight of
+// 9 rows 7.1, by blocks 8.1, of 14 9.0 and 8.5), and of up to this many where workgroups wait for one another (64 of 17 rows 44,
+// by blocks 61, of 24 57 and 63; beside twice the card's workgroups, 32 of 1 to 24 rows, it is 23 and 20).
 constexpr int FEW_ROWS = 12, MANY_FEW_ROWS = 24;
 
 // The list: every sequence that goes by blocks, at most, the stretches, and the cut sequences again (at most as many as
@@ -1035,8 +1035,8 @@ hipError_t launch_wkv_rows(const WkvRowsArgs& a, hipStream_t s)
     const unsigned heads = static_cast<unsigned>(a.heads), grid = static_cast<unsigned>(a.batch.sequences) * heads;
     const int over = grid <= 2 * CARD ? FEW_ROWS : MANY_FEW_ROWS;
     if (a.batch.max_rows <= over) {
-        // Eight waves a head where that leaves no workgroup waiting for another (seven sequences of 3 to 6 rows, 32 heads, 5.6 us, of four
-        // 6.9; 64 of one row 14.3 and 13.5).
+        // Eight waves a head where that leaves no workgroup waiting for another (seven sequences of 3 to 6 rows, 32 heads, 5.4 us, of four
+        // 6.6; 64 of one row 14.2 and 13.1).
         if (grid <= CARD)
             hipLaunchKernelGGL(wkv_few_kernel<8>, dim3(grid), dim3(512), 0, s, a, INT32_MAX, 0, 0, nullptr);
         else
