@@ -139,7 +139,8 @@ class Rwkv7RowsSession:
     # -- steps -----------------------------------------------------------------------------
     def step(self, sequences: Sequence[Sequence[int]], from_: Sequence[int], to: Sequence[int]) -> np.ndarray:
         """The next tokens of some sequences (16 in all, at most): sequence s goes on from slot from_[s] (-1: from the
-        beginning) and leaves its state in slot to[s] (-1: nowhere).  Returns the logits of every row [rows, vocab]."""
+        beginning) and leaves its state in slot to[s] (-1: nowhere; a sequence without tokens leaves none).  Returns the logits of
+        every row [rows, vocab]."""
         counts = [len(t) for t in sequences]
         rows = sum(counts)
         if not sequences or len(sequences) > ROWS or rows < 1 or rows > ROWS:
